@@ -391,6 +391,48 @@ LDB_API int ldb_apply_lesion_change(ldb_stream_t stream, const float* original, 
                                     const float* reconstruction, const uint8_t* lesion, float* out, int n0, int n1,
                                     int n2, int reach, uint8_t* workspace, size_t workspace_bytes, double* stats);
 
+/* -------------------------------------------------------------------------
+ * 8-bit transformer operators.  Values are e4m3 codes (1 byte) with one
+ * power-of-two scale (E8M0: a byte that stands for 2^(byte - 127)) per block:
+ * the smallest 2^e with max|y| <= 448 * 2^e over the block's finite values (1
+ * for a block of zeros); a value that is not finite becomes the NaN code.  Rows have
+ * a scale per 128 channels (the last block may be short), weights a scale per
+ * 128 x 128 block.  Row strides (`_ld`) count elements (bytes for codes and
+ * scales).  The reference has no 8-bit arithmetic; these are additions.
+ * ---------------------------------------------------------------------- */
+
+/* h = x + residual (residual null: h = x), stored rounded to `dtype` (h may
+ * be null), and codes / scales of h * rsqrt(mean(h^2) + eps) * gamma, computed in
+ * FP32 from the unrounded h (gamma f32, null = 1).  1..32768 channels; codes
+ * 16-byte aligned with codes_ld a multiple of 16; any x / residual / h strides
+ * (16-byte aligned rows of a multiple of 8 channels take wide accesses). */
+LDB_API int ldb_rms_norm_fp8(ldb_stream_t stream, const void* x, long long x_ld, const void* residual,
+                             long long residual_ld, int dtype, const float* gamma, float eps, void* h, long long h_ld,
+                             uint8_t* codes, long long codes_ld, uint8_t* scales, long long scales_ld, int rows,
+                             int channels);
+
+/* Codes and scales of the rows of x as they are. */
+LDB_API int ldb_quantize_fp8_rows(ldb_stream_t stream, const void* x, long long x_ld, int dtype, uint8_t* codes,
+                                  long long codes_ld, uint8_t* scales, long long scales_ld, int rows, int channels);
+
+/* Codes and scales of an (n, k) weight: scales[(row / 128) * scales_ld + column / 128]. */
+LDB_API int ldb_pack_weight_fp8(ldb_stream_t stream, const void* w, long long w_ld, int dtype, uint8_t* codes,
+                                long long codes_ld, uint8_t* scales, int scales_ld, int n, int k);
+
+/* out[m, n] = act(sum_k a[m, k] w[n, k] + bias[n] + residual[m, n]) of 8-bit
+ * rows a and an 8-bit weight w, accumulated in FP32 and rounded once to
+ * out_dtype (the residual has the output's type; bias f32; both may be null).
+ * Codes 16-byte aligned with strides a multiple of 16; row scales 4-byte
+ * aligned with a stride that is a multiple of 4; any n, k, out and residual
+ * strides.  The workspace (16-byte aligned) holds partial sums where few tiles
+ * are split over k. */
+LDB_API int ldb_matmul_fp8_workspace_size(int m, int n, int k, size_t* bytes);
+LDB_API int ldb_matmul_fp8(ldb_stream_t stream, const uint8_t* a, long long a_ld, const uint8_t* a_scales,
+                           long long a_scales_ld, const uint8_t* w, long long w_ld, const uint8_t* w_scales,
+                           long long w_scales_ld, const float* bias, const void* residual, long long residual_ld,
+                           void* out, long long out_ld, int m, int n, int k, int act, int out_dtype, void* workspace,
+                           size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -60,6 +60,7 @@ class ConvDesc(ctypes.Structure):
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_L = ctypes.c_longlong
 _SZ = ctypes.c_size_t
 
 # name -> (argtypes); every function returns int unless listed in _RESTYPES.
@@ -100,6 +101,11 @@ SIGNATURES: dict[str, list] = {
     "ldb_apply_lesion_change": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _SZ, _P],
     "ldb_hu_map": [_P, _P, _I, _I, ctypes.c_longlong, _P],
     "ldb_ct_normalize": [_P, _P, ctypes.c_longlong, _P, _I, _I],
+    "ldb_rms_norm_fp8": [_P, _P, _L, _P, _L, _I, _P, _F, _P, _L, _P, _L, _P, _L, _I, _I],
+    "ldb_quantize_fp8_rows": [_P, _P, _L, _I, _P, _L, _P, _L, _I, _I],
+    "ldb_pack_weight_fp8": [_P, _P, _L, _I, _P, _L, _P, _I, _I, _I],
+    "ldb_matmul_fp8_workspace_size": [_I, _I, _I, ctypes.POINTER(_SZ)],
+    "ldb_matmul_fp8": [_P, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P, _SZ],
 }
 _RESTYPES = {"ldb_last_error": ctypes.c_char_p, "ldb_launch_count": ctypes.c_ulonglong}
 

@@ -273,6 +273,30 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
       : "memory");
 }
 
+// D[tmem] (+)= (A 2^sa)[smem] * (B 2^sb)[smem]^T of 8-bit operands, f32
+// accumulator (kind::mxf8f6f4, K = 32): one E8M0 scale per row of A and of B
+// for each product, read from tensor memory (tmem_copy_scales lays them out).
+// The instruction descriptor names the byte of each 32-bit scale word to use.
+__device__ __forceinline__ void umma_ss_mx8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t sa_tmem, uint32_t sb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::
+          "r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+      : "memory");
+}
+
+// Copy the scales of 128 rows from shared memory (512 bytes: row r's 32-bit
+// word, one byte for each of four products along K, at (r % 32) * 16 +
+// (r / 32) * 4) to 4 TMEM columns, repeated in all four lane quarters: row r
+// at lane r % 32 of column r / 32, as the block-scaled products read them.
+// Ordered before the products this thread issues afterwards.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
 // Arrive once on an mbarrier when all previously issued MMAs of this thread
 // have completed (and finished reading their shared-memory operands).
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
@@ -440,6 +464,13 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int m, int n, uint32_t ab_
                                                       uint32_t b_mn_major) {
   return (1u << 4) | (ab_type << 7) | (ab_type << 10) | (a_mn_major << 15) | (b_mn_major << 16) |
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Instruction descriptor of kind::mxf8f6f4 with E4M3 operands, both K-major,
+// and E8M0 scales; sf_id (0..3) is the byte of the scale words that A and B use.
+__host__ __device__ constexpr uint32_t make_idesc_mx8(int m, int n, uint32_t sf_id) {
+  return (sf_id << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24) |
+         (sf_id << 29);
 }
 
 // ---------------------------------------------------------------- misc

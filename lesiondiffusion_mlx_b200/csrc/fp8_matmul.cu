@@ -1,0 +1,503 @@
+// Product of 8-bit rows and an 8-bit weight on the block-scaled tensor-core
+// path (tcgen05 kind::mxf8f6f4):
+//
+//   y[m, n] = act(sum_k a[m, k] w[n, k] 2^(ea[m, k/128] + ew[n/128, k/128])
+//                 + bias[n] + residual[m, n])
+//
+// The scales are powers of two (E8M0), so the tensor core applies them inside
+// the product, in FP32, and the accumulator stays in TMEM over the whole of K;
+// an FP32 scale per 128 channels would have to leave TMEM for every K block and
+// be applied in registers.  The hardware takes one scale byte per 32 elements
+// of K: the four products of a 128-channel block name the same byte of the
+// 32-bit scale word, and a word holds four consecutive blocks.
+//
+// One CTA per SM walks 128-row x BN-column tiles: warp 0 loads the code tiles
+// (TMA, 128-byte swizzle), warp 2 writes the scale words of each four blocks in
+// the order that tcgen05.cp spreads over TMEM lanes, one thread of warp 1 issues
+// scale copies and products, warps 4-7 drain the accumulator of one tile while
+// the next is computed in the other.  Grids with fewer tiles than SMs cut K into
+// ranges whose FP32 partial sums a second kernel adds in order.
+
+#include <algorithm>
+
+#include "fp8.cuh"
+#include "host_common.h"
+
+namespace ldb {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTileM = 128;
+constexpr int kMaxStages = 8;
+constexpr int kScaleStages = 4;                // ring of scale groups in shared memory
+constexpr int kScaleBytes = 512 + 1024;        // A words, then up to 256 B words
+constexpr int kMaxBn = 224;
+constexpr int kSmemBudget = 200 * 1024;        // code stages
+constexpr int kTmemCols = 512;
+static_assert(2 * kMaxBn + kScaleStages * 12 <= kTmemCols, "two accumulators and the scale sets");
+
+struct MatmulParams {
+  const uint8_t* a_scales;
+  const uint8_t* w_scales;
+  const float* bias;      // may be null
+  const void* residual;   // may be null
+  void* out;
+  float* partial;         // split > 1: [split][m][n]
+  long long a_scales_ld, w_scales_ld, res_ld, out_ld;
+  int m, n, k;
+  int bn, stages, box_m;
+  int tiles_m, tiles_n, split, kb_per_split;
+  int act, out_dtype;
+  int vec;  // out, residual and partial rows allow 16-byte accesses
+};
+
+// Scale words of tile row `row` (128-channel blocks kb .. kb + 3) of A; blocks
+// and rows outside the operand count as scale 1 (their codes are zero).
+__device__ __forceinline__ uint32_t a_scale_word(const MatmulParams& p, int row, int kb, int kblocks) {
+  if (row >= p.m) return 0x7F7F7F7Fu;
+  const uint8_t* s = p.a_scales + row * p.a_scales_ld + kb;
+  if (kb + 4 <= kblocks) return *reinterpret_cast<const uint32_t*>(s);
+  uint32_t w = 0x7F7F7F7Fu;
+  for (int j = 0; j < 4 && kb + j < kblocks; ++j) w = (w & ~(0xFFu << (8 * j))) | (static_cast<uint32_t>(s[j]) << (8 * j));
+  return w;
+}
+__device__ __forceinline__ uint32_t w_scale_word(const MatmulParams& p, int col, int kb, int kblocks) {
+  uint32_t w = 0x7F7F7F7Fu;
+  if (col >= p.n) return w;
+  const uint8_t* s = p.w_scales + (col / kFp8Block) * p.w_scales_ld + kb;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (kb + j < kblocks) w = (w & ~(0xFFu << (8 * j))) | (static_cast<uint32_t>(s[j]) << (8 * j));
+  return w;
+}
+
+// Tile and K range of work item i: rows vary fastest, so neighbouring CTAs
+// share a weight tile.
+struct Work {
+  int row0, col0, kb0, kb1, split;
+};
+__device__ __forceinline__ Work work_item(const MatmulParams& p, int i, int kblocks) {
+  Work w;
+  const int tm = i % p.tiles_m;
+  const int rest = i / p.tiles_m;
+  w.split = rest % p.split;
+  w.row0 = tm * kTileM;
+  w.col0 = (rest / p.split) * p.bn;
+  w.kb0 = w.split * p.kb_per_split;
+  w.kb1 = min(kblocks, w.kb0 + p.kb_per_split);
+  return w;
+}
+
+// 32 columns of one output row: bias, residual, activation, one rounding.
+template <typename T>
+__device__ __forceinline__ void finish32(const MatmulParams& p, int row, int col, float (&v)[32]) {
+  const bool full = p.vec && col + 32 <= p.n;
+  if (p.bias) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (full || col + j < p.n) v[j] += p.bias[col + j];
+  }
+  if (p.residual) {
+    const T* r = static_cast<const T*>(p.residual) + row * p.res_ld + col;
+    if (full) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float a[8];
+        load8<T>(r + 8 * c, a);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[8 * c + j] += a[j];
+      }
+    } else {
+      for (int j = 0; j < 32; ++j)
+        if (col + j < p.n) v[j] += to_f32<T>(r[j]);
+    }
+  }
+  if (p.act == LDB_ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = gelu_erf_f32(v[j]);
+  }
+  T* o = static_cast<T*>(p.out) + row * p.out_ld + col;
+  if (full) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float a[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = v[8 * c + j];
+      store8<T>(o + 8 * c, a);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col + j < p.n) o[j] = from_f32<T>(v[j]);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_matmul_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap wmap,
+                      const MatmulParams p, unsigned int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_bytes = kTileM * 128 + p.bn * 128;
+  uint8_t* s_scales = smem + p.stages * stage_bytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_scales + kScaleStages * kScaleBytes);
+  uint64_t* full = bars;                       // [kMaxStages] codes have landed
+  uint64_t* empty = full + kMaxStages;         // [kMaxStages] the products have read them
+  uint64_t* sf_full = empty + kMaxStages;      // [kScaleStages] scale words are written
+  uint64_t* sf_empty = sf_full + kScaleStages; // [kScaleStages] the copy and the products have read them
+  uint64_t* acc_full = sf_empty + kScaleStages;  // [2] a tile's products are done
+  uint64_t* acc_empty = acc_full + 2;            // [2] the epilogue has drained it
+  uint64_t* drain = acc_empty + 2;               // an aborting CTA's last products
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = warp_id();
+  const int lane = lane_id();
+  const int kblocks = (p.k + kFp8Block - 1) / kFp8Block;
+  const int items = p.tiles_m * p.tiles_n * p.split;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kMaxStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < kScaleStages; ++s) {
+      mbar_init(&sf_full[s], 32);
+      mbar_init(&sf_empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&acc_full[t], 1);
+      mbar_init(&acc_empty[t], 4);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&amap);
+    tma_prefetch_desc(&wmap);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_begin();
+
+  if (warp == 0) {
+    // -------------------------------------------------------------- codes
+    if (lane == 0) {
+      int st = 0;
+      uint32_t ph = 0;
+      int loads = 0;
+      const uint32_t bytes = static_cast<uint32_t>(p.box_m + p.bn) * 128;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+        const Work w = work_item(p, i, kblocks);
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          if (!mbar_wait(&empty[st], ph ^ 1u, abort_flag, status)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = smem + st * stage_bytes;
+          mbar_arrive_expect_tx(&full[st], bytes);
+          tma_load_2d(sa, &amap, &full[st], kb * 128, w.row0);
+          tma_load_2d(sa + kTileM * 128, &wmap, &full[st], kb * 128, w.col0);
+          ++loads;
+          if (++st == p.stages) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      if (*abort_flag) {
+        // Let the loads in flight land before the CTA gives up its shared memory.
+        volatile int never = 0;
+        for (int back = 1; back <= min(loads, p.stages); ++back) {
+          const int l = loads - back;
+          mbar_wait(&full[l % p.stages], static_cast<uint32_t>(l / p.stages) & 1u, &never, status);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ products
+    if (lane == 0) {
+      // Scale words in TMEM: a set of columns per ring slot, behind the two accumulators.
+      const int sfb_cols = 4 * ((p.bn + 127) / 128);
+      const uint32_t sf_cols = 4 + sfb_cols;
+      const uint32_t sf_base = tmem + kTmemCols - kScaleStages * sf_cols;
+      int st = 0, sst = 0, tile = 0;
+      uint32_t ph = 0, sph = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++tile) {
+        const Work w = work_item(p, i, kblocks);
+        const uint32_t acc = tmem + (tile & 1) * p.bn;
+        ok = mbar_wait(&acc_empty[tile & 1], (static_cast<uint32_t>(tile >> 1) & 1u) ^ 1u, abort_flag, status);
+        if (!ok) break;
+        tc_fence_after();
+        for (int kb = w.kb0; ok && kb < w.kb1; kb += 4) {
+          if (!mbar_wait(&sf_full[sst], sph, abort_flag, status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sfa = sf_base + sst * sf_cols;
+          const uint32_t sfb = sfa + 4;
+          const uint32_t s_addr = smem_u32(s_scales + sst * kScaleBytes);
+          tmem_copy_scales(sfa, make_smem_desc(s_addr, 0, 128, kSwizzleNone));
+          for (int c = 0; c < sfb_cols / 4; ++c)
+            tmem_copy_scales(sfb + 4 * c, make_smem_desc(s_addr + 512 + 512 * c, 0, 128, kSwizzleNone));
+          const int kend = min(w.kb1, kb + 4);
+          for (int b = kb; b < kend; ++b) {
+            if (!mbar_wait(&full[st], ph, abort_flag, status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(smem + st * stage_bytes);
+            const uint32_t w_addr = a_addr + kTileM * 128;
+            const uint32_t idesc = make_idesc_mx8(kTileM, p.bn, static_cast<uint32_t>(b - kb));
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              umma_ss_mx8(acc, make_smem_desc(a_addr + q * 32, 16, 1024, kSwizzle128),
+                          make_smem_desc(w_addr + q * 32, 16, 1024, kSwizzle128), idesc, sfa, sfb,
+                          (b > w.kb0 || q > 0) ? 1u : 0u);
+            umma_commit(&empty[st]);
+            if (++st == p.stages) {
+              st = 0;
+              ph ^= 1u;
+            }
+          }
+          umma_commit(&sf_empty[sst]);  // the copy and the products have read this slot
+          if (++sst == kScaleStages) {
+            sst = 0;
+            sph ^= 1u;
+          }
+        }
+        if (ok) umma_commit(&acc_full[tile & 1]);
+      }
+      if (*abort_flag) {
+        volatile int never = 0;
+        umma_commit(drain);
+        mbar_wait(drain, 0, &never, status);
+      }
+    }
+  } else if (warp == 2) {
+    // -------------------------------------------------------------- scales
+    int sst = 0;
+    uint32_t sph = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+      const Work w = work_item(p, i, kblocks);
+      for (int kb = w.kb0; kb < w.kb1; kb += 4) {
+        uint32_t a[4], b[8];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) a[c] = a_scale_word(p, w.row0 + 32 * c + lane, kb, kblocks);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) b[c] = 32 * c < p.bn ? w_scale_word(p, w.col0 + 32 * c + lane, kb, kblocks) : 0;
+        if (!warp_wait(&sf_empty[sst], sph ^ 1u, abort_flag, status)) {
+          ok = false;
+          break;
+        }
+        uint4* dst = reinterpret_cast<uint4*>(s_scales + sst * kScaleBytes);
+        dst[lane] = make_uint4(a[0], a[1], a[2], a[3]);
+        dst[32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
+        if (p.bn > 128) dst[64 + lane] = make_uint4(b[4], b[5], b[6], b[7]);
+        fence_proxy_async_smem();
+        mbar_arrive(&sf_full[sst]);
+        if (++sst == kScaleStages) {
+          sst = 0;
+          sph ^= 1u;
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------- epilogue
+    int tile = 0;
+    for (int i = blockIdx.x; i < items; i += gridDim.x, ++tile) {
+      const Work w = work_item(p, i, kblocks);
+      if (!warp_wait(&acc_full[tile & 1], static_cast<uint32_t>(tile >> 1) & 1u, abort_flag, status)) break;
+      tc_fence_after();
+      const int quarter = warp & 3;
+      const int row = w.row0 + quarter * 32 + lane;
+      const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (tile & 1) * p.bn;
+      const int cols = min(p.bn, p.n - w.col0);
+      if (w.row0 + quarter * 32 < p.m) {
+        for (int c = 0; c < cols; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(acc + c, r);
+          tmem_wait_ld();
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          if (row < p.m) {
+            if (p.split == 1) {
+              finish32<T>(p, row, w.col0 + c, v);
+            } else {
+              float* o = p.partial + (static_cast<long long>(w.split) * p.m + row) * p.n + w.col0 + c;
+              if (p.n % 4 == 0 && w.col0 + c + 32 <= p.n) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  reinterpret_cast<float4*>(o)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (w.col0 + c + j < p.n) o[j] = v[j];
+              }
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[tile & 1]);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Sum of the K ranges in their order, then the epilogue; one thread per value.
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_matmul_reduce_kernel(const MatmulParams p) {
+  pdl_begin();
+  const long long total = static_cast<long long>(p.m) * p.n;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const long long row = i / p.n;
+    const int col = static_cast<int>(i - row * p.n);
+    float v = 0.f;
+    for (int s = 0; s < p.split; ++s) v += p.partial[s * total + i];
+    if (p.bias) v += p.bias[col];
+    if (p.residual) v += to_f32<T>(static_cast<const T*>(p.residual)[row * p.res_ld + col]);
+    if (p.act == LDB_ACT_GELU) v = gelu_erf_f32(v);
+    static_cast<T*>(p.out)[row * p.out_ld + col] = from_f32<T>(v);
+  }
+}
+
+// Column tile, K ranges and ring depth from the extents alone.
+int plan(int m, int n, int k, MatmulParams* p) {
+  if (m <= 0 || n <= 0 || k <= 0) return fail(LDB_ERR_SHAPE, "matmul_fp8: %d x %d x %d", m, n, k);
+  const int sms = sm_count();
+  const int kblocks = (k + kFp8Block - 1) / kFp8Block;
+  p->m = m, p->n = n, p->k = k;
+  p->tiles_m = (m + kTileM - 1) / kTileM;
+  // Cycles of a CTA that walks `waves` tiles: a K block costs the products
+  // (2 cycles a column), not less than its loads; each tile a fixed start.
+  long long best = -1;
+  for (const int bn : {32, 64, 96, 128, 160, 192, kMaxBn}) {
+    const long long tiles = static_cast<long long>(p->tiles_m) * ((n + bn - 1) / bn);
+    const long long waves = (tiles + sms - 1) / sms;
+    const long long cost = waves * (static_cast<long long>(kblocks) * std::max(2 * bn, 160) + 1000);
+    if (best < 0 || cost < best) {
+      best = cost;
+      p->bn = bn;
+    }
+  }
+  p->tiles_n = (n + p->bn - 1) / p->bn;
+  const long long tiles = static_cast<long long>(p->tiles_m) * p->tiles_n;
+  p->split = 1;
+  if (tiles * 2 <= sms && kblocks >= 8) {
+    // K ranges of at least four blocks (one scale group), cut at groups
+    const int groups = (kblocks + 3) / 4;
+    p->split = std::max(1, std::min({static_cast<int>(sms / tiles), groups, 16}));
+  }
+  const int groups = (kblocks + 3) / 4;
+  p->kb_per_split = 4 * ((groups + p->split - 1) / p->split);
+  p->split = (kblocks + p->kb_per_split - 1) / p->kb_per_split;
+  p->stages = std::min(kMaxStages, kSmemBudget / (kTileM * 128 + p->bn * 128));
+  p->box_m = std::min(kTileM, (m + 7) / 8 * 8);
+  if (tiles * p->split > 0x7FFFFFFF) return fail(LDB_ERR_SHAPE, "matmul_fp8: too many tiles");
+  return LDB_OK;
+}
+
+size_t partial_bytes(const MatmulParams& p) {
+  return p.split > 1 ? static_cast<size_t>(p.split) * p.m * p.n * sizeof(float) : 0;
+}
+
+template <typename T>
+int launch(cudaStream_t stream, const CUtensorMap& amap, const CUtensorMap& wmap, const MatmulParams& p,
+           unsigned int* status) {
+  static unsigned long long configured = 0;
+  const int smem = 1024 + p.stages * (kTileM + p.bn) * 128 + kScaleStages * kScaleBytes + 512;
+  int rc = ensure_smem_attribute(reinterpret_cast<const void*>(fp8_matmul_kernel<T>),
+                                 1024 + kSmemBudget + kScaleStages * kScaleBytes + 512, &configured,
+                                 "matmul_fp8 shared memory");
+  if (rc != LDB_OK) return rc;
+  const int items = p.tiles_m * p.tiles_n * p.split;
+  rc = launch_kernel(fp8_matmul_kernel<T>, dim3(std::min(items, sm_count())), dim3(kThreads), smem, stream,
+                     "matmul_fp8 launch", amap, wmap, p, status);
+  if (rc != LDB_OK || p.split == 1) return rc;
+  const long long total = static_cast<long long>(p.m) * p.n;
+  const int blocks = static_cast<int>(std::min<long long>((total + 255) / 256, 4ll * sm_count()));
+  return launch_kernel(fp8_matmul_reduce_kernel<T>, dim3(blocks), dim3(256), 0, stream, "matmul_fp8 reduce launch", p);
+}
+
+}  // namespace
+}  // namespace ldb
+
+extern "C" {
+
+int ldb_matmul_fp8_workspace_size(int m, int n, int k, size_t* bytes) {
+  using namespace ldb;
+  if (!bytes) return fail(LDB_ERR_INVALID, "matmul_fp8: bytes is null");
+  MatmulParams p{};
+  const int rc = plan(m, n, k, &p);
+  if (rc == LDB_OK) *bytes = partial_bytes(p);
+  return rc;
+}
+
+int ldb_matmul_fp8(cudaStream_t stream, const uint8_t* a, long long a_ld, const uint8_t* a_scales,
+                   long long a_scales_ld, const uint8_t* w, long long w_ld, const uint8_t* w_scales,
+                   long long w_scales_ld, const float* bias, const void* residual, long long residual_ld, void* out,
+                   long long out_ld, int m, int n, int k, int act, int out_dtype, void* workspace,
+                   size_t workspace_bytes) {
+  using namespace ldb;
+  if (!a || !a_scales || !w || !w_scales || !out) return fail(LDB_ERR_INVALID, "matmul_fp8: null pointer");
+  if (out_dtype != LDB_F16 && out_dtype != LDB_F32 && out_dtype != LDB_BF16)
+    return fail(LDB_ERR_INVALID, "matmul_fp8: unknown output type %d", out_dtype);
+  if (act != LDB_ACT_NONE && act != LDB_ACT_GELU) return fail(LDB_ERR_INVALID, "matmul_fp8: unknown activation %d", act);
+  MatmulParams p{};
+  int rc = plan(m, n, k, &p);
+  if (rc != LDB_OK) return rc;
+  const int kblocks = (k + kFp8Block - 1) / kFp8Block;
+  if (a_ld < k || w_ld < k || a_scales_ld < kblocks || w_scales_ld < kblocks || out_ld < n ||
+      (residual && residual_ld < n))
+    return fail(LDB_ERR_SHAPE, "matmul_fp8: a row stride is shorter than its row");
+  if (a_ld % 16 || w_ld % 16 || reinterpret_cast<uintptr_t>(a) % 16 || reinterpret_cast<uintptr_t>(w) % 16)
+    return fail(LDB_ERR_ALIGNMENT, "matmul_fp8: codes need 16-byte aligned rows");
+  if (a_scales_ld % 4 || reinterpret_cast<uintptr_t>(a_scales) % 4)
+    return fail(LDB_ERR_ALIGNMENT, "matmul_fp8: row scales need 4-byte aligned rows");
+  const size_t need = partial_bytes(p);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return fail(LDB_ERR_WORKSPACE, "matmul_fp8 needs %zu workspace bytes (16-byte aligned), got %zu", need,
+                workspace_bytes);
+  unsigned int* status = device_status_ptr();
+  if (!status) return fail(LDB_ERR_CUDA, "matmul_fp8: no device status word");
+  p.a_scales = a_scales, p.a_scales_ld = a_scales_ld;
+  p.w_scales = w_scales, p.w_scales_ld = w_scales_ld;
+  p.bias = bias, p.residual = residual, p.res_ld = residual_ld;
+  p.out = out, p.out_ld = out_ld, p.partial = static_cast<float*>(workspace);
+  p.act = act, p.out_dtype = out_dtype;
+  const int es = out_dtype == LDB_F32 ? 4 : 2;
+  p.vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_ld * es % 16 == 0 &&
+          (!residual || (reinterpret_cast<uintptr_t>(residual) % 16 == 0 && residual_ld * es % 16 == 0));
+  CUtensorMap amap, wmap;
+  const uint64_t adims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(m)};
+  const uint64_t wdims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n)};
+  const uint64_t astride[1] = {static_cast<uint64_t>(a_ld)}, wstride[1] = {static_cast<uint64_t>(w_ld)};
+  const uint32_t abox[2] = {128, static_cast<uint32_t>(p.box_m)}, wbox[2] = {128, static_cast<uint32_t>(p.bn)};
+  rc = encode_tiled_u8(&amap, a, 2, adims, astride, abox, 128);
+  if (rc == LDB_OK) rc = encode_tiled_u8(&wmap, w, 2, wdims, wstride, wbox, 128);
+  if (rc != LDB_OK) return rc;
+  if (out_dtype == LDB_F16) return launch<__half>(stream, amap, wmap, p, status);
+  if (out_dtype == LDB_BF16) return launch<__nv_bfloat16>(stream, amap, wmap, p, status);
+  return launch<float>(stream, amap, wmap, p, status);
+}
+
+}  // extern "C"

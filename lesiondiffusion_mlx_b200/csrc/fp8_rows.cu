@@ -1,0 +1,318 @@
+// Row quantization to the 8-bit format of fp8.cuh: the root-mean-square norm
+// with the residual's addition, plain rows, and the one-time packing of
+// weights.
+//
+//   h = x + r                                (FP32; stored rounded to x's type)
+//   y = h * rsqrt(mean(h^2) + eps) * gamma   (FP32, from the unrounded h)
+//   code = e4m3(y * 2^-e), e per row and 128 channels
+//
+// Bound: HBM.  x and r are read once (2 x 2 bytes a channel in 16 bits), h and
+// the codes written once (2 + 1 bytes): the row stays in registers between the
+// sum of squares and the rounding, 8 consecutive channels a lane, so that 16
+// lanes hold the 128 channels of a scale and find its maximum with four
+// shuffles.  Rows of up to 1024 channels take one warp (no barrier), wider rows
+// a block; the grid is resident and walks the rows, keeping gamma in registers.
+
+#include <algorithm>
+
+#include "fp8.cuh"
+#include "host_common.h"
+
+namespace ldb {
+namespace {
+
+struct RowsParams {
+  const void* x;
+  const void* residual;  // may be null
+  const float* gamma;    // may be null (ones)
+  void* h;               // may be null
+  uint8_t* codes;
+  uint8_t* scales;
+  long long x_ld, r_ld, h_ld, codes_ld, scales_ld;
+  int rows, channels;
+  float eps;
+  int vec;  // channels, strides and addresses allow 16-byte accesses
+};
+
+// Eight channels from `c` on (zero past the row's end).
+template <typename T>
+__device__ __forceinline__ void load_row8(const T* row, int c, int channels, bool vec, float (&v)[8]) {
+  if (vec) {
+    load8<T>(row + c, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < channels ? to_f32<T>(row[c + j]) : 0.f;
+  }
+}
+
+// Quantize the 128 channels that 16 neighbouring lanes hold, 8 each; every
+// lane of the warp takes part, lanes with `live` store.
+__device__ __forceinline__ void quantize_block(float (&y)[8], bool live, bool first, uint8_t* codes, uint8_t* scale) {
+  float amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(y[j]));  // a NaN leaves the maximum as it is
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  // Infinities (rare): out of the maximum, and NaN before the rounding.
+  if (__any_sync(0xffffffffu, !fp8_is_finite(amax))) {
+    amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (fp8_is_finite(y[j])) {
+        amax = fmaxf(amax, fabsf(y[j]));
+      } else {
+        y[j] = fp8_nan();
+      }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  }
+  const int e = fp8_exponent(amax);
+  const float inv = fp8_pow2(-e);
+  if (live) {
+    uint2 packed;
+    packed.x = fp8_pack4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+    packed.y = fp8_pack4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv);
+    *reinterpret_cast<uint2*>(codes) = packed;
+    if (first) *scale = static_cast<uint8_t>(e + 127);
+  }
+}
+
+// WARPS warps per row (1: eight rows per 256-thread block), ITERS x 8 channels a lane.
+template <typename T, int WARPS, int ITERS, bool NORM>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) fp8_rows_kernel(const RowsParams p) {
+  __shared__ float s_part[WARPS == 1 ? 1 : WARPS];
+  constexpr int kLanes = WARPS * 32;
+  const int t = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int per_block = WARPS == 1 ? 8 : 1;
+  const int first_row = blockIdx.x * per_block + (WARPS == 1 ? threadIdx.x >> 5 : 0);
+  const int step = gridDim.x * per_block;
+
+  // gamma is a weight, not the previous kernel's output: read before the wait
+  // (the widest rows have no registers to keep it in and read it for each row).
+  constexpr bool kKeepGamma = NORM && WARPS < 32;
+  auto gamma_at = [&](int i, int j) {
+    const int c = (i * kLanes + t) * 8 + j;
+    return p.gamma && c < p.channels ? p.gamma[c] : 1.f;
+  };
+  float g[ITERS][8];
+  if constexpr (kKeepGamma) {
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[i][j] = gamma_at(i, j);
+  }
+  pdl_begin();
+  for (int row = first_row; row < p.rows; row += step) {
+    const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
+    const T* r = static_cast<const T*>(p.residual) + (p.residual ? row * p.r_ld : 0);
+    float v[ITERS][8];
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      const int c = (i * kLanes + t) * 8;
+      if (c < p.channels) {
+        load_row8<T>(x, c, p.channels, p.vec, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      }
+    }
+    if (p.residual) {
+#pragma unroll
+      for (int i = 0; i < ITERS; ++i) {
+        const int c = (i * kLanes + t) * 8;
+        if (c < p.channels) {
+          float a[8];
+          load_row8<T>(r, c, p.channels, p.vec, a);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] += a[j];
+        }
+      }
+    }
+    if (p.h) {
+      T* h = static_cast<T*>(p.h) + row * p.h_ld;
+#pragma unroll
+      for (int i = 0; i < ITERS; ++i) {
+        const int c = (i * kLanes + t) * 8;
+        if (c < p.channels) {
+          if (p.vec) {
+            store8<T>(h + c, v[i]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (c + j < p.channels) h[c + j] = from_f32<T>(v[i][j]);
+          }
+        }
+      }
+    }
+    if constexpr (NORM) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < ITERS; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(v[i][j], v[i][j], sum);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if constexpr (WARPS > 1) {
+        if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) sum += s_part[w];
+        __syncthreads();  // before the next row's partial sums
+      }
+      const float rstd = rsqrtf(sum / static_cast<float>(p.channels) + p.eps);
+#pragma unroll
+      for (int i = 0; i < ITERS; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rstd * (kKeepGamma ? g[i][j] : gamma_at(i, j));
+    }
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      const int c = (i * kLanes + t) * 8;
+      quantize_block(v[i], c < p.channels, c % kFp8Block == 0, p.codes + row * p.codes_ld + c,
+                     p.scales + row * p.scales_ld + c / kFp8Block);
+    }
+  }
+}
+
+template <typename T, bool NORM>
+int launch_rows(cudaStream_t stream, const RowsParams& p, const char* what) {
+  const int sms = sm_count();
+  const int c = p.channels;
+  // Blocks resident at once: 64 registers a thread allow four 256-thread blocks
+  // per SM; rows beyond them are walked by the same blocks.
+  if (c <= 1024) {
+    const int blocks = std::min((p.rows + 7) / 8, sms * 4);
+    auto k = c <= 256 ? fp8_rows_kernel<T, 1, 1, NORM>
+                      : (c <= 512 ? fp8_rows_kernel<T, 1, 2, NORM> : fp8_rows_kernel<T, 1, 4, NORM>);
+    return launch_kernel(k, dim3(blocks), dim3(256), 0, stream, what, p);
+  }
+  if (c <= 8192) {
+    const int blocks = std::min(p.rows, sms * 4);
+    auto k = c <= 2048 ? fp8_rows_kernel<T, 8, 1, NORM>
+                       : (c <= 4096 ? fp8_rows_kernel<T, 8, 2, NORM> : fp8_rows_kernel<T, 8, 4, NORM>);
+    return launch_kernel(k, dim3(blocks), dim3(256), 0, stream, what, p);
+  }
+  return launch_kernel(fp8_rows_kernel<T, 32, 4, NORM>, dim3(std::min(p.rows, sms)), dim3(1024), 0, stream, what, p);
+}
+
+int esize(int dtype) { return dtype == LDB_F32 ? 4 : 2; }
+
+bool aligned16(const void* p, long long ld, int es) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0);
+}
+
+int run_rows(cudaStream_t stream, RowsParams p, int dtype, bool norm, const char* what) {
+  if (p.rows != 0 && (!p.x || !p.codes || !p.scales)) return fail(LDB_ERR_INVALID, "%s: null pointer", what);
+  if (dtype != LDB_F16 && dtype != LDB_F32 && dtype != LDB_BF16)
+    return fail(LDB_ERR_INVALID, "%s: unknown element type %d", what, dtype);
+  if (p.rows < 0 || p.channels <= 0 || p.channels > 32768)
+    return fail(LDB_ERR_SHAPE, "%s: %d rows of %d channels (1..32768)", what, p.rows, p.channels);
+  const int blocks = (p.channels + kFp8Block - 1) / kFp8Block;
+  if (p.x_ld < p.channels || (p.residual && p.r_ld < p.channels) || (p.h && p.h_ld < p.channels) ||
+      p.codes_ld < p.channels || p.scales_ld < blocks)
+    return fail(LDB_ERR_SHAPE, "%s: a row stride is shorter than its row", what);
+  if (p.codes_ld % 16 || reinterpret_cast<uintptr_t>(p.codes) % 16)
+    return fail(LDB_ERR_ALIGNMENT, "%s: codes need 16-byte aligned rows", what);
+  if (p.rows == 0) return LDB_OK;
+  const int es = esize(dtype);
+  p.vec = p.channels % 8 == 0 && aligned16(p.x, p.x_ld, es) && aligned16(p.residual, p.r_ld, es) &&
+          aligned16(p.h, p.h_ld, es);
+  if (dtype == LDB_F16)
+    return norm ? launch_rows<__half, true>(stream, p, what) : launch_rows<__half, false>(stream, p, what);
+  if (dtype == LDB_BF16)
+    return norm ? launch_rows<__nv_bfloat16, true>(stream, p, what)
+                : launch_rows<__nv_bfloat16, false>(stream, p, what);
+  return norm ? launch_rows<float, true>(stream, p, what) : launch_rows<float, false>(stream, p, what);
+}
+
+// One 128 x 128 block of a weight: eight warps, 16 rows each, four columns a
+// lane held in registers between the maximum and the rounding.  Runs once per
+// weight; not tuned.
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_pack_weight_kernel(const T* w, long long w_ld, int n, int k, uint8_t* codes,
+                                                              long long codes_ld, uint8_t* scales, int scales_ld) {
+  __shared__ float s_max[8];
+  pdl_begin();
+  const int warp = warp_id(), lane = lane_id();
+  const int col = blockIdx.x * kFp8Block + lane * 4;
+  float v[16][4];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = blockIdx.y * kFp8Block + i * 8 + warp;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a = row < n && col + j < k ? to_f32<T>(w[row * w_ld + col + j]) : 0.f;
+      if (!fp8_is_finite(a)) a = fp8_nan();
+      v[i][j] = a;
+      amax = fmaxf(amax, fabsf(a));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (lane == 0) s_max[warp] = amax;
+  __syncthreads();
+  amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, s_max[i]);
+  const int e = fp8_exponent(amax);
+  const float inv = fp8_pow2(-e);
+  if (threadIdx.x == 0) scales[static_cast<long long>(blockIdx.y) * scales_ld + blockIdx.x] = static_cast<uint8_t>(e + 127);
+  if (col >= k) return;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = blockIdx.y * kFp8Block + i * 8 + warp;
+    if (row < n)
+      *reinterpret_cast<uint32_t*>(codes + row * codes_ld + col) =
+          fp8_pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+  }
+}
+
+}  // namespace
+}  // namespace ldb
+
+extern "C" {
+
+int ldb_rms_norm_fp8(cudaStream_t stream, const void* x, long long x_ld, const void* residual, long long residual_ld,
+                     int dtype, const float* gamma, float eps, void* h, long long h_ld, uint8_t* codes,
+                     long long codes_ld, uint8_t* scales, long long scales_ld, int rows, int channels) {
+  ldb::RowsParams p{x, residual, gamma, h, codes, scales, x_ld, residual_ld, h_ld, codes_ld, scales_ld,
+                    rows, channels, eps, 0};
+  return ldb::run_rows(stream, p, dtype, true, "rms_norm_fp8");
+}
+
+int ldb_quantize_fp8_rows(cudaStream_t stream, const void* x, long long x_ld, int dtype, uint8_t* codes,
+                          long long codes_ld, uint8_t* scales, long long scales_ld, int rows, int channels) {
+  ldb::RowsParams p{x, nullptr, nullptr, nullptr, codes, scales, x_ld, 0, 0, codes_ld, scales_ld,
+                    rows, channels, 0.f, 0};
+  return ldb::run_rows(stream, p, dtype, false, "quantize_fp8_rows");
+}
+
+int ldb_pack_weight_fp8(cudaStream_t stream, const void* w, long long w_ld, int dtype, uint8_t* codes,
+                        long long codes_ld, uint8_t* scales, int scales_ld, int n, int k) {
+  using namespace ldb;
+  if (!w || !codes || !scales) return fail(LDB_ERR_INVALID, "pack_weight_fp8: null pointer");
+  if (dtype != LDB_F16 && dtype != LDB_F32 && dtype != LDB_BF16)
+    return fail(LDB_ERR_INVALID, "pack_weight_fp8: unknown element type %d", dtype);
+  if (n <= 0 || k <= 0) return fail(LDB_ERR_SHAPE, "pack_weight_fp8: %d x %d", n, k);
+  const int kb = (k + kFp8Block - 1) / kFp8Block, nb = (n + kFp8Block - 1) / kFp8Block;
+  if (w_ld < k || codes_ld < k || scales_ld < kb)
+    return fail(LDB_ERR_SHAPE, "pack_weight_fp8: a row stride is shorter than its row");
+  if (nb > 65535) return fail(LDB_ERR_SHAPE, "pack_weight_fp8: at most 8388480 rows");
+  if (codes_ld % 16 || reinterpret_cast<uintptr_t>(codes) % 16)
+    return fail(LDB_ERR_ALIGNMENT, "pack_weight_fp8: codes need 16-byte aligned rows");
+  const dim3 grid(kb, nb);
+  const char* what = "pack_weight_fp8 launch";
+  if (dtype == LDB_F16)
+    return launch_kernel(fp8_pack_weight_kernel<__half>, grid, dim3(256), 0, stream, what,
+                         static_cast<const __half*>(w), w_ld, n, k, codes, codes_ld, scales, scales_ld);
+  if (dtype == LDB_BF16)
+    return launch_kernel(fp8_pack_weight_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, what,
+                         static_cast<const __nv_bfloat16*>(w), w_ld, n, k, codes, codes_ld, scales, scales_ld);
+  return launch_kernel(fp8_pack_weight_kernel<float>, grid, dim3(256), 0, stream, what, static_cast<const float*>(w),
+                       w_ld, n, k, codes, codes_ld, scales, scales_ld);
+}
+
+}  // extern "C"

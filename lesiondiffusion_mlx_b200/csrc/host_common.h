@@ -91,4 +91,8 @@ int encode_tiled_f16(CUtensorMap* map, const void* base, int rank, const uint64_
 int encode_tiled_f32(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
                      const uint64_t* strides_bytes, const uint32_t* box, int swizzle_bytes);
 
+// Same for 8-bit elements (e4m3 codes).
+int encode_tiled_u8(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                    const uint64_t* strides_bytes, const uint32_t* box, int swizzle_bytes);
+
 }  // namespace ldb
