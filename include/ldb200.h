@@ -433,6 +433,41 @@ LDB_API int ldb_matmul_fp8(ldb_stream_t stream, const uint8_t* a, long long a_ld
                            void* out, long long out_ld, int m, int n, int k, int act, int out_dtype, void* workspace,
                            size_t workspace_bytes);
 
+/* Paged 8-bit key/value cache: codes [pages][kv_heads][page][head_dim] and
+ * scales [pages][kv_heads] for keys and for values, each page's scale within
+ * 2^-96 .. 2^96; pages of 16, 32, 64 or 128 tokens, head_dim 32, 64 or 128.
+ * table (device, [batch][table_ld], `width` entries used) names the pages of
+ * each item's tokens in order.  A page number outside [0, pages), a position
+ * outside the table or a negative count is left out and sets status bit 1.
+ *
+ * ldb_kv_append_fp8 writes `tokens` rows of k and v ([batch][tokens][kv_heads *
+ * head_dim], element strides _ld and _batch) of each item, or the first
+ * counts[b] of them, from position start[b] on.  Where a touched page holds
+ * older tokens its scale is the larger of its own and the new tokens' and the
+ * older codes are rounded to it; otherwise it is the new tokens' alone.  Pages
+ * written by one call belong to one item. */
+LDB_API int ldb_kv_append_fp8(ldb_stream_t stream, const void* k, long long k_ld, long long k_batch, const void* v,
+                              long long v_ld, long long v_batch, int dtype, uint8_t* k_codes, uint8_t* v_codes,
+                              uint8_t* k_scales, uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim,
+                              const int* table, long long table_ld, int width, const int* start, const int* counts,
+                              int batch, int tokens);
+
+/* softmax(q k^T scale) v over the first lengths[b] cached tokens of each item:
+ * q and out [batch][queries][heads * head_dim] (f16 or bf16, element strides _ld
+ * and _batch), query head h reading key/value head h / (heads / kv_heads).
+ * causal: query i sees the keys up to lengths[b] - queries + i.  A query
+ * without keys gives zeros.  FP32 scores, sums and outputs with one rounding;
+ * the weights of the value product are rounded to f16.  At most 2048 items; a
+ * cache of at most 2^31 - 1 token rows.  The workspace (16-byte aligned) holds partial rows. */
+LDB_API int ldb_kv_attention_fp8_workspace_size(int batch, int queries, int heads, int kv_heads, int head_dim,
+                                                size_t* bytes);
+LDB_API int ldb_kv_attention_fp8(ldb_stream_t stream, const void* q, long long q_ld, long long q_batch, int dtype,
+                                 const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scales,
+                                 const uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim,
+                                 const int* table, long long table_ld, int width, const int* lengths, void* out,
+                                 long long out_ld, long long out_batch, int batch, int queries, int heads, float scale,
+                                 int causal, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -104,6 +104,10 @@ SIGNATURES: dict[str, list] = {
     "ldb_rms_norm_fp8": [_P, _P, _L, _P, _L, _I, _P, _F, _P, _L, _P, _L, _P, _L, _I, _I],
     "ldb_quantize_fp8_rows": [_P, _P, _L, _I, _P, _L, _P, _L, _I, _I],
     "ldb_pack_weight_fp8": [_P, _P, _L, _I, _P, _L, _P, _I, _I, _I],
+    "ldb_kv_append_fp8": [_P, _P, _L, _L, _P, _L, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _I, _I],
+    "ldb_kv_attention_fp8_workspace_size": [_I, _I, _I, _I, _I, ctypes.POINTER(_SZ)],
+    "ldb_kv_attention_fp8": [_P, _P, _L, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I,
+                             _F, _I, _P, _SZ],
     "ldb_matmul_fp8_workspace_size": [_I, _I, _I, ctypes.POINTER(_SZ)],
     "ldb_matmul_fp8": [_P, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P, _SZ],
 }

@@ -1,0 +1,189 @@
+// Writing new tokens into the paged 8-bit key/value cache.
+//
+// One block per touched (page, kv head) of K or V.  With `held` older tokens in
+// the page and e(new) the scale that the new values need (fp8.cuh):
+//
+//   e = held > 0 ? max(e_old, e(new)) : e(new)
+//   new codes = e4m3(x 2^-e);  if e > e_old, old codes = e4m3(code 2^(e_old - e))
+//
+// so a page that is filled token by token keeps one scale, and what it holds is
+// rounded again only when that scale grows.  Writing the same tokens at the
+// same place again changes nothing.
+//
+// Bound: HBM (2 bytes read and 1 written a value); a page's new values stay in
+// registers between the maximum and the rounding.  For one token it is the
+// launch.
+
+#include "host_common.h"
+#include "kv_cache.cuh"
+
+namespace ldb {
+namespace {
+
+struct AppendParams {
+  const void* src[2];      // new keys, new values
+  uint8_t* codes[2];
+  uint8_t* scales[2];
+  const int* table;
+  const int* start;        // [batch] first position written
+  const int* counts;       // [batch] tokens written, null: all `tokens`
+  long long src_ld[2], src_batch[2], table_ld;
+  int pages, kv_heads, page, width, dim, dim_shift, tokens;
+  int vec;  // 16-byte reads of eight values
+};
+
+constexpr int kAppendThreads = 256;
+constexpr int kAppendVecs = 128 * 128 / 8 / kAppendThreads;  // of the largest page, per thread
+
+__device__ __forceinline__ float block_max(float v, float* s_part) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if (lane_id() == 0) s_part[warp_id()] = v;
+  __syncthreads();
+  v = s_part[0];
+#pragma unroll
+  for (int w = 1; w < kAppendThreads / 32; ++w) v = fmaxf(v, s_part[w]);
+  return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p, unsigned int* status) {
+  __shared__ float s_part[kAppendThreads / 32];
+  __shared__ int s_old;
+  pdl_begin();
+  const int b = blockIdx.y / p.kv_heads, head = blockIdx.y % p.kv_heads, which = blockIdx.z;
+  const int start = p.start[b];
+  int count = p.counts ? p.counts[b] : p.tokens;
+  if (start < 0 || count < 0 || count > p.tokens) {
+    if (threadIdx.x == 0) set_bad_shape(status);
+    return;
+  }
+  const long long slot = start / p.page + blockIdx.x;
+  const long long page0 = slot * p.page;
+  const int first = static_cast<int>(max(0ll, page0 - start));                              // of the new tokens
+  const int last = static_cast<int>(min(static_cast<long long>(count), page0 + p.page - start));
+  if (first >= last) return;
+  const int held = static_cast<int>(max(0ll, start - page0));
+  const int id = slot < p.width ? p.table[b * p.table_ld + slot] : -1;
+  if (id < 0 || id >= p.pages) {
+    if (threadIdx.x == 0) set_bad_shape(status);
+    return;
+  }
+  const long long unit = static_cast<long long>(id) * p.kv_heads + head;
+  uint8_t* codes = p.codes[which] + unit * p.page * p.dim;
+  uint8_t* scale = p.scales[which] + unit;
+  const T* src = static_cast<const T*>(p.src[which]) + b * p.src_batch[which] + head * p.dim;
+  const int vshift = p.dim_shift - 3;  // vectors of eight per token
+  const int vecs = (last - first) << vshift;
+
+  if (threadIdx.x == 0) s_old = *scale;
+  float v[kAppendVecs][8];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < kAppendVecs; ++i) {
+    const int q = i * kAppendThreads + threadIdx.x;
+    if (q < vecs) {
+      const T* x = src + (first + (q >> vshift)) * p.src_ld[which] + ((q & ((1 << vshift) - 1)) << 3);
+      if (p.vec) {
+        load8<T>(x, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = to_f32<T>(x[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (!fp8_is_finite(v[i][j])) v[i][j] = fp8_nan();
+        amax = fmaxf(amax, fabsf(v[i][j]));
+      }
+    }
+  }
+  amax = block_max(amax, s_part);
+  const int e_old = s_old - 127;
+  int e = max(-kKvMaxExponent, min(kKvMaxExponent, fp8_exponent(amax)));
+  if (held > 0) e = amax == 0.f ? e_old : max(e, e_old);  // zeros ask for no scale
+  const float inv = fp8_pow2(-min(e, 127));
+#pragma unroll
+  for (int i = 0; i < kAppendVecs; ++i) {
+    const int q = i * kAppendThreads + threadIdx.x;
+    if (q < vecs) {
+      uint2 packed;
+      packed.x = fp8_pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+      packed.y = fp8_pack4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+      *reinterpret_cast<uint2*>(codes + ((static_cast<long long>(held) << p.dim_shift) + (q << 3))) = packed;
+    }
+  }
+  if (held > 0 && e > e_old) {
+    const float shrink = exp2f(static_cast<float>(max(e_old - e, -64)));  // below 2^-18 every code becomes 0
+    for (int q = threadIdx.x; q < held << vshift; q += kAppendThreads) {
+      uint2* at = reinterpret_cast<uint2*>(codes + (q << 3));
+      uint2 old = *at;
+      uint32_t* w = &old.x;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t word = h == 0 ? old.x : old.y;
+        const uint32_t lo = fp8_unpack2(word & 0xFFFFu), hi = fp8_unpack2(word >> 16);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+        const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        w[h] = fp8_pack4(a.x * shrink, a.y * shrink, c.x * shrink, c.y * shrink);
+      }
+      *at = old;
+    }
+  }
+  if (threadIdx.x == 0) *scale = static_cast<uint8_t>(e + 127);
+}
+
+}  // namespace
+}  // namespace ldb
+
+extern "C" {
+
+int ldb_kv_append_fp8(cudaStream_t stream, const void* k, long long k_ld, long long k_batch, const void* v,
+                      long long v_ld, long long v_batch, int dtype, uint8_t* k_codes, uint8_t* v_codes,
+                      uint8_t* k_scales, uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim,
+                      const int* table, long long table_ld, int width, const int* start, const int* counts, int batch,
+                      int tokens) {
+  using namespace ldb;
+  if (batch < 0 || tokens < 0) return fail(LDB_ERR_SHAPE, "kv_append: %d items of %d tokens", batch, tokens);
+  if (dtype != LDB_F16 && dtype != LDB_F32 && dtype != LDB_BF16)
+    return fail(LDB_ERR_INVALID, "kv_append: unknown element type %d", dtype);
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return fail(LDB_ERR_SHAPE, "kv_append: head_dim %d (32, 64 or 128)", head_dim);
+  if (page != 16 && page != 32 && page != 64 && page != 128)
+    return fail(LDB_ERR_SHAPE, "kv_append: pages of %d tokens (16, 32, 64 or 128)", page);
+  if (pages <= 0 || kv_heads <= 0 || width <= 0 || table_ld < width)
+    return fail(LDB_ERR_SHAPE, "kv_append: %d pages, %d heads, table of %d", pages, kv_heads, width);
+  if (batch == 0 || tokens == 0) return LDB_OK;
+  if (!k || !v || !k_codes || !v_codes || !k_scales || !v_scales || !table || !start)
+    return fail(LDB_ERR_INVALID, "kv_append: null pointer");
+  const long long row = static_cast<long long>(kv_heads) * head_dim;
+  if ((tokens > 1 && (k_ld < row || v_ld < row)) || static_cast<long long>(batch) * kv_heads > 65535)
+    return fail(LDB_ERR_SHAPE, "kv_append: row strides below %lld, or more than 65535 (item, head) pairs", row);
+  if (reinterpret_cast<uintptr_t>(k_codes) % 16 || reinterpret_cast<uintptr_t>(v_codes) % 16)
+    return fail(LDB_ERR_ALIGNMENT, "kv_append: codes must be 16-byte aligned");
+  unsigned int* status = device_status_ptr();
+  if (!status) return fail(LDB_ERR_CUDA, "kv_append: no device status word");
+  AppendParams p{};
+  p.src[0] = k, p.src[1] = v, p.codes[0] = k_codes, p.codes[1] = v_codes;
+  p.scales[0] = k_scales, p.scales[1] = v_scales;
+  p.src_ld[0] = k_ld, p.src_ld[1] = v_ld, p.src_batch[0] = k_batch, p.src_batch[1] = v_batch;
+  p.table = table, p.table_ld = table_ld, p.start = start, p.counts = counts;
+  p.pages = pages, p.kv_heads = kv_heads, p.page = page, p.width = width, p.dim = head_dim;
+  p.dim_shift = head_dim == 32 ? 5 : (head_dim == 64 ? 6 : 7);
+  p.tokens = tokens;
+  const int es = dtype == LDB_F32 ? 4 : 2;
+  p.vec = 1;
+  for (int i = 0; i < 2; ++i)
+    if (reinterpret_cast<uintptr_t>(p.src[i]) % 16 || p.src_ld[i] * es % 16 || p.src_batch[i] * es % 16) p.vec = 0;
+  // pages that a run of `tokens` can touch, wherever it starts
+  const long long touched = (static_cast<long long>(tokens) + page - 2) / page + 1;
+  const dim3 grid(static_cast<unsigned>(touched), batch * kv_heads, 2);
+  const char* what = "kv_append launch";
+  if (dtype == LDB_F16)
+    return launch_kernel(kv_append_kernel<__half>, grid, dim3(kAppendThreads), 0, stream, what, p, status);
+  if (dtype == LDB_BF16)
+    return launch_kernel(kv_append_kernel<__nv_bfloat16>, grid, dim3(kAppendThreads), 0, stream, what, p, status);
+  return launch_kernel(kv_append_kernel<float>, grid, dim3(kAppendThreads), 0, stream, what, p, status);
+}
+
+}  // extern "C"

@@ -1,0 +1,151 @@
+"""Paged 8-bit key/value cache: keys and values that are written once and read many times.
+
+The cache holds e4m3 codes in pages of tokens, ``(pages, kv_heads, page,
+head_dim)`` for keys and for values, with one power-of-two scale (E8M0) per
+page and head.  An item's tokens lie, in order, in the pages of its row of an
+int32 page table, so items can share pages (several seeds of one text context)
+and grow without moving.
+
+    cache = KvCacheFp8.empty(pages, kv_heads, head_dim, page=64, device="cuda")
+    kv_append(cache, k, v, table, start)          # tokens start .. start + L of every item
+    out = kv_attention(q, cache, table, lengths, scale=head_dim ** -0.5)
+
+Lengths and positions are device tensors; a page number or a length outside
+the cache is left out and sets the device status (``ldb_device_status``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib, instrument
+from .fp8 import CODES, SCALES
+from .ops import _DT, _ptr, _stream
+
+HEAD_DIMS = (32, 64, 128)
+PAGES = (16, 32, 64, 128)
+
+
+@dataclass(frozen=True)
+class KvCacheFp8:
+    """Codes ``k``, ``v`` ``(pages, kv_heads, page, head_dim)`` and scales ``(pages, kv_heads)``."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, head_dim: int, *, page: int = 64,
+              device: torch.device | str = "cuda") -> "KvCacheFp8":
+        """An unwritten cache of ``pages`` pages of ``page`` tokens (16, 32, 64 or 128)."""
+        if page not in PAGES or head_dim not in HEAD_DIMS:
+            raise ValueError(f"pages hold {PAGES} tokens of {HEAD_DIMS} channels, got {page} of {head_dim}")
+        codes = [torch.empty((pages, kv_heads, page, head_dim), dtype=CODES, device=device) for _ in range(2)]
+        scales = [torch.empty((pages, kv_heads), dtype=SCALES, device=device) for _ in range(2)]
+        return cls(*codes, *scales)
+
+
+def _check_cache(cache: KvCacheFp8, name: str) -> tuple[int, int, int, int]:
+    shape = cache.k.shape
+    if len(shape) != 4 or cache.v.shape != shape or cache.k.dtype != CODES or cache.v.dtype != CODES:
+        raise ValueError(f"{name}: k and v must be float8_e4m3fn (pages, kv_heads, page, head_dim)")
+    pages, heads, page, dim = shape
+    if page not in PAGES or dim not in HEAD_DIMS:
+        raise ValueError(f"{name}: pages hold {PAGES} tokens of {HEAD_DIMS} channels, got {page} of {dim}")
+    if (cache.k_scale.shape != (pages, heads) or cache.v_scale.shape != (pages, heads)
+            or cache.k_scale.dtype != SCALES or cache.v_scale.dtype != SCALES):
+        raise ValueError(f"{name}: scales must be float8_e8m0fnu ({pages}, {heads})")
+    device = cache.k.device
+    if device.type != "cuda":
+        raise ValueError(f"{name}: the cache must be on a CUDA device")
+    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        if not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{name}: the cache's tensors must be contiguous and on one device")
+    return pages, heads, page, dim
+
+
+def _check_index(t: torch.Tensor, ndim: int, batch: int, device: torch.device, name: str) -> None:
+    if t.dtype != torch.int32 or t.ndim != ndim or t.shape[0] != batch or t.device != device:
+        raise ValueError(f"{name} must be an int32 {ndim}-axis tensor of {batch} items on the cache's device")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must have unit stride along its last axis")
+
+
+def _table_ld(table: torch.Tensor) -> int:
+    if table.shape[1] == 0:
+        raise ValueError("the page table has no columns")
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+
+
+def kv_append(cache: KvCacheFp8, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, *,
+              counts: torch.Tensor | None = None) -> None:
+    """Write ``(B, L, kv_heads * head_dim)`` keys and values at positions ``start[b] ..`` of each item.
+
+    Only the first ``counts[b]`` of item ``b``'s tokens where given.  What a
+    page holds before ``start`` stays, rounded again if the page's scale has to
+    grow for the new tokens; anything at or after ``start`` in the touched
+    pages counts as unwritten.  Items written together must not share the
+    pages they write.  float16, bfloat16 or float32, any row and item stride."""
+    pages, heads, page, dim = _check_cache(cache, "kv_append")
+    if k.dtype not in _DT or v.dtype != k.dtype:
+        raise ValueError("kv_append: k and v must share dtype float16, bfloat16 or float32")
+    if k.ndim != 3 or v.shape != k.shape or k.shape[2] != heads * dim:
+        raise ValueError(f"kv_append: k and v must be (B, L, {heads * dim}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    device = cache.k.device
+    if k.device != device or v.device != device:
+        raise ValueError("kv_append: k and v must be on the cache's device")
+    if k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("kv_append: channel axis must have unit stride")
+    batch, tokens, _ = k.shape
+    _check_index(table, 2, batch, device, "kv_append: table")
+    _check_index(start, 1, batch, device, "kv_append: start")
+    if counts is not None:
+        _check_index(counts, 1, batch, device, "kv_append: counts")
+    with instrument.maybe_time("kv_append", 0.0):
+        _lib.call("ldb_kv_append_fp8", _stream(k), k.data_ptr(), k.stride(1), k.stride(0), v.data_ptr(), v.stride(1),
+                  v.stride(0), _DT[k.dtype], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+                  cache.v_scale.data_ptr(), pages, heads, page, dim, table.data_ptr(), _table_ld(table),
+                  table.shape[1], start.data_ptr(), _ptr(counts), batch, tokens)
+
+
+def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, lengths: torch.Tensor, *, scale: float,
+                 causal: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``softmax(q k^T * scale) v`` of ``(B, L, heads * head_dim)`` queries over each item's cached tokens.
+
+    ``heads`` is a multiple of the cache's; query head ``h`` reads key/value
+    head ``h // (heads / kv_heads)``.  Item ``b`` has ``lengths[b]`` tokens (0
+    included).  With ``causal`` the queries are the item's last ``L`` tokens:
+    query ``i`` sees the keys up to ``lengths[b] - L + i``.  A query that sees
+    no key gives zeros; a NaN among the keys or values a query does not see
+    does not reach it.  float16 or bfloat16, any row and item stride."""
+    pages, kv_heads, page, dim = _check_cache(cache, "kv_attention")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"kv_attention: queries must be float16 or bfloat16, got {q.dtype}")
+    device = cache.k.device
+    if q.ndim != 3 or q.device != device or q.shape[2] % (kv_heads * dim) or q.shape[2] == 0:
+        raise ValueError(f"kv_attention: queries must be (B, L, n * {kv_heads * dim}) on the cache's device, got "
+                         f"{tuple(q.shape)}")
+    if q.stride(2) != 1:
+        raise ValueError("kv_attention: channel axis must have unit stride")
+    batch, queries, width = q.shape
+    _check_index(table, 2, batch, device, "kv_attention: table")
+    _check_index(lengths, 1, batch, device, "kv_attention: lengths")
+    if out is None:
+        out = torch.empty((batch, queries, width), dtype=q.dtype, device=device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.stride(2) != 1:
+        raise ValueError("kv_attention: out must have q's shape, dtype and device, and unit channel stride")
+    heads = width // dim
+    need = ctypes.c_size_t(0)
+    _lib.call("ldb_kv_attention_fp8_workspace_size", batch, queries, heads, kv_heads, dim, ctypes.byref(need))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+    with instrument.maybe_time("kv_attention", 0.0):
+        _lib.call("ldb_kv_attention_fp8", _stream(q), q.data_ptr(), q.stride(1), q.stride(0), _DT[q.dtype],
+                  cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pages,
+                  kv_heads, page, dim, table.data_ptr(), _table_ld(table), table.shape[1], lengths.data_ptr(),
+                  out.data_ptr(), out.stride(1), out.stride(0), batch, queries, heads, float(scale), int(causal),
+                  ws.data_ptr(), need.value)
+    return out
