@@ -6,20 +6,26 @@
 // with one running reference per row, M = max_j (s[r, j] + ev_j), so that every
 // weight 2^(s + ev - M) of the value product lies in [0, 1] whatever the
 // pages' scales are, and is rounded to f16 once; the sum takes the same weight
-// times 2^-ev in FP32.  Codes are exact in f16; bf16 queries become f16 after
-// a power-of-two scaling of their row.
+// times 2^-ev in FP32.
+//
+// q k runs on the codes as they are (m16n8k32 e4m3): a query row is scaled by a
+// power of two and written as e4m3 parts, q = q0 + q1 / 16 + q2 / 256, two for
+// bf16 (8 significant bits), three for f16 (11), exactly but for channels
+// 2^-14 below the row's largest.  The first two parts of eight rows fill the 16 rows
+// of one product.  p v takes the values as f16 (exact) in the other
+// orientation, channels x rows, so that eight rows fill the eight columns of
+// a product and the scores' registers are its weight fragment as they are.
 //
 // Bound: HBM, the cached tokens (2 D bytes each) read once for a group's
-// heads.  The 16 rows of an m16n8k16 product are (query, head of the group)
-// pairs of one key/value head.  The cached tokens of all items and heads form one line of
-// 64-token tiles, cut into equal ranges, one per CTA (two CTAs per SM), so that
-// ragged lengths and preallocated tables leave no SM idle; a pair whose tiles
-// lie in several CTAs is merged by a second kernel, in order.  One warp fetches tiles (TMA,
-// swizzled) into a ring; four warps take them in turn, each with its own M, sum
-// and output, merged at the end of a pair.  A lane's 16-byte reads of a
+// heads.  The cached tokens of all items and heads form one line of 32-token
+// tiles, cut into equal ranges, one per warp, so that ragged lengths and
+// preallocated tables leave no SM idle.  A warp works by itself: it copies the
+// next tiles into its own ring (cp.async, swizzled) while it works on one, and
+// keeps M, sum and output in registers until a pair of item and head ends, so
+// that nothing waits for another warp.  A pair whose tiles lie in several
+// ranges is merged by a second kernel, in order.  A lane's 16-byte reads of a
 // swizzled row are free of bank conflicts, and the orders of channels (in q k)
-// and of output columns (in p v) are chosen so that these bytes are its
-// fragments.
+// and of output rows (in p v) are chosen so that these bytes are its fragments.
 
 #include <algorithm>
 
@@ -29,12 +35,14 @@
 namespace ldb {
 namespace {
 
-constexpr int kTile = 64;        // tokens per tile
-constexpr int kRows = 16;        // query rows of a product
-constexpr int kConsumers = 4;    // warps that take tiles in turn
-constexpr int kAttnThreads = (kConsumers + 1) * 32;
+constexpr int kTile = 32;        // tokens per tile
+constexpr int kGroupRows = 8;    // query rows of one product
+constexpr int kWarps = 4;        // per CTA; they share nothing but the tiles' line
 constexpr int kMaxBatch = 2048;
-constexpr int kCtasPerSm = 2;
+// Positions on the line that the start of a pair counts for: its page numbers,
+// scales and queries take a warp about as long as this many tiles.  (Without them a
+// batch of short items next to long ones ran 1.7 times as long.)
+constexpr int kStart = 3;
 constexpr float kFloor = -1.0e30f;  // reference of a row that has seen nothing
 
 struct AttnParams {
@@ -42,73 +50,71 @@ struct AttnParams {
   const void* q;
   void* out;
   long long q_ld, q_batch, out_ld, out_batch;
-  int queries, group, rows, row_tiles;  // rows = queries * group per key/value head
-  int causal, q_vec;
+  int queries, group, rows;  // rows = queries * group per key/value head
+  int tile_rows, row_tiles;
+  int causal, q_vec, out_vec;
   float scale_log2;
-  int ctas;
-  float* o_part;   // [cta][2][16][D]
-  float* ml_part;  // [cta][2][16][2]
+  int warps;       // of the grid
+  float* o_part;   // [warp][2][tile rows][D]
+  float* ml_part;  // [warp][2][tile rows][2]
+  // Pairs split over warps: (item, pair, first warp, warps, or 0 for a pair that
+  // is whole), by pair where there are fewer pairs than warps, else by first warp.
+  int4* open_part;
+  int open_by_pair;
+  unsigned int* status;
 };
 
-template <int D>
+// G groups of eight query rows per row tile.
+template <int D, int G>
 struct Cfg {
+  static constexpr int kRows = G * kGroupRows;
   static constexpr int kTileBytes = kTile * D;
-  static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = D == 128 ? 4 : (D == 64 ? 6 : 8);
-  static constexpr int kOffMeta = kStages * kStageBytes;            // [stage][4] (key factor, value exponent)
-  static constexpr int kOffO = kOffMeta + kStages * 4 * 8;          // [4][16][D] floats
-  static constexpr int kOffMl = kOffO + kConsumers * kRows * D * 4; // [4][16][2] floats
-  static constexpr int kOffBar = kOffMl + kConsumers * kRows * 8;
-  static constexpr int kOffBase = kOffBar + 2 * kStages * 8 + 16;   // [batch + 1] long long
+  static constexpr int kSlotBytes = 2 * kTileBytes;
+  // Tiles in flight: 16 KB a warp over eight to sixteen warps per SM, about
+  // three times what HBM's latency times its rate asks for.
+  static constexpr int kSlots = D == 128 ? 3 : (D == 64 ? 4 : 6);
+  static constexpr int kCtasPerSm = D == 128 ? 2 : 3;
+  static constexpr int kOffMeta = kWarps * kSlots * kSlotBytes;  // [warp][slot][2] (key factor, value exponent)
+  static constexpr int kOffBase = kOffMeta + kWarps * kSlots * 16;  // [batch + 1] int
 };
+int ctas_per_sm(int head_dim) { return head_dim == 128 ? Cfg<128, 1>::kCtasPerSm : Cfg<64, 1>::kCtasPerSm; }
 
 // ------------------------------------------------------------ division of the work
 
 __device__ __forceinline__ int tiles_of(int tokens) { return (tokens + kTile - 1) / kTile; }
+// Positions of one pair of an item: kStart, then one per tile (none without tokens).
+__device__ __forceinline__ int places_of(int tokens) { return tokens == 0 ? 0 : kStart + tiles_of(tokens); }
 
-// CTAs that share `total` tiles: at least one tile per consumer warp.
-__device__ __forceinline__ long long active_ctas(long long total, int ctas) {
-  return max(1ll, min(static_cast<long long>(ctas), (total + kConsumers - 1) / kConsumers));
-}
-__device__ __forceinline__ long long range_begin(long long cta, long long total, long long active) {
-  return cta * total / active;
-}
-
-struct Segment {
-  int b, pair, tile0, tiles, item_tiles;
-  bool whole;
-};
-
-// The segment that starts at tile u of the line (base: each item's first tile).
-__device__ __forceinline__ Segment segment_at(const long long* base, int batch, int pairs, long long u, long long end) {
-  int lo = 0, hi = batch;  // the last item whose first tile is at or before u
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (base[mid] <= u) {
-      lo = mid;
-    } else {
-      hi = mid;
-    }
+// `total` positions in ranges of equal length, the first ones one longer.
+struct Ranges {
+  int per, extra;
+  __device__ __forceinline__ Ranges(int total, int warps) : per(total / warps), extra(total % warps) {}
+  __device__ __forceinline__ int begin(int w) const { return w * per + min(w, extra); }
+  __device__ __forceinline__ int of(int u) const {
+    const int head = extra * (per + 1);
+    return u < head ? u / (per + 1) : extra + (u - head) / per;
   }
-  Segment g;
-  g.b = lo;
-  const long long rel = u - base[lo];
-  g.item_tiles = static_cast<int>((base[lo + 1] - base[lo]) / pairs);
-  g.pair = static_cast<int>(rel / g.item_tiles);
-  g.tile0 = static_cast<int>(rel - static_cast<long long>(g.pair) * g.item_tiles);
-  g.tiles = static_cast<int>(min(static_cast<long long>(g.item_tiles - g.tile0), end - u));
-  g.whole = g.tiles == g.item_tiles;
-  return g;
-}
+};
 
 // ------------------------------------------------------------------ fragments
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// D (16 x 8) += A (16 x 32) B (32 x 8), e4m3.
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// D (16 x 8) += A (16 x 16) B (16 x 8), f16.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -132,443 +138,581 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[W / 4]
   }
 }
 
-template <int D, typename T>
-__global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
-    kv_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                        const AttnParams p, unsigned int* status) {
-  using C = Cfg<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float2* s_meta = reinterpret_cast<float2*>(smem + C::kOffMeta);
-  float* s_o = reinterpret_cast<float*>(smem + C::kOffO);
-  float* s_ml = reinterpret_cast<float*>(smem + C::kOffMl);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  uint64_t* empty = full + C::kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + C::kStages);
-  long long* s_base = reinterpret_cast<long long*>(smem + C::kOffBase);
-  const int warp = warp_id(), lane = lane_id();
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    *abort_flag = 0;
-    fence_mbarrier_init();
-    tma_prefetch_desc(&kmap);
-    tma_prefetch_desc(&vmap);
+// Four values as e4m3, and what is left of them times 16 (exact): the next part's input.
+__device__ __forceinline__ uint32_t split_part(__half2 (&x)[2]) {
+  uint32_t codes = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint16_t part;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(part) : "r"(*reinterpret_cast<const uint32_t*>(&x[h])));
+    const uint32_t back = fp8_unpack2(part);
+    x[h] = __hmul2(__hsub2(x[h], *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(16.f));
+    codes |= static_cast<uint32_t>(part) << (16 * h);
   }
-  pdl_begin();
-  const int pairs = p.c.kv_heads * p.row_tiles;
-  if (warp == 0) {
-    // First tile of each item on the line.
-    long long sum = 0;
-    for (int b0 = 0; b0 < p.c.batch; b0 += 32) {
-      const int b = b0 + lane;
-      long long n = b < p.c.batch ? static_cast<long long>(tiles_of(kv_length(p.c, b, status))) * pairs : 0;
-      long long upto = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += other;
-      }
-      if (b < p.c.batch) s_base[b] = sum + upto - n;
-      sum += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    if (lane == 0) s_base[p.c.batch] = sum;
-  }
-  __syncthreads();
-  const long long total = s_base[p.c.batch];
-  const long long active = active_ctas(total, p.ctas);
-  if (static_cast<long long>(blockIdx.x) >= active) return;
-  const long long begin = range_begin(blockIdx.x, total, active);
-  const long long end = range_begin(blockIdx.x + 1, total, active);
-  const int page = p.c.page;
-  const int box = min(page, kTile);  // tokens per load
-
-  if (warp == kConsumers) {
-    // -------------------------------------------------------------- fetch
-    int seq = 0;
-    bool ok = true;
-    for (long long u = begin; ok && u < end;) {
-      const Segment g = segment_at(s_base, p.c.batch, pairs, u, end);
-      const int head = g.pair / p.row_tiles;
-      const int used = (kv_length(p.c, g.b, status) + page - 1) / page;  // pages that hold tokens
-      int batch0 = -32;  // first of the 32 pages whose numbers and scales the lanes hold
-      int id = -1;
-      float kf = 0.f, ev = 0.f;
-      for (int j = g.tile0; j < g.tile0 + g.tiles; ++j, ++seq) {
-        const int first = j * kTile / page;
-        if (first >= batch0 + 32 || batch0 < 0) {
-          batch0 = first;
-          const int at = batch0 + lane;
-          id = at < used ? p.c.table[g.b * p.c.table_ld + at] : -1;
-          if (at < used && (id < 0 || id >= p.c.pages)) {
-            set_bad_shape(status);
-            id = -1;
-          }
-          kf = 0.f;
-          ev = 0.f;
-          if (id >= 0) {
-            const long long unit = static_cast<long long>(id) * p.c.kv_heads + head;
-            kf = fp8_pow2(p.c.k_scale[unit] - 127) * p.scale_log2;
-            ev = static_cast<float>(p.c.v_scale[unit] - 127);
-          }
-        }
-        const int st = seq % C::kStages;
-        const int loads = kTile / box;  // pages of this tile (1 where a page holds two tiles)
-        const int mine = first + lane - batch0;
-        const int my_id = __shfl_sync(0xffffffffu, id, mine & 31);
-        const float my_kf = __shfl_sync(0xffffffffu, kf, mine & 31);
-        const float my_ev = __shfl_sync(0xffffffffu, ev, mine & 31);
-        ok = warp_wait(&empty[st], (static_cast<uint32_t>(seq / C::kStages) & 1u) ^ 1u, abort_flag, status);
-        if (!ok) break;
-        const bool load = lane < loads && my_id >= 0;
-        if (lane < loads) s_meta[st * 4 + lane] = make_float2(my_kf, my_ev);
-        const int count = __popc(__ballot_sync(0xffffffffu, load));
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(count) * 2 * box * D);
-        __syncwarp();
-        if (load) {
-          // rows of the (pages x heads x tokens, D) code matrix
-          const int row = (my_id * p.c.kv_heads + head) * page + (j * kTile) % page;
-          uint8_t* dst = smem + st * C::kStageBytes + lane * box * D;
-          tma_load_2d(dst, &kmap, &full[st], 0, row);
-          tma_load_2d(dst + C::kTileBytes, &vmap, &full[st], 0, row);
-        }
-      }
-      u += g.tiles;
-    }
-    if (*abort_flag) {
-      volatile int never = 0;
-      for (int back = 1; back <= min(seq, C::kStages); ++back)
-        mbar_wait(&full[(seq - back) % C::kStages], static_cast<uint32_t>((seq - back) / C::kStages) & 1u, &never, status);
-    }
-  } else {
-    // ------------------------------------------------------------ attend
-    // Lane (g, c): rows g and g + 8, key g of a group of eight, channels
-    // [c D/4, (c + 1) D/4) in q k; tokens 2c, 2c + 1, 2c + 8, 2c + 9 and
-    // channels [g D/8, (g + 1) D/8) in p v.
-    const int g = lane >> 2, c = lane & 3;
-    constexpr int kSteps = D / 16;  // products over the channels
-    constexpr int kCols = D / 8;    // groups of eight output columns
-    int seq = 0;
-    bool ok = true;
-    for (long long u = begin; u < end;) {
-      const Segment sg = segment_at(s_base, p.c.batch, pairs, u, end);
-      const int head = sg.pair / p.row_tiles, row0 = (sg.pair % p.row_tiles) * kRows;
-      const int len = kv_length(p.c, sg.b, status);
-      // Queries as f16 fragments, their rows' power-of-two factors, and the keys a row sees.
-      uint32_t qf[kSteps][4];
-      float qs[2];
-      int limit[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = row0 + g + 8 * h;
-        const bool live = r < p.rows;
-        const int i = live ? r / p.group : 0;
-        limit[h] = !live ? len : (p.causal ? min(len, len - p.queries + i + 1) : len);
-        float x[D / 4];
-        if (live) {
-          const T* src = static_cast<const T*>(p.q) + sg.b * p.q_batch + i * p.q_ld +
-                         (static_cast<long long>(head) * p.group + r % p.group) * D + c * (D / 4);
-          if (p.q_vec) {
-#pragma unroll
-            for (int k = 0; k < D / 32; ++k) {
-              float t[8];
-              load8<T>(src + 8 * k, t);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[8 * k + e] = t[e];
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < D / 4; ++k) x[k] = to_f32<T>(src[k]);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < D / 4; ++k) x[k] = 0.f;
-        }
-        qs[h] = 1.f;
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          // bf16 reaches past f16's range: bring the row's maximum to [1, 2)
-          float m = 0.f;
-#pragma unroll
-          for (int k = 0; k < D / 4; ++k) m = fmaxf(m, fabsf(x[k]));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-          const int e = min(126, max(-126, static_cast<int>(__float_as_uint(m) >> 23) - 127));
-          qs[h] = fp8_pow2(e);
-          const float inv = fp8_pow2(-e);
-#pragma unroll
-          for (int k = 0; k < D / 4; ++k) x[k] *= inv;
-        }
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          qf[s][h] = pack_half2(x[4 * s], x[4 * s + 1]);
-          qf[s][2 + h] = pack_half2(x[4 * s + 2], x[4 * s + 3]);
-        }
-      }
-      const int open = p.causal ? min(len, len - p.queries + row0 / p.group + 1) : len;  // keys that every row sees
-
-      float o[kCols][4];
-#pragma unroll
-      for (int j = 0; j < kCols; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-      float top[2] = {kFloor, kFloor}, sum[2] = {0.f, 0.f};
-
-      for (int t = 0; t < sg.tiles; ++t, ++seq) {
-        if ((seq & (kConsumers - 1)) != warp) continue;
-        const int st = seq % C::kStages;
-        if (ok) ok = warp_wait(&full[st], static_cast<uint32_t>(seq / C::kStages) & 1u, abort_flag, status);
-        if (!ok) continue;
-        const uint8_t* sk = smem + st * C::kStageBytes;
-        const uint8_t* sv = sk + C::kTileBytes;
-        const int j0 = (sg.tile0 + t) * kTile;
-        const bool masked = j0 + kTile > open;
-
-        // Scores of 8 keys at a time.
-        float s[8][4];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-          constexpr int W = D / 4 >= 16 ? 16 : D / 4;
-          uint32_t w[D / 16];
-#pragma unroll
-          for (int h = 0; h < (D / 4) / W; ++h) {
-            uint32_t part[W / 4];
-            lds_words<W>(sk + swizzle_offset((8 * n + g) * D + c * (D / 4) + h * W, D), part);
-#pragma unroll
-            for (int e = 0; e < W / 4; ++e) w[h * (W / 4) + e] = part[e];
-          }
-#pragma unroll
-          for (int k = 0; k < kSteps; ++k) mma16816(s[n], qf[k], fp8_unpack2(w[k] & 0xFFFFu), fp8_unpack2(w[k] >> 16));
-        }
-        uint32_t bad_lo = 0, bad_hi = 0;  // tokens some rows must not see whose values hold a NaN
-        if (masked && p.queries > 1) {
-          uint32_t any[2] = {0, 0};
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            for (int e = 0; e < D / 4; ++e)
-              any[h] |= nan_codes(reinterpret_cast<const uint32_t*>(sv + (lane + 32 * h) * D)[e]);
-          bad_lo = __ballot_sync(0xffffffffu, any[0] != 0);
-          bad_hi = __ballot_sync(0xffffffffu, any[1] != 0);
-        }
-        float mx[2] = {kFloor, kFloor};
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float2 meta = s_meta[st * 4 + 8 * n / box];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int h = e >> 1;
-            s[n][e] = fmaf(s[n][e], qs[h] * meta.x, meta.y);
-            if (masked) {
-              const int tok = 8 * n + 2 * c + (e & 1);
-              if (((tok < 32 ? bad_lo >> tok : bad_hi >> (tok - 32)) & 1u) != 0) s[n][e] = fp8_nan();
-              if (j0 + tok >= limit[h]) s[n][e] = -INFINITY;
-            }
-            mx[h] = fmaxf(mx[h], s[n][e]);
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-        }
-        if (__any_sync(0xffffffffu, mx[0] > top[0] || mx[1] > top[1])) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float m = fmaxf(top[h], mx[h]);
-            const float f = ex2_approx(top[h] - m);
-            top[h] = m;
-            sum[h] *= f;
-#pragma unroll
-            for (int j = 0; j < kCols; ++j) {
-              o[j][2 * h] *= f;
-              o[j][2 * h + 1] *= f;
-            }
-          }
-        }
-        // Weights 2^(s + ev - M), packed as the A fragments of p v.
-        uint32_t pf[8][2];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float undo = fp8_pow2(-static_cast<int>(s_meta[st * 4 + 8 * n / box].y));
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float a = ex2_approx(s[n][2 * h] - top[h]), b = ex2_approx(s[n][2 * h + 1] - top[h]);
-            sum[h] = fmaf(a + b, undo, sum[h]);
-            pf[n][h] = pack_half2(a, b);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          constexpr int W = D / 8;
-          uint32_t w[4][W / 4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int tok = 16 * k + 2 * c + (e & 1) + 8 * (e >> 1);
-            lds_words<W>(sv + swizzle_offset(tok * D + g * W, D), w[e]);
-            if (masked) {
-              const bool drop = j0 + tok >= len || (((tok < 32 ? bad_lo >> tok : bad_hi >> (tok - 32)) & 1u) != 0);
-#pragma unroll
-              for (int x = 0; x < W / 4; ++x)
-                if (drop) w[e][x] = 0;
-            }
-          }
-          const uint32_t a[4] = {pf[2 * k][0], pf[2 * k][1], pf[2 * k + 1][0], pf[2 * k + 1][1]};
-#pragma unroll
-          for (int x = 0; x < W / 4; ++x) {
-            // channels 4x .. 4x + 3 of tokens (2c, 2c + 1) and (2c + 8, 2c + 9), paired by channel
-            const uint32_t b0 = __byte_perm(w[0][x], w[1][x], 0x5140), b1 = __byte_perm(w[0][x], w[1][x], 0x7362);
-            const uint32_t c0 = __byte_perm(w[2][x], w[3][x], 0x5140), c1 = __byte_perm(w[2][x], w[3][x], 0x7362);
-            mma16816(o[4 * x], a, fp8_unpack2(b0 & 0xFFFFu), fp8_unpack2(c0 & 0xFFFFu));
-            mma16816(o[4 * x + 1], a, fp8_unpack2(b0 >> 16), fp8_unpack2(c0 >> 16));
-            mma16816(o[4 * x + 2], a, fp8_unpack2(b1 & 0xFFFFu), fp8_unpack2(c1 & 0xFFFFu));
-            mma16816(o[4 * x + 3], a, fp8_unpack2(b1 >> 16), fp8_unpack2(c1 >> 16));
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
-      }
-
-      // Merge the four warps.
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-        if (c == 0) {
-          s_ml[(warp * kRows + g + 8 * h) * 2] = top[h];
-          s_ml[(warp * kRows + g + 8 * h) * 2 + 1] = sum[h];
-        }
-      }
-      named_barrier(1, kConsumers * 32);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = g + 8 * h;
-        float m = kFloor;
-#pragma unroll
-        for (int w = 0; w < kConsumers; ++w) m = fmaxf(m, s_ml[(w * kRows + r) * 2]);
-        const float f = ex2_approx(top[h] - m);
-        // column n = 2c + e of group j is channel n D/8 + j
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int j = 0; j < kCols; ++j) s_o[(warp * kRows + r) * D + (2 * c + e) * kCols + j] = o[j][2 * h + e] * f;
-      }
-      named_barrier(1, kConsumers * 32);
-      const int slot = blockIdx.x * 2 + (sg.tile0 == 0 ? 1 : 0);
-      for (int at = threadIdx.x; at < kRows * D; at += kConsumers * 32) {
-        const int r = at / D, d = at % D;
-        if (row0 + r >= p.rows) continue;
-        float m = kFloor, l = 0.f, v = 0.f;
-#pragma unroll
-        for (int w = 0; w < kConsumers; ++w) m = fmaxf(m, s_ml[(w * kRows + r) * 2]);
-#pragma unroll
-        for (int w = 0; w < kConsumers; ++w) {
-          l = fmaf(s_ml[(w * kRows + r) * 2 + 1], ex2_approx(s_ml[(w * kRows + r) * 2] - m), l);
-          v += s_o[(w * kRows + r) * D + d];
-        }
-        if (sg.whole) {
-          const int i = (row0 + r) / p.group;
-          static_cast<T*>(p.out)[sg.b * p.out_batch + i * p.out_ld +
-                                 (static_cast<long long>(head) * p.group + (row0 + r) % p.group) * D + d] =
-              from_f32<T>(l == 0.f ? 0.f : v / l);
-        } else {
-          p.o_part[(static_cast<long long>(slot) * kRows + r) * D + d] = v;
-          if (d == 0) {
-            p.ml_part[(slot * kRows + r) * 2] = m;
-            p.ml_part[(slot * kRows + r) * 2 + 1] = l;
-          }
-        }
-      }
-      named_barrier(1, kConsumers * 32);
-      u += sg.tiles;
-    }
-  }
-}
-
-// One row of one (item, head, row tile): the partial results in the order of
-// their tiles; zeros for an item without tokens.
-template <int D, typename T>
-__global__ void __launch_bounds__(128) kv_attention_merge_kernel(const AttnParams p, unsigned int* status) {
-  __shared__ long long s_sum[2][4];
-  pdl_begin();
-  const int pairs = p.c.kv_heads * p.row_tiles;
-  const int b = blockIdx.x / pairs, pair = blockIdx.x % pairs;
-  long long total = 0, before = 0;
-  for (int i = threadIdx.x; i < p.c.batch; i += 128) {
-    const long long n = static_cast<long long>(tiles_of(kv_length(p.c, i, status))) * pairs;
-    total += n;
-    if (i < b) before += n;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
-  if (lane_id() == 0) {
-    s_sum[0][warp_id()] = total;
-    s_sum[1][warp_id()] = before;
-  }
-  __syncthreads();
-  total = s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3];
-  before = s_sum[1][0] + s_sum[1][1] + s_sum[1][2] + s_sum[1][3];
-  const int tiles = tiles_of(kv_length(p.c, b, status));
-  const int head = pair / p.row_tiles, r = blockIdx.y, row = (pair % p.row_tiles) * kRows + r;
-  if (row >= p.rows || static_cast<int>(threadIdx.x) >= D) return;
-  T* out = static_cast<T*>(p.out) + b * p.out_batch + (row / p.group) * p.out_ld +
-           (static_cast<long long>(head) * p.group + row % p.group) * D + threadIdx.x;
-  if (tiles == 0) {
-    *out = from_f32<T>(0.f);
-    return;
-  }
-  const long long active = active_ctas(total, p.ctas);
-  const long long u0 = before + static_cast<long long>(pair) * tiles, u1 = u0 + tiles;
-  long long first = u0 * active / total;  // the CTA whose range holds u0
-  while (range_begin(first + 1, total, active) <= u0) ++first;
-  while (range_begin(first, total, active) > u0) --first;
-  if (range_begin(first + 1, total, active) >= u1) return;  // one CTA had it all and wrote it
-  float m = kFloor;
-  for (long long cta = first; cta < active && range_begin(cta, total, active) < u1; ++cta) {
-    const long long slot = cta * 2 + (range_begin(cta, total, active) <= u0 ? 1 : 0);
-    m = fmaxf(m, p.ml_part[(slot * kRows + r) * 2]);
-  }
-  float l = 0.f, v = 0.f;
-  for (long long cta = first; cta < active && range_begin(cta, total, active) < u1; ++cta) {
-    const long long slot = cta * 2 + (range_begin(cta, total, active) <= u0 ? 1 : 0);
-    const float f = ex2_approx(p.ml_part[(slot * kRows + r) * 2] - m);
-    l = fmaf(p.ml_part[(slot * kRows + r) * 2 + 1], f, l);
-    v = fmaf(p.o_part[(slot * kRows + r) * D + threadIdx.x], f, v);
-  }
-  *out = from_f32<T>(l == 0.f ? 0.f : v / l);
-}
-
-size_t partial_floats(int ctas, int head_dim) { return static_cast<size_t>(ctas) * 2 * kRows * (head_dim + 2); }
-
-template <int D, typename T>
-int launch(cudaStream_t stream, const CUtensorMap& kmap, const CUtensorMap& vmap, const AttnParams& p,
-           unsigned int* status) {
-  static unsigned long long configured = 0;
-  const int most = 1024 + Cfg<D>::kOffBase + (kMaxBatch + 1) * 8;
-  int rc = ensure_smem_attribute(reinterpret_cast<const void*>(kv_attention_kernel<D, T>), most, &configured,
-                                 "kv_attention shared memory");
-  if (rc != LDB_OK) return rc;
-  const int smem = 1024 + Cfg<D>::kOffBase + (p.c.batch + 1) * 8;
-  rc = launch_kernel(kv_attention_kernel<D, T>, dim3(p.ctas), dim3(kAttnThreads), smem, stream, "kv_attention launch",
-                     kmap, vmap, p, status);
-  if (rc != LDB_OK) return rc;
-  const int pairs = p.c.batch * p.c.kv_heads * p.row_tiles;
-  return launch_kernel(kv_attention_merge_kernel<D, T>, dim3(pairs, std::min(kRows, p.rows)), dim3(128), 0, stream,
-                       "kv_attention merge launch", p, status);
+  return codes;
 }
 
 template <typename T>
-int launch_dim(cudaStream_t stream, const CUtensorMap& kmap, const CUtensorMap& vmap, const AttnParams& p, int head_dim,
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A run of tiles of one (item, head, row tile) pair, and the copies of its
+// tiles into the warp's ring.
+template <int D, int G>
+struct Fetch {
+  const KvView& c;
+  int b, head, used;      // pages that hold the item's tokens
+  int batch0;             // first of the 32 pages whose numbers and scales the lanes hold
+  int id;
+  float kf, ev;
+  float scale_log2;
+  unsigned int* status;
+
+  __device__ __forceinline__ Fetch(const KvView& view, float scale, unsigned int* st)
+      : c(view), scale_log2(scale), status(st) {}
+
+  __device__ __forceinline__ void start(int item, int h, int len) {
+    b = item;
+    head = h;
+    used = (len + c.page - 1) / c.page;
+    batch0 = -32;
+  }
+
+  // Copy tile j into the slot at `dst` (shared address) and its pages' factors to `meta`.
+  __device__ __forceinline__ void tile(int j, uint32_t dst, float2* meta) {
+    const int lane = lane_id();
+    const int shift = 31 - __clz(c.page);
+    const int first = (j * kTile) >> shift;
+    if (first - batch0 > (c.page < kTile ? 30 : 31)) {
+      batch0 = first;
+      const int at = batch0 + lane;
+      id = at < used ? c.table[b * c.table_ld + at] : -1;
+      if (at < used && (id < 0 || id >= c.pages)) {
+        set_bad_shape(status);
+        id = -1;
+      }
+      kf = 0.f;
+      ev = 0.f;
+      if (id >= 0) {
+        const long long unit = static_cast<long long>(id) * c.kv_heads + head;
+        kf = fp8_pow2(c.k_scale[unit] - 127) * scale_log2;
+        ev = static_cast<float>(c.v_scale[unit] - 127);
+      }
+    }
+    const int at = first - batch0;
+    const int id0 = __shfl_sync(0xffffffffu, id, at);
+    const float kf0 = __shfl_sync(0xffffffffu, kf, at), ev0 = __shfl_sync(0xffffffffu, ev, at);
+    int id1 = id0;
+    float kf1 = kf0, ev1 = ev0;
+    if (c.page < kTile) {
+      id1 = __shfl_sync(0xffffffffu, id, at + 1);
+      kf1 = __shfl_sync(0xffffffffu, kf, at + 1);
+      ev1 = __shfl_sync(0xffffffffu, ev, at + 1);
+    }
+    if (lane < 2) meta[lane] = lane == 0 ? make_float2(kf0, ev0) : make_float2(kf1, ev1);
+    // 16-byte unit q of a tile goes to its swizzled place: within 512 bytes the
+    // pattern depends on the lane, and for 128-byte rows on the parity of i.
+    constexpr int kUnits = kTile * D / 16 / 32;  // per lane, of K and of V
+    const uint32_t even = swizzle_offset(lane * 16, D), odd = swizzle_offset(512 + lane * 16, D) - 512;
+    const int inside = (j * kTile) & (c.page - 1);  // first row of the tile in its page
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // rows 0 .. 15 and 16 .. 31
+      const int page_id = h == 0 ? id0 : id1;
+      if (page_id < 0) continue;
+      const int row = c.page < kTile ? 0 : inside + 16 * h;
+      const long long off = ((static_cast<long long>(page_id) * c.kv_heads + head) * c.page + row) * D + lane * 16;
+#pragma unroll
+      for (int i = 0; i < kUnits / 2; ++i) {
+        const int at_i = h * (kUnits / 2) + i;
+        const uint32_t to = dst + at_i * 512 + ((at_i & 1) ? odd : even);
+        cp_async16(to, c.k + off + i * 512);
+        cp_async16(to + kTile * D, c.v + off + i * 512);
+      }
+    }
+  }
+};
+
+template <int D, int G, typename T>
+__global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
+    kv_attention_kernel(const AttnParams p, unsigned int* status) {
+  using C = Cfg<D, G>;
+  constexpr bool kThreeParts = std::is_same<T, __half>::value;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  int* s_base = reinterpret_cast<int*>(smem + C::kOffBase);
+  const int warp = warp_id(), lane = lane_id();
+  const int me = blockIdx.x * kWarps + warp;
+  pdl_begin();
+  const int pairs = p.c.kv_heads * p.row_tiles;
+  {
+    // First position of each item on the line: a scan over blocks of items.
+    __shared__ int s_warp[kWarps];
+    int before = 0, next = static_cast<int>(threadIdx.x) < p.c.batch ? kv_length(p.c, threadIdx.x, status) : 0;
+    for (int b0 = 0; b0 < p.c.batch; b0 += kWarps * 32) {
+      const int b = b0 + threadIdx.x;
+      const int n = b < p.c.batch ? places_of(next) * pairs : 0;
+      if (b + kWarps * 32 < p.c.batch) next = kv_length(p.c, b + kWarps * 32, status);
+      int upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += other;
+      }
+      if (lane == 31) s_warp[warp] = upto;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) upto += s_warp[w];
+      }
+      if (b < p.c.batch) s_base[b] = before + upto - n;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) before += s_warp[w];
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) s_base[p.c.batch] = before;
+    __syncthreads();
+  }
+  // Zeros for items without tokens, dealt out over the CTAs.
+  for (int b = blockIdx.x; b < p.c.batch; b += gridDim.x) {
+    if (s_base[b + 1] != s_base[b]) continue;
+    const int width = p.c.kv_heads * p.group * D;
+    for (long long i = threadIdx.x; i < static_cast<long long>(p.queries) * width; i += kWarps * 32)
+      static_cast<T*>(p.out)[b * p.out_batch + (i / width) * p.out_ld + i % width] = from_f32<T>(0.f);
+  }
+  const Ranges ranges(s_base[p.c.batch], p.warps);
+  const int begin = ranges.begin(me), end = ranges.begin(me + 1);
+  if (!p.open_by_pair && lane == 0) p.open_part[me] = make_int4(0, 0, 0, 0);
+  if (begin == end) return;
+
+  const uint32_t ring = smem_u32(smem + warp * C::kSlots * C::kSlotBytes);
+  const uint8_t* ring_ptr = smem + warp * C::kSlots * C::kSlotBytes;
+  float2* s_meta = reinterpret_cast<float2*>(smem + C::kOffMeta) + warp * C::kSlots * 2;
+
+  // Lane (g, c) holds, in q k, query row g of each group, keys 2c and 2c + 1
+  // of every eight, channels [c D/4, (c + 1) D/4) of key g; in p v, tokens 2c, 2c
+  // + 1, 2c + 8, 2c + 9 of every 16 and channels [g D/8, (g + 1) D/8), and the
+  // outputs of those channels for rows 2c and 2c + 1.
+  const int g = lane >> 2, c = lane & 3;
+  constexpr int kSteps = D / 32;  // q k products over the channels
+  constexpr int kMTiles = D / 16; // p v products over the channels
+  // Swizzled places of the lane's bytes: the rows 8 n + g of K and 16 k + 8 h
+  // + 2c (+ 1) of V have the same pattern for every n, k and h.
+  constexpr int kWk = D / 4 >= 16 ? 16 : D / 4;  // bytes per read of K
+  constexpr int kWv = D / 8;                     // bytes per read of V
+  uint32_t at_k[(D / 4) / kWk], at_v[2];
+#pragma unroll
+  for (int h = 0; h < (D / 4) / kWk; ++h) at_k[h] = swizzle_offset(g * D + c * (D / 4) + h * kWk, D);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) at_v[e] = C::kTileBytes + swizzle_offset((2 * c + e) * D + g * kWv, D);
+
+  // The item and pair where the range begins.
+  int b = 0;
+  for (int lo = 0, hi = p.c.batch; hi - lo > 1;) {
+    const int mid = (lo + hi) / 2;
+    if (s_base[mid] <= begin) {
+      lo = mid;
+    } else {
+      hi = mid;
+    }
+    b = lo;
+  }
+  Fetch<D, G> fetch(p.c, p.scale_log2, status);
+  int places = (s_base[b + 1] - s_base[b]) / pairs;
+  int pair = (begin - s_base[b]) / places;
+  int at = s_base[b] + pair * places;  // of the pair
+  for (; at < end; at += places, ++pair) {
+    if (pair == pairs) {
+      pair = 0;
+      do {
+        ++b;
+      } while (s_base[b + 1] == s_base[b]);  // (position `at` exists, so a later item has tokens)
+      places = (s_base[b + 1] - s_base[b]) / pairs;
+    }
+    const int item_tiles = places - kStart;
+    const int tile0 = max(0, begin - at - kStart), tiles = min(item_tiles, end - at - kStart) - tile0;
+    if (tiles <= 0) continue;
+    const int head = pair / p.row_tiles, row0 = (pair % p.row_tiles) * C::kRows;
+    const int len = kv_length(p.c, b, status);
+    // Queries as they are, on their way while the page numbers arrive.
+    uint32_t raw[G][D / 8];
+    int limit[G];  // the keys a row sees
+#pragma unroll
+    for (int r = 0; r < G; ++r) {
+      const int row = row0 + 8 * r + g;
+      const bool live = row < p.rows;
+      const int i = live ? row / p.group : 0;
+      limit[r] = !live ? len : (p.causal ? min(len, len - p.queries + i + 1) : len);
+      const T* src = static_cast<const T*>(p.q) + b * p.q_batch + i * p.q_ld +
+                     (static_cast<long long>(head) * p.group + (live ? row % p.group : 0)) * D + c * (D / 4);
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        if (!live) {
+          raw[r][4 * k] = raw[r][4 * k + 1] = raw[r][4 * k + 2] = raw[r][4 * k + 3] = 0;
+        } else if (p.q_vec) {
+          const uint4 t = reinterpret_cast<const uint4*>(src)[k];
+          raw[r][4 * k] = t.x, raw[r][4 * k + 1] = t.y, raw[r][4 * k + 2] = t.z, raw[r][4 * k + 3] = t.w;
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(src) + 8 * k;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) raw[r][4 * k + e] = h[2 * e] | static_cast<uint32_t>(h[2 * e + 1]) << 16;
+        }
+      }
+    }
+    fetch.start(b, head, len);
+#pragma unroll
+    for (int t = 0; t < C::kSlots - 1; ++t) {
+      if (t < tiles) fetch.tile(tile0 + t, ring + t * C::kSlotBytes, s_meta + 2 * t);
+      cp_async_commit();
+    }
+
+    // Queries in parts, and their rows' power-of-two factors.
+    uint32_t q01[G][kSteps][4];                   // parts 0 and 1 of four + four channels
+    uint32_t q2[G][kThreeParts ? kSteps : 1][2];  // part 2
+    float qs[G];
+#pragma unroll
+    for (int r = 0; r < G; ++r) {
+      // the row's largest magnitude to [128, 256); a NaN stays one, an infinity makes the row's factor one
+      float m = 0.f;
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) {
+        const float2 x = unpack2<T>(raw[r][k]);
+        m = fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y)));
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const int e = m > 0.f ? min(126, max(-119, static_cast<int>(__float_as_uint(m) >> 23) - 127)) : 0;
+      qs[r] = fp8_is_finite(m) ? fp8_pow2(e - 7) : fp8_nan();
+      const float inv = fp8_pow2(7 - e);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 x = unpack2<T>(raw[r][4 * s + 2 * h]), y = unpack2<T>(raw[r][4 * s + 2 * h + 1]);
+          __half2 t[2] = {__floats2half2_rn(x.x * inv, x.y * inv), __floats2half2_rn(y.x * inv, y.y * inv)};
+          q01[r][s][2 * h] = split_part(t);
+          q01[r][s][2 * h + 1] = split_part(t);
+          if constexpr (kThreeParts) q2[r][s][h] = split_part(t);
+        }
+    }
+    const int open = p.causal ? min(len, len - p.queries + row0 / p.group + 1) : len;  // keys that every row sees
+
+    float o[G][kMTiles][4];
+#pragma unroll
+    for (int r = 0; r < G; ++r)
+#pragma unroll
+      for (int j = 0; j < kMTiles; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][j][e] = 0.f;
+    float top[G], sum[G];
+#pragma unroll
+    for (int r = 0; r < G; ++r) top[r] = kFloor, sum[r] = 0.f;
+
+    int slot = 0;
+#pragma unroll 1
+    for (int t = 0; t < tiles; ++t) {
+      // The slot of tile t - 1 is free: start tile t + kSlots - 1, then wait for tile t.
+      {
+        const int into = slot == 0 ? C::kSlots - 1 : slot - 1;
+        if (t + C::kSlots - 1 < tiles)
+          fetch.tile(tile0 + t + C::kSlots - 1, ring + into * C::kSlotBytes, s_meta + 2 * into);
+        cp_async_commit();
+      }
+      cp_async_wait<C::kSlots - 1>();
+      __syncwarp();
+      const uint8_t* sk = ring_ptr + slot * C::kSlotBytes;
+      const float2 meta[2] = {s_meta[2 * slot], s_meta[2 * slot + 1]};
+      const int j0 = (tile0 + t) * kTile;
+      const bool masked = j0 + kTile > open;
+
+      // Scores plus the value scale's exponent, eight keys at a time.
+      float s[G][4][2];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        uint32_t w[D / 16];
+#pragma unroll
+        for (int h = 0; h < (D / 4) / kWk; ++h) {
+          uint32_t part[kWk / 4];
+          lds_words<kWk>(sk + at_k[h] + n * 8 * D, part);
+#pragma unroll
+          for (int e = 0; e < kWk / 4; ++e) w[h * (kWk / 4) + e] = part[e];
+        }
+#pragma unroll
+        for (int r = 0; r < G; ++r) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k)
+            mma_e4m3(d, q01[r][k][0], q01[r][k][1], q01[r][k][2], q01[r][k][3], w[2 * k], w[2 * k + 1]);
+          if constexpr (kThreeParts) {
+            float d2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) mma_e4m3(d2, q2[r][k][0], 0u, q2[r][k][1], 0u, w[2 * k], w[2 * k + 1]);
+            d[2] = fmaf(d2[0], 0.0625f, d[2]);
+            d[3] = fmaf(d2[1], 0.0625f, d[3]);
+          }
+          const float f = qs[r] * meta[n >> 1].x;
+          s[r][n][0] = fmaf(fmaf(d[2], 0.0625f, d[0]), f, meta[n >> 1].y);
+          s[r][n][1] = fmaf(fmaf(d[3], 0.0625f, d[1]), f, meta[n >> 1].y);
+        }
+      }
+      uint32_t bad = 0;  // tokens some rows must not see whose values hold a NaN
+      if (masked) {
+        if (p.queries > 1) {
+          uint32_t any = 0;
+          for (int e = 0; e < D / 4; ++e)
+            any |= nan_codes(reinterpret_cast<const uint32_t*>(sk + C::kTileBytes + lane * D)[e]);
+          bad = __ballot_sync(0xffffffffu, any != 0);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int tok = 8 * n + 2 * c + e;
+#pragma unroll
+            for (int r = 0; r < G; ++r) {
+              if ((bad >> tok) & 1u) s[r][n][e] = fp8_nan();
+              if (j0 + tok >= limit[r]) s[r][n][e] = -INFINITY;
+            }
+          }
+      }
+      float mx[G];
+      bool grew = false;
+#pragma unroll
+      for (int r = 0; r < G; ++r) {
+        mx[r] = kFloor;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) mx[r] = fmaxf(mx[r], fmaxf(s[r][n][0], s[r][n][1]));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+        grew |= mx[r] > top[r];
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int r = 0; r < G; ++r) {
+          const float m = fmaxf(top[r], mx[r]);
+          const float f = ex2_approx(top[r] - m);
+          top[r] = m;
+          sum[r] *= f;
+          const float f0 = __shfl_sync(0xffffffffu, f, 8 * c), f1 = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+#pragma unroll
+          for (int j = 0; j < kMTiles; ++j) {
+            o[r][j][0] *= f0;
+            o[r][j][1] *= f1;
+            o[r][j][2] *= f0;
+            o[r][j][3] *= f1;
+          }
+        }
+      }
+      // Weights 2^(s + ev - M): the fragments of p v as they are.
+      uint32_t pf[G][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float undo = fp8_pow2(-static_cast<int>(meta[n >> 1].y));
+#pragma unroll
+        for (int r = 0; r < G; ++r) {
+          const float a = ex2_approx(s[r][n][0] - top[r]), bb = ex2_approx(s[r][n][1] - top[r]);
+          sum[r] = fmaf(a + bb, undo, sum[r]);
+          pf[r][n] = pack_half2(a, bb);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t w[4][kWv / 4];  // tokens 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lds_words<kWv>(sk + at_v[e & 1] + (16 * k + 8 * (e >> 1)) * D, w[e]);
+          if (masked) {
+            const int tok = 16 * k + 2 * c + (e & 1) + 8 * (e >> 1);
+            const bool drop = j0 + tok >= len || ((bad >> tok) & 1u) != 0;
+#pragma unroll
+            for (int x = 0; x < kWv / 4; ++x)
+              if (drop) w[e][x] = 0;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < kWv / 4; ++x) {
+          // channels 4x .. 4x + 3 of tokens (2c, 2c + 1) and (2c + 8, 2c + 9), paired by channel
+          const uint32_t b0 = __byte_perm(w[0][x], w[1][x], 0x5140), b1 = __byte_perm(w[0][x], w[1][x], 0x7362);
+          const uint32_t c0 = __byte_perm(w[2][x], w[3][x], 0x5140), c1 = __byte_perm(w[2][x], w[3][x], 0x7362);
+          const uint32_t v0 = fp8_unpack2(b0 & 0xFFFFu), v1 = fp8_unpack2(b0 >> 16);
+          const uint32_t v2 = fp8_unpack2(c0 & 0xFFFFu), v3 = fp8_unpack2(c0 >> 16);
+          const uint32_t v4 = fp8_unpack2(b1 & 0xFFFFu), v5 = fp8_unpack2(b1 >> 16);
+          const uint32_t v6 = fp8_unpack2(c1 & 0xFFFFu), v7 = fp8_unpack2(c1 >> 16);
+#pragma unroll
+          for (int r = 0; r < G; ++r) {
+            mma_f16(o[r][2 * x], v0, v1, v2, v3, pf[r][2 * k], pf[r][2 * k + 1]);
+            mma_f16(o[r][2 * x + 1], v4, v5, v6, v7, pf[r][2 * k], pf[r][2 * k + 1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (++slot == C::kSlots) slot = 0;
+    }
+
+    // The pair's rows, or this range's part of them.
+    const bool whole = tiles == item_tiles;
+    const int part = me * 2 + (tile0 == 0 ? 1 : 0);
+#pragma unroll
+    for (int r = 0; r < G; ++r) {
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+      if (!whole && c == 0) {
+        float* ml = p.ml_part + (static_cast<long long>(part) * C::kRows + 8 * r + g) * 2;
+        ml[0] = top[r];
+        ml[1] = sum[r];
+      }
+      const float l[2] = {__shfl_sync(0xffffffffu, sum[r], 8 * c), __shfl_sync(0xffffffffu, sum[r], 8 * c + 4)};
+      // products j: rows g and g + 8 are channels g D/8 + 2j and + 1
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = row0 + 8 * r + 2 * c + e;
+        if (row >= p.rows) continue;
+        if (whole) {
+          const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];
+          T* dst = static_cast<T*>(p.out) + b * p.out_batch + (row / p.group) * p.out_ld +
+                   (static_cast<long long>(head) * p.group + row % p.group) * D + g * (D / 8);
+          if (D >= 64 && p.out_vec) {
+#pragma unroll
+            for (int j = 0; j < kMTiles / 4; ++j) {
+              const float v[8] = {o[r][4 * j][e] * inv,     o[r][4 * j][2 + e] * inv,     o[r][4 * j + 1][e] * inv,
+                                  o[r][4 * j + 1][2 + e] * inv, o[r][4 * j + 2][e] * inv, o[r][4 * j + 2][2 + e] * inv,
+                                  o[r][4 * j + 3][e] * inv, o[r][4 * j + 3][2 + e] * inv};
+              store8<T>(dst + 8 * j, v);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kMTiles; ++j) {
+              dst[2 * j] = from_f32<T>(o[r][j][e] * inv);
+              dst[2 * j + 1] = from_f32<T>(o[r][j][2 + e] * inv);
+            }
+          }
+        } else {
+          float* dst = p.o_part + (static_cast<long long>(part) * C::kRows + 8 * r + 2 * c + e) * D + g * (D / 8);
+#pragma unroll
+          for (int j = 0; j < kMTiles / 2; ++j)
+            reinterpret_cast<float4*>(dst)[j] =
+                make_float4(o[r][2 * j][e], o[r][2 * j][2 + e], o[r][2 * j + 1][e], o[r][2 * j + 1][2 + e]);
+        }
+      }
+    }
+    // The warp that starts a pair says who goes on with it.
+    if (tile0 == 0 && lane == 0 && (p.open_by_pair || !whole))
+      p.open_part[p.open_by_pair ? b * pairs + pair : me] =
+          make_int4(b, pair, me, whole ? 0 : ranges.of(at + kStart + item_tiles - 1) - me + 1);
+  }
+}
+
+// Row blockIdx.y of a pair whose tiles lie in several ranges: its parts, one
+// per warp from the one that starts it.  The threads weigh the parts first (the
+// references' maximum is order-free, the sums go through a fixed tree), then the
+// block's groups of D / 4 threads, four channels each, add every k-th part in order, and
+// the groups' sums are added in order.  Small blocks: most have nothing to do.
+constexpr int kMergeThreads = 256;
+template <int D, typename T>
+__global__ void __launch_bounds__(kMergeThreads) kv_attention_merge_kernel(const AttnParams p) {
+  constexpr int kLanes = D / 4, kGroups = kMergeThreads / kLanes;
+  __shared__ float4 s_v[kGroups][kLanes];
+  __shared__ float s_red[2][kMergeThreads / 32], s_f[kMergeThreads];
+  pdl_begin();
+  int4 at = p.open_part[blockIdx.x];
+  if (p.open_by_pair && kv_length(p.c, blockIdx.x / (p.c.kv_heads * p.row_tiles), p.status) == 0) at.w = 0;  // not written
+  const int first = at.z, count = at.w, r = blockIdx.y;
+  const int row = (at.y % p.row_tiles) * p.tile_rows + r;
+  if (count == 0 || row >= p.rows) return;
+  const int head = at.y / p.row_tiles;
+  const int group = threadIdx.x / kLanes, lane4 = threadIdx.x % kLanes;
+  // slot 1 of the warp that starts the pair, slot 0 of those that go on with it
+  auto part = [&](int i) { return (static_cast<long long>(first + i) * 2 + (i == 0 ? 1 : 0)) * p.tile_rows + r; };
+  float m = kFloor;
+  for (int i = threadIdx.x; i < count; i += kMergeThreads) m = fmaxf(m, p.ml_part[part(i) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane_id() == 0) s_red[0][warp_id()] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 32; ++w) m = fmaxf(m, s_red[0][w]);
+  float l = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < count; i0 += kMergeThreads) {
+    if (i0) __syncthreads();  // the round before has read s_f
+    const int i = i0 + threadIdx.x;
+    if (i < count) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.ml_part + part(i) * 2);
+      s_f[threadIdx.x] = ex2_approx(ml.x - m);
+      l = fmaf(ml.y, s_f[threadIdx.x], l);
+    }
+    __syncthreads();
+    const int n = min(count - i0, kMergeThreads);
+#pragma unroll 8
+    for (int k = group; k < n; k += kGroups) {
+      const float4 o = reinterpret_cast<const float4*>(p.o_part + part(i0 + k) * D)[lane4];
+      const float f = s_f[k];
+      v.x = fmaf(o.x, f, v.x), v.y = fmaf(o.y, f, v.y), v.z = fmaf(o.z, f, v.z), v.w = fmaf(o.w, f, v.w);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (lane_id() == 0) s_red[1][warp_id()] = l;
+  s_v[group][lane4] = v;
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) >= D) return;
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 32; ++w) l += s_red[1][w];
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) sum += reinterpret_cast<const float*>(s_v[k])[threadIdx.x];
+  static_cast<T*>(p.out)[at.x * p.out_batch + (row / p.group) * p.out_ld +
+                         (static_cast<long long>(head) * p.group + row % p.group) * D + threadIdx.x] =
+      from_f32<T>(l == 0.f ? 0.f : sum / l);
+}
+
+// Partial rows of every warp, and the pairs left open.
+size_t workspace_bytes_of(int warps, int rows, int head_dim) {
+  return static_cast<size_t>(warps) * (2ull * rows * (head_dim + 2) * sizeof(float) + sizeof(int4));
+}
+
+// Groups of eight query rows that one pass over the cache serves: as few as
+// hold the rows, so that a lane's output stays in registers (8 D / 32 a group).
+int row_groups(long long rows) { return rows <= 8 ? 1 : 2; }
+
+template <int D, int G, typename T>
+int launch(cudaStream_t stream, const AttnParams& p, unsigned int* status) {
+  static unsigned long long configured = 0;
+  int rc = ensure_smem_attribute(reinterpret_cast<const void*>(kv_attention_kernel<D, G, T>),
+                                 Cfg<D, G>::kOffBase + (kMaxBatch + 1) * 4, &configured, "kv_attention shared memory");
+  if (rc != LDB_OK) return rc;
+  rc = launch_kernel(kv_attention_kernel<D, G, T>, dim3(p.warps / kWarps), dim3(kWarps * 32),
+                     Cfg<D, G>::kOffBase + (p.c.batch + 1) * 4, stream, "kv_attention launch", p, status);
+  if (rc != LDB_OK) return rc;
+  return launch_kernel(kv_attention_merge_kernel<D, T>,
+                       dim3(p.open_by_pair ? p.c.batch * p.c.kv_heads * p.row_tiles : p.warps, std::min(p.tile_rows, p.rows)),
+                       dim3(kMergeThreads), 0, stream,
+                       "kv_attention merge launch", p);
+}
+
+template <int D, typename T>
+int launch_groups(cudaStream_t stream, const AttnParams& p,
+                  unsigned int* status) {
+  return p.tile_rows == 8 ? launch<D, 1, T>(stream, p, status)
+                          : launch<D, 2, T>(stream, p, status);
+}
+
+template <typename T>
+int launch_dim(cudaStream_t stream, const AttnParams& p, int head_dim,
                unsigned int* status) {
-  if (head_dim == 32) return launch<32, T>(stream, kmap, vmap, p, status);
-  if (head_dim == 64) return launch<64, T>(stream, kmap, vmap, p, status);
-  return launch<128, T>(stream, kmap, vmap, p, status);
+  if (head_dim == 32) return launch_groups<32, T>(stream, p, status);
+  if (head_dim == 64) return launch_groups<64, T>(stream, p, status);
+  return launch_groups<128, T>(stream, p, status);
 }
 
 }  // namespace
@@ -582,7 +726,8 @@ int ldb_kv_attention_fp8_workspace_size(int batch, int queries, int heads, int k
   if (batch < 0 || queries < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads ||
       (head_dim != 32 && head_dim != 64 && head_dim != 128))
     return fail(LDB_ERR_SHAPE, "kv_attention: %d heads over %d of width %d (32, 64 or 128)", heads, kv_heads, head_dim);
-  *bytes = partial_floats(kCtasPerSm * sm_count(), head_dim) * sizeof(float);
+  const int rows = kGroupRows * row_groups(static_cast<long long>(queries) * (heads / kv_heads));
+  *bytes = workspace_bytes_of(ctas_per_sm(head_dim) * sm_count() * kWarps, rows, head_dim);
   return LDB_OK;
 }
 
@@ -623,25 +768,24 @@ int ldb_kv_attention_fp8(cudaStream_t stream, const void* q, long long q_ld, lon
   p.out = out, p.out_ld = out_ld, p.out_batch = out_batch;
   p.queries = queries, p.group = heads / kv_heads;
   const long long group_rows = static_cast<long long>(queries) * p.group;
-  const long long row_tiles = (group_rows + kRows - 1) / kRows;
-  if (group_rows > 0x7FFFFFFFll || row_tiles * kv_heads * batch > 0x7FFFFFFFll)
-    return fail(LDB_ERR_SHAPE, "kv_attention: too many query rows");
+  p.tile_rows = kGroupRows * row_groups(group_rows);
+  const long long row_tiles = (group_rows + p.tile_rows - 1) / p.tile_rows;
+  const long long tiles = kStart + (static_cast<long long>(width) * page + kTile - 1) / kTile;
+  if (group_rows > 0x7FFFFFFFll || row_tiles * kv_heads > 0x7FFFFFFFll || row_tiles * kv_heads * batch * tiles > 0x7FFFFFFFll)
+    return fail(LDB_ERR_SHAPE, "kv_attention: too many query rows over too long a table");
   p.rows = static_cast<int>(group_rows), p.row_tiles = static_cast<int>(row_tiles);
   p.causal = causal != 0;
   p.q_vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_ld % 8 == 0 && q_batch % 8 == 0;
+  p.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_ld % 8 == 0 && out_batch % 8 == 0;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.ctas = kCtasPerSm * sm_count();
+  p.warps = ctas_per_sm(head_dim) * sm_count() * kWarps;
   p.o_part = static_cast<float*>(workspace);
-  p.ml_part = p.o_part + static_cast<size_t>(p.ctas) * 2 * kRows * head_dim;
-  CUtensorMap kmap, vmap;
-  const uint64_t dims[2] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(rows_all)};
-  const uint64_t strides[1] = {static_cast<uint64_t>(head_dim)};
-  const uint32_t box[2] = {static_cast<uint32_t>(head_dim), static_cast<uint32_t>(std::min(page, kTile))};
-  rc = encode_tiled_u8(&kmap, k_codes, 2, dims, strides, box, head_dim);
-  if (rc == LDB_OK) rc = encode_tiled_u8(&vmap, v_codes, 2, dims, strides, box, head_dim);
-  if (rc != LDB_OK) return rc;
-  return dtype == LDB_F16 ? launch_dim<__half>(stream, kmap, vmap, p, head_dim, status)
-                          : launch_dim<__nv_bfloat16>(stream, kmap, vmap, p, head_dim, status);
+  p.ml_part = p.o_part + static_cast<size_t>(p.warps) * 2 * p.tile_rows * head_dim;
+  p.open_by_pair = row_tiles * kv_heads * batch <= p.warps;
+  p.status = status;
+  p.open_part = reinterpret_cast<int4*>(p.ml_part + static_cast<size_t>(p.warps) * 2 * p.tile_rows * 2);
+  return dtype == LDB_F16 ? launch_dim<__half>(stream, p, head_dim, status)
+                          : launch_dim<__nv_bfloat16>(stream, p, head_dim, status);
 }
 
 }  // extern "C"
