@@ -30,7 +30,7 @@
 #include <algorithm>
 
 #include "host_common.h"
-#include "kv_cache.cuh"
+#include "kv_attention.cuh"
 
 namespace ldb {
 namespace {
@@ -41,7 +41,7 @@ constexpr int kWarps = 4;        // per CTA; they share nothing but the tiles' l
 constexpr int kMaxBatch = 2048;
 // Positions on the line that the start of a pair counts for: its page numbers,
 // scales and queries take a warp about as long as this many tiles.  (Without them a
-// batch of short items next to long ones ran 1.7 times as long.)
+// batch of 384 items of 2 to 1024 tokens took 166 us instead of 86.)
 constexpr int kStart = 3;
 constexpr float kFloor = -1.0e30f;  // reference of a row that has seen nothing
 
@@ -122,8 +122,6 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
-
 // W bytes (4, 8 or 16) at a 16-byte unit of a swizzled tile.
 template <int W>
 __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[W / 4]) {
@@ -136,26 +134,6 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[W / 4]
   } else {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
-}
-
-// Four values as e4m3, and what is left of them times 16 (exact): the next part's input.
-__device__ __forceinline__ uint32_t split_part(__half2 (&x)[2]) {
-  uint32_t codes = 0;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint16_t part;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(part) : "r"(*reinterpret_cast<const uint32_t*>(&x[h])));
-    const uint32_t back = fp8_unpack2(part);
-    x[h] = __hmul2(__hsub2(x[h], *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(16.f));
-    codes |= static_cast<uint32_t>(part) << (16 * h);
-  }
-  return codes;
-}
-
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -385,7 +363,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
       float m = 0.f;
 #pragma unroll
       for (int k = 0; k < D / 8; ++k) {
-        const float2 x = unpack2<T>(raw[r][k]);
+        const float2 x = kv_unpack2<T>(raw[r][k]);
         m = fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y)));
       }
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
@@ -397,11 +375,11 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
       for (int s = 0; s < kSteps; ++s)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float2 x = unpack2<T>(raw[r][4 * s + 2 * h]), y = unpack2<T>(raw[r][4 * s + 2 * h + 1]);
+          const float2 x = kv_unpack2<T>(raw[r][4 * s + 2 * h]), y = kv_unpack2<T>(raw[r][4 * s + 2 * h + 1]);
           __half2 t[2] = {__floats2half2_rn(x.x * inv, x.y * inv), __floats2half2_rn(y.x * inv, y.y * inv)};
-          q01[r][s][2 * h] = split_part(t);
-          q01[r][s][2 * h + 1] = split_part(t);
-          if constexpr (kThreeParts) q2[r][s][h] = split_part(t);
+          q01[r][s][2 * h] = kv_split_part<16>(t);
+          q01[r][s][2 * h + 1] = kv_split_part<16>(t);
+          if constexpr (kThreeParts) q2[r][s][h] = kv_split_part<16>(t);
         }
     }
     const int open = p.causal ? min(len, len - p.queries + row0 / p.group + 1) : len;  // keys that every row sees
@@ -469,7 +447,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
         if (p.queries > 1) {
           uint32_t any = 0;
           for (int e = 0; e < D / 4; ++e)
-            any |= nan_codes(reinterpret_cast<const uint32_t*>(sk + C::kTileBytes + lane * D)[e]);
+            any |= kv_nan_codes(reinterpret_cast<const uint32_t*>(sk + C::kTileBytes + lane * D)[e]);
           bad = __ballot_sync(0xffffffffu, any != 0);
         }
 #pragma unroll
@@ -685,6 +663,9 @@ size_t workspace_bytes_of(int warps, int rows, int head_dim) {
 // hold the rows, so that a lane's output stays in registers (8 D / 32 a group).
 int row_groups(long long rows) { return rows <= 8 ? 1 : 2; }
 
+// Rows from which on the 128-row tiles of the many-row kernel are the faster.
+constexpr long long kTileRows = 17;
+
 template <int D, int G, typename T>
 int launch(cudaStream_t stream, const AttnParams& p, unsigned int* status) {
   static unsigned long long configured = 0;
@@ -726,8 +707,10 @@ int ldb_kv_attention_fp8_workspace_size(int batch, int queries, int heads, int k
   if (batch < 0 || queries < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads ||
       (head_dim != 32 && head_dim != 64 && head_dim != 128))
     return fail(LDB_ERR_SHAPE, "kv_attention: %d heads over %d of width %d (32, 64 or 128)", heads, kv_heads, head_dim);
-  const int rows = kGroupRows * row_groups(static_cast<long long>(queries) * (heads / kv_heads));
-  *bytes = workspace_bytes_of(ctas_per_sm(head_dim) * sm_count() * kWarps, rows, head_dim);
+  const long long rows = static_cast<long long>(queries) * (heads / kv_heads);
+  *bytes = rows >= kTileRows ? kv_tile_workspace(batch, kv_heads, rows, head_dim)
+                             : workspace_bytes_of(ctas_per_sm(head_dim) * sm_count() * kWarps,
+                                                  kGroupRows * row_groups(rows), head_dim);
   return LDB_OK;
 }
 
@@ -757,26 +740,36 @@ int ldb_kv_attention_fp8(cudaStream_t stream, const void* q, long long q_ld, lon
     return fail(LDB_ERR_SHAPE, "kv_attention: a row stride is below %lld", row);
   if (reinterpret_cast<uintptr_t>(k_codes) % 16 || reinterpret_cast<uintptr_t>(v_codes) % 16)
     return fail(LDB_ERR_ALIGNMENT, "kv_attention: codes must be 16-byte aligned");
-  if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(LDB_ERR_WORKSPACE, "kv_attention needs %zu workspace bytes (16-byte aligned), got %zu", need,
                 workspace_bytes);
   unsigned int* status = device_status_ptr();
   if (!status) return fail(LDB_ERR_CUDA, "kv_attention: no device status word");
+  const KvView view{k_codes, v_codes, k_scales, v_scales, table, lengths, table_ld, pages, kv_heads, page, width, batch};
+  const long long group_rows = static_cast<long long>(queries) * (heads / kv_heads);
+  if (group_rows > 0x7FFFFF00ll) return fail(LDB_ERR_SHAPE, "kv_attention: too many query rows");
+  const int q_vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_ld % 8 == 0 && q_batch % 8 == 0;
+  const int out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_ld % 8 == 0 && out_batch % 8 == 0;
+  if (group_rows >= kTileRows) {
+    KvTileParams t{};
+    t.c = view;
+    t.q = q, t.q_ld = q_ld, t.q_batch = q_batch, t.q_vec = q_vec;
+    t.out = out, t.out_ld = out_ld, t.out_batch = out_batch, t.out_vec = out_vec;
+    t.queries = queries, t.group = heads / kv_heads, t.rows = static_cast<int>(group_rows), t.causal = causal != 0;
+    return kv_attention_tiles(stream, t, head_dim, dtype, scale, workspace, status);
+  }
   AttnParams p{};
-  p.c = KvView{k_codes, v_codes, k_scales, v_scales, table, lengths, table_ld, pages, kv_heads, page, width, batch};
-  p.q = q, p.q_ld = q_ld, p.q_batch = q_batch;
-  p.out = out, p.out_ld = out_ld, p.out_batch = out_batch;
+  p.c = view;
+  p.q = q, p.q_ld = q_ld, p.q_batch = q_batch, p.q_vec = q_vec;
+  p.out = out, p.out_ld = out_ld, p.out_batch = out_batch, p.out_vec = out_vec;
   p.queries = queries, p.group = heads / kv_heads;
-  const long long group_rows = static_cast<long long>(queries) * p.group;
   p.tile_rows = kGroupRows * row_groups(group_rows);
   const long long row_tiles = (group_rows + p.tile_rows - 1) / p.tile_rows;
   const long long tiles = kStart + (static_cast<long long>(width) * page + kTile - 1) / kTile;
-  if (group_rows > 0x7FFFFFFFll || row_tiles * kv_heads > 0x7FFFFFFFll || row_tiles * kv_heads * batch * tiles > 0x7FFFFFFFll)
-    return fail(LDB_ERR_SHAPE, "kv_attention: too many query rows over too long a table");
+  if (row_tiles * kv_heads > 0x7FFFFFFFll || row_tiles * kv_heads * batch * tiles > 0x7FFFFFFFll)
+    return fail(LDB_ERR_SHAPE, "kv_attention: too many heads over too long a table");
   p.rows = static_cast<int>(group_rows), p.row_tiles = static_cast<int>(row_tiles);
   p.causal = causal != 0;
-  p.q_vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_ld % 8 == 0 && q_batch % 8 == 0;
-  p.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_ld % 8 == 0 && out_batch % 8 == 0;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.warps = ctas_per_sm(head_dim) * sm_count() * kWarps;
   p.o_part = static_cast<float*>(workspace);
