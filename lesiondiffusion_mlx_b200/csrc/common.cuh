@@ -273,18 +273,49 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
       : "memory");
 }
 
-// D[tmem] (+)= (A 2^sa)[smem] * (B 2^sb)[smem]^T of 8-bit operands, f32
+// The forms below are for a whole warp: every lane calls them with the same
+// operands and one elected lane (the same each time) issues.  In convergent
+// code the descriptors stay in uniform registers; issued from a `lane == 0`
+// branch each product costs its thread about 100 cycles, twice what a
+// 128 x 128 product takes at the tensor core.
+
+// D[tmem] (+)= (A 2^sa)[smem] * (B 2^sb)[smem]^T of e4m3 operands, f32
 // accumulator (kind::mxf8f6f4, K = 32): one E8M0 scale per row of A and of B
 // for each product, read from tensor memory (tmem_copy_scales lays them out).
 // The instruction descriptor names the byte of each 32-bit scale word to use.
 __device__ __forceinline__ void umma_ss_mx8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                             uint32_t sa_tmem, uint32_t sb_tmem, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::
+      "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::
           "r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+      : "memory");
+}
+
+// D[tmem] (+)= A[smem] * B[smem]^T of e4m3 operands, f32 accumulator (K = 32).
+__device__ __forceinline__ void umma_ss_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// umma_ts of a whole warp.
+__device__ __forceinline__ void umma_ts_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -292,9 +323,23 @@ __device__ __forceinline__ void umma_ss_mx8(uint32_t d_tmem, uint64_t a_desc, ui
 // word, one byte for each of four products along K, at (r % 32) * 16 +
 // (r / 32) * 4) to 4 TMEM columns, repeated in all four lane quarters: row r
 // at lane r % 32 of column r / 32, as the block-scaled products read them.
-// Ordered before the products this thread issues afterwards.
+// Ordered before the products the elected lane issues afterwards.
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}\n" ::"r"(taddr),
+      "l"(desc)
+      : "memory");
+}
+
+// umma_commit of the products (and scale copies) the elected lane has issued.
+__device__ __forceinline__ void umma_commit_warp(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
+      : "memory");
 }
 
 // Arrive once on an mbarrier when all previously issued MMAs of this thread

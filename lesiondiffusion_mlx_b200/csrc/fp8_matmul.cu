@@ -13,8 +13,8 @@
 //
 // One CTA per SM walks 128-row x BN-column tiles: warp 0 loads the code tiles
 // (TMA, 128-byte swizzle), warp 2 writes the scale words of each four blocks in
-// the order that tcgen05.cp spreads over TMEM lanes, one thread of warp 1 issues
-// scale copies and products, warps 4-7 drain the accumulator of one tile while
+// the order that tcgen05.cp spreads over TMEM lanes, warp 1 issues scale
+// copies and products, warps 4-7 drain the accumulator of one tile while
 // the next is computed in the other.  Grids with fewer tiles than SMs cut K into
 // ranges whose FP32 partial sums a second kernel adds in order.
 
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
-    if (lane == 0) {
+    {
       // Scale words in TMEM: a set of columns per ring slot, behind the two accumulators.
       const int sfb_cols = 4 * ((p.bn + 127) / 128);
       const uint32_t sf_cols = 4 + sfb_cols;
@@ -235,11 +235,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++tile) {
         const Work w = work_item(p, i, kblocks);
         const uint32_t acc = tmem + (tile & 1) * p.bn;
-        ok = mbar_wait(&acc_empty[tile & 1], (static_cast<uint32_t>(tile >> 1) & 1u) ^ 1u, abort_flag, status);
+        ok = warp_wait(&acc_empty[tile & 1], (static_cast<uint32_t>(tile >> 1) & 1u) ^ 1u, abort_flag, status);
         if (!ok) break;
         tc_fence_after();
         for (int kb = w.kb0; ok && kb < w.kb1; kb += 4) {
-          if (!mbar_wait(&sf_full[sst], sph, abort_flag, status)) {
+          if (!warp_wait(&sf_full[sst], sph, abort_flag, status)) {
             ok = false;
             break;
           }
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_copy_scales(sfb + 4 * c, make_smem_desc(s_addr + 512 + 512 * c, 0, 128, kSwizzleNone));
           const int kend = min(w.kb1, kb + 4);
           for (int b = kb; b < kend; ++b) {
-            if (!mbar_wait(&full[st], ph, abort_flag, status)) {
+            if (!warp_wait(&full[st], ph, abort_flag, status)) {
               ok = false;
               break;
             }
@@ -265,23 +265,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               umma_ss_mx8(acc, make_smem_desc(a_addr + q * 32, 16, 1024, kSwizzle128),
                           make_smem_desc(w_addr + q * 32, 16, 1024, kSwizzle128), idesc, sfa, sfb,
                           (b > w.kb0 || q > 0) ? 1u : 0u);
-            umma_commit(&empty[st]);
+            umma_commit_warp(&empty[st]);
             if (++st == p.stages) {
               st = 0;
               ph ^= 1u;
             }
           }
-          umma_commit(&sf_empty[sst]);  // the copy and the products have read this slot
+          umma_commit_warp(&sf_empty[sst]);  // the copy and the products have read this slot
           if (++sst == kScaleStages) {
             sst = 0;
             sph ^= 1u;
           }
         }
-        if (ok) umma_commit(&acc_full[tile & 1]);
+        if (ok) umma_commit_warp(&acc_full[tile & 1]);
       }
       if (*abort_flag) {
         volatile int never = 0;
-        umma_commit(drain);
+        umma_commit_warp(drain);
         mbar_wait(drain, 0, &never, status);
       }
     }

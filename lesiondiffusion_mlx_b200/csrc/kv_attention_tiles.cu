@@ -47,7 +47,6 @@ struct Cfg {
   static constexpr int kPartBytes = kM * D;  // one part of a query tile
   static constexpr int kRawBytes = kN * D;   // codes of a block of K or V
   static constexpr int kSubD = D == 32 ? 32 : 64;  // channels of one f16 value tile
-  static constexpr int kSubs = D / kSubD;
   static constexpr int kSubRow = kSubD * 2;
   static constexpr uint32_t kVLayout = kSubD == 64 ? kSwizzle128 : kSwizzle64;
   static constexpr int kV16Bytes = kN * D * 2;
@@ -88,17 +87,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
-}
-
-// D[tmem] (+)= A[smem] B[smem]^T of e4m3 operands, f32 accumulator.
-__device__ __forceinline__ void umma_ss_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                           uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
 }
 
 // The CTA's share of the work.
@@ -253,9 +241,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 1) {
       // --------------------------------------------------------- products
-      if (lane == 0 && sp.nblocks > 0) {
+      if (sp.nblocks > 0) {
         constexpr uint32_t idesc_qk = (1u << 4) | (kN >> 3 << 17) | (kM >> 4 << 24);  // e4m3 x e4m3 -> f32
-        constexpr uint32_t idesc_pv = make_idesc_f16(kM, C::kSubD, 0u, 0u, 1u);
+        constexpr uint32_t idesc_pv = make_idesc_f16(kM, D, 0u, 0u, 1u);
         auto scores = [&](int t, int j) {
           const uint32_t k_addr = smem_u32(smem + C::kOffK + (j & 1) * C::kRawBytes);
 #pragma unroll
@@ -266,38 +254,35 @@ __global__ void __launch_bounds__(kThreads, 1)
               umma_ss_f8(tmem + t * 128, make_smem_desc(q_addr + k * 32, 16, 8 * D, C::kLayout),
                          make_smem_desc(k_addr + k * 32, 16, 8 * D, C::kLayout), idesc_qk, (part > 0 || k > 0) ? 1u : 0u);
           }
-          umma_commit(&s_full[t]);
+          umma_commit_warp(&s_full[t]);
         };
         auto values = [&](int t, int j) {
           const uint32_t v_addr = smem_u32(smem + C::kOffV16 + (j & 1) * C::kV16Bytes);
           const uint32_t p_tmem = C::kSeparateP ? tmem + 256 + t * 128 + 64 : tmem + t * 128;
 #pragma unroll
-          for (int sub = 0; sub < C::kSubs; ++sub)
-#pragma unroll
-            for (int k = 0; k < kN / 16; ++k)
-              umma_ts(tmem + 256 + t * 128 + sub * C::kSubD, p_tmem + k * 8,
-                      make_smem_desc(v_addr + sub * kN * C::kSubRow + k * 16 * C::kSubRow, 128 * C::kSubRow,
-                                     8 * C::kSubRow, C::kVLayout),
-                      idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
-          umma_commit(&pv_done[t]);
+          for (int k = 0; k < kN / 16; ++k)  // (value tiles of 64 channels lie kN rows apart)
+            umma_ts_warp(tmem + 256 + t * 128, p_tmem + k * 8,
+                         make_smem_desc(v_addr + k * 16 * C::kSubRow, kN * C::kSubRow, 8 * C::kSubRow, C::kVLayout),
+                         idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+          umma_commit_warp(&pv_done[t]);
         };
-        bool ok = mbar_wait(q_full, 0, abort_flag, status);
+        bool ok = warp_wait(q_full, 0, abort_flag, status);
         for (int j = 0; ok && j <= sp.nblocks; ++j) {
           const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u, was = static_cast<uint32_t>(j - 1) & 1u;
-          if (j < sp.nblocks) ok = mbar_wait(&k_full[j & 1], ph, abort_flag, status);
+          if (j < sp.nblocks) ok = warp_wait(&k_full[j & 1], ph, abort_flag, status);
           if (ok && j > 0)
-            ok = mbar_wait(&v16_full[(j - 1) & 1], static_cast<uint32_t>((j - 1) >> 1) & 1u, abort_flag, status);
+            ok = warp_wait(&v16_full[(j - 1) & 1], static_cast<uint32_t>((j - 1) >> 1) & 1u, abort_flag, status);
           if constexpr (C::kSeparateP) {
             for (int t = 0; ok && j < sp.nblocks && t < sp.tiles; ++t) {
               // the softmax has the scores of the block before in registers
-              if (j > 0) ok = mbar_wait(&s_free[t], was, abort_flag, status);
+              if (j > 0) ok = warp_wait(&s_free[t], was, abort_flag, status);
               if (!ok) break;
               tc_fence_after();
               scores(t, j);
             }
-            if (ok && j < sp.nblocks) umma_commit(&k_empty[j & 1]);
+            if (ok && j < sp.nblocks) umma_commit_warp(&k_empty[j & 1]);
             for (int t = 0; ok && j > 0 && t < sp.tiles; ++t) {
-              ok = mbar_wait(&p_ready[t], was, abort_flag, status);
+              ok = warp_wait(&p_ready[t], was, abort_flag, status);
               if (!ok) break;
               tc_fence_after();
               values(t, j - 1);
@@ -305,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             for (int t = 0; ok && t < sp.tiles; ++t) {
               if (j > 0) {
-                ok = mbar_wait(&p_ready[t], was, abort_flag, status);
+                ok = warp_wait(&p_ready[t], was, abort_flag, status);
                 if (!ok) break;
                 tc_fence_after();
                 values(t, j - 1);
@@ -315,18 +300,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 scores(t, j);
               }
             }
-            if (ok && j < sp.nblocks) umma_commit(&k_empty[j & 1]);
+            if (ok && j < sp.nblocks) umma_commit_warp(&k_empty[j & 1]);
           }
-          if (ok && j > 0) umma_commit(&v16_empty[(j - 1) & 1]);
+          if (ok && j > 0) umma_commit_warp(&v16_empty[(j - 1) & 1]);
         }
-        umma_commit(drain);
+        umma_commit_warp(drain);
         volatile int never = 0;
         mbar_wait(drain, 0, &never, status);
       }
     } else {
       // -------------------------------------------------- values to f16
       const int tid = threadIdx.x - 64;
-      constexpr int kUnits = D / 16;  // 16-byte units of a token
+      constexpr int kUnits = D / 16;      // 16-byte units of a token
+      constexpr int kStep = 64 / kUnits;  // tokens of a round (a multiple of eight: one swizzle pattern for all rounds)
+      // 16 channels are two units of a f16 row; lanes of the second value tile
+      // write theirs in the other order (the same banks otherwise).
+      const int tok0 = tid / kUnits, chunk = tid % kUnits, sub = chunk * 16 / C::kSubD;
+      const bool swap = sub & 1;
+      const int at_raw = swizzle_offset(tid * 16, D);
+      const int at_out = tok0 * C::kSubRow + (chunk * 32) % C::kSubRow;
+      const int at_first = sub * kN * C::kSubRow + swizzle_offset(at_out + (swap ? 16 : 0), C::kSubRow);
+      const int at_second = sub * kN * C::kSubRow + swizzle_offset(at_out + (swap ? 0 : 16), C::kSubRow);
       bool ok = true;
       for (int j = 0; ok && j < sp.nblocks; ++j) {
         const int st = j & 1;
@@ -352,23 +346,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) s_bad[st * 4 + h] = bad[h];
           }
         }
-#pragma unroll 4
-        for (int u = tid; u < kN * kUnits; u += 64) {
-          const int tok = u / kUnits, chunk = u % kUnits;
-          uint4 w = *reinterpret_cast<const uint4*>(raw + swizzle_offset(u * 16, D));
+        // unit tid + 64 n: the same channels of every kStep-th token
+        auto convert = [&](int n, uint4 w) {
           if (masked) {
+            const int tok = tok0 + n * kStep;
             const uint32_t word = tok < 64 ? (tok < 32 ? bad[0] : bad[1]) : (tok < 96 ? bad[2] : bad[3]);
             if (j0 + tok >= sp.len || ((word >> (tok & 31)) & 1u)) w = make_uint4(0, 0, 0, 0);
           }
           const uint4 lo = make_uint4(fp8_unpack2(w.x), fp8_unpack2(w.x >> 16), fp8_unpack2(w.y), fp8_unpack2(w.y >> 16));
           const uint4 hi = make_uint4(fp8_unpack2(w.z), fp8_unpack2(w.z >> 16), fp8_unpack2(w.w), fp8_unpack2(w.w >> 16));
-          // channels 16 chunk .. + 15: two units of a f16 row; the second value tile's lanes
-          // write theirs in the other order (the same banks otherwise)
-          const int sub = chunk * 16 / C::kSubD, at = tok * C::kSubRow + (chunk * 32) % C::kSubRow;
-          uint8_t* dst = out + sub * kN * C::kSubRow;
-          const bool swap = sub & 1;
-          *reinterpret_cast<uint4*>(dst + swizzle_offset(at + (swap ? 16 : 0), C::kSubRow)) = swap ? hi : lo;
-          *reinterpret_cast<uint4*>(dst + swizzle_offset(at + (swap ? 0 : 16), C::kSubRow)) = swap ? lo : hi;
+          *reinterpret_cast<uint4*>(out + n * kStep * C::kSubRow + at_first) = swap ? hi : lo;
+          *reinterpret_cast<uint4*>(out + n * kStep * C::kSubRow + at_second) = swap ? lo : hi;
+        };
+#pragma unroll
+        for (int n0 = 0; n0 < kN / kStep; n0 += 4) {
+          uint4 w[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) w[n] = *reinterpret_cast<const uint4*>(raw + (n0 + n) * kStep * D + at_raw);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) convert(n0 + n, w[n]);
         }
         fence_proxy_async_smem();
         mbar_arrive(&v16_full[st]);
