@@ -136,12 +136,17 @@ def library() -> ctypes.CDLL:
         return _lib
 
 
+_functions: dict[str, object] = {}
+
+
 def call(name: str, *args) -> int:
     """Invoke ``name`` and raise ``LdbError`` on a negative status."""
-    lib = library()
-    rc = getattr(lib, name)(*args)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(library(), name)
+    rc = fn(*args)
     if rc < 0:
-        raise LdbError(name, rc, lib.ldb_last_error().decode(errors="replace"))
+        raise LdbError(name, rc, library().ldb_last_error().decode(errors="replace"))
     return rc
 
 

@@ -14,8 +14,9 @@
 // One CTA per SM walks 128-row x BN-column tiles: warp 0 loads the code tiles
 // (TMA, 128-byte swizzle), warp 2 writes the scale words of each four blocks in
 // the order that tcgen05.cp spreads over TMEM lanes, warp 1 issues scale
-// copies and products, warps 4-7 drain the accumulator of one tile while
-// the next is computed in the other.  Grids with fewer tiles than SMs cut K into
+// copies and products, warps 4-11 drain the accumulator of one tile while
+// the next is computed in the other (two warps per 32 rows, alternating 32-column chunks,
+// staged in shared memory for TMA stores where the output allows them).  Grids with fewer tiles than SMs cut K into
 // ranges whose FP32 partial sums a second kernel adds in order.
 
 #include <algorithm>
@@ -26,13 +27,15 @@
 namespace ldb {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = (4 + kEpilogueWarps) * 32;
 constexpr int kTileM = 128;
 constexpr int kMaxStages = 8;
 constexpr int kScaleStages = 4;                // ring of scale groups in shared memory
 constexpr int kScaleBytes = 512 + 1024;        // A words, then up to 256 B words
 constexpr int kMaxBn = 224;
-constexpr int kSmemBudget = 200 * 1024;        // code stages
+constexpr int kStagingBytes = 4096;            // per epilogue warp: 32 x 32 outputs, twice for 16-bit ones
+constexpr int kSmemBudget = 184 * 1024;        // code stages
 constexpr int kTmemCols = 512;
 static_assert(2 * kMaxBn + kScaleStages * 12 <= kTmemCols, "two accumulators and the scale sets");
 
@@ -48,7 +51,8 @@ struct MatmulParams {
   int bn, stages, box_m;
   int tiles_m, tiles_n, split, kb_per_split;
   int act, out_dtype;
-  int vec;  // out, residual and partial rows allow 16-byte accesses
+  int vec;       // out and residual rows allow 16-byte accesses and TMA stores
+  int bias_vec;  // so does the bias
 };
 
 // Scale words of tile row `row` (128-channel blocks kb .. kb + 3) of A; blocks
@@ -88,18 +92,71 @@ __device__ __forceinline__ Work work_item(const MatmulParams& p, int i, int kblo
   return w;
 }
 
-// 32 columns of one output row: bias, residual, activation, one rounding.
+// Paired FP32 arithmetic (sm_100 f32x2 instructions).
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
+
+// 0.5 y (1 + erf(y / sqrt 2)) of two values, as max(y, 0) - 0.5 |y| erfc(|y| /
+// sqrt 2), which does not cancel, with erfc by formula 7.1.26 of Abramowitz and Stegun
+// (error at most 1.5e-7): ten operations a value.  With erff, and one warp per
+// 32 rows, the epilogue of a short K took twice the time of everything else.
+__device__ __forceinline__ void gelu2(float& y0, float& y1) {
+  const uint64_t a = pack2(fabsf(y0), fabsf(y1));
+  const uint64_t z = mul2(a, both(0.70710678118654752f));
+  float d0, d1, e0, e1;
+  unpack2(fma2(z, both(0.3275911f), both(1.f)), d0, d1);
+  const uint64_t t = pack2(rcp_approx(d0), rcp_approx(d1));
+  uint64_t q = fma2(both(1.061405429f), t, both(-1.453152027f));
+  q = fma2(q, t, both(1.421413741f));
+  q = fma2(q, t, both(-0.284496736f));
+  q = fma2(q, t, both(0.254829592f));
+  unpack2(mul2(mul2(z, z), both(-1.4426950408889634f)), e0, e1);
+  q = mul2(mul2(q, t), pack2(ex2_approx(e0), ex2_approx(e1)));  // erfc(z)
+  unpack2(fma2(mul2(a, both(-0.5f)), q, pack2(fmaxf(y0, 0.f), fmaxf(y1, 0.f))), y0, y1);
+}
+__device__ __forceinline__ float gelu1(float y) {
+  float other = 0.f;
+  gelu2(y, other);
+  return y;
+}
+
+// 32 columns of one output row before the rounding: bias, residual, activation.
 template <typename T>
 __device__ __forceinline__ void finish32(const MatmulParams& p, int row, int col, float (&v)[32]) {
-  const bool full = p.vec && col + 32 <= p.n;
+  const bool full = col + 32 <= p.n;
   if (p.bias) {
+    if (full && p.bias_vec) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (full || col + j < p.n) v[j] += p.bias[col + j];
+      for (int j = 0; j < 8; ++j) {
+        const float4 b = reinterpret_cast<const float4*>(p.bias + col)[j];
+        v[4 * j] += b.x, v[4 * j + 1] += b.y, v[4 * j + 2] += b.z, v[4 * j + 3] += b.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col + j < p.n) v[j] += p.bias[col + j];
+    }
   }
-  if (p.residual) {
+  if (p.residual && row < p.m) {
     const T* r = static_cast<const T*>(p.residual) + row * p.res_ld + col;
-    if (full) {
+    if (full && p.vec) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         float a[8];
@@ -108,39 +165,27 @@ __device__ __forceinline__ void finish32(const MatmulParams& p, int row, int col
         for (int j = 0; j < 8; ++j) v[8 * c + j] += a[j];
       }
     } else {
+#pragma unroll
       for (int j = 0; j < 32; ++j)
         if (col + j < p.n) v[j] += to_f32<T>(r[j]);
     }
   }
   if (p.act == LDB_ACT_GELU) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = gelu_erf_f32(v[j]);
-  }
-  T* o = static_cast<T*>(p.out) + row * p.out_ld + col;
-  if (full) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      float a[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] = v[8 * c + j];
-      store8<T>(o + 8 * c, a);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col + j < p.n) o[j] = from_f32<T>(v[j]);
+    for (int j = 0; j < 32; j += 2) gelu2(v[j], v[j + 1]);
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_matmul_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap wmap,
-                      const MatmulParams p, unsigned int* status) {
+                      const __grid_constant__ CUtensorMap omap, const MatmulParams p, unsigned int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stage_bytes = kTileM * 128 + p.bn * 128;
   uint8_t* s_scales = smem + p.stages * stage_bytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_scales + kScaleStages * kScaleBytes);
+  uint8_t* s_out = s_scales + kScaleStages * kScaleBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_out + kEpilogueWarps * kStagingBytes);
   uint64_t* full = bars;                       // [kMaxStages] codes have landed
   uint64_t* empty = full + kMaxStages;         // [kMaxStages] the products have read them
   uint64_t* sf_full = empty + kMaxStages;      // [kScaleStages] scale words are written
@@ -167,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&acc_full[t], 1);
-      mbar_init(&acc_empty[t], 4);
+      mbar_init(&acc_empty[t], kEpilogueWarps);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -316,45 +361,76 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------- epilogue
-    int tile = 0;
+    constexpr int kRowBytes = 32 * sizeof(T);            // of a staged chunk
+    constexpr int kBuffers = kStagingBytes / (32 * kRowBytes);
+    uint8_t* staging = s_out + (warp - 4) * kStagingBytes;
+    const int quarter = warp & 3;
+    const bool staged = p.vec && p.split == 1;
+    int tile = 0, buffer = 0;
     for (int i = blockIdx.x; i < items; i += gridDim.x, ++tile) {
       const Work w = work_item(p, i, kblocks);
       if (!warp_wait(&acc_full[tile & 1], static_cast<uint32_t>(tile >> 1) & 1u, abort_flag, status)) break;
       tc_fence_after();
-      const int quarter = warp & 3;
-      const int row = w.row0 + quarter * 32 + lane;
+      const int row0 = w.row0 + quarter * 32, row = row0 + lane;
       const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (tile & 1) * p.bn;
-      const int cols = min(p.bn, p.n - w.col0);
-      if (w.row0 + quarter * 32 < p.m) {
-        for (int c = 0; c < cols; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(acc + c, r);
-          tmem_wait_ld();
-          float v[32];
+      const int cols = row0 < p.m ? min(p.bn, p.n - w.col0) : 0;
+      for (int c = 32 * ((warp - 4) >> 2); c < cols; c += 64) {
+        uint32_t r[32];
+        tmem_ld32(acc + c, r);
+        tmem_wait_ld();
+        float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        const int col = w.col0 + c;
+        if (p.split > 1) {
           if (row < p.m) {
-            if (p.split == 1) {
-              finish32<T>(p, row, w.col0 + c, v);
+            float* o = p.partial + (static_cast<long long>(w.split) * p.m + row) * p.n + col;
+            if (p.n % 4 == 0 && col + 32 <= p.n) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                reinterpret_cast<float4*>(o)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             } else {
-              float* o = p.partial + (static_cast<long long>(w.split) * p.m + row) * p.n + w.col0 + c;
-              if (p.n % 4 == 0 && w.col0 + c + 32 <= p.n) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  reinterpret_cast<float4*>(o)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (w.col0 + c + j < p.n) o[j] = v[j];
-              }
+              for (int j = 0; j < 32; ++j)
+                if (col + j < p.n) o[j] = v[j];
             }
           }
+          continue;
+        }
+        finish32<T>(p, row, col, v);
+        if (staged) {
+          // the store before last (16-bit) or last (FP32) has read this buffer
+          uint8_t* out = staging + buffer * 32 * kRowBytes;
+          if (lane == 0) bulk_wait_group_read<kBuffers - 1>();
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < kRowBytes / 16; ++h) {
+            constexpr int kPer = 16 / sizeof(T);
+            uint4 packed;
+            T* e = reinterpret_cast<T*>(&packed);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) e[j] = from_f32<T>(v[h * kPer + j]);
+            *reinterpret_cast<uint4*>(out + swizzle_offset(lane * kRowBytes + h * 16, kRowBytes)) = packed;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&omap, out, col, row0);  // rows and columns outside the output are left out
+            bulk_commit_group();
+          }
+          if (++buffer == kBuffers) buffer = 0;
+        } else if (row < p.m) {
+          T* o = static_cast<T*>(p.out) + row * p.out_ld + col;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (col + j < p.n) o[j] = from_f32<T>(v[j]);
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[tile & 1]);
     }
+    if (lane == 0) bulk_wait_group_all();
   }
   __syncwarp();
   tc_fence_before();
@@ -375,7 +451,7 @@ __global__ void __launch_bounds__(256) fp8_matmul_reduce_kernel(const MatmulPara
     for (int s = 0; s < p.split; ++s) v += p.partial[s * total + i];
     if (p.bias) v += p.bias[col];
     if (p.residual) v += to_f32<T>(static_cast<const T*>(p.residual)[row * p.res_ld + col]);
-    if (p.act == LDB_ACT_GELU) v = gelu_erf_f32(v);
+    if (p.act == LDB_ACT_GELU) v = gelu1(v);
     static_cast<T*>(p.out)[row * p.out_ld + col] = from_f32<T>(v);
   }
 }
@@ -387,29 +463,33 @@ int plan(int m, int n, int k, MatmulParams* p) {
   const int kblocks = (k + kFp8Block - 1) / kFp8Block;
   p->m = m, p->n = n, p->k = k;
   p->tiles_m = (m + kTileM - 1) / kTileM;
-  // Cycles of a CTA that walks `waves` tiles: a K block costs the products
-  // (2 cycles a column), not less than its loads; each tile a fixed start.
+  // Cycles of a CTA that walks `waves` tiles.  A K block moves 128 rows of A and
+  // bn of the weight through shared memory twice (in, and out to the tensor
+  // core) at 128 bytes a cycle; the epilogue takes 12 to 24 cycles a column (GELU) and
+  // runs beside the next tile's products.  K ranges (few tiles, long K; cut at
+  // groups of four blocks) cost the second kernel, most of it on the host.
   long long best = -1;
+  const int groups = (kblocks + 3) / 4;
   for (const int bn : {32, 64, 96, 128, 160, 192, kMaxBn}) {
-    const long long tiles = static_cast<long long>(p->tiles_m) * ((n + bn - 1) / bn);
-    const long long waves = (tiles + sms - 1) / sms;
-    const long long cost = waves * (static_cast<long long>(kblocks) * std::max(2 * bn, 160) + 1000);
+    const int tiles_n = (n + bn - 1) / bn;
+    const long long tiles = static_cast<long long>(p->tiles_m) * tiles_n;
+    int split = 1;
+    if (tiles * 2 <= sms && kblocks >= 8) split = std::max(1, std::min({static_cast<int>(sms / tiles), groups, 16}));
+    const int per = 4 * ((groups + split - 1) / split);
+    split = (kblocks + per - 1) / per;
+    const long long waves = (tiles * split + sms - 1) / sms;
+    const long long main = static_cast<long long>(std::min(per, kblocks)) * (256 + 2 * bn);
+    const long long cost =
+        waves * (std::max<long long>(main, 16 * bn) + 1000) + (split > 1 ? 6000 : 0);
     if (best < 0 || cost < best) {
       best = cost;
       p->bn = bn;
+      p->tiles_n = tiles_n;
+      p->split = split;
+      p->kb_per_split = per;
     }
   }
-  p->tiles_n = (n + p->bn - 1) / p->bn;
   const long long tiles = static_cast<long long>(p->tiles_m) * p->tiles_n;
-  p->split = 1;
-  if (tiles * 2 <= sms && kblocks >= 8) {
-    // K ranges of at least four blocks (one scale group), cut at groups
-    const int groups = (kblocks + 3) / 4;
-    p->split = std::max(1, std::min({static_cast<int>(sms / tiles), groups, 16}));
-  }
-  const int groups = (kblocks + 3) / 4;
-  p->kb_per_split = 4 * ((groups + p->split - 1) / p->split);
-  p->split = (kblocks + p->kb_per_split - 1) / p->kb_per_split;
   p->stages = std::min(kMaxStages, kSmemBudget / (kTileM * 128 + p->bn * 128));
   p->box_m = std::min(kTileM, (m + 7) / 8 * 8);
   if (tiles * p->split > 0x7FFFFFFF) return fail(LDB_ERR_SHAPE, "matmul_fp8: too many tiles");
@@ -424,14 +504,28 @@ template <typename T>
 int launch(cudaStream_t stream, const CUtensorMap& amap, const CUtensorMap& wmap, const MatmulParams& p,
            unsigned int* status) {
   static unsigned long long configured = 0;
-  const int smem = 1024 + p.stages * (kTileM + p.bn) * 128 + kScaleStages * kScaleBytes + 512;
-  int rc = ensure_smem_attribute(reinterpret_cast<const void*>(fp8_matmul_kernel<T>),
-                                 1024 + kSmemBudget + kScaleStages * kScaleBytes + 512, &configured,
+  constexpr int kFixed = 1024 + kScaleStages * kScaleBytes + kEpilogueWarps * kStagingBytes + 512;
+  static_assert(kFixed + kSmemBudget <= 232448, "shared memory");
+  const int smem = kFixed + p.stages * (kTileM + p.bn) * 128;
+  CUtensorMap omap = amap;  // (not used without TMA stores)
+  int rc = LDB_OK;
+  if (p.vec && p.split == 1) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(p.n), static_cast<uint64_t>(p.m)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(p.out_ld) * sizeof(T)};
+    const uint32_t box[2] = {32, 32};
+    if (sizeof(T) == 4) {
+      rc = encode_tiled_f32(&omap, p.out, 2, dims, strides, box, 128);
+    } else {
+      rc = encode_tiled_f16(&omap, p.out, 2, dims, strides, box, 64, p.out_dtype == LDB_BF16);
+    }
+    if (rc != LDB_OK) return rc;
+  }
+  rc = ensure_smem_attribute(reinterpret_cast<const void*>(fp8_matmul_kernel<T>), kFixed + kSmemBudget, &configured,
                                  "matmul_fp8 shared memory");
   if (rc != LDB_OK) return rc;
   const int items = p.tiles_m * p.tiles_n * p.split;
   rc = launch_kernel(fp8_matmul_kernel<T>, dim3(std::min(items, sm_count())), dim3(kThreads), smem, stream,
-                     "matmul_fp8 launch", amap, wmap, p, status);
+                     "matmul_fp8 launch", amap, wmap, omap, p, status);
   if (rc != LDB_OK || p.split == 1) return rc;
   const long long total = static_cast<long long>(p.m) * p.n;
   const int blocks = static_cast<int>(std::min<long long>((total + 255) / 256, 4ll * sm_count()));
@@ -487,6 +581,7 @@ int ldb_matmul_fp8(cudaStream_t stream, const uint8_t* a, long long a_ld, const 
   const int es = out_dtype == LDB_F32 ? 4 : 2;
   p.vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_ld * es % 16 == 0 &&
           (!residual || (reinterpret_cast<uintptr_t>(residual) % 16 == 0 && residual_ld * es % 16 == 0));
+  p.bias_vec = reinterpret_cast<uintptr_t>(bias) % 16 == 0;
   CUtensorMap amap, wmap;
   const uint64_t adims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(m)};
   const uint64_t wdims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n)};

@@ -11,7 +11,7 @@
 // sum of squares and the rounding, 8 consecutive channels a lane, so that 16
 // lanes hold the 128 channels of a scale and find its maximum with four
 // shuffles.  Rows of up to 1024 channels take one warp (no barrier), wider rows
-// a block; the grid is resident and walks the rows, keeping gamma in registers.
+// a block; the grid is resident and walks the rows.
 
 #include <algorithm>
 
@@ -80,7 +80,7 @@ __device__ __forceinline__ void quantize_block(float (&y)[8], bool live, bool fi
 
 // WARPS warps per row (1: eight rows per 256-thread block), ITERS x 8 channels a lane.
 template <typename T, int WARPS, int ITERS, bool NORM>
-__global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) fp8_rows_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32, WARPS == 32 ? 1 : 4) fp8_rows_kernel(const RowsParams p) {
   __shared__ float s_part[WARPS == 1 ? 1 : WARPS];
   constexpr int kLanes = WARPS * 32;
   const int t = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
@@ -88,19 +88,13 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) fp8_rows_kernel
   const int first_row = blockIdx.x * per_block + (WARPS == 1 ? threadIdx.x >> 5 : 0);
   const int step = gridDim.x * per_block;
 
-  // gamma is a weight, not the previous kernel's output: read before the wait
-  // (the widest rows have no registers to keep it in and read it for each row).
-  constexpr bool kKeepGamma = NORM && WARPS < 32;
-  auto gamma_at = [&](int i, int j) {
-    const int c = (i * kLanes + t) * 8 + j;
-    return p.gamma && c < p.channels ? p.gamma[c] : 1.f;
-  };
-  float g[ITERS][8];
-  if constexpr (kKeepGamma) {
-#pragma unroll
-    for (int i = 0; i < ITERS; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) g[i][j] = gamma_at(i, j);
+  // gamma is a weight, not the previous kernel's output: staged in shared
+  // memory before the wait (in registers it took a third of them, and half the warps).
+  extern __shared__ float s_gamma[];
+  if constexpr (NORM) {
+    for (int c = threadIdx.x; c < ITERS * kLanes * 8; c += blockDim.x)
+      s_gamma[c] = p.gamma && c < p.channels ? p.gamma[c] : 1.f;
+    __syncthreads();
   }
   pdl_begin();
   for (int row = first_row; row < p.rows; row += step) {
@@ -163,9 +157,12 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) fp8_rows_kernel
       }
       const float rstd = rsqrtf(sum / static_cast<float>(p.channels) + p.eps);
 #pragma unroll
-      for (int i = 0; i < ITERS; ++i)
+      for (int i = 0; i < ITERS; ++i) {
+        float g[8];
+        load8<float>(s_gamma + (i * kLanes + t) * 8, g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rstd * (kKeepGamma ? g[i][j] : gamma_at(i, j));
+        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rstd * g[j];
+      }
     }
 #pragma unroll
     for (int i = 0; i < ITERS; ++i) {
@@ -182,19 +179,26 @@ int launch_rows(cudaStream_t stream, const RowsParams& p, const char* what) {
   const int c = p.channels;
   // Blocks resident at once: 64 registers a thread allow four 256-thread blocks
   // per SM; rows beyond them are walked by the same blocks.
+  auto smem = [](int lanes, int iters) { return NORM ? static_cast<size_t>(lanes) * iters * 8 * sizeof(float) : 0; };
   if (c <= 1024) {
     const int blocks = std::min((p.rows + 7) / 8, sms * 4);
-    auto k = c <= 256 ? fp8_rows_kernel<T, 1, 1, NORM>
-                      : (c <= 512 ? fp8_rows_kernel<T, 1, 2, NORM> : fp8_rows_kernel<T, 1, 4, NORM>);
-    return launch_kernel(k, dim3(blocks), dim3(256), 0, stream, what, p);
+    const int iters = c <= 256 ? 1 : (c <= 512 ? 2 : 4);
+    auto k = iters == 1 ? fp8_rows_kernel<T, 1, 1, NORM>
+                        : (iters == 2 ? fp8_rows_kernel<T, 1, 2, NORM> : fp8_rows_kernel<T, 1, 4, NORM>);
+    return launch_kernel(k, dim3(blocks), dim3(256), smem(32, iters), stream, what, p);
   }
   if (c <= 8192) {
     const int blocks = std::min(p.rows, sms * 4);
-    auto k = c <= 2048 ? fp8_rows_kernel<T, 8, 1, NORM>
-                       : (c <= 4096 ? fp8_rows_kernel<T, 8, 2, NORM> : fp8_rows_kernel<T, 8, 4, NORM>);
-    return launch_kernel(k, dim3(blocks), dim3(256), 0, stream, what, p);
+    const int iters = c <= 2048 ? 1 : (c <= 4096 ? 2 : 4);
+    auto k = iters == 1 ? fp8_rows_kernel<T, 8, 1, NORM>
+                        : (iters == 2 ? fp8_rows_kernel<T, 8, 2, NORM> : fp8_rows_kernel<T, 8, 4, NORM>);
+    return launch_kernel(k, dim3(blocks), dim3(256), smem(256, iters), stream, what, p);
   }
-  return launch_kernel(fp8_rows_kernel<T, 32, 4, NORM>, dim3(std::min(p.rows, sms)), dim3(1024), 0, stream, what, p);
+  static unsigned long long configured = 0;
+  auto k = fp8_rows_kernel<T, 32, 4, NORM>;
+  const int rc = ensure_smem_attribute(reinterpret_cast<const void*>(k), static_cast<int>(smem(1024, 4)), &configured, what);
+  if (rc != LDB_OK) return rc;
+  return launch_kernel(k, dim3(std::min(p.rows, sms)), dim3(1024), smem(1024, 4), stream, what, p);
 }
 
 int esize(int dtype) { return dtype == LDB_F32 ? 4 : 2; }

@@ -33,7 +33,7 @@ struct AppendParams {
 };
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendVecs = 128 * 128 / 8 / kAppendThreads;  // of the largest page, per thread
+constexpr int kMaxVecs = 128 * 128 / 8 / kAppendThreads;  // vectors of eight per thread, of the largest page
 
 __device__ __forceinline__ float block_max(float v, float* s_part) {
 #pragma unroll
@@ -47,8 +47,12 @@ __device__ __forceinline__ float block_max(float v, float* s_part) {
   return v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p, unsigned int* status) {
+// VECS: vectors of eight values per thread that a whole page takes.  The
+// values stay as they came (four registers a vector in 16 bits) until they
+// are rounded, so that enough blocks are resident to cover the chain of
+// dependent reads (position, page number, values).
+template <typename T, int VECS>
+__global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) == 4 ? 3 : 6) kv_append_kernel(const AppendParams p, unsigned int* status) {
   __shared__ float s_part[kAppendThreads / 32];
   __shared__ int s_old;
   pdl_begin();
@@ -78,23 +82,33 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
   const int vecs = (last - first) << vshift;
 
   if (threadIdx.x == 0) s_old = *scale;
-  float v[kAppendVecs][8];
+  uint4 raw[VECS][sizeof(T) / 2];
   float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < kAppendVecs; ++i) {
+  for (int i = 0; i < VECS; ++i) {
     const int q = i * kAppendThreads + threadIdx.x;
     if (q < vecs) {
       const T* x = src + (first + (q >> vshift)) * p.src_ld[which] + ((q & ((1 << vshift) - 1)) << 3);
       if (p.vec) {
-        load8<T>(x, v[i]);
-      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = to_f32<T>(x[j]);
+        for (int h = 0; h < static_cast<int>(sizeof(T) / 2); ++h) raw[i][h] = reinterpret_cast<const uint4*>(x)[h];
+      } else {
+        T t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = x[j];
+#pragma unroll
+        for (int h = 0; h < static_cast<int>(sizeof(T) / 2); ++h) raw[i][h] = reinterpret_cast<const uint4*>(t)[h];
       }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    if (i * kAppendThreads + static_cast<int>(threadIdx.x) < vecs) {
+      const T* v = reinterpret_cast<const T*>(raw[i]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (!fp8_is_finite(v[i][j])) v[i][j] = fp8_nan();
-        amax = fmaxf(amax, fabsf(v[i][j]));
+        const float a = fabsf(to_f32<T>(v[j]));
+        if (fp8_is_finite(a)) amax = fmaxf(amax, a);
       }
     }
   }
@@ -104,12 +118,19 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
   if (held > 0) e = amax == 0.f ? e_old : max(e, e_old);  // zeros ask for no scale
   const float inv = fp8_pow2(-min(e, 127));
 #pragma unroll
-  for (int i = 0; i < kAppendVecs; ++i) {
+  for (int i = 0; i < VECS; ++i) {
     const int q = i * kAppendThreads + threadIdx.x;
     if (q < vecs) {
+      const T* v = reinterpret_cast<const T*>(raw[i]);
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        y[j] = to_f32<T>(v[j]) * inv;
+        if (!fp8_is_finite(y[j])) y[j] = fp8_nan();
+      }
       uint2 packed;
-      packed.x = fp8_pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-      packed.y = fp8_pack4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+      packed.x = fp8_pack4(y[0], y[1], y[2], y[3]);
+      packed.y = fp8_pack4(y[4], y[5], y[6], y[7]);
       *reinterpret_cast<uint2*>(codes + ((static_cast<long long>(held) << p.dim_shift) + (q << 3))) = packed;
     }
   }
@@ -131,6 +152,14 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
     }
   }
   if (threadIdx.x == 0) *scale = static_cast<uint8_t>(e + 127);
+}
+
+template <typename T>
+int launch_append(cudaStream_t stream, dim3 grid, const AppendParams& p, unsigned int* status) {
+  const int vecs = (p.page * p.dim / 8 + kAppendThreads - 1) / kAppendThreads;
+  auto k = vecs == 1 ? kv_append_kernel<T, 1>
+                     : (vecs == 2 ? kv_append_kernel<T, 2> : (vecs <= 4 ? kv_append_kernel<T, 4> : kv_append_kernel<T, 8>));
+  return launch_kernel(k, grid, dim3(kAppendThreads), 0, stream, "kv_append launch", p, status);
 }
 
 }  // namespace
@@ -178,12 +207,9 @@ int ldb_kv_append_fp8(cudaStream_t stream, const void* k, long long k_ld, long l
   // pages that a run of `tokens` can touch, wherever it starts
   const long long touched = (static_cast<long long>(tokens) + page - 2) / page + 1;
   const dim3 grid(static_cast<unsigned>(touched), batch * kv_heads, 2);
-  const char* what = "kv_append launch";
-  if (dtype == LDB_F16)
-    return launch_kernel(kv_append_kernel<__half>, grid, dim3(kAppendThreads), 0, stream, what, p, status);
-  if (dtype == LDB_BF16)
-    return launch_kernel(kv_append_kernel<__nv_bfloat16>, grid, dim3(kAppendThreads), 0, stream, what, p, status);
-  return launch_kernel(kv_append_kernel<float>, grid, dim3(kAppendThreads), 0, stream, what, p, status);
+  if (dtype == LDB_F16) return launch_append<__half>(stream, grid, p, status);
+  if (dtype == LDB_BF16) return launch_append<__nv_bfloat16>(stream, grid, p, status);
+  return launch_append<float>(stream, grid, p, status);
 }
 
 }  // extern "C"

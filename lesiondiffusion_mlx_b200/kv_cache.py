@@ -17,20 +17,19 @@ the cache is left out and sets the device status (``ldb_device_status``).
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
-from . import _lib, instrument
-from .fp8 import CODES, SCALES
-from .ops import _DT, _ptr, _stream
+from . import _lib
+from .fp8 import CODES, SCALES, _launch, _raw_stream
+from .ops import _DT
 
 HEAD_DIMS = (32, 64, 128)
 PAGES = (16, 32, 64, 128)
 
 
-@dataclass(frozen=True)
-class KvCacheFp8:
+class KvCacheFp8(NamedTuple):
     """Codes ``k``, ``v`` ``(pages, kv_heads, page, head_dim)`` and scales ``(pages, kv_heads)``."""
 
     k: torch.Tensor
@@ -49,23 +48,22 @@ class KvCacheFp8:
         return cls(*codes, *scales)
 
 
-def _check_cache(cache: KvCacheFp8, name: str) -> tuple[int, int, int, int]:
-    shape = cache.k.shape
-    if len(shape) != 4 or cache.v.shape != shape or cache.k.dtype != CODES or cache.v.dtype != CODES:
+def _check_cache(cache: KvCacheFp8, name: str) -> tuple[torch.Size, torch.device]:
+    k, v, k_scale, v_scale = cache
+    shape, device = k.shape, k.device
+    if len(shape) != 4 or v.shape != shape or k.dtype != CODES or v.dtype != CODES:
         raise ValueError(f"{name}: k and v must be float8_e4m3fn (pages, kv_heads, page, head_dim)")
-    pages, heads, page, dim = shape
-    if page not in PAGES or dim not in HEAD_DIMS:
-        raise ValueError(f"{name}: pages hold {PAGES} tokens of {HEAD_DIMS} channels, got {page} of {dim}")
-    if (cache.k_scale.shape != (pages, heads) or cache.v_scale.shape != (pages, heads)
-            or cache.k_scale.dtype != SCALES or cache.v_scale.dtype != SCALES):
-        raise ValueError(f"{name}: scales must be float8_e8m0fnu ({pages}, {heads})")
-    device = cache.k.device
-    if device.type != "cuda":
+    if shape[2] not in PAGES or shape[3] not in HEAD_DIMS:
+        raise ValueError(f"{name}: pages hold {PAGES} tokens of {HEAD_DIMS} channels, got {shape[2]} of {shape[3]}")
+    if (k_scale.shape != shape[:2] or v_scale.shape != shape[:2] or k_scale.dtype != SCALES
+            or v_scale.dtype != SCALES):
+        raise ValueError(f"{name}: scales must be float8_e8m0fnu {tuple(shape[:2])}")
+    if not k.is_cuda:
         raise ValueError(f"{name}: the cache must be on a CUDA device")
-    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
-        if not t.is_contiguous() or t.device != device:
-            raise ValueError(f"{name}: the cache's tensors must be contiguous and on one device")
-    return pages, heads, page, dim
+    if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()
+            and v.device == device and k_scale.device == device and v_scale.device == device):
+        raise ValueError(f"{name}: the cache's tensors must be contiguous and on one device")
+    return shape, device
 
 
 def _check_index(t: torch.Tensor, ndim: int, batch: int, device: torch.device, name: str) -> None:
@@ -75,10 +73,13 @@ def _check_index(t: torch.Tensor, ndim: int, batch: int, device: torch.device, n
         raise ValueError(f"{name} must have unit stride along its last axis")
 
 
-def _table_ld(table: torch.Tensor) -> int:
-    if table.shape[1] == 0:
-        raise ValueError("the page table has no columns")
-    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+def _check_table(table: torch.Tensor, batch: int, device: torch.device, name: str) -> tuple[int, int]:
+    """(columns, row stride) of the page table."""
+    _check_index(table, 2, batch, device, name)
+    width = table.shape[1]
+    if width == 0:
+        raise ValueError(f"{name} has no columns")
+    return width, table.stride(0) if batch > 1 else width
 
 
 def kv_append(cache: KvCacheFp8, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, *,
@@ -90,26 +91,25 @@ def kv_append(cache: KvCacheFp8, k: torch.Tensor, v: torch.Tensor, table: torch.
     grow for the new tokens; anything at or after ``start`` in the touched
     pages counts as unwritten.  Items written together must not share the
     pages they write.  float16, bfloat16 or float32, any row and item stride."""
-    pages, heads, page, dim = _check_cache(cache, "kv_append")
+    (pages, heads, page, dim), device = _check_cache(cache, "kv_append")
     if k.dtype not in _DT or v.dtype != k.dtype:
         raise ValueError("kv_append: k and v must share dtype float16, bfloat16 or float32")
     if k.ndim != 3 or v.shape != k.shape or k.shape[2] != heads * dim:
         raise ValueError(f"kv_append: k and v must be (B, L, {heads * dim}), got {tuple(k.shape)} and {tuple(v.shape)}")
-    device = cache.k.device
     if k.device != device or v.device != device:
         raise ValueError("kv_append: k and v must be on the cache's device")
-    if k.stride(2) != 1 or v.stride(2) != 1:
+    (k_batch, k_ld, k_step), (v_batch, v_ld, v_step) = k.stride(), v.stride()
+    if k_step != 1 or v_step != 1:
         raise ValueError("kv_append: channel axis must have unit stride")
     batch, tokens, _ = k.shape
-    _check_index(table, 2, batch, device, "kv_append: table")
+    width, table_ld = _check_table(table, batch, device, "kv_append: table")
     _check_index(start, 1, batch, device, "kv_append: start")
     if counts is not None:
         _check_index(counts, 1, batch, device, "kv_append: counts")
-    with instrument.maybe_time("kv_append", 0.0):
-        _lib.call("ldb_kv_append_fp8", _stream(k), k.data_ptr(), k.stride(1), k.stride(0), v.data_ptr(), v.stride(1),
-                  v.stride(0), _DT[k.dtype], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-                  cache.v_scale.data_ptr(), pages, heads, page, dim, table.data_ptr(), _table_ld(table),
-                  table.shape[1], start.data_ptr(), _ptr(counts), batch, tokens)
+    _launch("kv_append", 0.0, "ldb_kv_append_fp8", _raw_stream(k.get_device()), k.data_ptr(), k_ld, k_batch,
+            v.data_ptr(), v_ld, v_batch, _DT[k.dtype], cache.k.data_ptr(), cache.v.data_ptr(),
+            cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pages, heads, page, dim, table.data_ptr(), table_ld,
+            width, start.data_ptr(), None if counts is None else counts.data_ptr(), batch, tokens)
 
 
 def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, lengths: torch.Tensor, *, scale: float,
@@ -122,30 +122,32 @@ def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, length
     query ``i`` sees the keys up to ``lengths[b] - L + i``.  A query that sees
     no key gives zeros; a NaN among the keys or values a query does not see
     does not reach it.  float16 or bfloat16, any row and item stride."""
-    pages, kv_heads, page, dim = _check_cache(cache, "kv_attention")
+    (pages, kv_heads, page, dim), device = _check_cache(cache, "kv_attention")
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"kv_attention: queries must be float16 or bfloat16, got {q.dtype}")
-    device = cache.k.device
     if q.ndim != 3 or q.device != device or q.shape[2] % (kv_heads * dim) or q.shape[2] == 0:
         raise ValueError(f"kv_attention: queries must be (B, L, n * {kv_heads * dim}) on the cache's device, got "
                          f"{tuple(q.shape)}")
-    if q.stride(2) != 1:
+    batch, queries, channels = q.shape
+    q_batch, q_ld, q_step = q.stride()
+    if q_step != 1:
         raise ValueError("kv_attention: channel axis must have unit stride")
-    batch, queries, width = q.shape
-    _check_index(table, 2, batch, device, "kv_attention: table")
+    width, table_ld = _check_table(table, batch, device, "kv_attention: table")
     _check_index(lengths, 1, batch, device, "kv_attention: lengths")
     if out is None:
-        out = torch.empty((batch, queries, width), dtype=q.dtype, device=device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.stride(2) != 1:
         raise ValueError("kv_attention: out must have q's shape, dtype and device, and unit channel stride")
-    heads = width // dim
-    need = ctypes.c_size_t(0)
+    out_batch, out_ld, _ = out.stride()
+    heads = channels // dim
+    need = ctypes.c_size_t()
     _lib.call("ldb_kv_attention_fp8_workspace_size", batch, queries, heads, kv_heads, dim, ctypes.byref(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-    with instrument.maybe_time("kv_attention", 0.0):
-        _lib.call("ldb_kv_attention_fp8", _stream(q), q.data_ptr(), q.stride(1), q.stride(0), _DT[q.dtype],
-                  cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pages,
-                  kv_heads, page, dim, table.data_ptr(), _table_ld(table), table.shape[1], lengths.data_ptr(),
-                  out.data_ptr(), out.stride(1), out.stride(0), batch, queries, heads, float(scale), int(causal),
-                  ws.data_ptr(), need.value)
+    ws_ptr = None
+    if need.value:
+        ws = q.new_empty(need.value, dtype=torch.uint8)
+        ws_ptr = ws.data_ptr()
+    _launch("kv_attention", 0.0, "ldb_kv_attention_fp8", _raw_stream(q.get_device()), q.data_ptr(), q_ld, q_batch,
+            _DT[q.dtype], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+            pages, kv_heads, page, dim, table.data_ptr(), table_ld, width, lengths.data_ptr(), out.data_ptr(), out_ld,
+            out_batch, batch, queries, heads, scale, int(causal), ws_ptr, need.value)
     return out
