@@ -12,11 +12,15 @@
 // 32-bit scale word, and a word holds four consecutive blocks.
 //
 // One CTA per SM walks 128-row x BN-column tiles: warp 0 loads the code tiles
-// (TMA, 128-byte swizzle), warp 2 writes the scale words of each four blocks in
+// (TMA, 128-byte swizzle), warps 2-3 write the scale words of each four blocks in
 // the order that tcgen05.cp spreads over TMEM lanes, warp 1 issues scale
 // copies and products, warps 4-11 drain the accumulator of one tile while
 // the next is computed in the other (two warps per 32 rows, alternating 32-column chunks,
-// staged in shared memory for TMA stores where the output allows them).  Grids with fewer tiles than SMs cut K into
+// staged in shared memory for TMA stores where the output allows them).  PAIR:
+// two CTAs run one 256-row tile (cta_group::2), each staging its own rows and
+// half of the weight columns: 30 KB a K block where one CTA alone moves 44 KB
+// for 128 x 224 outputs, in and out of shared memory at 128 bytes a cycle, which
+// is what bounds it (704 cycles a K block against 448 of products).  Grids with fewer tiles than SMs cut K into
 // ranges whose FP32 partial sums a second kernel adds in order.
 
 #include <algorithm>
@@ -48,7 +52,7 @@ struct MatmulParams {
   float* partial;         // split > 1: [split][m][n]
   long long a_scales_ld, w_scales_ld, res_ld, out_ld;
   int m, n, k;
-  int bn, stages, box_m;
+  int pair, bn, stages, box_m;
   int tiles_m, tiles_n, split, kb_per_split;
   int act, out_dtype;
   int vec;       // out and residual rows allow 16-byte accesses and TMA stores
@@ -65,27 +69,18 @@ __device__ __forceinline__ uint32_t a_scale_word(const MatmulParams& p, int row,
   for (int j = 0; j < 4 && kb + j < kblocks; ++j) w = (w & ~(0xFFu << (8 * j))) | (static_cast<uint32_t>(s[j]) << (8 * j));
   return w;
 }
-__device__ __forceinline__ uint32_t w_scale_word(const MatmulParams& p, int col, int kb, int kblocks) {
-  uint32_t w = 0x7F7F7F7Fu;
-  if (col >= p.n) return w;
-  const uint8_t* s = p.w_scales + (col / kFp8Block) * p.w_scales_ld + kb;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (kb + j < kblocks) w = (w & ~(0xFFu << (8 * j))) | (static_cast<uint32_t>(s[j]) << (8 * j));
-  return w;
-}
-
 // Tile and K range of work item i: rows vary fastest, so neighbouring CTAs
 // share a weight tile.
 struct Work {
   int row0, col0, kb0, kb1, split;
 };
-__device__ __forceinline__ Work work_item(const MatmulParams& p, int i, int kblocks) {
+template <bool PAIR>
+__device__ __forceinline__ Work work_item(const MatmulParams& p, int i, int kblocks, int rank) {
   Work w;
   const int tm = i % p.tiles_m;
   const int rest = i / p.tiles_m;
   w.split = rest % p.split;
-  w.row0 = tm * kTileM;
+  w.row0 = PAIR ? (2 * tm + rank) * kTileM : tm * kTileM;
   w.col0 = (rest / p.split) * p.bn;
   w.kb0 = w.split * p.kb_per_split;
   w.kb1 = min(kblocks, w.kb0 + p.kb_per_split);
@@ -176,13 +171,14 @@ __device__ __forceinline__ void finish32(const MatmulParams& p, int row, int col
   }
 }
 
-template <typename T>
+template <typename T, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_matmul_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap wmap,
                       const __grid_constant__ CUtensorMap omap, const MatmulParams p, unsigned int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int stage_bytes = kTileM * 128 + p.bn * 128;
+  const int w_rows = PAIR ? p.bn / 2 : p.bn;  // weight columns this CTA stages
+  const int stage_bytes = kTileM * 128 + w_rows * 128;
   uint8_t* s_scales = smem + p.stages * stage_bytes;
   uint8_t* s_out = s_scales + kScaleStages * kScaleBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_out + kEpilogueWarps * kStagingBytes);
@@ -200,6 +196,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = lane_id();
   const int kblocks = (p.k + kFp8Block - 1) / kFp8Block;
   const int items = p.tiles_m * p.tiles_n * p.split;
+  const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
+  const int item0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, item_step = PAIR ? gridDim.x >> 1 : gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) {
@@ -207,12 +205,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kScaleStages; ++s) {
-      mbar_init(&sf_full[s], 32);
+      mbar_init(&sf_full[s], PAIR ? 64 : 32);  // (a pair's barriers of arrival are the leader's)
       mbar_init(&sf_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&acc_full[t], 1);
-      mbar_init(&acc_empty[t], kEpilogueWarps);
+      mbar_init(&acc_empty[t], PAIR ? 2 * kEpilogueWarps : kEpilogueWarps);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -223,11 +221,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&wmap);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, kTmemCols);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_slot, kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, kTmemCols);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist before any arrival from the other
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_begin();
@@ -238,19 +242,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       int st = 0;
       uint32_t ph = 0;
       int loads = 0;
-      const uint32_t bytes = static_cast<uint32_t>(p.box_m + p.bn) * 128;
+      const uint32_t bytes = static_cast<uint32_t>(p.box_m + w_rows) * 128;
       bool ok = true;
-      for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-        const Work w = work_item(p, i, kblocks);
+      for (int i = item0; ok && i < items; i += item_step) {
+        const Work w = work_item<PAIR>(p, i, kblocks, rank);
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!mbar_wait(&empty[st], ph ^ 1u, abort_flag, status)) {
             ok = false;
             break;
           }
           uint8_t* sa = smem + st * stage_bytes;
-          mbar_arrive_expect_tx(&full[st], bytes);
-          tma_load_2d(sa, &amap, &full[st], kb * 128, w.row0);
-          tma_load_2d(sa + kTileM * 128, &wmap, &full[st], kb * 128, w.col0);
+          if constexpr (PAIR) {
+            // the loads of both CTAs complete on the leader's barrier, which counts both's bytes
+            if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * bytes);
+            const uint32_t bar = mapa_shared(smem_u32(&full[st]), 0);
+            tma_load_2d_pair(sa, &amap, bar, kb * 128, w.row0);
+            tma_load_2d_pair(sa + kTileM * 128, &wmap, bar, kb * 128, w.col0 + rank * w_rows);
+          } else {
+            mbar_arrive_expect_tx(&full[st], bytes);
+            tma_load_2d(sa, &amap, &full[st], kb * 128, w.row0);
+            tma_load_2d(sa + kTileM * 128, &wmap, &full[st], kb * 128, w.col0);
+          }
           ++loads;
           if (++st == p.stages) {
             st = 0;
@@ -258,8 +270,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (*abort_flag) {
-        // Let the loads in flight land before the CTA gives up its shared memory.
+      if (*abort_flag && rank == 0) {
+        // Let the loads in flight land before the CTA gives up its shared memory
+        // (a pair's CTAs give it up together).
         volatile int never = 0;
         for (int back = 1; back <= min(loads, p.stages); ++back) {
           const int l = loads - back;
@@ -269,7 +282,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
-    {
+    if (rank == 0) {  // (the leader's, with pairs)
+      auto copy = [](uint32_t to, uint64_t desc) {
+        if constexpr (PAIR) {
+          tmem_copy_scales_pair(to, desc);
+        } else {
+          tmem_copy_scales(to, desc);
+        }
+      };
+      auto product = [](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t more) {
+        if constexpr (PAIR) {
+          umma_ss_mx8_pair(d, a, b, idesc, sa, sb, more);
+        } else {
+          umma_ss_mx8(d, a, b, idesc, sa, sb, more);
+        }
+      };
+      auto commit = [](uint64_t* bar) {
+        if constexpr (PAIR) {
+          umma_commit_pair_warp(bar, 3);  // in both CTAs
+        } else {
+          umma_commit_warp(bar);
+        }
+      };
       // Scale words in TMEM: a set of columns per ring slot, behind the two accumulators.
       const int sfb_cols = 4 * ((p.bn + 127) / 128);
       const uint32_t sf_cols = 4 + sfb_cols;
@@ -277,8 +311,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int st = 0, sst = 0, tile = 0;
       uint32_t ph = 0, sph = 0;
       bool ok = true;
-      for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++tile) {
-        const Work w = work_item(p, i, kblocks);
+      for (int i = item0; ok && i < items; i += item_step, ++tile) {
+        const Work w = work_item<PAIR>(p, i, kblocks, rank);
         const uint32_t acc = tmem + (tile & 1) * p.bn;
         ok = warp_wait(&acc_empty[tile & 1], (static_cast<uint32_t>(tile >> 1) & 1u) ^ 1u, abort_flag, status);
         if (!ok) break;
@@ -292,9 +326,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t sfa = sf_base + sst * sf_cols;
           const uint32_t sfb = sfa + 4;
           const uint32_t s_addr = smem_u32(s_scales + sst * kScaleBytes);
-          tmem_copy_scales(sfa, make_smem_desc(s_addr, 0, 128, kSwizzleNone));
-          for (int c = 0; c < sfb_cols / 4; ++c)
-            tmem_copy_scales(sfb + 4 * c, make_smem_desc(s_addr + 512 + 512 * c, 0, 128, kSwizzleNone));
+          copy(sfa, make_smem_desc(s_addr, 0, 128, kSwizzleNone));
+          for (int c = 0; c < sfb_cols / 4; ++c) copy(sfb + 4 * c, make_smem_desc(s_addr + 512 + 512 * c, 0, 128, kSwizzleNone));
           const int kend = min(w.kb1, kb + 4);
           for (int b = kb; b < kend; ++b) {
             if (!warp_wait(&full[st], ph, abort_flag, status)) {
@@ -304,59 +337,101 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             const uint32_t a_addr = smem_u32(smem + st * stage_bytes);
             const uint32_t w_addr = a_addr + kTileM * 128;
-            const uint32_t idesc = make_idesc_mx8(kTileM, p.bn, static_cast<uint32_t>(b - kb));
+            const uint32_t idesc = make_idesc_mx8(PAIR ? 2 * kTileM : kTileM, p.bn, static_cast<uint32_t>(b - kb));
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              umma_ss_mx8(acc, make_smem_desc(a_addr + q * 32, 16, 1024, kSwizzle128),
-                          make_smem_desc(w_addr + q * 32, 16, 1024, kSwizzle128), idesc, sfa, sfb,
-                          (b > w.kb0 || q > 0) ? 1u : 0u);
-            umma_commit_warp(&empty[st]);
+              product(acc, make_smem_desc(a_addr + q * 32, 16, 1024, kSwizzle128),
+                      make_smem_desc(w_addr + q * 32, 16, 1024, kSwizzle128), idesc, sfa, sfb,
+                      (b > w.kb0 || q > 0) ? 1u : 0u);
+            commit(&empty[st]);
             if (++st == p.stages) {
               st = 0;
               ph ^= 1u;
             }
           }
-          umma_commit_warp(&sf_empty[sst]);  // the copy and the products have read this slot
+          commit(&sf_empty[sst]);  // the copy and the products have read this slot
           if (++sst == kScaleStages) {
             sst = 0;
             sph ^= 1u;
           }
         }
-        if (ok) umma_commit_warp(&acc_full[tile & 1]);
+        if (ok) commit(&acc_full[tile & 1]);
       }
       if (*abort_flag) {
         volatile int never = 0;
-        umma_commit_warp(drain);
+        if constexpr (PAIR) {
+          umma_commit_pair_warp(drain, 1);
+        } else {
+          umma_commit_warp(drain);
+        }
         mbar_wait(drain, 0, &never, status);
       }
     }
-  } else if (warp == 2) {
+  } else if (warp < 4) {
     // -------------------------------------------------------------- scales
-    int sst = 0;
+    // Warps 2 and 3 take the groups in turn, each with its next group's words
+    // on their way while one's are written: with one warp their latency was
+    // longer than the products of four blocks.
+    int i = item0, kb = 0;
+    Work w = work_item<PAIR>(p, min(i, items - 1), kblocks, rank);
+    kb = w.kb0;
+    auto advance = [&]() {  // to the next group
+      kb += 4;
+      if (kb >= w.kb1) {
+        i += item_step;
+        if (i < items) {
+          w = work_item<PAIR>(p, i, kblocks, rank);
+          kb = w.kb0;
+        }
+      }
+    };
+    uint32_t a[4], byte = 0x7F;
+    // A tile's columns lie in at most three 128-column blocks: lane 4 n + j
+    // reads byte j of block n's word.
+    auto load = [&]() {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) a[c] = a_scale_word(p, w.row0 + 32 * c + lane, kb, kblocks);
+      const int block = w.col0 / kFp8Block + (lane >> 2), at = kb + (lane & 3);
+      byte = lane < 12 && block * kFp8Block < p.n && at < kblocks ? p.w_scales[block * p.w_scales_ld + at] : 0x7F;
+    };
+    if (warp == 3 && i < items) advance();
+    if (i < items) load();
+    int sst = warp - 2;
     uint32_t sph = 0;
-    bool ok = true;
-    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      const Work w = work_item(p, i, kblocks);
-      for (int kb = w.kb0; kb < w.kb1; kb += 4) {
-        uint32_t a[4], b[8];
+    while (i < items) {
+      const int col = w.col0 % kFp8Block + lane;
+      const uint4 rows = make_uint4(a[0], a[1], a[2], a[3]);
+      uint32_t words[3];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) a[c] = a_scale_word(p, w.row0 + 32 * c + lane, kb, kblocks);
+      for (int n = 0; n < 3; ++n) {
+        words[n] = 0;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) b[c] = 32 * c < p.bn ? w_scale_word(p, w.col0 + 32 * c + lane, kb, kblocks) : 0;
-        if (!warp_wait(&sf_empty[sst], sph ^ 1u, abort_flag, status)) {
-          ok = false;
-          break;
-        }
-        uint4* dst = reinterpret_cast<uint4*>(s_scales + sst * kScaleBytes);
-        dst[lane] = make_uint4(a[0], a[1], a[2], a[3]);
-        dst[32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
-        if (p.bn > 128) dst[64 + lane] = make_uint4(b[4], b[5], b[6], b[7]);
-        fence_proxy_async_smem();
+        for (int j = 0; j < 4; ++j) words[n] |= __shfl_sync(0xffffffffu, byte, 4 * n + j) << (8 * j);
+      }
+      advance();
+      if (i < items) advance();
+      if (i < items) load();
+      uint32_t b[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const int n = (col + 32 * c) / kFp8Block;
+        b[c] = n == 0 ? words[0] : (n == 1 ? words[1] : words[2]);
+      }
+      if (!warp_wait(&sf_empty[sst], sph ^ 1u, abort_flag, status)) break;
+      uint4* dst = reinterpret_cast<uint4*>(s_scales + sst * kScaleBytes);
+      dst[lane] = rows;
+      dst[32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
+      if (p.bn > 128) dst[64 + lane] = make_uint4(b[4], b[5], b[6], b[7]);
+      fence_proxy_async_smem();
+      if constexpr (PAIR) {
+        mbar_arrive_cluster(mapa_shared(smem_u32(&sf_full[sst]), 0));
+      } else {
         mbar_arrive(&sf_full[sst]);
-        if (++sst == kScaleStages) {
-          sst = 0;
-          sph ^= 1u;
-        }
+      }
+      sst += 2;
+      if (sst >= kScaleStages) {
+        sst -= kScaleStages;
+        sph ^= 1u;
       }
     }
   } else if (warp >= 4) {
@@ -367,8 +442,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3;
     const bool staged = p.vec && p.split == 1;
     int tile = 0, buffer = 0;
-    for (int i = blockIdx.x; i < items; i += gridDim.x, ++tile) {
-      const Work w = work_item(p, i, kblocks);
+    for (int i = item0; i < items; i += item_step, ++tile) {
+      const Work w = work_item<PAIR>(p, i, kblocks, rank);
       if (!warp_wait(&acc_full[tile & 1], static_cast<uint32_t>(tile >> 1) & 1u, abort_flag, status)) break;
       tc_fence_after();
       const int row0 = w.row0 + quarter * 32, row = row0 + lane;
@@ -428,15 +503,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[tile & 1]);
+      if (lane == 0) {
+        if constexpr (PAIR) {
+          mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[tile & 1]), 0));
+        } else {
+          mbar_arrive(&acc_empty[tile & 1]);
+        }
+      }
     }
     if (lane == 0) bulk_wait_group_all();
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the leader's products read both CTAs' memory
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_dealloc_pair(tmem, kTmemCols);
+    } else {
+      tmem_dealloc(tmem, kTmemCols);
+    }
+  }
 }
 
 // Sum of the K ranges in their order, then the epilogue; one thread per value.
@@ -462,35 +550,46 @@ int plan(int m, int n, int k, MatmulParams* p) {
   const int sms = sm_count();
   const int kblocks = (k + kFp8Block - 1) / kFp8Block;
   p->m = m, p->n = n, p->k = k;
-  p->tiles_m = (m + kTileM - 1) / kTileM;
   // Cycles of a CTA that walks `waves` tiles.  A K block moves 128 rows of A and
-  // bn of the weight through shared memory twice (in, and out to the tensor
-  // core) at 128 bytes a cycle; the epilogue takes 12 to 24 cycles a column (GELU) and
-  // runs beside the next tile's products.  K ranges (few tiles, long K; cut at
-  // groups of four blocks) cost the second kernel, most of it on the host.
+  // its share of the weight through shared memory twice (in, and out to the tensor
+  // core) at 128 bytes a cycle, and takes 2 cycles a column of products; the epilogue takes
+  // about 32 cycles a column and runs beside the next tile's products.  K ranges
+  // (few tiles, long K; cut at groups of four blocks) cost the second kernel, most of it
+  // on the host; pairs start and end later.  Measured on one B200, us: 6400 x
+  // 1024 x 1024 with residual 16.5 alone, 18.9 in pairs; 8190 x 4096 x 4096 156
+  // alone, 125 in pairs; 6400 x 1024 x 256 with GELU 13.3 at 128 columns, 17.3 at 64, 14.9 at 224.
   long long best = -1;
   const int groups = (kblocks + 3) / 4;
-  for (const int bn : {32, 64, 96, 128, 160, 192, kMaxBn}) {
-    const int tiles_n = (n + bn - 1) / bn;
-    const long long tiles = static_cast<long long>(p->tiles_m) * tiles_n;
-    int split = 1;
-    if (tiles * 2 <= sms && kblocks >= 8) split = std::max(1, std::min({static_cast<int>(sms / tiles), groups, 16}));
-    const int per = 4 * ((groups + split - 1) / split);
-    split = (kblocks + per - 1) / per;
-    const long long waves = (tiles * split + sms - 1) / sms;
-    const long long main = static_cast<long long>(std::min(per, kblocks)) * (256 + 2 * bn);
-    const long long cost =
-        waves * (std::max<long long>(main, 16 * bn) + 1000) + (split > 1 ? 6000 : 0);
-    if (best < 0 || cost < best) {
-      best = cost;
-      p->bn = bn;
-      p->tiles_n = tiles_n;
-      p->split = split;
-      p->kb_per_split = per;
+  for (const int pair : {0, 1}) {
+    if (pair && m <= kTileM) continue;
+    const int tiles_m = (m + kTileM * (1 + pair) - 1) / (kTileM * (1 + pair));
+    for (const int bn : {32, 64, 96, 128, 160, 192, kMaxBn}) {
+      const int tiles_n = (n + bn - 1) / bn;
+      const long long tiles = static_cast<long long>(tiles_m) * tiles_n;
+      const int slots = pair ? sms / 2 : sms;
+      int split = 1;
+      if (!pair && tiles * 2 <= sms && kblocks >= 8)
+        split = std::max(1, std::min({static_cast<int>(sms / tiles), groups, 16}));
+      const int per = 4 * ((groups + split - 1) / split);
+      split = (kblocks + per - 1) / per;
+      const long long waves = (tiles * split + slots - 1) / slots;
+      const long long main =
+          static_cast<long long>(std::min(per, kblocks)) * (pair ? std::max(2 * bn, 256 + bn) : 256 + 2 * bn);
+      const long long cost =
+          waves * (std::max<long long>(main, 32 * bn) + 1000) + (split > 1 ? 6000 : 0) + (pair ? 5000 : 0);
+      if (best < 0 || cost < best) {
+        best = cost;
+        p->pair = pair;
+        p->bn = bn;
+        p->tiles_m = tiles_m;
+        p->tiles_n = tiles_n;
+        p->split = split;
+        p->kb_per_split = per;
+      }
     }
   }
   const long long tiles = static_cast<long long>(p->tiles_m) * p->tiles_n;
-  p->stages = std::min(kMaxStages, kSmemBudget / (kTileM * 128 + p->bn * 128));
+  p->stages = std::min(kMaxStages, kSmemBudget / (kTileM * 128 + (p->pair ? p->bn / 2 : p->bn) * 128));
   p->box_m = std::min(kTileM, (m + 7) / 8 * 8);
   if (tiles * p->split > 0x7FFFFFFF) return fail(LDB_ERR_SHAPE, "matmul_fp8: too many tiles");
   return LDB_OK;
@@ -506,7 +605,7 @@ int launch(cudaStream_t stream, const CUtensorMap& amap, const CUtensorMap& wmap
   static unsigned long long configured = 0;
   constexpr int kFixed = 1024 + kScaleStages * kScaleBytes + kEpilogueWarps * kStagingBytes + 512;
   static_assert(kFixed + kSmemBudget <= 232448, "shared memory");
-  const int smem = kFixed + p.stages * (kTileM + p.bn) * 128;
+  const int smem = kFixed + p.stages * (kTileM + (p.pair ? p.bn / 2 : p.bn)) * 128;
   CUtensorMap omap = amap;  // (not used without TMA stores)
   int rc = LDB_OK;
   if (p.vec && p.split == 1) {
@@ -520,11 +619,20 @@ int launch(cudaStream_t stream, const CUtensorMap& amap, const CUtensorMap& wmap
     }
     if (rc != LDB_OK) return rc;
   }
-  rc = ensure_smem_attribute(reinterpret_cast<const void*>(fp8_matmul_kernel<T>), kFixed + kSmemBudget, &configured,
-                                 "matmul_fp8 shared memory");
+  if (p.pair) {
+    static unsigned long long pair_configured = 0;
+    rc = ensure_smem_attribute(reinterpret_cast<const void*>(fp8_matmul_kernel<T, true>), kFixed + kSmemBudget,
+                               &pair_configured, "matmul_fp8 shared memory");
+    if (rc != LDB_OK) return rc;
+    const int pairs = std::min(p.tiles_m * p.tiles_n, sm_count() / 2);
+    return launch_kernel_cluster(fp8_matmul_kernel<T, true>, dim3(2 * pairs), dim3(kThreads), smem, stream,
+                                 "matmul_fp8 (CTA pairs) launch", 2u, amap, wmap, omap, p, status);
+  }
+  rc = ensure_smem_attribute(reinterpret_cast<const void*>(fp8_matmul_kernel<T, false>), kFixed + kSmemBudget,
+                             &configured, "matmul_fp8 shared memory");
   if (rc != LDB_OK) return rc;
   const int items = p.tiles_m * p.tiles_n * p.split;
-  rc = launch_kernel(fp8_matmul_kernel<T>, dim3(std::min(items, sm_count())), dim3(kThreads), smem, stream,
+  rc = launch_kernel(fp8_matmul_kernel<T, false>, dim3(std::min(items, sm_count())), dim3(kThreads), smem, stream,
                      "matmul_fp8 launch", amap, wmap, omap, p, status);
   if (rc != LDB_OK || p.split == 1) return rc;
   const long long total = static_cast<long long>(p.m) * p.n;
@@ -586,7 +694,7 @@ int ldb_matmul_fp8(cudaStream_t stream, const uint8_t* a, long long a_ld, const 
   const uint64_t adims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(m)};
   const uint64_t wdims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n)};
   const uint64_t astride[1] = {static_cast<uint64_t>(a_ld)}, wstride[1] = {static_cast<uint64_t>(w_ld)};
-  const uint32_t abox[2] = {128, static_cast<uint32_t>(p.box_m)}, wbox[2] = {128, static_cast<uint32_t>(p.bn)};
+  const uint32_t abox[2] = {128, static_cast<uint32_t>(p.box_m)}, wbox[2] = {128, static_cast<uint32_t>(p.pair ? p.bn / 2 : p.bn)};
   rc = encode_tiled_u8(&amap, a, 2, adims, astride, abox, 128);
   if (rc == LDB_OK) rc = encode_tiled_u8(&wmap, w, 2, wdims, wstride, wbox, 128);
   if (rc != LDB_OK) return rc;

@@ -197,6 +197,25 @@ def test_matmul(cuda_device, dtype, m, n, k, bias, residual, gelu):
     assert _lib.device_status(reset=True) == 0
 
 
+@pytest.mark.parametrize("dtype,m,n,k,bias,residual,gelu", [
+    (torch.float16, 513, 2304, 2048, True, False, True), (torch.bfloat16, 2050, 4100, 1024, False, True, False),
+    (torch.float32, 700, 1600, 1500, True, True, False), (torch.float16, 1025, 1001, 2050, False, False, False),
+    (torch.bfloat16, 300, 520, 4096, True, True, True)])
+def test_matmul_many_rows_over_a_long_k(cuda_device, dtype, m, n, k, bias, residual, gelu):
+    """Sizes at which two CTAs share a tile, with ragged last tiles on every side."""
+    rows, weight, av, wv = operands(m, n, k, cuda_device, m + n + k)
+    g = torch.Generator().manual_seed(1)
+    b = torch.randn(n, generator=g) if bias else None
+    r = torch.randn(m, n, generator=g).to(dtype) if residual else None
+    args = dict(residual=None if r is None else r.to(cuda_device),
+                act=_lib.LDB_ACT_GELU if gelu else _lib.LDB_ACT_NONE, out_dtype=dtype)
+    got = fp8.matmul_fp8(rows, weight, None if b is None else b.to(cuda_device), **args)
+    want, size = oracle.matmul(av, wv, b, r, gelu)
+    check_product(got, want, size, dtype, slope=1.5 if gelu else 1.0)
+    assert torch.equal(fp8.matmul_fp8(rows, weight, None if b is None else b.to(cuda_device), **args), got)
+    assert _lib.device_status(reset=True) == 0
+
+
 def test_matmul_leading_axes_strides_and_repeats(cuda_device):
     rows, weight, av, wv = operands(60, 72, 256, cuda_device, 4)
     shaped = fp8.Fp8Rows(rows.codes.view(3, 20, 256), rows.scales.view(torch.uint8).as_strided((3, 20, 2), (80, 4, 1))
