@@ -37,7 +37,7 @@ static_assert(128 * kRegsWg0 + 256 * kRegsSoftmax <= kThreads * 168, "register s
 constexpr int kM = 128;      // rows per tile
 constexpr int kN = 128;      // tokens per block
 constexpr int kMeta = 4;     // ring of page factors
-constexpr int kGroups = 8;   // of 16 tokens, each of one page
+constexpr int kGroups = 8;   // of 16 tokens, each of one page (pages under 64 tokens; else the groups come in fours)
 constexpr float kFloor = -1.0e30f;  // reference of a row that has seen nothing
 constexpr float kGrow = 8.f;        // a reference follows its row's maximum once that is 2^8 above
 
@@ -54,8 +54,8 @@ struct Cfg {
   static constexpr int kOffK = 2 * PARTS * kPartBytes;
   static constexpr int kOffV = kOffK + kStages * kRawBytes;
   static constexpr int kOffV16 = kOffV + kStages * kRawBytes;
-  static constexpr int kOffMeta = kOffV16 + 2 * kV16Bytes;  // [kMeta][8] (key factor, value exponent)
-  static constexpr int kOffBad = kOffMeta + kMeta * kGroups * 8;  // [2][4] tokens whose values hold a NaN
+  static constexpr int kOffMeta = kOffV16 + 2 * kV16Bytes;  // [kMeta][8] (key factor, value exponent, 2^-exponent)
+  static constexpr int kOffBad = kOffMeta + kMeta * kGroups * 16;  // [2][4] tokens whose values hold a NaN
   static constexpr int kOffBar = kOffBad + 2 * 16;
   static constexpr int kSmem = 1024 + kOffBar + 256;
   // TMEM: S_t at 128 t, O_t at 256 + 128 t.  D = 128: the weights overwrite
@@ -89,6 +89,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// Each lane writes 8 consecutive 32-bit columns of its own TMEM lane.
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 // The CTA's share of the work.
 struct Span {
   int b, head, row0, tiles, len, jb0, nblocks, open;
@@ -111,7 +118,10 @@ __device__ __forceinline__ Span span_of(const KvTileParams& p, unsigned int* sta
   return s;
 }
 
-template <int D, typename T>
+// FINE: pages under 64 tokens, whose factors change every 16 columns of a
+// block; otherwise every 64.  (Fetching them every 16 columns for all pages
+// made the softmax, which bounds the kernel, a third longer.)
+template <int D, typename T, bool FINE>
 __global__ void __launch_bounds__(kThreads, 1)
     kv_tiles_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                     const KvTileParams p, unsigned int* status) {
@@ -119,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<D, PARTS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float2* s_meta = reinterpret_cast<float2*>(smem + C::kOffMeta);
+  float4* s_meta = reinterpret_cast<float4*>(smem + C::kOffMeta);
   uint32_t* s_bad = reinterpret_cast<uint32_t*>(smem + C::kOffBad);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* q_full = bars;                 // the query parts are written
@@ -212,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = warp_wait(&k_empty[st], ph ^ 1u, abort_flag, status);
         if (!ok) break;
         // (slot ms: the scores of block j - 2 are done, so the softmax of block j - 4 is)
-        if (lane < kGroups) s_meta[ms * kGroups + lane] = make_float2(gk, ge);
+        if (lane < kGroups) s_meta[ms * kGroups + lane] = make_float4(gk, ge, fp8_pow2(-static_cast<int>(ge)), 0.f);
         const bool load = lane < loads && my_id >= 0;
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, load)) * box * D;
         const int row = (my_id * p.c.kv_heads + sp.head) * p.c.page;
@@ -468,22 +478,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      const float2* meta = s_meta + (j % kMeta) * kGroups;
+      const float4* meta = s_meta + (j % kMeta) * kGroups;
+      constexpr int kCols = FINE ? 16 : 64;  // columns of one page
+      auto factor = [&](float kf) {
+        const float f = qs * kf;
+        return f < 1.2e-38f ? 1.2e-38f : f;  // (-inf times zero would be a NaN)
+      };
       float mx = kFloor;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        float m = max3(__uint_as_float(sr[16 * g]), __uint_as_float(sr[16 * g + 1]), __uint_as_float(sr[16 * g + 2]));
-        float n = max3(__uint_as_float(sr[16 * g + 3]), __uint_as_float(sr[16 * g + 4]), __uint_as_float(sr[16 * g + 5]));
+      for (int c0 = 0; c0 < kN; c0 += kCols) {
+        // independent chains of 3-input maxima, folded
+        float m4[4];
 #pragma unroll
-        for (int c = 6; c < 14; c += 4) {
-          m = max3(m, __uint_as_float(sr[16 * g + c]), __uint_as_float(sr[16 * g + c + 1]));
-          n = max3(n, __uint_as_float(sr[16 * g + c + 2]), __uint_as_float(sr[16 * g + c + 3]));
-        }
-        m = max3(m, __uint_as_float(sr[16 * g + 14]), __uint_as_float(sr[16 * g + 15]));
-        const float2 v = meta[g];
-        float f = qs * v.x;
-        if (f < 1.2e-38f) f = 1.2e-38f;  // -inf times zero would be a NaN
-        mx = fmaxf(mx, fmaf(fmaxf(m, n), f, v.y));
+        for (int k = 0; k < 4; ++k)
+          m4[k] = fmaxf(__uint_as_float(sr[c0 + 2 * k]), __uint_as_float(sr[c0 + 2 * k + 1]));
+#pragma unroll
+        for (int c = 8; c < kCols; c += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            m4[k] = max3(m4[k], __uint_as_float(sr[c0 + c + 2 * k]), __uint_as_float(sr[c0 + c + 2 * k + 1]));
+        const float4 v = meta[c0 / 16];
+        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), factor(v.x), v.y));
       }
       const bool first = j == 0;
       const bool grow = first || mx - top > kGrow;
@@ -513,30 +528,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         top = next;
       }
 #pragma unroll
-      for (int c0 = 0; c0 < kN; c0 += 32) {
-        uint32_t packed[16];
+      for (int c0 = 0; c0 < kN; c0 += kCols) {
+        const float4 v = meta[c0 / 16];
+        const float f = factor(v.x);
+        const uint64_t f2 = pack2(f, f), shift = pack2(v.y - top, v.y - top);
+        uint64_t sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 v = meta[c0 / 16 + h];
-          float f = qs * v.x;
-          if (f < 1.2e-38f) f = 1.2e-38f;
-          const uint64_t f2 = pack2(f, f), shift = pack2(v.y - top, v.y - top);
-          uint64_t sum2 = pack2(0.f, 0.f);
+        for (int h = 0; h < kCols; h += 16) {
+          uint32_t packed[8];
 #pragma unroll
           for (int c = 0; c < 16; c += 2) {
-            const int at = c0 + 16 * h + c;
+            const int at = c0 + h + c;
             float x0, x1;
             unpack2(fma2(pack2(__uint_as_float(sr[at]), __uint_as_float(sr[at + 1])), f2, shift), x0, x1);
             const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
-            sum2 = add2(sum2, pack2(e0, e1));
+            sum2[(c >> 1) & 1] = add2(sum2[(c >> 1) & 1], pack2(e0, e1));
             const __half2 w = __floats2half2_rn(e0, e1);
-            packed[8 * h + c / 2] = *reinterpret_cast<const uint32_t*>(&w);
+            packed[c / 2] = *reinterpret_cast<const uint32_t*>(&w);
           }
-          float a, b;
-          unpack2(sum2, a, b);
-          l = fmaf(a + b, fp8_pow2(-static_cast<int>(v.y)), l);
+          tmem_st8(tmem_p + ((c0 + h) >> 1), packed);
         }
-        tmem_st16(tmem_p + (c0 >> 1), packed);
+        float a, b;
+        unpack2(add2(sum2[0], sum2[1]), a, b);
+        l = fmaf(a + b, v.z, l);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -628,11 +642,11 @@ __global__ void __launch_bounds__(256) kv_tiles_merge_kernel(const KvTileParams 
   for (int c = 0; c < D / 32; ++c) dst[32 * c + lane] = from_f32<T>(v[c] * inv);
 }
 
-template <int D, typename T>
+template <int D, typename T, bool FINE>
 int launch(cudaStream_t stream, const KvTileParams& p, unsigned int* status) {
   using C = Cfg<D, std::is_same<T, __half>::value ? 3 : 2>;
   static unsigned long long configured = 0;
-  int rc = ensure_smem_attribute(reinterpret_cast<const void*>(kv_tiles_kernel<D, T>), C::kSmem, &configured,
+  int rc = ensure_smem_attribute(reinterpret_cast<const void*>(kv_tiles_kernel<D, T, FINE>), C::kSmem, &configured,
                                  "kv_attention shared memory");
   if (rc != LDB_OK) return rc;
   CUtensorMap kmap, vmap;
@@ -643,7 +657,7 @@ int launch(cudaStream_t stream, const KvTileParams& p, unsigned int* status) {
   rc = encode_tiled_u8(&kmap, p.c.k, 2, dims, strides, box, D);
   if (rc == LDB_OK) rc = encode_tiled_u8(&vmap, p.c.v, 2, dims, strides, box, D);
   if (rc != LDB_OK) return rc;
-  rc = launch_kernel(kv_tiles_kernel<D, T>, dim3(p.row_blocks * p.splits, p.c.kv_heads, p.c.batch), dim3(kThreads),
+  rc = launch_kernel(kv_tiles_kernel<D, T, FINE>, dim3(p.row_blocks * p.splits, p.c.kv_heads, p.c.batch), dim3(kThreads),
                      C::kSmem, stream, "kv_attention tiles launch", kmap, vmap, p, status);
   if (rc != LDB_OK || p.splits == 1) return rc;
   const long long rows = static_cast<long long>(p.c.batch) * p.c.kv_heads * p.rows;
@@ -651,11 +665,16 @@ int launch(cudaStream_t stream, const KvTileParams& p, unsigned int* status) {
                        "kv_attention tiles merge launch", p);
 }
 
+template <int D, typename T>
+int launch_page(cudaStream_t stream, const KvTileParams& p, unsigned int* status) {
+  return p.c.page < 64 ? launch<D, T, true>(stream, p, status) : launch<D, T, false>(stream, p, status);
+}
+
 template <typename T>
 int launch_dim(cudaStream_t stream, const KvTileParams& p, int head_dim, unsigned int* status) {
-  if (head_dim == 32) return launch<32, T>(stream, p, status);
-  if (head_dim == 64) return launch<64, T>(stream, p, status);
-  return launch<128, T>(stream, p, status);
+  if (head_dim == 32) return launch_page<32, T>(stream, p, status);
+  if (head_dim == 64) return launch_page<64, T>(stream, p, status);
+  return launch_page<128, T>(stream, p, status);
 }
 
 }  // namespace
