@@ -14,6 +14,8 @@
 // registers between the maximum and the rounding.  For one token it is the
 // launch.
 
+#include <type_traits>
+
 #include "host_common.h"
 #include "kv_cache.cuh"
 
@@ -47,6 +49,24 @@ __device__ __forceinline__ float block_max(float v, float* s_part) {
   return v;
 }
 
+// Largest magnitude of eight values (NaN left out), two at a time in 16 bits.
+template <typename T>
+__device__ __forceinline__ float max_of8(const uint4 (&raw)[sizeof(T) / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    const float* v = reinterpret_cast<const float*>(raw);
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+    return m;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* v = reinterpret_cast<const T2*>(raw);
+    const T2 m = __hmax2(__hmax2(__habs2(v[0]), __habs2(v[1])), __hmax2(__habs2(v[2]), __habs2(v[3])));
+    const float a = to_f32<T>(m.x), b = to_f32<T>(m.y);
+    return fmaxf(fmaxf(a, b), 0.f);  // (a NaN, left where all are one, counts nothing)
+  }
+}
+
 // VECS: vectors of eight values per thread that a whole page takes.  The
 // values stay as they came (four registers a vector in 16 bits) until they
 // are rounded, so that enough blocks are resident to cover the chain of
@@ -69,19 +89,11 @@ __global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) 
   const int last = static_cast<int>(min(static_cast<long long>(count), page0 + p.page - start));
   if (first >= last) return;
   const int held = static_cast<int>(max(0ll, start - page0));
-  const int id = slot < p.width ? p.table[b * p.table_ld + slot] : -1;
-  if (id < 0 || id >= p.pages) {
-    if (threadIdx.x == 0) set_bad_shape(status);
-    return;
-  }
-  const long long unit = static_cast<long long>(id) * p.kv_heads + head;
-  uint8_t* codes = p.codes[which] + unit * p.page * p.dim;
-  uint8_t* scale = p.scales[which] + unit;
+  const int id = slot < p.width ? p.table[b * p.table_ld + slot] : -1;  // (looked at once the values are on their way)
   const T* src = static_cast<const T*>(p.src[which]) + b * p.src_batch[which] + head * p.dim;
   const int vshift = p.dim_shift - 3;  // vectors of eight per token
   const int vecs = (last - first) << vshift;
 
-  if (threadIdx.x == 0) s_old = *scale;
   uint4 raw[VECS][sizeof(T) / 2];
   float amax = 0.f;
 #pragma unroll
@@ -101,19 +113,35 @@ __global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) 
       }
     }
   }
+  if (id < 0 || id >= p.pages) {
+    if (threadIdx.x == 0) set_bad_shape(status);
+    return;
+  }
+  const long long unit = static_cast<long long>(id) * p.kv_heads + head;
+  uint8_t* codes = p.codes[which] + unit * p.page * p.dim;
+  uint8_t* scale = p.scales[which] + unit;
+  if (held > 0 && threadIdx.x == 0) s_old = *scale;
 #pragma unroll
-  for (int i = 0; i < VECS; ++i) {
-    if (i * kAppendThreads + static_cast<int>(threadIdx.x) < vecs) {
-      const T* v = reinterpret_cast<const T*>(raw[i]);
+  for (int i = 0; i < VECS; ++i)
+    if (i * kAppendThreads + static_cast<int>(threadIdx.x) < vecs) amax = fmaxf(amax, max_of8<T>(raw[i]));
+  amax = block_max(amax, s_part);
+  const bool infinite = !fp8_is_finite(amax);  // (rare: infinities become NaN and leave the maximum)
+  if (infinite) {
+    amax = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = fabsf(to_f32<T>(v[j]));
-        if (fp8_is_finite(a)) amax = fmaxf(amax, a);
+    for (int i = 0; i < VECS; ++i) {
+      if (i * kAppendThreads + static_cast<int>(threadIdx.x) < vecs) {
+        const T* v = reinterpret_cast<const T*>(raw[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float a = fabsf(to_f32<T>(v[j]));
+          if (fp8_is_finite(a)) amax = fmaxf(amax, a);
+        }
       }
     }
+    amax = block_max(amax, s_part);
   }
-  amax = block_max(amax, s_part);
-  const int e_old = s_old - 127;
+  const int e_old = held > 0 ? s_old - 127 : 0;
   int e = max(-kKvMaxExponent, min(kKvMaxExponent, fp8_exponent(amax)));
   if (held > 0) e = amax == 0.f ? e_old : max(e, e_old);  // zeros ask for no scale
   const float inv = fp8_pow2(-min(e, 127));
@@ -126,7 +154,7 @@ __global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) 
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         y[j] = to_f32<T>(v[j]) * inv;
-        if (!fp8_is_finite(y[j])) y[j] = fp8_nan();
+        if (infinite && !fp8_is_finite(y[j])) y[j] = fp8_nan();
       }
       uint2 packed;
       packed.x = fp8_pack4(y[0], y[1], y[2], y[3]);
