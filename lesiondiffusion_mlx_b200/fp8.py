@@ -71,17 +71,24 @@ def _quantized(x: torch.Tensor, k: int) -> tuple[Fp8Rows, int, int]:
     lead = x.shape[:-1]
     blocks = (k + 127) // 128
     ld, s_ld = (k + 15) // 16 * 16, (blocks + 3) // 4 * 4
-    codes = x.new_empty((*lead, ld), dtype=CODES)
+    codes = (torch.empty_like(x, dtype=CODES, memory_format=torch.contiguous_format) if ld == k
+             else x.new_empty((*lead, ld), dtype=CODES))
     scales = x.new_empty((*lead, s_ld), dtype=SCALES)
     return Fp8Rows(codes if ld == k else codes[..., :k], scales if s_ld == blocks else scales[..., :blocks]), ld, s_ld
 
 
-def _launch(kind: str, flops: float, name: str, *args) -> None:
-    if instrument.active() is None:  # (a context manager costs a tenth of a single token's call)
-        _lib.call(name, *args)
-    else:
+def _launcher(kind: str, flops: float = 0.0):
+    """``_lib.call``, inside the active timer's measurement if there is one.
+
+    (A context manager around every call costs a tenth of a single token's.)"""
+    if instrument.active() is None:
+        return _lib.call
+
+    def call(name: str, *args) -> None:
         with instrument.maybe_time(kind, flops):
             _lib.call(name, *args)
+
+    return call
 
 
 def _check_input(x: torch.Tensor, name: str) -> None:
@@ -110,10 +117,10 @@ def rms_norm_fp8(x: torch.Tensor, gamma: torch.Tensor | None, *, residual: torch
         if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
             raise ValueError("rms_norm_fp8: residual must have x's shape, dtype and device")
         r_ld = _flat(residual, "rms_norm_fp8: residual")[2]
-        h = x.new_empty(x.shape)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
         residual_ptr, h_ptr = residual.data_ptr(), h.data_ptr()
     out, ld, s_ld = _quantized(x, c)
-    _launch("rms_norm_fp8", 0.0, "ldb_rms_norm_fp8", _raw_stream(x.get_device()), x.data_ptr(), x_ld, residual_ptr,
+    _launcher("rms_norm_fp8")("ldb_rms_norm_fp8", _raw_stream(x.get_device()), x.data_ptr(), x_ld, residual_ptr,
             r_ld, _DT[x.dtype], None if gamma is None else gamma.data_ptr(), eps, h_ptr, c, out.codes.data_ptr(), ld,
             out.scales.data_ptr(), s_ld, rows, c)
     return out, x if h is None else h
@@ -124,7 +131,7 @@ def quantize_rows(x: torch.Tensor) -> Fp8Rows:
     _check_input(x, "quantize_rows: x")
     rows, k, x_ld = _flat(x, "quantize_rows: x")
     out, ld, s_ld = _quantized(x, k)
-    _launch("quantize_rows", 0.0, "ldb_quantize_fp8_rows", _raw_stream(x.get_device()), x.data_ptr(), x_ld,
+    _launcher("quantize_rows")("ldb_quantize_fp8_rows", _raw_stream(x.get_device()), x.data_ptr(), x_ld,
             _DT[x.dtype], out.codes.data_ptr(), ld, out.scales.data_ptr(), s_ld, rows, k)
     return out
 
@@ -137,8 +144,8 @@ def pack_weight_fp8(weight: torch.Tensor) -> Fp8Weight:
     n, k, ld = _flat(weight, "pack_weight_fp8: weight")
     codes = torch.zeros((n, (k + 15) // 16 * 16), dtype=torch.uint8, device=weight.device).view(CODES)
     scales = torch.empty(((n + 127) // 128, (k + 127) // 128), dtype=SCALES, device=weight.device)
-    _lib.call("ldb_pack_weight_fp8", _raw_stream(weight.get_device()), weight.data_ptr(), ld, _DT[weight.dtype], codes.data_ptr(),
-              codes.shape[1], scales.data_ptr(), scales.shape[1], n, k)
+    _lib.call("ldb_pack_weight_fp8", _raw_stream(weight.get_device()), weight.data_ptr(), ld, _DT[weight.dtype],
+              codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1], n, k)
     return Fp8Weight(codes[:, :k], scales)
 
 
@@ -200,7 +207,7 @@ def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, *, re
     if need.value:
         ws = codes.new_empty(need.value, dtype=torch.uint8)
         ws_ptr = ws.data_ptr()
-    _launch("matmul_fp8", 2.0 * m * n * k, "ldb_matmul_fp8", _raw_stream(codes.get_device()), codes.data_ptr(), a_ld,
+    _launcher("matmul_fp8", 2.0 * m * n * k)("ldb_matmul_fp8", _raw_stream(codes.get_device()), codes.data_ptr(), a_ld,
             scales.data_ptr(), s_ld, w_codes.data_ptr(), w_ld, w_scales.data_ptr(), ws_ld, bias_ptr, residual_ptr,
             r_ld, out.data_ptr(), out_ld, m, n, k, act, _DT[out_dtype], ws_ptr, need.value)
     return out

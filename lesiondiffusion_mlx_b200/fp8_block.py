@@ -127,10 +127,10 @@ def random_weights(channels: int, context: int, heads: int, kv_heads: int, head_
     def dense(n: int, k: int) -> torch.Tensor:
         return torch.randn(n, k, generator=g) * k ** -0.5
 
-    return {"norm1": 1 + 0.1 * torch.randn(channels, generator=g), "norm2": 1 + 0.1 * torch.randn(channels, generator=g),
-            "to_q": dense(heads * head_dim, channels), "to_k": dense(kv_heads * head_dim, context),
-            "to_v": dense(kv_heads * head_dim, context), "to_out": dense(channels, heads * head_dim),
-            "ff1": dense(hidden, channels), "ff2": dense(channels, hidden),
+    norm1, norm2 = (1 + 0.1 * torch.randn(channels, generator=g) for _ in range(2))
+    return {"norm1": norm1, "norm2": norm2, "to_q": dense(heads * head_dim, channels),
+            "to_k": dense(kv_heads * head_dim, context), "to_v": dense(kv_heads * head_dim, context),
+            "to_out": dense(channels, heads * head_dim), "ff1": dense(hidden, channels), "ff2": dense(channels, hidden),
             "ff1.bias": 0.02 * torch.randn(hidden, generator=g), "ff2.bias": 0.02 * torch.randn(channels, generator=g)}
 
 

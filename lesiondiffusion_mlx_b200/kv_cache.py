@@ -22,7 +22,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .fp8 import CODES, SCALES, _launch, _raw_stream
+from .fp8 import CODES, SCALES, _launcher, _raw_stream
 from .ops import _DT
 
 HEAD_DIMS = (32, 64, 128)
@@ -106,7 +106,7 @@ def kv_append(cache: KvCacheFp8, k: torch.Tensor, v: torch.Tensor, table: torch.
     _check_index(start, 1, batch, device, "kv_append: start")
     if counts is not None:
         _check_index(counts, 1, batch, device, "kv_append: counts")
-    _launch("kv_append", 0.0, "ldb_kv_append_fp8", _raw_stream(k.get_device()), k.data_ptr(), k_ld, k_batch,
+    _launcher("kv_append")("ldb_kv_append_fp8", _raw_stream(k.get_device()), k.data_ptr(), k_ld, k_batch,
             v.data_ptr(), v_ld, v_batch, _DT[k.dtype], cache.k.data_ptr(), cache.v.data_ptr(),
             cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pages, heads, page, dim, table.data_ptr(), table_ld,
             width, start.data_ptr(), None if counts is None else counts.data_ptr(), batch, tokens)
@@ -135,7 +135,7 @@ def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, length
     width, table_ld = _check_table(table, batch, device, "kv_attention: table")
     _check_index(lengths, 1, batch, device, "kv_attention: lengths")
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.stride(2) != 1:
         raise ValueError("kv_attention: out must have q's shape, dtype and device, and unit channel stride")
     out_batch, out_ld, _ = out.stride()
@@ -146,7 +146,7 @@ def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, length
     if need.value:
         ws = q.new_empty(need.value, dtype=torch.uint8)
         ws_ptr = ws.data_ptr()
-    _launch("kv_attention", 0.0, "ldb_kv_attention_fp8", _raw_stream(q.get_device()), q.data_ptr(), q_ld, q_batch,
+    _launcher("kv_attention")("ldb_kv_attention_fp8", _raw_stream(q.get_device()), q.data_ptr(), q_ld, q_batch,
             _DT[q.dtype], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
             pages, kv_heads, page, dim, table.data_ptr(), table_ld, width, lengths.data_ptr(), out.data_ptr(), out_ld,
             out_batch, batch, queries, heads, scale, int(causal), ws_ptr, need.value)
