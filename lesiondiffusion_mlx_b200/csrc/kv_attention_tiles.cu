@@ -691,7 +691,9 @@ size_t kv_tile_workspace(int batch, int kv_heads, long long rows, int head_dim) 
 
 int kv_attention_tiles(cudaStream_t stream, KvTileParams p, int head_dim, int dtype, float scale, void* workspace,
                        unsigned int* status) {
-  p.splits = kv_tile_splits(p.c.batch, p.c.kv_heads, p.rows);
+  // (at least two blocks of the longest item a range)
+  const long long blocks = (static_cast<long long>(p.c.width) * p.c.page + kN - 1) / kN;
+  p.splits = static_cast<int>(std::min<long long>(kv_tile_splits(p.c.batch, p.c.kv_heads, p.rows), (blocks + 1) / 2));
   p.row_blocks = (p.rows + 2 * kM - 1) / (2 * kM);
   p.negate = scale < 0.f;
   p.scale_log2 = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
