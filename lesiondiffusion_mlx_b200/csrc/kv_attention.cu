@@ -26,6 +26,12 @@
 // ranges is merged by a second kernel, in order.  A lane's 16-byte reads of a
 // swizzled row are free of bank conflicts, and the orders of channels (in q k)
 // and of output rows (in p v) are chosen so that these bytes are its fragments.
+//
+// One B200, 8 heads of 128 shared by 4 bf16 queries each: 131072 tokens 58 us
+// (50 in this kernel, 5.4 TB/s; the start and the merge are the rest), 48 items
+// of up to 8192 tokens 77.5 us (5.2 TB/s).  Tiles fetched by one warp per CTA
+// with TMA and shared by four others took 74 and 154 us: the fetch was bound by
+// the issue of its loads, and every change of pair by the four warps' barriers.
 
 #include <algorithm>
 

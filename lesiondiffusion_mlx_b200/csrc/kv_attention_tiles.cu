@@ -20,7 +20,13 @@
 //
 // Bound: 4 D flops and one exponential per score; at D = 128 the tensor core
 // (1024 cycles per 128 x 128 tile) and the exponentials (1024 cycles) ask for
-// as much.
+// as much.  One B200: 4 prompts of 2048 tokens over up to 8000, 32 heads of 128
+// over 8, bf16, 492 us (745 TFLOP/s); 6400 f16 tokens over 77, 4 heads of 64,
+// 10.6 us.  A block of two tiles takes 4700 cycles: 2000 from a tile's weights to
+// its next scores (718 for the value product, 977 for the scores, whose operands
+// take 128 bytes a cycle of shared memory), 420 for the maximum, 340 for the
+// reference, 1600 for the weights.  Four softmax warpgroups with half a row a
+// thread took 626 us instead of 527, scores read from TMEM twice 581.
 
 #include <algorithm>
 
