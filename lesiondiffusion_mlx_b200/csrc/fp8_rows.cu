@@ -96,19 +96,19 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32,
   constexpr int kLanes = WARPS * 32;
   const int t = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
   const int per_block = WARPS == 1 ? 8 : 1;
-  const int first_row = blockIdx.x * per_block + (WARPS == 1 ? threadIdx.x >> 5 : 0);
-  const int step = gridDim.x * per_block;
+  // (unsigned: the last step may pass 2^31)
+  const unsigned first_row = blockIdx.x * per_block + (WARPS == 1 ? threadIdx.x >> 5 : 0);
+  const unsigned step = gridDim.x * per_block, rows = p.rows;
 
-  // gamma is a weight, not the previous kernel's output: staged in shared
-  // memory before the wait (in registers it took a third of them, and half the warps).
+  pdl_begin();
+  // gamma in shared memory: in registers it took a third of them, and half the warps.
   extern __shared__ float s_gamma[];
   if constexpr (NORM) {
     for (int c = threadIdx.x; c < ITERS * kLanes * 8; c += blockDim.x)
       s_gamma[c] = p.gamma && c < p.channels ? p.gamma[c] : 1.f;
     __syncthreads();
   }
-  pdl_begin();
-  for (int row = first_row; row < p.rows; row += step) {
+  for (unsigned row = first_row; row < rows; row += step) {
     const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
     const T* r = static_cast<const T*>(p.residual) + (p.residual ? row * p.r_ld : 0);
     float v[ITERS][8];
@@ -192,7 +192,7 @@ int launch_rows(cudaStream_t stream, const RowsParams& p, const char* what) {
   auto smem = [](int lanes, int iters) { return NORM ? static_cast<size_t>(lanes) * iters * 8 * sizeof(float) : 0; };
   if (c <= 1024) {
     const int iters = c <= 256 ? 1 : (c <= 512 ? 2 : 4);
-    const int blocks = std::min((p.rows + 7) / 8, sms * resident_blocks(1, iters, sizeof(T)));
+    const int blocks = std::min((p.rows - 1) / 8 + 1, sms * resident_blocks(1, iters, sizeof(T)));
     auto k = iters == 1 ? fp8_rows_kernel<T, 1, 1, NORM>
                         : (iters == 2 ? fp8_rows_kernel<T, 1, 2, NORM> : fp8_rows_kernel<T, 1, 4, NORM>);
     return launch_kernel(k, dim3(blocks), dim3(256), smem(32, iters), stream, what, p);

@@ -291,3 +291,20 @@ def test_refusals(cuda_device):
     with pytest.raises(_lib.LdbError, match="16-byte"):
         odd = torch.zeros(4, 200, device=cuda_device, dtype=torch.uint8)[:, 1:65].view(fp8.CODES)
         fp8.matmul_fp8(fp8.Fp8Rows(odd, rows.scales), weight)
+
+
+def test_rms_norm_reads_gamma_after_its_producer(cuda_device):
+    """gamma written by the launch right before: the norm has to wait for it."""
+    c = 2048
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    x = torch.randn(1, c, device=cuda_device, generator=g)
+    rows = fp8.quantize_rows(torch.randn(1, c, device=cuda_device, generator=g))
+    for seed in range(20):
+        weight = fp8.pack_weight_fp8(torch.randn(c, c, device=cuda_device, generator=g))
+        torch.cuda.synchronize()
+        gamma = fp8.matmul_fp8(rows, weight, out_dtype=torch.float32)
+        got, _ = fp8.rms_norm_fp8(x, gamma[0])
+        torch.cuda.synchronize()
+        want, _ = fp8.rms_norm_fp8(x, gamma[0])
+        assert torch.equal(got.codes.view(torch.uint8), want.codes.view(torch.uint8)), seed
+        assert torch.equal(got.scales.view(torch.uint8), want.scales.view(torch.uint8)), seed
