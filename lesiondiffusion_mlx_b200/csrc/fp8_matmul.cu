@@ -555,7 +555,9 @@ __global__ void __launch_bounds__(256) fp8_matmul_reduce_kernel(const MatmulPara
 
 // Column tile, K ranges and ring depth from the extents alone.
 int plan(int m, int n, int k, MatmulParams* p) {
-  if (m <= 0 || n <= 0 || k <= 0) return fail(LDB_ERR_SHAPE, "matmul_fp8: %d x %d x %d", m, n, k);
+  constexpr int kMost = 0x7FFFFE00;  // (rows and columns of a whole last tile still count in 32 bits)
+  if (m <= 0 || n <= 0 || k <= 0 || m > kMost || n > kMost || k > kMost)
+    return fail(LDB_ERR_SHAPE, "matmul_fp8: %d x %d x %d", m, n, k);
   const int sms = sm_count();
   const int kblocks = (k + kFp8Block - 1) / kFp8Block;
   p->m = m, p->n = n, p->k = k;

@@ -31,6 +31,8 @@ SCALES = torch.float8_e8m0fnu
 # bound by the host: building a torch.cuda.Stream to read its handle takes longer than a launch.)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
+_MAX_ROWS = 2 ** 31 - 1  # the library counts rows in 32 bits
+
 
 class Fp8Rows(NamedTuple):
     """``(..., K)`` e4m3 codes and ``(..., ceil(K / 128))`` E8M0 scales.
@@ -56,6 +58,8 @@ def _flat(t: torch.Tensor, name: str) -> tuple[int, int, int]:
         ld, step = t.stride()
         if step != 1 and k != 1:
             raise ValueError(f"{name}: channel axis must have unit stride")
+        if rows > _MAX_ROWS:
+            raise ValueError(f"{name}: {rows} rows (at most {_MAX_ROWS})")
         return rows, k, ld if rows > 1 or ld > k else k
     if t.ndim < 2:
         raise ValueError(f"{name}: expected (..., channels) with at least two axes")
@@ -63,6 +67,8 @@ def _flat(t: torch.Tensor, name: str) -> tuple[int, int, int]:
     rows = t.shape[0] * per
     if t.shape[0] > 1 and per and t.stride(0) != per * ld:
         raise ValueError(f"{name}: tensor must be dense over its rows")
+    if rows > _MAX_ROWS:
+        raise ValueError(f"{name}: {rows} rows (at most {_MAX_ROWS})")
     return rows, k, max(ld, k) if rows <= 1 else ld
 
 

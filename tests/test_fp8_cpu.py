@@ -71,3 +71,15 @@ def test_python_refuses_what_does_not_fit():
         fp8.matmul_fp8(rows, weight)
     with pytest.raises(ValueError, match="float8"):
         fp8.matmul_fp8(fp8.Fp8Rows(x, rows.scales), weight)
+
+
+def test_extents_past_32_bits_are_refused_not_wrapped():
+    need = ctypes.c_size_t(0)
+    for m, n, k in ((2 ** 31 - 1, 8, 128), (8, 2 ** 31 - 1, 128), (8, 8, 2 ** 31 - 1)):
+        with pytest.raises(_lib.LdbError) as e:
+            _lib.call("ldb_matmul_fp8_workspace_size", m, n, k, ctypes.byref(need))
+        assert e.value.code == -2
+    with pytest.raises(ValueError, match="at most"):
+        fp8._flat(torch.zeros(1, 1).expand(2 ** 32 + 1, 1), "x")
+    with pytest.raises(ValueError, match="at most"):
+        fp8._flat(torch.zeros(1, 1, 1).expand(2 ** 16, 2 ** 16, 1), "x")
