@@ -142,8 +142,9 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[W / 4]
   }
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// 16 bytes: the first `bytes` of them from src, then zeros.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -187,7 +188,7 @@ struct Fetch {
         id = -1;
       }
       kf = 0.f;
-      ev = 0.f;
+      ev = -INFINITY;  // (tokens of no page weigh nothing)
       if (id >= 0) {
         const long long unit = static_cast<long long>(id) * c.kv_heads + head;
         kf = fp8_pow2(c.k_scale[unit] - 127) * scale_log2;
@@ -213,15 +214,15 @@ struct Fetch {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // rows 0 .. 15 and 16 .. 31
       const int page_id = h == 0 ? id0 : id1;
-      if (page_id < 0) continue;
       const int row = c.page < kTile ? 0 : inside + 16 * h;
-      const long long off = ((static_cast<long long>(page_id) * c.kv_heads + head) * c.page + row) * D + lane * 16;
+      const long long off = ((static_cast<long long>(max(page_id, 0)) * c.kv_heads + head) * c.page + row) * D + lane * 16;
+      const uint32_t bytes = page_id < 0 ? 0u : 16u;  // zeros for what has no page
 #pragma unroll
       for (int i = 0; i < kUnits / 2; ++i) {
         const int at_i = h * (kUnits / 2) + i;
         const uint32_t to = dst + at_i * 512 + ((at_i & 1) ? odd : even);
-        cp_async16(to, c.k + off + i * 512);
-        cp_async16(to + kTile * D, c.v + off + i * 512);
+        cp_async16(to, c.k + off + i * 512, bytes);
+        cp_async16(to + kTile * D, c.v + off + i * 512, bytes);
       }
     }
   }
@@ -275,7 +276,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
       for (int i = (blockIdx.x + b) % gridDim.x; i < p.queries; i += gridDim.x) {
         T* row = static_cast<T*>(p.out) + b * p.out_batch + i * p.out_ld;
         if (p.out_vec) {
-          for (int d = threadIdx.x; d < width / 8; d += kWarps * 32) reinterpret_cast<uint4*>(row)[d] = make_uint4(0, 0, 0, 0);
+          for (int d = threadIdx.x; d < width / 8; d += kWarps * 32)
+            reinterpret_cast<uint4*>(row)[d] = make_uint4(0, 0, 0, 0);
         } else {
           for (int d = threadIdx.x; d < width; d += kWarps * 32) row[d] = from_f32<T>(0.f);
         }
@@ -457,13 +459,13 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
           s[r][n][1] = fmaf(fmaf(d[3], 0.0625f, d[1]), f, meta[n >> 1].y);
         }
       }
-      uint32_t bad = 0;  // tokens some rows must not see whose values hold a NaN
+      uint32_t bad = 0;  // tokens whose values hold a NaN, where some rows may not see them
       if (masked) {
-        if (p.queries > 1) {
+        if (p.causal && p.queries > 1) {
           uint32_t any = 0;
           for (int e = 0; e < D / 4; ++e)
             any |= kv_nan_codes(reinterpret_cast<const uint32_t*>(sk + C::kTileBytes + lane * D)[e]);
-          bad = __ballot_sync(0xffffffffu, any != 0);
+          bad = __ballot_sync(0xffffffffu, any != 0 && j0 + lane < len);
         }
 #pragma unroll
         for (int n = 0; n < 4; ++n)
@@ -471,10 +473,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
           for (int e = 0; e < 2; ++e) {
             const int tok = 8 * n + 2 * c + e;
 #pragma unroll
-            for (int r = 0; r < G; ++r) {
-              if ((bad >> tok) & 1u) s[r][n][e] = fp8_nan();
+            for (int r = 0; r < G; ++r)
               if (j0 + tok >= limit[r]) s[r][n][e] = -INFINITY;
-            }
           }
       }
       float mx[G];
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
       uint32_t pf[G][4];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const float undo = fp8_pow2(-static_cast<int>(meta[n >> 1].y));
+        const float undo = fp8_pow2(-max(static_cast<int>(meta[n >> 1].y), -127));
 #pragma unroll
         for (int r = 0; r < G; ++r) {
           const float a = ex2_approx(s[r][n][0] - top[r]), bb = ex2_approx(s[r][n][1] - top[r]);
@@ -525,10 +525,11 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
           lds_words<kWv>(sk + at_v[e & 1] + (16 * k + 8 * (e >> 1)) * D, w[e]);
           if (masked) {
             const int tok = 16 * k + 2 * c + (e & 1) + 8 * (e >> 1);
-            const bool drop = j0 + tok >= len || ((bad >> tok) & 1u) != 0;
 #pragma unroll
-            for (int x = 0; x < kWv / 4; ++x)
-              if (drop) w[e][x] = 0;
+            for (int x = 0; x < kWv / 4; ++x) {
+              if (j0 + tok >= len) w[e][x] = 0;
+              if ((bad >> tok) & 1u) w[e][x] = kv_without_nan(w[e][x]);
+            }
           }
         }
 #pragma unroll
@@ -546,6 +547,21 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
             mma_f16(o[r][2 * x + 1], v4, v5, v6, v7, pf[r][2 * k], pf[r][2 * k + 1]);
           }
         }
+      }
+      // The NaN that the product left out, to the rows that see its token.
+      for (uint32_t rest = bad; rest; rest &= rest - 1) {
+        const int tok = __ffs(rest) - 1;
+        uint32_t w[kWv / 4];
+        lds_words<kWv>(sk + C::kTileBytes + swizzle_offset(tok * D + g * kWv, D), w);
+#pragma unroll
+        for (int r = 0; r < G; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bool seen = j0 + tok < __shfl_sync(0xffffffffu, limit[r], 8 * c + 4 * e);
+#pragma unroll
+            for (int x = 0; x < D / 8; ++x)  // channel g D/8 + x
+              if (seen && ((kv_nan_codes(w[x / 4]) >> (8 * (x % 4))) & 0x80u)) o[r][x / 2][2 * (x % 2) + e] = fp8_nan();
+          }
       }
       __syncwarp();
       if (++slot == C::kSlots) slot = 0;
@@ -617,7 +633,8 @@ __global__ void __launch_bounds__(kMergeThreads) kv_attention_merge_kernel(const
   __shared__ float s_red[2][kMergeThreads / 32], s_f[kMergeThreads];
   pdl_begin();
   int4 at = p.open_part[blockIdx.x];
-  if (p.open_by_pair && kv_length(p.c, blockIdx.x / (p.c.kv_heads * p.row_tiles), p.status) == 0) at.w = 0;  // not written
+  if (p.open_by_pair && kv_length(p.c, blockIdx.x / (p.c.kv_heads * p.row_tiles), p.status) == 0)
+    at.w = 0;  // not written
   const int first = at.z, count = at.w, r = blockIdx.y;
   const int row = (at.y % p.row_tiles) * p.tile_rows + r;
   if (count == 0 || row >= p.rows) return;
@@ -693,22 +710,18 @@ int launch(cudaStream_t stream, const AttnParams& p, unsigned int* status) {
   rc = launch_kernel(kv_attention_kernel<D, G, T>, dim3(p.warps / kWarps), dim3(kWarps * 32),
                      Cfg<D, G>::kOffBase + (p.c.batch + 1) * 4, stream, "kv_attention launch", p, status);
   if (rc != LDB_OK) return rc;
-  return launch_kernel(kv_attention_merge_kernel<D, T>,
-                       dim3(p.open_by_pair ? p.c.batch * p.c.kv_heads * p.row_tiles : p.warps, std::min(p.tile_rows, p.rows)),
-                       dim3(kMergeThreads), 0, stream,
+  const dim3 grid(p.open_by_pair ? p.c.batch * p.c.kv_heads * p.row_tiles : p.warps, std::min(p.tile_rows, p.rows));
+  return launch_kernel(kv_attention_merge_kernel<D, T>, grid, dim3(kMergeThreads), 0, stream,
                        "kv_attention merge launch", p);
 }
 
 template <int D, typename T>
-int launch_groups(cudaStream_t stream, const AttnParams& p,
-                  unsigned int* status) {
-  return p.tile_rows == 8 ? launch<D, 1, T>(stream, p, status)
-                          : launch<D, 2, T>(stream, p, status);
+int launch_groups(cudaStream_t stream, const AttnParams& p, unsigned int* status) {
+  return p.tile_rows == 8 ? launch<D, 1, T>(stream, p, status) : launch<D, 2, T>(stream, p, status);
 }
 
 template <typename T>
-int launch_dim(cudaStream_t stream, const AttnParams& p, int head_dim,
-               unsigned int* status) {
+int launch_dim(cudaStream_t stream, const AttnParams& p, int head_dim, unsigned int* status) {
   if (head_dim == 32) return launch_groups<32, T>(stream, p, status);
   if (head_dim == 64) return launch_groups<64, T>(stream, p, status);
   return launch_groups<128, T>(stream, p, status);
@@ -748,14 +761,15 @@ int ldb_kv_attention_fp8(cudaStream_t stream, const void* q, long long q_ld, lon
   if (pages <= 0 || width <= 0 || table_ld < width || static_cast<long long>(width) * page > 0x7FFFFFFFll)
     return fail(LDB_ERR_SHAPE, "kv_attention: %d pages, table of %d", pages, width);
   const long long rows_all = static_cast<long long>(pages) * kv_heads * page;
-  if (rows_all > 0x7FFFFFFFll) return fail(LDB_ERR_SHAPE, "kv_attention: cache of %lld token rows (2^31 - 1)", rows_all);
+  if (rows_all > 0x7FFFFFFFll)
+    return fail(LDB_ERR_SHAPE, "kv_attention: cache of %lld token rows (2^31 - 1)", rows_all);
   if (batch > kMaxBatch) return fail(LDB_ERR_SHAPE, "kv_attention: at most %d items, got %d", kMaxBatch, batch);
   if (batch == 0 || queries == 0) return LDB_OK;
   if (!q || !k_codes || !v_codes || !k_scales || !v_scales || !table || !lengths || !out)
     return fail(LDB_ERR_INVALID, "kv_attention: null pointer");
   const long long row = static_cast<long long>(heads) * head_dim;
-  if (queries > 1 && (q_ld < row || out_ld < row))
-    return fail(LDB_ERR_SHAPE, "kv_attention: a row stride is below %lld", row);
+  if ((queries > 1 && (q_ld < row || out_ld < row)) || (batch > 1 && out_batch < row))
+    return fail(LDB_ERR_SHAPE, "kv_attention: a row stride, or the output's item stride, is below %lld", row);
   if (reinterpret_cast<uintptr_t>(k_codes) % 16 || reinterpret_cast<uintptr_t>(v_codes) % 16)
     return fail(LDB_ERR_ALIGNMENT, "kv_attention: codes must be 16-byte aligned");
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
@@ -763,7 +777,8 @@ int ldb_kv_attention_fp8(cudaStream_t stream, const void* q, long long q_ld, lon
                 workspace_bytes);
   unsigned int* status = device_status_ptr();
   if (!status) return fail(LDB_ERR_CUDA, "kv_attention: no device status word");
-  const KvView view{k_codes, v_codes, k_scales, v_scales, table, lengths, table_ld, pages, kv_heads, page, width, batch};
+  const KvView view{k_codes,  v_codes, k_scales, v_scales, table, lengths,
+                    table_ld, pages,   kv_heads, page,     width, batch};
   const long long group_rows = static_cast<long long>(queries) * (heads / kv_heads);
   if (group_rows > 0x7FFFFF00ll) return fail(LDB_ERR_SHAPE, "kv_attention: too many query rows");
   const int q_vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_ld % 8 == 0 && q_batch % 8 == 0;

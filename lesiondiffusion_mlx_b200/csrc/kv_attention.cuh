@@ -1,5 +1,5 @@
 // What the two cache-attention kernels share: the split of a query into e4m3
-// parts, the NaN test of packed codes, and the many-row kernel's interface.
+// parts, the NaN tests of packed codes, and the many-row kernel's interface.
 #pragma once
 
 #include <type_traits>
@@ -33,6 +33,9 @@ __device__ __forceinline__ float2 kv_unpack2(uint32_t w) {
 
 // Non-zero if one of four codes is a NaN (0x7F or 0xFF).
 __device__ __forceinline__ uint32_t kv_nan_codes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+// The same codes with each NaN turned into zero.
+__device__ __forceinline__ uint32_t kv_without_nan(uint32_t w) { return w & ~((kv_nan_codes(w) >> 7) * 0xFFu); }
 
 struct KvTileParams {
   KvView c;

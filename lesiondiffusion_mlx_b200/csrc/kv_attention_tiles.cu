@@ -21,8 +21,8 @@
 // Bound: 4 D flops and one exponential per score; at D = 128 the tensor core
 // (1024 cycles per 128 x 128 tile) and the exponentials (1024 cycles) ask for
 // as much.  One B200: 4 prompts of 2048 tokens over up to 8000, 32 heads of 128
-// over 8, bf16, 492 us (745 TFLOP/s); 6400 f16 tokens over 77, 4 heads of 64,
-// 10.6 us.  A block of two tiles takes 4700 cycles: 2000 from a tile's weights to
+// over 8, bf16, 480 us (764 TFLOP/s); 6400 f16 tokens over 77, 4 heads of 64,
+// 10.0 us.  A block of two tiles takes 4700 cycles: 2000 from a tile's weights to
 // its next scores (718 for the value product, 977 for the scores, whose operands
 // take 128 bytes a cycle of shared memory), 420 for the maximum, 340 for the
 // reference, 1600 for the weights.  Four softmax warpgroups with half a row a
@@ -61,8 +61,8 @@ struct Cfg {
   static constexpr int kOffV = kOffK + kStages * kRawBytes;
   static constexpr int kOffV16 = kOffV + kStages * kRawBytes;
   static constexpr int kOffMeta = kOffV16 + 2 * kV16Bytes;  // [kMeta][8] (key factor, value exponent, 2^-exponent)
-  static constexpr int kOffBad = kOffMeta + kMeta * kGroups * 16;  // [2][4] tokens whose values hold a NaN
-  static constexpr int kOffBar = kOffBad + 2 * 16;
+  static constexpr int kOffBad = kOffMeta + kMeta * kGroups * 16;  // NaN met among values that not every row sees
+  static constexpr int kOffBar = kOffBad + 16;
   static constexpr int kSmem = 1024 + kOffBar + 256;
   // TMEM: S_t at 128 t, O_t at 256 + 128 t.  D = 128: the weights overwrite
   // their scores; narrower heads have room for them behind O_t, so that the next block's
@@ -173,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < kMeta; ++s) mbar_init(&meta_full[s], 1);
     mbar_init(q_full, p.rows - (p.row_blocks - 1 - static_cast<int>(blockIdx.x) / p.splits) * 2 * kM > kM ? 8 : 4);
     *abort_flag = 0;
+    *s_bad = 0;
     fence_mbarrier_init();
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             id = -1;
           }
           kf = p.scale_log2;
-          ev = 0.f;
+          ev = -INFINITY;  // (tokens of no page weigh nothing)
           if (id >= 0) {
             const long long unit = static_cast<long long>(id) * p.c.kv_heads + sp.head;
             kf = fp8_pow2(p.c.k_scale[unit] - 127) * p.scale_log2;
@@ -228,8 +229,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = warp_wait(&k_empty[st], ph ^ 1u, abort_flag, status);
         if (!ok) break;
         // (slot ms: the scores of block j - 2 are done, so the softmax of block j - 4 is)
-        if (lane < kGroups) s_meta[ms * kGroups + lane] = make_float4(gk, ge, fp8_pow2(-static_cast<int>(ge)), 0.f);
+        if (lane < kGroups)
+          s_meta[ms * kGroups + lane] = make_float4(gk, ge, fp8_pow2(-max(static_cast<int>(ge), -127)), 0.f);
         const bool load = lane < loads && my_id >= 0;
+        // pages that the table should name and does not: zeros in their place
+        const uint32_t holes = __ballot_sync(0xffffffffu, lane < loads && my_id < 0 && first + lane < used);
+        auto blank = [&](uint8_t* codes) {
+          for (uint32_t rest = holes; rest; rest &= rest - 1) {
+            uint4* at = reinterpret_cast<uint4*>(codes + (__ffs(rest) - 1) * box * D);
+            for (int i = lane; i < box * D / 16; i += 32) at[i] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        };
+        if (holes) blank(smem + C::kOffK + st * C::kRawBytes);
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, load)) * box * D;
         const int row = (my_id * p.c.kv_heads + sp.head) * p.c.page;
         __syncwarp();
@@ -242,6 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++k_loads;
         ok = warp_wait(&v_empty[st], ph ^ 1u, abort_flag, status);
         if (!ok) break;
+        if (holes) blank(smem + C::kOffV + st * C::kRawBytes);
+        __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&v_full[st], bytes);
         __syncwarp();
         if (load) tma_load_2d(smem + C::kOffV + st * C::kRawBytes + lane * box * D, &vmap, &v_full[st], 0, row);
@@ -268,7 +282,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < D / 32; ++k)
               umma_ss_f8(tmem + t * 128, make_smem_desc(q_addr + k * 32, 16, 8 * D, C::kLayout),
-                         make_smem_desc(k_addr + k * 32, 16, 8 * D, C::kLayout), idesc_qk, (part > 0 || k > 0) ? 1u : 0u);
+                         make_smem_desc(k_addr + k * 32, 16, 8 * D, C::kLayout), idesc_qk,
+                         (part > 0 || k > 0) ? 1u : 0u);
           }
           umma_commit_warp(&s_full[t]);
         };
@@ -347,40 +362,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint8_t* raw = smem + C::kOffV + st * C::kRawBytes;
         uint8_t* out = smem + C::kOffV16 + st * C::kV16Bytes;
         const int j0 = (sp.jb0 + j) * kN;
-        const bool masked = j0 + kN > sp.open;
-        uint32_t bad[4] = {0, 0, 0, 0};
-        if (masked) {
-          // A token that holds a NaN: its values become zero, and the softmax
-          // gives the NaN to the rows that see it.  (Both warps test all tokens:
-          // neither has to wait for the other.)
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const int tok = lane + 32 * h;
-            uint32_t any = 0;
-            for (int e = 0; e < D / 4; ++e) any |= kv_nan_codes(reinterpret_cast<const uint32_t*>(raw + tok * D)[e]);
-            bad[h] = __ballot_sync(0xffffffffu, any != 0 && j0 + tok < sp.len);
-            if (lane == 0) s_bad[st * 4 + h] = bad[h];
-          }
-        }
         // unit tid + 64 n: the same channels of every kStep-th token
-        auto convert = [&](int n, uint4 w) {
-          if (masked) {
-            const int tok = tok0 + n * kStep;
-            const uint32_t word = tok < 64 ? (tok < 32 ? bad[0] : bad[1]) : (tok < 96 ? bad[2] : bad[3]);
-            if (j0 + tok >= sp.len || ((word >> (tok & 31)) & 1u)) w = make_uint4(0, 0, 0, 0);
+        auto convert = [&](int n, uint4 w, auto masked) {
+          if constexpr (decltype(masked)::value) {
+            // Where some rows may not see a token its NaN becomes zero here, and
+            // the rows that do see it get the NaN at the end.
+            if (j0 + tok0 + n * kStep >= sp.len) w = make_uint4(0, 0, 0, 0);
+            if (kv_nan_codes(w.x) | kv_nan_codes(w.y) | kv_nan_codes(w.z) | kv_nan_codes(w.w)) {
+              *s_bad = 1;
+              w = make_uint4(kv_without_nan(w.x), kv_without_nan(w.y), kv_without_nan(w.z), kv_without_nan(w.w));
+            }
           }
-          const uint4 lo = make_uint4(fp8_unpack2(w.x), fp8_unpack2(w.x >> 16), fp8_unpack2(w.y), fp8_unpack2(w.y >> 16));
-          const uint4 hi = make_uint4(fp8_unpack2(w.z), fp8_unpack2(w.z >> 16), fp8_unpack2(w.w), fp8_unpack2(w.w >> 16));
+          const uint4 lo =
+              make_uint4(fp8_unpack2(w.x), fp8_unpack2(w.x >> 16), fp8_unpack2(w.y), fp8_unpack2(w.y >> 16));
+          const uint4 hi =
+              make_uint4(fp8_unpack2(w.z), fp8_unpack2(w.z >> 16), fp8_unpack2(w.w), fp8_unpack2(w.w >> 16));
           *reinterpret_cast<uint4*>(out + n * kStep * C::kSubRow + at_first) = swap ? hi : lo;
           *reinterpret_cast<uint4*>(out + n * kStep * C::kSubRow + at_second) = swap ? lo : hi;
         };
+        auto block = [&](auto masked) {
 #pragma unroll
-        for (int n0 = 0; n0 < kN / kStep; n0 += 4) {
-          uint4 w[4];
+          for (int n0 = 0; n0 < kN / kStep; n0 += 4) {
+            uint4 w[4];
 #pragma unroll
-          for (int n = 0; n < 4; ++n) w[n] = *reinterpret_cast<const uint4*>(raw + (n0 + n) * kStep * D + at_raw);
+            for (int n = 0; n < 4; ++n) w[n] = *reinterpret_cast<const uint4*>(raw + (n0 + n) * kStep * D + at_raw);
 #pragma unroll
-          for (int n = 0; n < 4; ++n) convert(n0 + n, w[n]);
+            for (int n = 0; n < 4; ++n) convert(n0 + n, w[n], masked);
+          }
+        };
+        // (two loops: with the test inside one the prompts of the head comment took 641 us instead of 493)
+        if (j0 + kN > sp.open) {
+          block(std::true_type{});
+        } else {
+          block(std::false_type{});
         }
         fence_proxy_async_smem();
         mbar_arrive(&v16_full[st]);
@@ -401,10 +415,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem_s = tmem + t * 128 + lane_base;
     const uint32_t tmem_o = tmem + 256 + t * 128 + lane_base;
     const uint32_t tmem_p = C::kSeparateP ? tmem_o + 64 : tmem_s;
+    const int limit = p.causal && live ? min(sp.len, sp.len - p.queries + i + 1) : sp.len;  // keys that the row sees
     float qs = 1.f;
     if (t < sp.tiles && sp.nblocks > 0) {
       // Query row in parts: the largest magnitude to [128, 256); a NaN stays
-      // one, an infinity makes the row's factor one.
+      // one, an infinity makes the row's factor one (of a row that sees any key).
       const T* src = static_cast<const T*>(p.q) + sp.b * p.q_batch + i * p.q_ld +
                      (static_cast<long long>(sp.head) * p.group + gq) * D;
       uint32_t raw[D / 2];
@@ -428,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         m = fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y)));
       }
       const int e = m > 0.f ? min(126, max(-119, static_cast<int>(__float_as_uint(m) >> 23) - 127)) : 0;
-      qs = fp8_is_finite(m) ? fp8_pow2(e - 7) : fp8_nan();
+      qs = fp8_is_finite(m) || limit <= 0 ? fp8_pow2(e - 7) : fp8_nan();
       const float inv = p.negate ? -fp8_pow2(7 - e) : fp8_pow2(7 - e);
 #pragma unroll
       for (int chunk = 0; chunk < D / 16; ++chunk) {
@@ -442,14 +457,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
 #pragma unroll
         for (int part = 0; part < PARTS; ++part)
-          *reinterpret_cast<uint4*>(smem + (t * PARTS + part) * C::kPartBytes + swizzle_offset(local * D + chunk * 16, D)) =
+          *reinterpret_cast<uint4*>(smem + (t * PARTS + part) * C::kPartBytes +
+                                    swizzle_offset(local * D + chunk * 16, D)) =
               make_uint4(parts[part][0], parts[part][1], parts[part][2], parts[part][3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
-    const int limit = p.causal && live ? min(sp.len, sp.len - p.queries + i + 1) : sp.len;
     float top = kFloor, l = 0.f;
     bool ok = t < sp.tiles;
     for (int j = 0; ok && j < sp.nblocks; ++j) {
@@ -470,19 +485,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&s_free[t]);
       }
       const int j0 = (sp.jb0 + j) * kN;
-      if (j0 + kN > sp.open) {
-        // hidden keys count nothing; a token with a NaN among its values counts as NaN
-        ok = warp_wait(&v16_full[j & 1], static_cast<uint32_t>(j >> 1) & 1u, abort_flag, status);
-        if (!ok) break;
+      if (j0 + kN > sp.open) {  // hidden keys count nothing
 #pragma unroll
-        for (int c0 = 0; c0 < kN; c0 += 32) {
-          const uint32_t bad = s_bad[(j & 1) * 4 + c0 / 32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            if ((bad >> c) & 1u) sr[c0 + c] = 0x7FC00000u;
-            if (j0 + c0 + c >= limit) sr[c0 + c] = 0xFF800000u;
-          }
-        }
+        for (int c = 0; c < kN; ++c)
+          if (j0 + c >= limit) sr[c] = 0xFF800000u;
       }
       const float4* meta = s_meta + (j % kMeta) * kGroups;
       constexpr int kCols = FINE ? 16 : 64;  // columns of one page
@@ -564,7 +570,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&p_ready[t]);
     }
     if (ok && sp.nblocks > 0)
-      ok = warp_wait(&pv_done[t], static_cast<uint32_t>(sp.nblocks - 1) & 1u, abort_flag, status);
+      ok = warp_wait(&pv_done[t], static_cast<uint32_t>(sp.nblocks - 1) & 1u, abort_flag, status) &&
+           warp_wait(&v16_full[(sp.nblocks - 1) & 1], static_cast<uint32_t>((sp.nblocks - 1) >> 1) & 1u, abort_flag,
+                     status);  // (done as well: orders the reads of s_bad)
     if (ok) {
       tc_fence_after();
       const int split = blockIdx.x % p.splits;
@@ -607,6 +615,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (p.splits > 1 && live) *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(top, l);
       tc_fence_before();
+      if (sp.nblocks > 0 && live && *s_bad != 0) {
+        // Rare: NaN among the values of the blocks that `open` cuts, whose product
+        // left them out.  Looked up again in the cache, token by token, by each row.
+        const int to = min(limit, (sp.jb0 + sp.nblocks) * kN);
+        for (int tok = max(sp.jb0, max(sp.open, 0) / kN) * kN; tok < to; ++tok) {
+          const int id = p.c.table[sp.b * p.c.table_ld + tok / p.c.page];
+          if (id < 0 || id >= p.c.pages) continue;
+          const uint8_t* v =
+              p.c.v + ((static_cast<long long>(id) * p.c.kv_heads + sp.head) * p.c.page + tok % p.c.page) * D;
+          for (int c = 0; c < D; ++c) {
+            if ((v[c] & 0x7F) != 0x7F) continue;
+            if (p.splits > 1) {
+              p.o_part[part * D + c] = fp8_nan();
+            } else {
+              dst[c] = from_f32<T>(fp8_nan());
+            }
+          }
+        }
+      }
     }
   }
   __syncwarp();
@@ -663,8 +690,8 @@ int launch(cudaStream_t stream, const KvTileParams& p, unsigned int* status) {
   rc = encode_tiled_u8(&kmap, p.c.k, 2, dims, strides, box, D);
   if (rc == LDB_OK) rc = encode_tiled_u8(&vmap, p.c.v, 2, dims, strides, box, D);
   if (rc != LDB_OK) return rc;
-  rc = launch_kernel(kv_tiles_kernel<D, T, FINE>, dim3(p.row_blocks * p.splits, p.c.kv_heads, p.c.batch), dim3(kThreads),
-                     C::kSmem, stream, "kv_attention tiles launch", kmap, vmap, p, status);
+  rc = launch_kernel(kv_tiles_kernel<D, T, FINE>, dim3(p.row_blocks * p.splits, p.c.kv_heads, p.c.batch),
+                     dim3(kThreads), C::kSmem, stream, "kv_attention tiles launch", kmap, vmap, p, status);
   if (rc != LDB_OK || p.splits == 1) return rc;
   const long long rows = static_cast<long long>(p.c.batch) * p.c.kv_heads * p.rows;
   return launch_kernel(kv_tiles_merge_kernel<D, T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, stream,
@@ -706,7 +733,8 @@ int kv_attention_tiles(cudaStream_t stream, KvTileParams p, int head_dim, int dt
   p.o_part = static_cast<float*>(workspace);
   p.ml_part = p.o_part + static_cast<size_t>(p.splits) * p.c.batch * p.c.kv_heads * p.rows * head_dim;
   if (static_cast<long long>(p.row_blocks) * p.splits > 0x7FFFFFFFll || p.c.kv_heads > 65535 || p.c.batch > 65535)
-    return fail(LDB_ERR_SHAPE, "kv_attention: %d row blocks, %d heads, %d items", p.row_blocks, p.c.kv_heads, p.c.batch);
+    return fail(LDB_ERR_SHAPE, "kv_attention: %d row blocks, %d heads, %d items", p.row_blocks, p.c.kv_heads,
+                p.c.batch);
   return dtype == LDB_F16 ? launch_dim<__half>(stream, p, head_dim, status)
                           : launch_dim<__nv_bfloat16>(stream, p, head_dim, status);
 }

@@ -266,3 +266,78 @@ def test_refusals(cuda_device):
         kv_cache.kv_append(cache, q, q, table, one, counts=ints([1, 1], cuda_device))
     with pytest.raises(ValueError, match="share dtype"):
         kv_cache.kv_append(cache, q, q.float(), table, one)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("queries,group,dim,page", [(1, 4, 128, 64), (5, 2, 64, 16), (12, 1, 32, 32), (7, 2, 128, 128),
+                                                    (70, 1, 64, 64), (130, 2, 128, 16), (300, 1, 32, 128)])
+def test_attention_nan_values_stay_in_their_channel(cuda_device, dtype, causal, queries, group, dim, page):
+    """NaN values in tokens that all, some or none of the queries see: exactly the formula's outputs are NaN."""
+    heads, lengths = 2, [310, 37]
+    table, pages = make_table(2, 320 // page + 1, cuda_device, 21)
+    cache = make_cache(pages, heads, dim, page, cuda_device, 22)
+    for b, head, tok, channel, code in ((0, 0, 309, 3, 0x7F), (0, 1, 305, 0, 0xFF), (0, 1, 306, dim - 1, 0x7F),
+                                        (0, 0, 290, 17, 0x7F), (0, 1, 12, 9, 0xFF), (1, 0, 36, 1, 0x7F),
+                                        (1, 1, 20, 30, 0x7F)):
+        cache.v.view(torch.uint8)[int(table[b, tok // page]), head, tok % page, channel] = code
+    want = host(cache)
+    q = torch.randn(2, queries, heads * group * dim, generator=torch.Generator().manual_seed(23)).to(dtype)
+    ref = oracle.attention(q, *want, table, lengths, group, dim ** -0.5, causal)
+    got = kv_cache.kv_attention(q.to(cuda_device), cache, table.to(cuda_device), ints(lengths, cuda_device),
+                                scale=dim ** -0.5, causal=causal)
+    nan = torch.isnan(ref["out"])
+    assert nan.any() and not nan.all()
+    assert torch.equal(torch.isnan(got.cpu().view(nan.shape)), nan)
+    finite = {k: torch.where(torch.isnan(x), torch.zeros_like(x), x) for k, x in ref.items()}
+    check_attention(torch.where(nan.to(cuda_device), 0.0, got.view(nan.shape)), finite, dtype)
+
+
+@pytest.mark.parametrize("queries", [9, 60, 200])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_attention_queries_without_keys_are_zero_whatever_they_hold(cuda_device, queries, value):
+    heads, dim, page, n = 1, 64, 64, 6  # the first queries - 6 queries see nothing
+    table, pages = make_table(1, 1, cuda_device, 31)
+    cache = make_cache(pages, heads, dim, page, cuda_device, 32)
+    q = torch.randn(1, queries, dim, generator=torch.Generator().manual_seed(33)).to(torch.float16)
+    ref = oracle.attention(q, *host(cache), table, [n], 1, 0.125, True)
+    q[0, 1, 5] = value
+    got = kv_cache.kv_attention(q.to(cuda_device), cache, table.to(cuda_device), ints([n], cuda_device), scale=0.125,
+                                causal=True)
+    assert (got[0, : queries - n] == 0).all()
+    check_attention(got, ref, torch.float16)
+    q[0, -2, 5] = value  # one that sees keys becomes NaN, and no other does
+    got = kv_cache.kv_attention(q.to(cuda_device), cache, table.to(cuda_device), ints([n], cuda_device), scale=0.125,
+                                causal=True)
+    assert torch.isnan(got[0, -2]).all()
+    rest = [i for i in range(queries) if i != queries - 2]
+    check_attention(got[:, rest], {k: x[:, rest] for k, x in ref.items()}, torch.float16)
+
+
+@pytest.mark.parametrize("queries,group,dim,page", [(1, 4, 128, 64), (3, 1, 64, 16), (3, 4, 32, 32), (20, 2, 128, 128),
+                                                    (90, 1, 64, 16), (130, 2, 128, 64), (64, 1, 32, 128)])
+@pytest.mark.parametrize("lost", [-1, 1 << 20])
+def test_attention_leaves_out_pages_outside_the_cache(cuda_device, queries, group, dim, page, lost):
+    """The result without the tokens of such a page, and a status bit; an item with no other page gives zeros."""
+    heads, dtype = 2, torch.bfloat16
+    lengths = [3 * page + 5, page - 3]
+    table, pages = make_table(2, 4, cuda_device, 41)
+    cache = make_cache(pages, heads, dim, page, cuda_device, 42)
+    q = torch.randn(2, queries, heads * group * dim, generator=torch.Generator().manual_seed(43)).to(dtype)
+    kept = table.clone()
+    kept[0, :3] = table[0, [0, 2, 3]]
+    ref = oracle.attention(q, *host(cache), kept, [2 * page + 5, 0], group, dim ** -0.5, False)
+    holes = table.clone()
+    holes[0, 1], holes[1, 0] = lost, lost
+    got = kv_cache.kv_attention(q.to(cuda_device), cache, holes.to(cuda_device), ints(lengths, cuda_device),
+                                scale=dim ** -0.5)
+    assert _lib.device_status(reset=True) == 2
+    check_attention(got, ref, dtype)
+
+
+def test_attention_refuses_items_that_overlap_in_the_output(cuda_device):
+    cache = make_cache(4, 1, 64, 32, cuda_device, 1)
+    table, lengths = ints([[0], [1]], cuda_device), ints([3, 3], cuda_device)
+    q = torch.zeros(2, 1, 64, device=cuda_device, dtype=torch.float16)
+    with pytest.raises(_lib.LdbError, match="item stride"):
+        kv_cache.kv_attention(q, cache, table, lengths, scale=1.0, out=q[:1].expand(2, 1, 64))
