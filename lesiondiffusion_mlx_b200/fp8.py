@@ -16,6 +16,7 @@ launches on the current stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -53,20 +54,22 @@ class Fp8Weight(NamedTuple):
 
 def _flat(t: torch.Tensor, name: str) -> tuple[int, int, int]:
     """(rows, channels, row stride) of a channels-last tensor dense over its rows."""
-    if t.ndim == 2:
-        rows, k = t.shape
+    shape = t.shape
+    if len(shape) < 2:
+        raise ValueError(f"{name}: expected (..., channels) with at least two axes")
+    k = shape[-1]
+    if t.is_contiguous() and k:
+        rows, ld = t.numel() // k, k
+    elif len(shape) == 2:
+        rows = shape[0]
         ld, step = t.stride()
         if step != 1 and k != 1:
             raise ValueError(f"{name}: channel axis must have unit stride")
-        if rows > _MAX_ROWS:
-            raise ValueError(f"{name}: {rows} rows (at most {_MAX_ROWS})")
-        return rows, k, ld if rows > 1 or ld > k else k
-    if t.ndim < 2:
-        raise ValueError(f"{name}: expected (..., channels) with at least two axes")
-    per, k, ld = _rows(t)
-    rows = t.shape[0] * per
-    if t.shape[0] > 1 and per and t.stride(0) != per * ld:
-        raise ValueError(f"{name}: tensor must be dense over its rows")
+    else:
+        per, k, ld = _rows(t)
+        rows = shape[0] * per
+        if shape[0] > 1 and per and t.stride(0) != per * ld:
+            raise ValueError(f"{name}: tensor must be dense over its rows")
     if rows > _MAX_ROWS:
         raise ValueError(f"{name}: {rows} rows (at most {_MAX_ROWS})")
     return rows, k, max(ld, k) if rows <= 1 else ld
@@ -79,8 +82,12 @@ def _quantized(x: torch.Tensor, k: int) -> tuple[Fp8Rows, int, int]:
     ld, s_ld = (k + 15) // 16 * 16, (blocks + 3) // 4 * 4
     codes = (torch.empty_like(x, dtype=CODES, memory_format=torch.contiguous_format) if ld == k
              else x.new_empty((*lead, ld), dtype=CODES))
-    scales = x.new_empty((*lead, s_ld), dtype=SCALES)
-    return Fp8Rows(codes if ld == k else codes[..., :k], scales if s_ld == blocks else scales[..., :blocks]), ld, s_ld
+    strides, step = [1], s_ld
+    for n in reversed(lead):
+        strides.insert(0, step)
+        step *= n
+    scales = x.new_empty_strided((*lead, blocks), strides, dtype=SCALES)
+    return Fp8Rows(codes if ld == k else codes[..., :k], scales), ld, s_ld
 
 
 def _launcher(kind: str, flops: float = 0.0):
@@ -95,6 +102,14 @@ def _launcher(kind: str, flops: float = 0.0):
             _lib.call(name, *args)
 
     return call
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(name: str, device: int, *sizes: int) -> int:
+    """What the library's ``name`` says for these sizes (asking costs a token's call a tenth of its time)."""
+    need = ctypes.c_size_t()
+    _lib.call(name, *sizes, ctypes.byref(need))
+    return need.value
 
 
 def _check_input(x: torch.Tensor, name: str) -> None:
@@ -208,12 +223,12 @@ def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, *, re
         raise ValueError("matmul_fp8: all tensors must be on one device")
     if m == 0:
         return out
-    need = ctypes.c_size_t()
-    _lib.call("ldb_matmul_fp8_workspace_size", m, n, k, ctypes.byref(need))
-    if need.value:
-        ws = codes.new_empty(need.value, dtype=torch.uint8)
+    device = codes.get_device()
+    need = _workspace_bytes("ldb_matmul_fp8_workspace_size", device, m, n, k)
+    if need:
+        ws = codes.new_empty(need, dtype=torch.uint8)
         ws_ptr = ws.data_ptr()
-    _launcher("matmul_fp8", 2.0 * m * n * k)("ldb_matmul_fp8", _raw_stream(codes.get_device()), codes.data_ptr(), a_ld,
+    _launcher("matmul_fp8", 2.0 * m * n * k)("ldb_matmul_fp8", _raw_stream(device), codes.data_ptr(), a_ld,
             scales.data_ptr(), s_ld, w_codes.data_ptr(), w_ld, w_scales.data_ptr(), ws_ld, bias_ptr, residual_ptr,
-            r_ld, out.data_ptr(), out_ld, m, n, k, act, _DT[out_dtype], ws_ptr, need.value)
+            r_ld, out.data_ptr(), out_ld, m, n, k, act, _DT[out_dtype], ws_ptr, need)
     return out

@@ -16,13 +16,12 @@ the cache is left out and sets the device status (``ldb_device_status``).
 
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from .fp8 import CODES, SCALES, _launcher, _raw_stream
+from .fp8 import CODES, SCALES, _launcher, _raw_stream, _workspace_bytes
 from .ops import _DT
 
 HEAD_DIMS = (32, 64, 128)
@@ -140,14 +139,14 @@ def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, length
         raise ValueError("kv_attention: out must have q's shape, dtype and device, and unit channel stride")
     out_batch, out_ld, _ = out.stride()
     heads = channels // dim
-    need = ctypes.c_size_t()
-    _lib.call("ldb_kv_attention_fp8_workspace_size", batch, queries, heads, kv_heads, dim, ctypes.byref(need))
+    index = q.get_device()
+    need = _workspace_bytes("ldb_kv_attention_fp8_workspace_size", index, batch, queries, heads, kv_heads, dim)
     ws_ptr = None
-    if need.value:
-        ws = q.new_empty(need.value, dtype=torch.uint8)
+    if need:
+        ws = q.new_empty(need, dtype=torch.uint8)
         ws_ptr = ws.data_ptr()
-    _launcher("kv_attention")("ldb_kv_attention_fp8", _raw_stream(q.get_device()), q.data_ptr(), q_ld, q_batch,
+    _launcher("kv_attention")("ldb_kv_attention_fp8", _raw_stream(index), q.data_ptr(), q_ld, q_batch,
             _DT[q.dtype], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
             pages, kv_heads, page, dim, table.data_ptr(), table_ld, width, lengths.data_ptr(), out.data_ptr(), out_ld,
-            out_batch, batch, queries, heads, scale, int(causal), ws_ptr, need.value)
+            out_batch, batch, queries, heads, scale, int(causal), ws_ptr, need)
     return out
