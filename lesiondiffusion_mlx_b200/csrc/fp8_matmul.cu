@@ -140,7 +140,8 @@ __device__ __forceinline__ float gelu1(float y) {
   return y;
 }
 
-// 32 columns of one output row before the rounding: bias, residual, activation.
+// 32 columns of one output row before the rounding: bias, residual, activation
+// (outputs and residuals that allow 16-byte accesses).
 template <typename T>
 __device__ __forceinline__ void finish32(const MatmulParams& p, int row, int col, float (&v)[32]) {
   const bool full = col + 32 <= p.n;
@@ -159,7 +160,7 @@ __device__ __forceinline__ void finish32(const MatmulParams& p, int row, int col
   }
   if (p.residual && row < p.m) {
     const T* r = static_cast<const T*>(p.residual) + row * p.res_ld + col;
-    if (full && p.vec) {
+    if (full) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         float a[8];
@@ -179,7 +180,58 @@ __device__ __forceinline__ void finish32(const MatmulParams& p, int row, int col
   }
 }
 
-template <typename T, bool PAIR>
+// The same for outputs that allow no 16-byte accesses: 32 x 32 FP32 values staged
+// in shared memory, a column per lane, so that a warp's accesses are one row
+// each.  (A row per lane, value by value: 12983 x 358 -> 1961 took 253 us instead
+// of 59; whole rows of 1960 columns take 27.)
+template <typename T>
+__device__ __forceinline__ void finish_rows(const MatmulParams& p, int split, int row0, int col, const uint8_t* staging) {
+  const int lane = lane_id(), rows = min(32, p.m - row0);
+  const int c = col + lane;
+  const bool live = c < p.n;
+  const bool last = p.split == 1;  // else a range's partial sums
+  const float bias = last && p.bias && live ? p.bias[c] : 0.f;
+  const T* res = static_cast<const T*>(p.residual) + (p.residual ? row0 * p.res_ld + c : 0);
+  float* part = p.partial + (static_cast<long long>(split) * p.m + row0) * p.n + c;
+  T* out = static_cast<T*>(p.out) + row0 * p.out_ld + c;
+  T a[32];  // all rows' loads in flight together
+  if (last && p.residual) {
+#pragma unroll
+    for (int u = 0; u < 32; ++u) a[u] = live && u < rows ? res[u * p.res_ld] : from_f32<T>(0.f);
+  }
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 8) {
+    if (r0 >= rows) break;
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      v[u] = *reinterpret_cast<const float*>(staging + swizzle_offset((r0 + u) * 128 + lane * 4, 128));
+    if (!last) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (live && r0 + u < rows) part[static_cast<long long>(r0 + u) * p.n] = v[u];
+      continue;
+    }
+    if (p.bias) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] += bias;
+    }
+    if (p.residual) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] += to_f32<T>(a[r0 + u]);
+    }
+    if (p.act == LDB_ACT_GELU) {
+#pragma unroll
+      for (int u = 0; u < 8; u += 2) gelu2(v[u], v[u + 1]);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (live && r0 + u < rows) out[(r0 + u) * p.out_ld] = from_f32<T>(v[u]);
+  }
+}
+
+// WHOLE: 16-byte accesses to the rows of what is written (and the residual's).
+template <typename T, bool PAIR, bool WHOLE>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_matmul_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap wmap,
                       const __grid_constant__ CUtensorMap omap, const MatmulParams p, unsigned int* status) {
@@ -449,7 +501,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kBuffers = kStagingBytes / (32 * kRowBytes);
     uint8_t* staging = s_out + (warp - 4) * kStagingBytes;
     const int quarter = warp & 3;
-    const bool staged = p.vec && p.split == 1;
     int tile = 0, buffer = 0;
     for (int i = item0; i < items; i += item_step, ++tile) {
       const Work w = work_item<PAIR>(p, i, kblocks, rank);
@@ -466,23 +517,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
         const int col = w.col0 + c;
-        if (p.split > 1) {
+        if constexpr (!WHOLE) {
+#pragma unroll
+          for (int h = 0; h < 8; ++h)
+            *reinterpret_cast<float4*>(staging + swizzle_offset(lane * 128 + h * 16, 128)) =
+                make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+          __syncwarp();
+          finish_rows<T>(p, w.split, row0, col, staging);
+          __syncwarp();
+        } else if (p.split > 1) {
           if (row < p.m) {
             float* o = p.partial + (static_cast<long long>(w.split) * p.m + row) * p.n + col;
-            if (p.n % 4 == 0 && col + 32 <= p.n) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8; ++j)
+              if (col + 4 * j < p.n)
                 reinterpret_cast<float4*>(o)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (col + j < p.n) o[j] = v[j];
-            }
           }
-          continue;
-        }
-        finish32<T>(p, row, col, v);
-        if (staged) {
+        } else {
+          finish32<T>(p, row, col, v);
           // the store before last (16-bit) or last (FP32) has read this buffer
           uint8_t* out = staging + buffer * 32 * kRowBytes;
           if (lane == 0) bulk_wait_group_read<kBuffers - 1>();
@@ -503,11 +555,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             bulk_commit_group();
           }
           if (++buffer == kBuffers) buffer = 0;
-        } else if (row < p.m) {
-          T* o = static_cast<T*>(p.out) + row * p.out_ld + col;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (col + j < p.n) o[j] = from_f32<T>(v[j]);
         }
       }
       tc_fence_before();
@@ -610,7 +657,7 @@ size_t partial_bytes(const MatmulParams& p) {
   return p.split > 1 ? static_cast<size_t>(p.split) * p.m * p.n * sizeof(float) : 0;
 }
 
-template <typename T>
+template <typename T, bool WHOLE>
 int launch(cudaStream_t stream, const CUtensorMap& amap, const CUtensorMap& wmap, const MatmulParams& p,
            unsigned int* status) {
   static unsigned long long configured = 0;
@@ -619,7 +666,7 @@ int launch(cudaStream_t stream, const CUtensorMap& amap, const CUtensorMap& wmap
   const int smem = kFixed + p.stages * (kTileM + (p.pair ? p.bn / 2 : p.bn)) * 128;
   CUtensorMap omap = amap;  // (not used without TMA stores)
   int rc = LDB_OK;
-  if (p.vec && p.split == 1) {
+  if (WHOLE && p.split == 1) {
     const uint64_t dims[2] = {static_cast<uint64_t>(p.n), static_cast<uint64_t>(p.m)};
     const uint64_t strides[1] = {static_cast<uint64_t>(p.out_ld) * sizeof(T)};
     const uint32_t box[2] = {32, 32};
@@ -632,23 +679,30 @@ int launch(cudaStream_t stream, const CUtensorMap& amap, const CUtensorMap& wmap
   }
   if (p.pair) {
     static unsigned long long pair_configured = 0;
-    rc = ensure_smem_attribute(reinterpret_cast<const void*>(fp8_matmul_kernel<T, true>), kFixed + kSmemBudget,
+    rc = ensure_smem_attribute(reinterpret_cast<const void*>(fp8_matmul_kernel<T, true, WHOLE>), kFixed + kSmemBudget,
                                &pair_configured, "matmul_fp8 shared memory");
     if (rc != LDB_OK) return rc;
     const int pairs = std::min(p.tiles_m * p.tiles_n, sm_count() / 2);
-    return launch_kernel_cluster(fp8_matmul_kernel<T, true>, dim3(2 * pairs), dim3(kThreads), smem, stream,
+    return launch_kernel_cluster(fp8_matmul_kernel<T, true, WHOLE>, dim3(2 * pairs), dim3(kThreads), smem, stream,
                                  "matmul_fp8 (CTA pairs) launch", 2u, amap, wmap, omap, p, status);
   }
-  rc = ensure_smem_attribute(reinterpret_cast<const void*>(fp8_matmul_kernel<T, false>), kFixed + kSmemBudget,
+  rc = ensure_smem_attribute(reinterpret_cast<const void*>(fp8_matmul_kernel<T, false, WHOLE>), kFixed + kSmemBudget,
                              &configured, "matmul_fp8 shared memory");
   if (rc != LDB_OK) return rc;
   const int items = p.tiles_m * p.tiles_n * p.split;
-  rc = launch_kernel(fp8_matmul_kernel<T, false>, dim3(std::min(items, sm_count())), dim3(kThreads), smem, stream,
+  rc = launch_kernel(fp8_matmul_kernel<T, false, WHOLE>, dim3(std::min(items, sm_count())), dim3(kThreads), smem, stream,
                      "matmul_fp8 launch", amap, wmap, omap, p, status);
   if (rc != LDB_OK || p.split == 1) return rc;
   const long long total = static_cast<long long>(p.m) * p.n;
   const int blocks = static_cast<int>(std::min<long long>((total + 255) / 256, 4ll * sm_count()));
   return launch_kernel(fp8_matmul_reduce_kernel<T>, dim3(blocks), dim3(256), 0, stream, "matmul_fp8 reduce launch", p);
+}
+
+template <typename T>
+int launch_rows(cudaStream_t stream, const CUtensorMap& amap, const CUtensorMap& wmap, const MatmulParams& p,
+                unsigned int* status) {
+  const bool whole = p.split > 1 ? p.n % 4 == 0 : p.vec != 0;
+  return whole ? launch<T, true>(stream, amap, wmap, p, status) : launch<T, false>(stream, amap, wmap, p, status);
 }
 
 }  // namespace
@@ -711,9 +765,9 @@ int ldb_matmul_fp8(cudaStream_t stream, const uint8_t* a, long long a_ld, const 
   rc = encode_tiled_u8(&amap, a, 2, adims, astride, abox, 128);
   if (rc == LDB_OK) rc = encode_tiled_u8(&wmap, w, 2, wdims, wstride, wbox, 128);
   if (rc != LDB_OK) return rc;
-  if (out_dtype == LDB_F16) return launch<__half>(stream, amap, wmap, p, status);
-  if (out_dtype == LDB_BF16) return launch<__nv_bfloat16>(stream, amap, wmap, p, status);
-  return launch<float>(stream, amap, wmap, p, status);
+  if (out_dtype == LDB_F16) return launch_rows<__half>(stream, amap, wmap, p, status);
+  if (out_dtype == LDB_BF16) return launch_rows<__nv_bfloat16>(stream, amap, wmap, p, status);
+  return launch_rows<float>(stream, amap, wmap, p, status);
 }
 
 }  // extern "C"

@@ -308,3 +308,28 @@ def test_rms_norm_reads_gamma_after_its_producer(cuda_device):
         want, _ = fp8.rms_norm_fp8(x, gamma[0])
         assert torch.equal(got.codes.view(torch.uint8), want.codes.view(torch.uint8)), seed
         assert torch.equal(got.scales.view(torch.uint8), want.scales.view(torch.uint8)), seed
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k,residual,gelu", [(1, 33, 130, True, False), (37, 61, 4096, True, True),
+                                                 (130, 257, 2500, False, False), (333, 999, 200, True, True),
+                                                 (1030, 1027, 2050, True, False), (2051, 1601, 140, False, True)])
+def test_matmul_narrow_outputs(cuda_device, dtype, m, n, k, residual, gelu):
+    """Outputs and residuals without 16-byte rows, inside wider ones whose other values stay."""
+    rows, weight, av, wv = operands(m, n, k, cuda_device, m + n + k)
+    g = torch.Generator().manual_seed(2)
+    b = torch.randn(n, generator=g)
+    r = torch.randn(m, n + 2, generator=g).to(dtype)[:, 1 : n + 1] if residual else None
+    wide = torch.full((m + 1, n + 4), 3.0, dtype=dtype, device=cuda_device)
+    out = wide[:m, 1 : n + 1]
+    wide_r = None
+    if residual:
+        wide_r = torch.zeros(m, n + 2, dtype=dtype, device=cuda_device)
+        wide_r[:, 1 : n + 1] = r.to(cuda_device)
+        wide_r = wide_r[:, 1 : n + 1]
+    fp8.matmul_fp8(rows, weight, b.to(cuda_device), residual=wide_r, out=out, out_dtype=dtype,
+                   act=_lib.LDB_ACT_GELU if gelu else _lib.LDB_ACT_NONE)
+    want, size = oracle.matmul(av, wv, b, r, gelu)
+    check_product(out, want, size, dtype, slope=1.5 if gelu else 1.0)
+    assert (wide[m:] == 3).all() and (wide[:, :1] == 3).all() and (wide[:, n + 1:] == 3).all()
+    assert _lib.device_status(reset=True) == 0
