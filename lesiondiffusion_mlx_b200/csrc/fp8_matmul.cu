@@ -185,7 +185,8 @@ __device__ __forceinline__ void finish32(const MatmulParams& p, int row, int col
 // each.  (A row per lane, value by value: 12983 x 358 -> 1961 took 253 us instead
 // of 59; whole rows of 1960 columns take 27.)
 template <typename T>
-__device__ __forceinline__ void finish_rows(const MatmulParams& p, int split, int row0, int col, const uint8_t* staging) {
+__device__ __forceinline__ void finish_rows(const MatmulParams& p, int split, int row0, int col,
+                                            const uint8_t* staging) {
   const int lane = lane_id(), rows = min(32, p.m - row0);
   const int c = col + lane;
   const bool live = c < p.n;

@@ -215,7 +215,8 @@ struct Fetch {
     for (int h = 0; h < 2; ++h) {  // rows 0 .. 15 and 16 .. 31
       const int page_id = h == 0 ? id0 : id1;
       const int row = c.page < kTile ? 0 : inside + 16 * h;
-      const long long off = ((static_cast<long long>(max(page_id, 0)) * c.kv_heads + head) * c.page + row) * D + lane * 16;
+      const long long off =
+          ((static_cast<long long>(max(page_id, 0)) * c.kv_heads + head) * c.page + row) * D + lane * 16;
       const uint32_t bytes = page_id < 0 ? 0u : 16u;  // zeros for what has no page
 #pragma unroll
       for (int i = 0; i < kUnits / 2; ++i) {
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
       }
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const int e = m > 0.f ? min(126, max(-119, static_cast<int>(__float_as_uint(m) >> 23) - 127)) : 0;
+      const int e = kv_query_exponent(m);
       qs[r] = fp8_is_finite(m) ? fp8_pow2(e - 7) : fp8_nan();
       const float inv = fp8_pow2(7 - e);
 #pragma unroll

@@ -37,6 +37,11 @@ __device__ __forceinline__ uint32_t kv_nan_codes(uint32_t w) { return ((w & 0x7F
 // The same codes with each NaN turned into zero.
 __device__ __forceinline__ uint32_t kv_without_nan(uint32_t w) { return w & ~((kv_nan_codes(w) >> 7) * 0xFFu); }
 
+// The power of two of a row's largest magnitude, within what its factors can express.
+__device__ __forceinline__ int kv_query_exponent(float m) {
+  return m > 0.f ? min(126, max(-119, static_cast<int>(__float_as_uint(m) >> 23) - 127)) : 0;
+}
+
 struct KvTileParams {
   KvView c;
   const void* q;

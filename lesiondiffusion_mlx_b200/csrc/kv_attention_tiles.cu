@@ -219,18 +219,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const int off = first - batch0;
-        // factors of the block's eight groups of 16 tokens
-        const int of_group = off + ((lane & 7) * 16 >> shift);
-        const float gk = __shfl_sync(0xffffffffu, kf, of_group & 31);
-        const float ge = __shfl_sync(0xffffffffu, ev, of_group & 31);
         const int my_id = __shfl_sync(0xffffffffu, id, (off + lane) & 31);
         const int st = j & 1, ms = j % kMeta;
         const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u;
         ok = warp_wait(&k_empty[st], ph ^ 1u, abort_flag, status);
         if (!ok) break;
-        // (slot ms: the scores of block j - 2 are done, so the softmax of block j - 4 is)
-        if (lane < kGroups)
-          s_meta[ms * kGroups + lane] = make_float4(gk, ge, fp8_pow2(-max(static_cast<int>(ge), -127)), 0.f);
         const bool load = lane < loads && my_id >= 0;
         // pages that the table should name and does not: zeros in their place
         const uint32_t holes = __ballot_sync(0xffffffffu, lane < loads && my_id < 0 && first + lane < used);
@@ -245,13 +238,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, load)) * box * D;
         const int row = (my_id * p.c.kv_heads + sp.head) * p.c.page;
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&meta_full[ms]);
-          mbar_arrive_expect_tx(&k_full[st], bytes);
-        }
+        if (lane == 0) mbar_arrive_expect_tx(&k_full[st], bytes);
         __syncwarp();
         if (load) tma_load_2d(smem + C::kOffK + st * C::kRawBytes + lane * box * D, &kmap, &k_full[st], 0, row);
         ++k_loads;
+        // Factors of the block's eight groups of 16 tokens, once the loads are on their
+        // way (slot ms: the scores of block j - 2 are done, so the softmax of block j - 4 is).
+        const int of_group = off + ((lane & 7) * 16 >> shift);
+        const float gk = __shfl_sync(0xffffffffu, kf, of_group & 31);
+        const float ge = __shfl_sync(0xffffffffu, ev, of_group & 31);
+        if (lane < kGroups)
+          s_meta[ms * kGroups + lane] = make_float4(gk, ge, fp8_pow2(-max(static_cast<int>(ge), -127)), 0.f);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&meta_full[ms]);
         ok = warp_wait(&v_empty[st], ph ^ 1u, abort_flag, status);
         if (!ok) break;
         if (holes) blank(smem + C::kOffV + st * C::kRawBytes);
@@ -418,49 +417,73 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int limit = p.causal && live ? min(sp.len, sp.len - p.queries + i + 1) : sp.len;  // keys that the row sees
     float qs = 1.f;
     if (t < sp.tiles && sp.nblocks > 0) {
-      // Query row in parts: the largest magnitude to [128, 256); a NaN stays
+      // Query rows in parts: the largest magnitude to [128, 256); a NaN stays
       // one, an infinity makes the row's factor one (of a row that sees any key).
+      // D / 8 neighbouring lanes read a row, eight channels each: with a row per
+      // lane it took 10500 cycles at D = 128 in three parts, now 8400.
+      constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes of a row, rows at a time
       const T* src = static_cast<const T*>(p.q) + sp.b * p.q_batch + i * p.q_ld +
                      (static_cast<long long>(sp.head) * p.group + gq) * D;
-      uint32_t raw[D / 2];
+      const int part_lane = lane % kLanes;
+      auto rows_from = [&](int n0, uint4(&raw)[4]) {
 #pragma unroll
-      for (int k = 0; k < D / 8; ++k) {
-        if (!live) {
-          raw[4 * k] = raw[4 * k + 1] = raw[4 * k + 2] = raw[4 * k + 3] = 0;
-        } else if (p.q_vec) {
-          const uint4 v = reinterpret_cast<const uint4*>(src)[k];
-          raw[4 * k] = v.x, raw[4 * k + 1] = v.y, raw[4 * k + 2] = v.z, raw[4 * k + 3] = v.w;
-        } else {
-          const uint16_t* h = reinterpret_cast<const uint16_t*>(src) + 8 * k;
+        for (int n = 0; n < 4; ++n) {
+          const int from = (n0 + n) * kRows + lane / kLanes;  // row of the warp, and the lane that owns it
+          const T* at = reinterpret_cast<const T*>(__shfl_sync(
+                            0xffffffffu, reinterpret_cast<unsigned long long>(src), from & 31)) + 8 * part_lane;
+          raw[n] = make_uint4(0, 0, 0, 0);
+          if (from < 32 && sp.row0 + t * kM + quarter * 32 + from < p.rows) {
+            if (p.q_vec) {
+              raw[n] = *reinterpret_cast<const uint4*>(at);
+            } else {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(at);
+              raw[n] = make_uint4(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16,
+                                  h[4] | static_cast<uint32_t>(h[5]) << 16, h[6] | static_cast<uint32_t>(h[7]) << 16);
+            }
+          }
+        }
+      };
+      float top_of = 0.f;  // largest magnitude of the lane's own row
+      uint4 next[4];
+      rows_from(0, next);
+#pragma unroll 1
+      for (int n0 = 0; n0 < kLanes; n0 += 4) {
+        uint4 raw[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) raw[4 * k + e] = h[2 * e] | static_cast<uint32_t>(h[2 * e + 1]) << 16;
+        for (int k = 0; k < 4; ++k) raw[k] = next[k];
+        rows_from(n0 + 4, next);
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) {
+          const int n = n0 + k4;
+          const uint32_t w[4] = {raw[k4].x, raw[k4].y, raw[k4].z, raw[k4].w};
+          float m = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 x = kv_unpack2<T>(w[k]);
+            m = fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y)));
+          }
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const float own = __shfl_sync(0xffffffffu, m, (lane % kRows) * kLanes);
+          if (lane / kRows == n) top_of = own;
+          const float factor = fp8_pow2(7 - kv_query_exponent(m));
+          const float inv = p.negate ? -factor : factor;
+          uint32_t parts[PARTS][2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float2 x = kv_unpack2<T>(w[2 * k]), y = kv_unpack2<T>(w[2 * k + 1]);
+            __half2 rest[2] = {__floats2half2_rn(x.x * inv, x.y * inv), __floats2half2_rn(y.x * inv, y.y * inv)};
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) parts[part][k] = kv_split_part<1>(rest);
+          }
+          const int at = swizzle_offset((quarter * 32 + n * kRows + lane / kLanes) * D + 8 * part_lane, D);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part)
+            *reinterpret_cast<uint2*>(smem + (t * PARTS + part) * C::kPartBytes + at) =
+                make_uint2(parts[part][0], parts[part][1]);
         }
       }
-      float m = 0.f;
-#pragma unroll
-      for (int k = 0; k < D / 2; ++k) {
-        const float2 x = kv_unpack2<T>(raw[k]);
-        m = fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y)));
-      }
-      const int e = m > 0.f ? min(126, max(-119, static_cast<int>(__float_as_uint(m) >> 23) - 127)) : 0;
-      qs = fp8_is_finite(m) || limit <= 0 ? fp8_pow2(e - 7) : fp8_nan();
-      const float inv = p.negate ? -fp8_pow2(7 - e) : fp8_pow2(7 - e);
-#pragma unroll
-      for (int chunk = 0; chunk < D / 16; ++chunk) {
-        uint32_t parts[PARTS][4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float2 x = kv_unpack2<T>(raw[8 * chunk + 2 * w]), y = kv_unpack2<T>(raw[8 * chunk + 2 * w + 1]);
-          __half2 rest[2] = {__floats2half2_rn(x.x * inv, x.y * inv), __floats2half2_rn(y.x * inv, y.y * inv)};
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) parts[part][w] = kv_split_part<1>(rest);
-        }
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part)
-          *reinterpret_cast<uint4*>(smem + (t * PARTS + part) * C::kPartBytes +
-                                    swizzle_offset(local * D + chunk * 16, D)) =
-              make_uint4(parts[part][0], parts[part][1], parts[part][2], parts[part][3]);
-      }
+      qs = fp8_is_finite(top_of) || limit <= 0 ? fp8_pow2(kv_query_exponent(top_of) - 7) : fp8_nan();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
@@ -581,7 +604,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       T* dst = static_cast<T*>(p.out) + sp.b * p.out_batch + i * p.out_ld +
                (static_cast<long long>(sp.head) * p.group + gq) * D;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
+      // (one range: rows to shared memory, where the queries were, and from there D /
+      // 8 lanes a row; stored a row per lane they took 6000 cycles at D = 128, now 4200)
+      constexpr int kChunks = D / 8, kSpread = kChunks < 8 ? kChunks - 1 : 7;  // 16-byte pieces of an output row
+      uint8_t* rows = smem + t * PARTS * C::kPartBytes + quarter * 32 * D * 2;
+      static_assert(PARTS >= 2, "an output tile fits where its queries were");
+#pragma unroll 2
       for (int c0 = 0; c0 < D; c0 += 16) {
         uint32_t r[16];
         if (sp.nblocks > 0) {
@@ -591,8 +619,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < 16; ++c) r[c] = 0;
         }
-        if (!live) continue;
         if (p.splits > 1) {
+          if (!live) continue;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             reinterpret_cast<float4*>(p.o_part + part * D + c0)[c] =
@@ -604,14 +632,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             float v[8];
 #pragma unroll
             for (int c = 0; c < 8; ++c) v[c] = __uint_as_float(r[8 * h + c]) * inv;
-            if (p.out_vec) {
-              store8<T>(dst + c0 + 8 * h, v);
-            } else {
-#pragma unroll
-              for (int c = 0; c < 8; ++c) dst[c0 + 8 * h + c] = from_f32<T>(v[c]);
-            }
+            store8<T>(reinterpret_cast<T*>(rows + lane * D * 2 + ((c0 / 8 + h) ^ (lane & kSpread)) * 16), v);
           }
         }
+      }
+      if (p.splits == 1) {
+        __syncwarp();
+        constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+#pragma unroll 4
+        for (int n = 0; n < kLanes; ++n) {
+          const int from = n * kRows + lane / kLanes, chunk = lane % kLanes;
+          T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from)) +
+                  8 * chunk;
+          if (sp.row0 + t * kM + quarter * 32 + from >= p.rows) continue;
+          const uint4 v = *reinterpret_cast<const uint4*>(rows + from * D * 2 + (chunk ^ (from & kSpread)) * 16);
+          if (p.out_vec) {
+            *reinterpret_cast<uint4*>(to) = v;
+          } else {
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) to[c] = e[c];
+          }
+        }
+        __syncwarp();
       }
       if (p.splits > 1 && live) *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(top, l);
       tc_fence_before();
@@ -712,9 +755,10 @@ int launch_dim(cudaStream_t stream, const KvTileParams& p, int head_dim, unsigne
 
 }  // namespace
 
+// Most ranges of tokens: grids of up to four waves may be cut, to up to four waves.
 int kv_tile_splits(int batch, int kv_heads, long long rows) {
   const long long ctas = (rows + 2 * kM - 1) / (2 * kM) * kv_heads * batch;
-  return static_cast<int>(std::max(1ll, std::min(32ll, sm_count() / std::max(1ll, ctas))));
+  return static_cast<int>(std::max(1ll, std::min(32ll, 4ll * sm_count() / std::max(1ll, ctas))));
 }
 
 size_t kv_tile_workspace(int batch, int kv_heads, long long rows, int head_dim) {
@@ -724,10 +768,21 @@ size_t kv_tile_workspace(int batch, int kv_heads, long long rows, int head_dim) 
 
 int kv_attention_tiles(cudaStream_t stream, KvTileParams p, int head_dim, int dtype, float scale, void* workspace,
                        unsigned int* status) {
-  // (at least two blocks of the longest item a range)
+  // Ranges from the table's capacity, in the time of a block of 128 tokens: a
+  // CTA's start and end take about five, the partial rows are written and read
+  // once, and there is a second kernel.  (The lengths are on the device; shorter and
+  // ragged items leave the order of the counts about as it is.)  7 items of up to 19724
+  // tokens, 523 causal queries, 4 heads of 32: 324 us in one range, 149 in five.
   const long long blocks = (static_cast<long long>(p.c.width) * p.c.page + kN - 1) / kN;
-  p.splits = static_cast<int>(std::min<long long>(kv_tile_splits(p.c.batch, p.c.kv_heads, p.rows), (blocks + 1) / 2));
   p.row_blocks = (p.rows + 2 * kM - 1) / (2 * kM);
+  const long long ctas = static_cast<long long>(p.row_blocks) * p.c.kv_heads * p.c.batch, sms = sm_count();
+  const double merge = static_cast<double>(p.c.batch) * p.c.kv_heads * p.rows * head_dim * 8 / 12e6;  // a range
+  double best = 0;
+  for (int s = 1; s <= std::min<long long>(kv_tile_splits(p.c.batch, p.c.kv_heads, p.rows), (blocks + 1) / 2); ++s) {
+    const double cost = static_cast<double>((ctas * s + sms - 1) / sms) * ((blocks + s - 1) / s + 5) +
+                        (s > 1 ? 2 + merge * s : 0);
+    if (s == 1 || cost < best) best = cost, p.splits = s;
+  }
   p.negate = scale < 0.f;
   p.scale_log2 = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
   p.o_part = static_cast<float*>(workspace);
