@@ -12,8 +12,8 @@
 // lanes hold the 128 channels of a scale and find its maximum with four
 // shuffles.  Rows of up to 1024 channels take one warp (no barrier), wider rows
 // a block; the grid is resident and walks the rows.  One B200: 51201 x 1000 bf16
-// with a residual 69 us (5.2 TB/s, 0.81 of the copy rate), 6400 x 256 f16 3.5
-// us, one row 2.1 us.
+// with a residual 68 us (5.3 TB/s, 0.82 of the copy rate), 6400 x 256 f16 3.8
+// us, one row 2.4 us.
 
 #include <algorithm>
 
@@ -33,17 +33,31 @@ struct RowsParams {
   long long x_ld, r_ld, h_ld, codes_ld, scales_ld;
   int rows, channels;
   float eps;
-  int vec;  // channels, strides and addresses allow 16-byte accesses
 };
 
-// Eight channels from `c` on (zero past the row's end).
-template <typename T>
-__device__ __forceinline__ void load_row8(const T* row, int c, int channels, bool vec, float (&v)[8]) {
-  if (vec) {
-    load8<T>(row + c, v);
+// A lane's eight channels: consecutive where channels, strides and addresses allow
+// 16-byte accesses (VEC), else every 32nd, so that a warp's narrow accesses are
+// consecutive (4937 x 6189 bf16 with a residual took 126 us with eight consecutive
+// channels a lane, 76 so; 4937 x 6192 takes 49).
+template <bool VEC>
+__device__ __forceinline__ int channel_of(int warp, int lane, int j) {
+  return VEC ? (warp * 32 + lane) * 8 + j : warp * 256 + j * 32 + lane;
+}
+// Eight channels (zero past the row's end).
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_row8(const T* row, int warp, int lane, int channels, float (&v)[8]) {
+  if constexpr (VEC) {
+    load8<T>(row + channel_of<VEC>(warp, lane, 0), v);
   } else {
+    const T* at = row + channel_of<VEC>(warp, lane, 0);
+    const int left = channels - channel_of<VEC>(warp, lane, 0);
+    if (warp * 256 + 256 <= channels) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < channels ? to_f32<T>(row[c + j]) : 0.f;
+      for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(at[32 * j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 32 * j < left ? to_f32<T>(at[32 * j]) : 0.f;
+    }
   }
 }
 
@@ -80,6 +94,40 @@ __device__ __forceinline__ void quantize_block(float (&y)[8], bool live, bool fi
   }
 }
 
+// The same for lanes that hold every 32nd of 256 channels, which are two blocks;
+// `left` channels from the lane's first on.
+__device__ __forceinline__ void quantize_strided(float (&y)[8], int left, uint8_t* codes, uint8_t* scales) {
+  float amax[2];
+  auto maxima = [&]() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      amax[h] = fmaxf(fmaxf(fabsf(y[4 * h]), fabsf(y[4 * h + 1])), fmaxf(fabsf(y[4 * h + 2]), fabsf(y[4 * h + 3])));
+      amax[h] = fmaxf(amax[h], 0.f);  // (NaN alone counts nothing)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) amax[h] = fmaxf(amax[h], __shfl_xor_sync(0xffffffffu, amax[h], o));
+    }
+  };
+  maxima();
+  if (!fp8_is_finite(fmaxf(amax[0], amax[1]))) {  // infinities (rare): NaN, and out of the maxima
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (!fp8_is_finite(y[j])) y[j] = fp8_nan();
+    maxima();
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int e = fp8_exponent(amax[h]);
+    const float inv = fp8_pow2(-e);
+#pragma unroll
+    for (int j = 4 * h; j < 4 * h + 4; j += 2) {
+      const uint32_t pair = fp8_pack2(y[j] * inv, y[j + 1] * inv);
+      if (32 * j < left) codes[32 * j] = static_cast<uint8_t>(pair);
+      if (32 * j + 32 < left) codes[32 * j + 32] = static_cast<uint8_t>(pair >> 8);
+    }
+    if (lane_id() == 0 && 128 * h < left) scales[h] = static_cast<uint8_t>(e + 127);
+  }
+}
+
 // Blocks per SM: the kernel waits for memory, so as many as its registers
 // allow (51201 x 1000 bf16: 73.4 us with four, 69.1 with five, 84 with six, which spill;
 // 6400 x 256 f16: 4.1, 3.8 and 3.5 us).
@@ -88,13 +136,13 @@ constexpr int resident_blocks(int warps, int iters, int element_bytes) {
 }
 
 // WARPS warps per row (1: eight rows per 256-thread block), ITERS x 8 channels a lane.
-template <typename T, int WARPS, int ITERS, bool NORM>
+template <typename T, int WARPS, int ITERS, bool NORM, bool VEC>
 __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32,
                                   WARPS == 32 ? 1 : resident_blocks(WARPS, ITERS, sizeof(T)))
     fp8_rows_kernel(const RowsParams p) {
   __shared__ float s_part[WARPS == 1 ? 1 : WARPS];
   constexpr int kLanes = WARPS * 32;
-  const int t = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int lane = lane_id(), in_row = WARPS == 1 ? 0 : warp_id();
   const int per_block = WARPS == 1 ? 8 : 1;
   // (unsigned: the last step may pass 2^31)
   const unsigned first_row = blockIdx.x * per_block + (WARPS == 1 ? threadIdx.x >> 5 : 0);
@@ -114,9 +162,9 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32,
     float v[ITERS][8];
 #pragma unroll
     for (int i = 0; i < ITERS; ++i) {
-      const int c = (i * kLanes + t) * 8;
-      if (c < p.channels) {
-        load_row8<T>(x, c, p.channels, p.vec, v[i]);
+      const int warp = i * WARPS + in_row;
+      if (channel_of<VEC>(warp, lane, 0) < p.channels) {
+        load_row8<T, VEC>(x, warp, lane, p.channels, v[i]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
@@ -125,10 +173,10 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32,
     if (p.residual) {
 #pragma unroll
       for (int i = 0; i < ITERS; ++i) {
-        const int c = (i * kLanes + t) * 8;
-        if (c < p.channels) {
+        const int warp = i * WARPS + in_row;
+        if (channel_of<VEC>(warp, lane, 0) < p.channels) {
           float a[8];
-          load_row8<T>(r, c, p.channels, p.vec, a);
+          load_row8<T, VEC>(r, warp, lane, p.channels, a);
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[i][j] += a[j];
         }
@@ -138,15 +186,16 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32,
       T* h = static_cast<T*>(p.h) + row * p.h_ld;
 #pragma unroll
       for (int i = 0; i < ITERS; ++i) {
-        const int c = (i * kLanes + t) * 8;
-        if (c < p.channels) {
-          if (p.vec) {
-            store8<T>(h + c, v[i]);
-          } else {
+        const int warp = i * WARPS + in_row;
+        if constexpr (VEC) {
+          const int c = channel_of<VEC>(warp, lane, 0);
+          if (c < p.channels) store8<T>(h + c, v[i]);
+        } else {
+          T* at = h + channel_of<VEC>(warp, lane, 0);
+          const int left = p.channels - channel_of<VEC>(warp, lane, 0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (c + j < p.channels) h[c + j] = from_f32<T>(v[i][j]);
-          }
+          for (int j = 0; j < 8; ++j)
+            if (32 * j < left) at[32 * j] = from_f32<T>(v[i][j]);
         }
       }
     }
@@ -169,22 +218,33 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32,
       const float rstd = rsqrtf(sum / static_cast<float>(p.channels) + p.eps);
 #pragma unroll
       for (int i = 0; i < ITERS; ++i) {
+        const int warp = i * WARPS + in_row;
         float g[8];
-        load8<float>(s_gamma + (i * kLanes + t) * 8, g);
+        if constexpr (VEC) {
+          load8<float>(s_gamma + channel_of<VEC>(warp, lane, 0), g);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[j] = s_gamma[channel_of<VEC>(warp, lane, j)];
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rstd * g[j];
       }
     }
 #pragma unroll
     for (int i = 0; i < ITERS; ++i) {
-      const int c = (i * kLanes + t) * 8;
-      quantize_block(v[i], c < p.channels, c % kFp8Block == 0, p.codes + row * p.codes_ld + c,
-                     p.scales + row * p.scales_ld + c / kFp8Block);
+      const int c = channel_of<VEC>(i * WARPS + in_row, lane, 0);
+      uint8_t* codes = p.codes + row * p.codes_ld + c;
+      uint8_t* scales = p.scales + row * p.scales_ld + c / kFp8Block;
+      if constexpr (VEC) {
+        quantize_block(v[i], c < p.channels, c % kFp8Block == 0, codes, scales);
+      } else {
+        quantize_strided(v[i], p.channels - c, codes, scales);
+      }
     }
   }
 }
 
-template <typename T, bool NORM>
+template <typename T, bool NORM, bool VEC>
 int launch_rows(cudaStream_t stream, const RowsParams& p, const char* what) {
   const int sms = sm_count();
   const int c = p.channels;
@@ -193,23 +253,29 @@ int launch_rows(cudaStream_t stream, const RowsParams& p, const char* what) {
   if (c <= 1024) {
     const int iters = c <= 256 ? 1 : (c <= 512 ? 2 : 4);
     const int blocks = std::min((p.rows - 1) / 8 + 1, sms * resident_blocks(1, iters, sizeof(T)));
-    auto k = iters == 1 ? fp8_rows_kernel<T, 1, 1, NORM>
-                        : (iters == 2 ? fp8_rows_kernel<T, 1, 2, NORM> : fp8_rows_kernel<T, 1, 4, NORM>);
+    auto k = iters == 1 ? fp8_rows_kernel<T, 1, 1, NORM, VEC>
+                        : (iters == 2 ? fp8_rows_kernel<T, 1, 2, NORM, VEC> : fp8_rows_kernel<T, 1, 4, NORM, VEC>);
     return launch_kernel(k, dim3(blocks), dim3(256), smem(32, iters), stream, what, p);
   }
   if (c <= 8192) {
     const int iters = c <= 2048 ? 1 : (c <= 4096 ? 2 : 4);
     const int blocks = std::min(p.rows, sms * resident_blocks(8, iters, sizeof(T)));
-    auto k = iters == 1 ? fp8_rows_kernel<T, 8, 1, NORM>
-                        : (iters == 2 ? fp8_rows_kernel<T, 8, 2, NORM> : fp8_rows_kernel<T, 8, 4, NORM>);
+    auto k = iters == 1 ? fp8_rows_kernel<T, 8, 1, NORM, VEC>
+                        : (iters == 2 ? fp8_rows_kernel<T, 8, 2, NORM, VEC> : fp8_rows_kernel<T, 8, 4, NORM, VEC>);
     return launch_kernel(k, dim3(blocks), dim3(256), smem(256, iters), stream, what, p);
   }
   static unsigned long long configured = 0;
-  auto k = fp8_rows_kernel<T, 32, 4, NORM>;
+  auto k = fp8_rows_kernel<T, 32, 4, NORM, VEC>;
   const int rc =
       ensure_smem_attribute(reinterpret_cast<const void*>(k), static_cast<int>(smem(1024, 4)), &configured, what);
   if (rc != LDB_OK) return rc;
   return launch_kernel(k, dim3(std::min(p.rows, sms)), dim3(1024), smem(1024, 4), stream, what, p);
+}
+
+template <typename T>
+int launch_vec(cudaStream_t stream, const RowsParams& p, bool norm, bool vec, const char* what) {
+  if (norm) return vec ? launch_rows<T, true, true>(stream, p, what) : launch_rows<T, true, false>(stream, p, what);
+  return vec ? launch_rows<T, false, true>(stream, p, what) : launch_rows<T, false, false>(stream, p, what);
 }
 
 int esize(int dtype) { return dtype == LDB_F32 ? 4 : 2; }
@@ -232,14 +298,11 @@ int run_rows(cudaStream_t stream, RowsParams p, int dtype, bool norm, const char
     return fail(LDB_ERR_ALIGNMENT, "%s: codes need 16-byte aligned rows", what);
   if (p.rows == 0) return LDB_OK;
   const int es = esize(dtype);
-  p.vec = p.channels % 8 == 0 && aligned16(p.x, p.x_ld, es) && aligned16(p.residual, p.r_ld, es) &&
-          aligned16(p.h, p.h_ld, es);
-  if (dtype == LDB_F16)
-    return norm ? launch_rows<__half, true>(stream, p, what) : launch_rows<__half, false>(stream, p, what);
-  if (dtype == LDB_BF16)
-    return norm ? launch_rows<__nv_bfloat16, true>(stream, p, what)
-                : launch_rows<__nv_bfloat16, false>(stream, p, what);
-  return norm ? launch_rows<float, true>(stream, p, what) : launch_rows<float, false>(stream, p, what);
+  const bool vec = p.channels % 8 == 0 && aligned16(p.x, p.x_ld, es) && aligned16(p.residual, p.r_ld, es) &&
+                   aligned16(p.h, p.h_ld, es);
+  if (dtype == LDB_F16) return launch_vec<__half>(stream, p, norm, vec, what);
+  if (dtype == LDB_BF16) return launch_vec<__nv_bfloat16>(stream, p, norm, vec, what);
+  return launch_vec<float>(stream, p, norm, vec, what);
 }
 
 // One 128 x 128 block of a weight: eight warps, 16 rows each, four columns a
@@ -295,14 +358,14 @@ int ldb_rms_norm_fp8(cudaStream_t stream, const void* x, long long x_ld, const v
                      int dtype, const float* gamma, float eps, void* h, long long h_ld, uint8_t* codes,
                      long long codes_ld, uint8_t* scales, long long scales_ld, int rows, int channels) {
   ldb::RowsParams p{x, residual, gamma, h, codes, scales, x_ld, residual_ld, h_ld, codes_ld, scales_ld,
-                    rows, channels, eps, 0};
+                    rows, channels, eps};
   return ldb::run_rows(stream, p, dtype, true, "rms_norm_fp8");
 }
 
 int ldb_quantize_fp8_rows(cudaStream_t stream, const void* x, long long x_ld, int dtype, uint8_t* codes,
                           long long codes_ld, uint8_t* scales, long long scales_ld, int rows, int channels) {
   ldb::RowsParams p{x, nullptr, nullptr, nullptr, codes, scales, x_ld, 0, 0, codes_ld, scales_ld,
-                    rows, channels, 0.f, 0};
+                    rows, channels, 0.f};
   return ldb::run_rows(stream, p, dtype, false, "quantize_fp8_rows");
 }
 

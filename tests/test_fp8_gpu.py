@@ -333,3 +333,20 @@ def test_matmul_narrow_outputs(cuda_device, dtype, m, n, k, residual, gelu):
     check_product(out, want, size, dtype, slope=1.5 if gelu else 1.0)
     assert (wide[m:] == 3).all() and (wide[:, :1] == 3).all() and (wide[:, n + 1:] == 3).all()
     assert _lib.device_status(reset=True) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,c", [(3, 127), (9, 129), (40, 257), (5, 1023), (6, 2051), (3, 8191), (2, 20003)])
+def test_quantize_narrow_rows_is_exact(cuda_device, dtype, rows, c):
+    """Rows without 16-byte accesses, with infinities and NaN, inside wider ones whose other values stay."""
+    wide = torch.randn(rows, c + 3, generator=torch.Generator().manual_seed(rows + c)) * 2.0 ** 3
+    wide[:, 1 + c // 2], wide[rows - 1, c] = float("inf"), float("nan")
+    wide = wide.to(dtype)
+    x = wide[:, 1 : c + 1]
+    got = fp8.quantize_rows(wide.to(cuda_device)[:, 1 : c + 1])
+    codes, e = oracle.quantize_rows(x.double())
+    have = got.codes.cpu().double()
+    assert torch.equal(torch.isnan(have), torch.isnan(codes))
+    assert torch.equal(have.nan_to_num(0.0), codes.nan_to_num(0.0))
+    assert torch.equal(got.scales.view(torch.uint8).cpu().long() - 127, e.long())
+    assert _lib.device_status(reset=True) == 0
