@@ -458,9 +458,12 @@ LDB_API int ldb_kv_append_fp8(ldb_stream_t stream, const void* k, long long k_ld
  * causal: query i sees the keys up to lengths[b] - queries + i.  A query
  * without keys gives zeros.  FP32 scores, sums and outputs with one rounding;
  * the weights of the value product are rounded to f16.  At most 2048 items; a
- * cache of at most 2^31 - 1 token rows.  The workspace (16-byte aligned) holds partial rows. */
+ * cache of at most 2^31 - 1 token rows.  The workspace (16-byte aligned) holds
+ * partial rows: bytes for any table, or for one of `capacity` = width * page tokens. */
 LDB_API int ldb_kv_attention_fp8_workspace_size(int batch, int queries, int heads, int kv_heads, int head_dim,
                                                 size_t* bytes);
+LDB_API int ldb_kv_attention_fp8_table_workspace_size(int batch, int queries, int heads, int kv_heads, int head_dim,
+                                                      long long capacity, size_t* bytes);
 LDB_API int ldb_kv_attention_fp8(ldb_stream_t stream, const void* q, long long q_ld, long long q_batch, int dtype,
                                  const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scales,
                                  const uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim,

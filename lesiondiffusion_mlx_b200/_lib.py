@@ -106,6 +106,7 @@ SIGNATURES: dict[str, list] = {
     "ldb_pack_weight_fp8": [_P, _P, _L, _I, _P, _L, _P, _I, _I, _I],
     "ldb_kv_append_fp8": [_P, _P, _L, _L, _P, _L, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _I, _I],
     "ldb_kv_attention_fp8_workspace_size": [_I, _I, _I, _I, _I, ctypes.POINTER(_SZ)],
+    "ldb_kv_attention_fp8_table_workspace_size": [_I, _I, _I, _I, _I, _L, ctypes.POINTER(_SZ)],
     "ldb_kv_attention_fp8": [_P, _P, _L, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I,
                              _F, _I, _P, _SZ],
     "ldb_matmul_fp8_workspace_size": [_I, _I, _I, ctypes.POINTER(_SZ)],

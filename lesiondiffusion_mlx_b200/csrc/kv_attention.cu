@@ -733,17 +733,22 @@ int launch_dim(cudaStream_t stream, const AttnParams& p, int head_dim, unsigned 
 
 extern "C" {
 
-int ldb_kv_attention_fp8_workspace_size(int batch, int queries, int heads, int kv_heads, int head_dim, size_t* bytes) {
+int ldb_kv_attention_fp8_table_workspace_size(int batch, int queries, int heads, int kv_heads, int head_dim,
+                                              long long capacity, size_t* bytes) {
   using namespace ldb;
   if (!bytes) return fail(LDB_ERR_INVALID, "kv_attention: bytes is null");
   if (batch < 0 || queries < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads ||
       (head_dim != 32 && head_dim != 64 && head_dim != 128))
     return fail(LDB_ERR_SHAPE, "kv_attention: %d heads over %d of width %d (32, 64 or 128)", heads, kv_heads, head_dim);
   const long long rows = static_cast<long long>(queries) * (heads / kv_heads);
-  *bytes = rows >= kTileRows ? kv_tile_workspace(batch, kv_heads, rows, head_dim)
+  *bytes = rows >= kTileRows ? kv_tile_workspace(batch, kv_heads, rows, head_dim, capacity)
                              : workspace_bytes_of(ctas_per_sm(head_dim) * sm_count() * kWarps,
                                                   kGroupRows * row_groups(rows), head_dim);
   return LDB_OK;
+}
+
+int ldb_kv_attention_fp8_workspace_size(int batch, int queries, int heads, int kv_heads, int head_dim, size_t* bytes) {
+  return ldb_kv_attention_fp8_table_workspace_size(batch, queries, heads, kv_heads, head_dim, -1, bytes);
 }
 
 int ldb_kv_attention_fp8(cudaStream_t stream, const void* q, long long q_ld, long long q_batch, int dtype,
@@ -755,7 +760,9 @@ int ldb_kv_attention_fp8(cudaStream_t stream, const void* q, long long q_ld, lon
   using namespace ldb;
   if (dtype != LDB_F16 && dtype != LDB_BF16) return fail(LDB_ERR_INVALID, "kv_attention: queries must be f16 or bf16");
   size_t need = 0;
-  int rc = ldb_kv_attention_fp8_workspace_size(batch, queries, heads, kv_heads, head_dim, &need);
+  int rc = ldb_kv_attention_fp8_table_workspace_size(batch, queries, heads, kv_heads, head_dim,
+                                                     static_cast<long long>(std::max(width, 0)) * std::max(page, 0),
+                                                     &need);
   if (rc != LDB_OK) return rc;
   if (page != 16 && page != 32 && page != 64 && page != 128)
     return fail(LDB_ERR_SHAPE, "kv_attention: pages of %d tokens (16, 32, 64 or 128)", page);

@@ -55,10 +55,9 @@ struct KvTileParams {
   float* ml_part;    // [split][batch][kv head][row][2]
 };
 
-// Ranges of tokens that the many-row kernel runs separately, the bytes of their
-// partial rows, and the kernel itself (p's shapes and pointers filled in).
-int kv_tile_splits(int batch, int kv_heads, long long rows);
-size_t kv_tile_workspace(int batch, int kv_heads, long long rows, int head_dim);
+// The many-row kernel (p's shapes and pointers filled in), and the bytes of the
+// partial rows of its ranges for a table of `capacity` tokens (negative: any).
+size_t kv_tile_workspace(int batch, int kv_heads, long long rows, int head_dim, long long capacity);
 int kv_attention_tiles(cudaStream_t stream, KvTileParams p, int head_dim, int dtype, float scale, void* workspace,
                        unsigned int* status);
 

@@ -753,36 +753,39 @@ int launch_dim(cudaStream_t stream, const KvTileParams& p, int head_dim, unsigne
   return launch_page<128, T>(stream, p, status);
 }
 
-}  // namespace
-
-// Most ranges of tokens: grids of up to four waves may be cut, to up to four waves.
-int kv_tile_splits(int batch, int kv_heads, long long rows) {
-  const long long ctas = (rows + 2 * kM - 1) / (2 * kM) * kv_heads * batch;
-  return static_cast<int>(std::max(1ll, std::min(32ll, 4ll * sm_count() / std::max(1ll, ctas))));
+// Ranges of tokens, from the table's capacity, in the time of a block of 128
+// tokens: a CTA's start and end take about five, the partial rows are written
+// and read once, and there is a second kernel; at most four waves.  (The lengths are
+// on the device; shorter and ragged items leave the order of the counts about as
+// it is.)  7 items of up to 19724 tokens, 523 causal queries, 4 heads of 32: 324 us in
+// one range, 149 in five.
+int kv_tile_splits(int batch, int kv_heads, long long rows, int head_dim, long long capacity) {
+  const long long ctas = (rows + 2 * kM - 1) / (2 * kM) * kv_heads * batch, sms = sm_count();
+  const long long blocks = (capacity + kN - 1) / kN;
+  const long long most = std::min({32ll, 4 * sms / std::max(1ll, ctas), (blocks + 1) / 2});
+  const double merge = static_cast<double>(batch) * kv_heads * rows * head_dim * 8 / 12e6;  // of a range
+  double best = static_cast<double>((ctas + sms - 1) / sms) * (blocks + 5);
+  int splits = 1;
+  for (int s = 2; s <= most; ++s) {
+    const double cost = static_cast<double>((ctas * s + sms - 1) / sms) * ((blocks + s - 1) / s + 5) + 2 + merge * s;
+    if (cost < best) best = cost, splits = s;
+  }
+  return splits;
 }
 
-size_t kv_tile_workspace(int batch, int kv_heads, long long rows, int head_dim) {
-  const int splits = kv_tile_splits(batch, kv_heads, rows);
-  return splits == 1 ? 0 : static_cast<size_t>(splits) * batch * kv_heads * rows * (head_dim + 2) * sizeof(float);
+}  // namespace
+
+size_t kv_tile_workspace(int batch, int kv_heads, long long rows, int head_dim, long long capacity) {
+  const long long ctas = (rows + 2 * kM - 1) / (2 * kM) * kv_heads * batch;
+  const long long splits = capacity < 0 ? std::min(32ll, 4ll * sm_count() / std::max(1ll, ctas))
+                                        : kv_tile_splits(batch, kv_heads, rows, head_dim, capacity);
+  return splits <= 1 ? 0 : static_cast<size_t>(splits) * batch * kv_heads * rows * (head_dim + 2) * sizeof(float);
 }
 
 int kv_attention_tiles(cudaStream_t stream, KvTileParams p, int head_dim, int dtype, float scale, void* workspace,
                        unsigned int* status) {
-  // Ranges from the table's capacity, in the time of a block of 128 tokens: a
-  // CTA's start and end take about five, the partial rows are written and read
-  // once, and there is a second kernel.  (The lengths are on the device; shorter and
-  // ragged items leave the order of the counts about as it is.)  7 items of up to 19724
-  // tokens, 523 causal queries, 4 heads of 32: 324 us in one range, 149 in five.
-  const long long blocks = (static_cast<long long>(p.c.width) * p.c.page + kN - 1) / kN;
   p.row_blocks = (p.rows + 2 * kM - 1) / (2 * kM);
-  const long long ctas = static_cast<long long>(p.row_blocks) * p.c.kv_heads * p.c.batch, sms = sm_count();
-  const double merge = static_cast<double>(p.c.batch) * p.c.kv_heads * p.rows * head_dim * 8 / 12e6;  // a range
-  double best = 0;
-  for (int s = 1; s <= std::min<long long>(kv_tile_splits(p.c.batch, p.c.kv_heads, p.rows), (blocks + 1) / 2); ++s) {
-    const double cost = static_cast<double>((ctas * s + sms - 1) / sms) * ((blocks + s - 1) / s + 5) +
-                        (s > 1 ? 2 + merge * s : 0);
-    if (s == 1 || cost < best) best = cost, p.splits = s;
-  }
+  p.splits = kv_tile_splits(p.c.batch, p.c.kv_heads, p.rows, head_dim, static_cast<long long>(p.c.width) * p.c.page);
   p.negate = scale < 0.f;
   p.scale_log2 = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
   p.o_part = static_cast<float*>(workspace);

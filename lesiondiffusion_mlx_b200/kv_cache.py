@@ -140,7 +140,8 @@ def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, length
     out_batch, out_ld, _ = out.stride()
     heads = channels // dim
     index = q.get_device()
-    need = _workspace_bytes("ldb_kv_attention_fp8_workspace_size", index, batch, queries, heads, kv_heads, dim)
+    need = _workspace_bytes("ldb_kv_attention_fp8_table_workspace_size", index, batch, queries, heads, kv_heads, dim,
+                            width * page)
     ws_ptr = None
     if need:
         ws = q.new_empty(need, dtype=torch.uint8)

@@ -61,3 +61,18 @@ def test_python_refuses_what_does_not_fit():
     bad = kv_cache.KvCacheFp8(cache.k, cache.v, cache.k_scale[:1], cache.v_scale)
     with pytest.raises(ValueError, match="scales"):
         kv_cache.kv_attention(torch.zeros(1, 1, 64), bad, index, index[0], scale=1.0)
+
+
+def test_workspace_of_a_table_is_within_that_of_any():
+    def size(name, *args):
+        need = ctypes.c_size_t(0)
+        _lib.call(name, *args, ctypes.byref(need))
+        return need.value
+
+    for batch, queries, heads, kv_heads, dim in ((1, 1, 8, 2, 128), (7, 523, 4, 4, 32), (3, 100, 8, 1, 64), (40, 60, 8, 8, 32),
+                                                 (64, 4000, 8, 8, 128)):
+        most = size("ldb_kv_attention_fp8_workspace_size", batch, queries, heads, kv_heads, dim)
+        for capacity in (16, 77, 1000, 19724, 130000, 2 ** 31 - 1):
+            got = size("ldb_kv_attention_fp8_table_workspace_size", batch, queries, heads, kv_heads, dim, capacity)
+            assert got <= most, (batch, queries, capacity)
+    assert size("ldb_kv_attention_fp8_table_workspace_size", 1, 6400, 4, 4, 64, 77) == 0  # one block: nothing to join
