@@ -1,6 +1,6 @@
 // Writing new tokens into the paged 8-bit key/value cache.
 //
-// One block per touched (page, kv head) of K or V.  With `held` older tokens in
+// One warp or block per touched (page, kv head) of K or V.  With `held` older tokens in
 // the page and e(new) the scale that the new values need (fp8.cuh):
 //
 //   e = held > 0 ? max(e_old, e(new)) : e(new)
@@ -12,9 +12,9 @@
 //
 // Bound: HBM (2 bytes read and 1 written a value); a page's new values stay in
 // registers between the maximum and the rounding.  For one token it is the
-// launch.  One B200: 4 x 2049 tokens of 8 x 128 bf16 13.1 us (3.8 TB/s: a
-// block's reads depend on one another, and two waves of blocks do not fill the
-// gaps), one token of 32 items 4.0 us.
+// launch.  One B200: 4 x 2049 tokens of 8 x 128 bf16 13.2 us (3.8 TB/s: a unit's
+// reads depend on one another, and the grid is not many times what is
+// resident), one token of 32 items 2.6 us.
 
 #include <type_traits>
 
@@ -37,17 +37,21 @@ struct AppendParams {
 };
 
 constexpr int kAppendThreads = 256;
-constexpr int kMaxVecs = 128 * 128 / 8 / kAppendThreads;  // vectors of eight per thread, of the largest page
+constexpr int kMaxVecs = 8;  // vectors of eight per thread
 
-__device__ __forceinline__ float block_max(float v, float* s_part) {
+// The largest value of a unit's threads.
+template <int WARPS>
+__device__ __forceinline__ float unit_max(float v, float* s_part) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if (lane_id() == 0) s_part[warp_id()] = v;
-  __syncthreads();
-  v = s_part[0];
+  if constexpr (WARPS > 1) {
+    __syncthreads();
+    if (lane_id() == 0) s_part[warp_id()] = v;
+    __syncthreads();
+    v = s_part[0];
 #pragma unroll
-  for (int w = 1; w < kAppendThreads / 32; ++w) v = fmaxf(v, s_part[w]);
+    for (int w = 1; w < WARPS; ++w) v = fmaxf(v, s_part[w]);
+  }
   return v;
 }
 
@@ -69,24 +73,31 @@ __device__ __forceinline__ float max_of8(const uint4 (&raw)[sizeof(T) / 2]) {
   }
 }
 
-// VECS: vectors of eight values per thread that a whole page takes.  The
-// values stay as they came (four registers a vector in 16 bits) until they
-// are rounded, so that enough blocks are resident to cover the chain of
-// dependent reads (position, page number, values).
-template <typename T, int VECS>
-__global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) == 4 ? 3 : 6)
+// WARPS of a unit (a page of one head), VECS vectors of eight values per thread
+// that a whole page takes: a warp up to 256 vectors, eight units to a block, and
+// the fewest warps above, a unit a block.  (4 x 2049 tokens, 8 heads: of 64 in pages
+// of 16, 19.2 us with 256 threads a unit, 6.9 so; of 64 in pages of 64, 8.6 and
+// 7.0; of 128 in pages of 64, 12.9 and 13.2; one token of 32 items 4.0 and 2.6.)  The
+// values stay as they came (four registers a vector in 16 bits) until they are
+// rounded, so that enough warps are resident to cover the chain of dependent
+// reads (position, page number, values).
+template <typename T, int VECS, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? kAppendThreads : WARPS * 32,
+                                  (sizeof(T) == 4 ? 3 : (VECS == kMaxVecs ? 4 : 6)) * (WARPS == 1 ? 1 : 8 / WARPS))
     kv_append_kernel(const AppendParams p, unsigned int* status) {
+  constexpr int kUnitThreads = WARPS * 32;
   __shared__ float s_part[kAppendThreads / 32];
-  __shared__ int s_old;
   pdl_begin();
-  const int b = blockIdx.y / p.kv_heads, head = blockIdx.y % p.kv_heads, which = blockIdx.z;
+  const int thread = WARPS == 1 ? lane_id() : threadIdx.x;
+  const int u = WARPS == 1 ? blockIdx.x * (kAppendThreads / 32) + warp_id() : blockIdx.x;
+  const int b = blockIdx.y, head = u % p.kv_heads, which = blockIdx.z;
   const int start = p.start[b];
   int count = p.counts ? p.counts[b] : p.tokens;
   if (start < 0 || count < 0 || count > p.tokens) {
-    if (threadIdx.x == 0) set_bad_shape(status);
+    if (thread == 0) set_bad_shape(status);
     return;
   }
-  const long long slot = start / p.page + blockIdx.x;
+  const long long slot = static_cast<long long>(start / p.page) + u / p.kv_heads;
   const long long page0 = slot * p.page;
   const int first = static_cast<int>(max(0ll, page0 - start));                              // of the new tokens
   const int last = static_cast<int>(min(static_cast<long long>(count), page0 + p.page - start));
@@ -101,7 +112,7 @@ __global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) 
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
-    const int q = i * kAppendThreads + threadIdx.x;
+    const int q = i * kUnitThreads + thread;
     if (q < vecs) {
       const T* x = src + (first + (q >> vshift)) * p.src_ld[which] + ((q & ((1 << vshift) - 1)) << 3);
       if (p.vec) {
@@ -117,23 +128,23 @@ __global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) 
     }
   }
   if (id < 0 || id >= p.pages) {
-    if (threadIdx.x == 0) set_bad_shape(status);
+    if (thread == 0) set_bad_shape(status);
     return;
   }
   const long long unit = static_cast<long long>(id) * p.kv_heads + head;
   uint8_t* codes = p.codes[which] + unit * p.page * p.dim;
   uint8_t* scale = p.scales[which] + unit;
-  if (held > 0 && threadIdx.x == 0) s_old = *scale;
+  const int old_scale = held > 0 ? *scale : 127;
 #pragma unroll
   for (int i = 0; i < VECS; ++i)
-    if (i * kAppendThreads + static_cast<int>(threadIdx.x) < vecs) amax = fmaxf(amax, max_of8<T>(raw[i]));
-  amax = block_max(amax, s_part);
+    if (i * kUnitThreads + thread < vecs) amax = fmaxf(amax, max_of8<T>(raw[i]));
+  amax = unit_max<WARPS>(amax, s_part);
   const bool infinite = !fp8_is_finite(amax);  // (rare: infinities become NaN and leave the maximum)
   if (infinite) {
     amax = 0.f;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      if (i * kAppendThreads + static_cast<int>(threadIdx.x) < vecs) {
+      if (i * kUnitThreads + thread < vecs) {
         const T* v = reinterpret_cast<const T*>(raw[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -142,15 +153,15 @@ __global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) 
         }
       }
     }
-    amax = block_max(amax, s_part);
+    amax = unit_max<WARPS>(amax, s_part);
   }
-  const int e_old = held > 0 ? s_old - 127 : 0;
+  const int e_old = old_scale - 127;
   int e = max(-kKvMaxExponent, min(kKvMaxExponent, fp8_exponent(amax)));
   if (held > 0) e = amax == 0.f ? e_old : max(e, e_old);  // zeros ask for no scale
   const float inv = fp8_pow2(-min(e, 127));
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
-    const int q = i * kAppendThreads + threadIdx.x;
+    const int q = i * kUnitThreads + thread;
     if (q < vecs) {
       const T* v = reinterpret_cast<const T*>(raw[i]);
       float y[8];
@@ -167,7 +178,7 @@ __global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) 
   }
   if (held > 0 && e > e_old) {
     const float shrink = exp2f(static_cast<float>(max(e_old - e, -64)));  // below 2^-18 every code becomes 0
-    for (int q = threadIdx.x; q < held << vshift; q += kAppendThreads) {
+    for (int q = thread; q < held << vshift; q += kUnitThreads) {
       uint2* at = reinterpret_cast<uint2*>(codes + (q << 3));
       uint2 old = *at;
       uint32_t* w = &old.x;
@@ -182,16 +193,25 @@ __global__ void __launch_bounds__(kAppendThreads, VECS == kMaxVecs || sizeof(T) 
       *at = old;
     }
   }
-  if (threadIdx.x == 0) *scale = static_cast<uint8_t>(e + 127);
+  if (WARPS == 1) __syncwarp();  // all have read the old one
+  if (thread == 0) *scale = static_cast<uint8_t>(e + 127);
 }
 
 template <typename T>
-int launch_append(cudaStream_t stream, dim3 grid, const AppendParams& p, unsigned int* status) {
-  const int vecs = (p.page * p.dim / 8 + kAppendThreads - 1) / kAppendThreads;
-  auto k = vecs == 1 ? kv_append_kernel<T, 1>
-                     : (vecs == 2 ? kv_append_kernel<T, 2>
-                                  : (vecs <= 4 ? kv_append_kernel<T, 4> : kv_append_kernel<T, kMaxVecs>));
-  return launch_kernel(k, grid, dim3(kAppendThreads), 0, stream, "kv_append launch", p, status);
+int launch_append(cudaStream_t stream, long long units, int batch, const AppendParams& p, unsigned int* status) {
+  const int vecs = p.page * p.dim / 8;  // 64 .. 2048, a power of two
+  auto k = vecs <= 64    ? kv_append_kernel<T, 2, 1>
+           : vecs <= 128 ? kv_append_kernel<T, 4, 1>
+           : vecs <= 256 ? kv_append_kernel<T, kMaxVecs, 1>
+           : vecs <= 512 ? kv_append_kernel<T, kMaxVecs, 2>
+           : vecs <= 1024 ? kv_append_kernel<T, kMaxVecs, 4>
+                          : kv_append_kernel<T, kMaxVecs, 8>;
+  const long long blocks = vecs <= 256 ? (units + kAppendThreads / 32 - 1) / (kAppendThreads / 32) : units;
+  if (blocks > 0x7FFFFFFFll || units > 0x7FFFFF00ll)
+    return fail(LDB_ERR_SHAPE, "kv_append: %lld pages and heads of an item", units);
+  const dim3 grid(static_cast<unsigned>(blocks), batch, 2);
+  const int threads = vecs <= 256 ? kAppendThreads : vecs / kMaxVecs;
+  return launch_kernel(k, grid, dim3(threads), 0, stream, "kv_append launch", p, status);
 }
 
 }  // namespace
@@ -238,10 +258,10 @@ int ldb_kv_append_fp8(cudaStream_t stream, const void* k, long long k_ld, long l
     if (reinterpret_cast<uintptr_t>(p.src[i]) % 16 || p.src_ld[i] * es % 16 || p.src_batch[i] * es % 16) p.vec = 0;
   // pages that a run of `tokens` can touch, wherever it starts
   const long long touched = (static_cast<long long>(tokens) + page - 2) / page + 1;
-  const dim3 grid(static_cast<unsigned>(touched), batch * kv_heads, 2);
-  if (dtype == LDB_F16) return launch_append<__half>(stream, grid, p, status);
-  if (dtype == LDB_BF16) return launch_append<__nv_bfloat16>(stream, grid, p, status);
-  return launch_append<float>(stream, grid, p, status);
+  const long long units = touched * kv_heads;
+  if (dtype == LDB_F16) return launch_append<__half>(stream, units, batch, p, status);
+  if (dtype == LDB_BF16) return launch_append<__nv_bfloat16>(stream, units, batch, p, status);
+  return launch_append<float>(stream, units, batch, p, status);
 }
 
 }  // extern "C"

@@ -341,3 +341,25 @@ def test_attention_refuses_items_that_overlap_in_the_output(cuda_device):
     q = torch.zeros(2, 1, 64, device=cuda_device, dtype=torch.float16)
     with pytest.raises(_lib.LdbError, match="item stride"):
         kv_cache.kv_attention(q, cache, table, lengths, scale=1.0, out=q[:1].expand(2, 1, 64))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_append_every_page_size(cuda_device, dtype, dim, page):
+    """Each page of each head width, over older tokens, with a short item, three heads and an infinity."""
+    heads, tokens, start, counts = 3, 2 * page + 5, [0, page - 1, 7], [2 * page + 5, page + 3, 0]
+    table, pages = make_table(3, 4, cuda_device, dim + page)
+    cache = make_cache(pages, heads, dim, page, cuda_device, page)
+    want = host(cache)
+    g = torch.Generator().manual_seed(dim)
+    k, v = (torch.randn(3, tokens, heads * dim, generator=g) for _ in range(2))
+    k[1] *= 64
+    v[0, 3, 5] = float("inf")
+    k, v = k.to(dtype), v.to(dtype)
+    kv_cache.kv_append(cache, k.to(cuda_device), v.to(cuda_device), table.to(cuda_device), ints(start, cuda_device),
+                       counts=ints(counts, cuda_device))
+    for (codes, e), new in zip(((want[0], want[1]), (want[2], want[3])), (k, v)):
+        oracle.append(codes, e, new.view(3, tokens, heads, dim), table, start, counts)
+    same_cache(cache, want)
+    assert _lib.device_status(reset=True) == 0
