@@ -25,9 +25,9 @@
 // KB for 128 x 224 outputs, in and out of shared memory at 128 bytes a cycle,
 // which is what bounds it (704 cycles a K block against 448 of products).
 //
-// One B200: 8190 x 4096 x 4096 bf16 with a residual 125 us (2200 TFLOP/s, 1.31
-// of the bf16 burst rate; tensor pipe 68 % active, 627 cycles for a K block's 448
-// of products); 6400 x 256 -> 1024 with GELU 13.4 us, bound by the epilogue; one
+// One B200: 8190 x 4096 x 4096 bf16 with a residual 124 us (2210 TFLOP/s, 1.32
+// of the bf16 burst rate; tensor pipe 69 % active, 627 cycles for a K block's 448
+// of products); 6400 x 256 -> 1024 with GELU 14.4 us, bound by the epilogue; one
 // row times 8192 x 2048 8.6 us, the start of the pipeline (2.6 us of weight).
 
 #include <algorithm>

@@ -25,8 +25,11 @@
 // 10.0 us.  A block of two tiles takes 4700 cycles: 2000 from a tile's weights to
 // its next scores (718 for the value product, 977 for the scores, whose operands
 // take 128 bytes a cycle of shared memory), 420 for the maximum, 340 for the
-// reference, 1600 for the weights.  Four softmax warpgroups with half a row a
-// thread took 626 us instead of 527, scores read from TMEM twice 581.
+// reference, 1600 for the weights.  Slower: four softmax warpgroups with half a row
+// a thread (626 us where two took 527), scores read from TMEM twice (581), and the
+// first 64 of the next scores before the value product, in the half of the scores'
+// columns that the weights leave free (742 where this took 480: products of half
+// the width read the queries twice).
 
 #include <algorithm>
 
