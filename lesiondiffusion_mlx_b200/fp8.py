@@ -80,14 +80,16 @@ def _quantized(x: torch.Tensor, k: int) -> tuple[Fp8Rows, int, int]:
     lead = x.shape[:-1]
     blocks = (k + 127) // 128
     ld, s_ld = (k + 15) // 16 * 16, (blocks + 3) // 4 * 4
-    codes = (torch.empty_like(x, dtype=CODES, memory_format=torch.contiguous_format) if ld == k
-             else x.new_empty((*lead, ld), dtype=CODES))
-    strides, step = [1], s_ld
+    per_row, rows = [], 1  # rows between neighbours of each leading axis
     for n in reversed(lead):
-        strides.insert(0, step)
-        step *= n
-    scales = x.new_empty_strided((*lead, blocks), strides, dtype=SCALES)
-    return Fp8Rows(codes if ld == k else codes[..., :k], scales), ld, s_ld
+        per_row.insert(0, rows)
+        rows *= n
+    if ld == k:
+        codes = torch.empty_like(x, dtype=CODES, memory_format=torch.contiguous_format)
+    else:  # (the padding behind the last row too)
+        codes = x.new_empty(rows * ld, dtype=CODES).as_strided((*lead, k), [n * ld for n in per_row] + [1])
+    scales = x.new_empty_strided((*lead, blocks), [n * s_ld for n in per_row] + [1], dtype=SCALES)
+    return Fp8Rows(codes, scales), ld, s_ld
 
 
 def _launcher(kind: str, flops: float = 0.0):
