@@ -27,9 +27,9 @@
 // swizzled row are free of bank conflicts, and the orders of channels (in q k)
 // and of output rows (in p v) are chosen so that these bytes are its fragments.
 //
-// One B200, 8 heads of 128 shared by 4 bf16 queries each: 131072 tokens 58 us
-// (50 in this kernel, 5.4 TB/s; the start and the merge are the rest), 48 items
-// of up to 8192 tokens 77.5 us (5.2 TB/s).  Tiles fetched by one warp per CTA
+// One B200, 8 heads of 128 shared by 4 bf16 queries each: 131072 tokens 54.5
+// us (50 in this kernel, 5.4 TB/s; the start and the merge are the rest), 48 items
+// of up to 8192 tokens 77 us (5.2 TB/s).  Tiles fetched by one warp per CTA
 // with TMA and shared by four others took 74 and 154 us: the fetch was bound by
 // the issue of its loads, and every change of pair by the four warps' barriers.
 
@@ -626,12 +626,11 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
 // references' maximum is order-free, the sums go through a fixed tree), then the
 // block's groups of D / 4 threads, four channels each, add every k-th part in order, and
 // the groups' sums are added in order.  Small blocks: most have nothing to do.
-constexpr int kMergeThreads = 256;
-template <int D, typename T>
-__global__ void __launch_bounds__(kMergeThreads) kv_attention_merge_kernel(const AttnParams p) {
-  constexpr int kLanes = D / 4, kGroups = kMergeThreads / kLanes;
+template <int D, typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_attention_merge_kernel(const AttnParams p) {
+  constexpr int kLanes = D / 4, kGroups = THREADS / kLanes;
   __shared__ float4 s_v[kGroups][kLanes];
-  __shared__ float s_red[2][kMergeThreads / 32], s_f[kMergeThreads];
+  __shared__ float s_red[2][THREADS / 32], s_f[THREADS];
   pdl_begin();
   int4 at = p.open_part[blockIdx.x];
   if (p.open_by_pair && kv_length(p.c, blockIdx.x / (p.c.kv_heads * p.row_tiles), p.status) == 0)
@@ -644,16 +643,16 @@ __global__ void __launch_bounds__(kMergeThreads) kv_attention_merge_kernel(const
   // slot 1 of the warp that starts the pair, slot 0 of those that go on with it
   auto part = [&](int i) { return (static_cast<long long>(first + i) * 2 + (i == 0 ? 1 : 0)) * p.tile_rows + r; };
   float m = kFloor;
-  for (int i = threadIdx.x; i < count; i += kMergeThreads) m = fmaxf(m, p.ml_part[part(i) * 2]);
+  for (int i = threadIdx.x; i < count; i += THREADS) m = fmaxf(m, p.ml_part[part(i) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane_id() == 0) s_red[0][warp_id()] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kMergeThreads / 32; ++w) m = fmaxf(m, s_red[0][w]);
+  for (int w = 0; w < THREADS / 32; ++w) m = fmaxf(m, s_red[0][w]);
   float l = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < count; i0 += kMergeThreads) {
+  for (int i0 = 0; i0 < count; i0 += THREADS) {
     if (i0) __syncthreads();  // the round before has read s_f
     const int i = i0 + threadIdx.x;
     if (i < count) {
@@ -662,7 +661,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv_attention_merge_kernel(const
       l = fmaf(ml.y, s_f[threadIdx.x], l);
     }
     __syncthreads();
-    const int n = min(count - i0, kMergeThreads);
+    const int n = min(count - i0, THREADS);
 #pragma unroll 8
     for (int k = group; k < n; k += kGroups) {
       const float4 o = reinterpret_cast<const float4*>(p.o_part + part(i0 + k) * D)[lane4];
@@ -678,7 +677,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv_attention_merge_kernel(const
   if (static_cast<int>(threadIdx.x) >= D) return;
   l = 0.f;
 #pragma unroll
-  for (int w = 0; w < kMergeThreads / 32; ++w) l += s_red[1][w];
+  for (int w = 0; w < THREADS / 32; ++w) l += s_red[1][w];
   float sum = 0.f;
 #pragma unroll
   for (int k = 0; k < kGroups; ++k) sum += reinterpret_cast<const float*>(s_v[k])[threadIdx.x];
@@ -711,9 +710,22 @@ int launch(cudaStream_t stream, const AttnParams& p, unsigned int* status) {
   rc = launch_kernel(kv_attention_kernel<D, G, T>, dim3(p.warps / kWarps), dim3(kWarps * 32),
                      Cfg<D, G>::kOffBase + (p.c.batch + 1) * 4, stream, "kv_attention launch", p, status);
   if (rc != LDB_OK) return rc;
-  const dim3 grid(p.open_by_pair ? p.c.batch * p.c.kv_heads * p.row_tiles : p.warps, std::min(p.tile_rows, p.rows));
-  return launch_kernel(kv_attention_merge_kernel<D, T>, grid, dim3(kMergeThreads), 0, stream,
-                       "kv_attention merge launch", p);
+  if (p.open_by_pair) {
+    const int pairs = p.c.batch * p.c.kv_heads * p.row_tiles;
+    const dim3 grid(pairs, std::min(p.tile_rows, p.rows));
+    // Parts of a pair, at most.  More threads add up many parts (32768 tokens, 8
+    // rows: 22.2 us with 1024, 26.3 with 256; 4 heads of 64 14.6 and 23.3) and start later
+    // (77 tokens, 24 rows: 13.2 and 10.7).
+    const long long parts =
+        std::min<long long>(p.warps / pairs, static_cast<long long>(p.c.width) * p.c.page / kTile);
+    if (parts >= 64)
+      return launch_kernel(kv_attention_merge_kernel<D, T, 1024>, grid, dim3(1024), 0, stream,
+                           "kv_attention merge launch", p);
+    return launch_kernel(kv_attention_merge_kernel<D, T, 256>, grid, dim3(256), 0, stream,
+                         "kv_attention merge launch", p);
+  }
+  return launch_kernel(kv_attention_merge_kernel<D, T, 256>, dim3(p.warps, std::min(p.tile_rows, p.rows)), dim3(256), 0,
+                       stream, "kv_attention merge launch", p);
 }
 
 template <int D, typename T>
