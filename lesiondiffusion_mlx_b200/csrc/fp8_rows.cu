@@ -61,6 +61,8 @@ __device__ __forceinline__ void load_row8(const T* row, int warp, int lane, int 
   }
 }
 
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+
 // Quantize the 128 channels that 16 neighbouring lanes hold, 8 each; every
 // lane of the warp takes part, lanes with `live` store.
 __device__ __forceinline__ void quantize_block(float (&y)[8], bool live, bool first, uint8_t* codes, uint8_t* scale) {
@@ -149,11 +151,32 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32,
   const unsigned step = gridDim.x * per_block, rows = p.rows;
 
   pdl_begin();
-  // gamma in shared memory: in registers it took a third of them, and half the warps.
+  // gamma in shared memory: in registers it took a third of them, and half the
+  // warps.  The first row's values come to L1 meanwhile.
   extern __shared__ float s_gamma[];
   if constexpr (NORM) {
-    for (int c = threadIdx.x; c < ITERS * kLanes * 8; c += blockDim.x)
-      s_gamma[c] = p.gamma && c < p.channels ? p.gamma[c] : 1.f;
+    if (first_row < rows) {
+#pragma unroll
+      for (int i = 0; i < ITERS; ++i) {
+        const int c = channel_of<VEC>(i * WARPS + in_row, lane, 0);
+        if (c >= p.channels) continue;
+        prefetch_l1(static_cast<const T*>(p.x) + first_row * p.x_ld + c);
+        if (p.residual) prefetch_l1(static_cast<const T*>(p.residual) + first_row * p.r_ld + c);
+      }
+    }
+    const bool whole = p.gamma && p.channels % 4 == 0 && reinterpret_cast<uintptr_t>(p.gamma) % 16 == 0;
+    for (int c = threadIdx.x * 4; c < ITERS * kLanes * 8; c += blockDim.x * 4) {
+      float4 g = make_float4(1.f, 1.f, 1.f, 1.f);
+      if (whole) {
+        if (c < p.channels) g = *reinterpret_cast<const float4*>(p.gamma + c);
+      } else if (p.gamma) {
+        float* e = &g.x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c + k < p.channels) e[k] = p.gamma[c + k];
+      }
+      *reinterpret_cast<float4*>(s_gamma + c) = g;
+    }
     __syncthreads();
   }
   for (unsigned row = first_row; row < rows; row += step) {
