@@ -623,12 +623,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < 16; ++c) r[c] = 0;
         }
         if (p.splits > 1) {
-          if (!live) continue;
+          if (live) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            reinterpret_cast<float4*>(p.o_part + part * D + c0)[c] =
-                make_float4(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1]), __uint_as_float(r[4 * c + 2]),
-                            __uint_as_float(r[4 * c + 3]));
+            for (int c = 0; c < 4; ++c)
+              reinterpret_cast<float4*>(p.o_part + part * D + c0)[c] =
+                  make_float4(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1]), __uint_as_float(r[4 * c + 2]),
+                              __uint_as_float(r[4 * c + 3]));
+          }
+          __syncwarp();  // the next read of TMEM is the whole warp's
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
