@@ -4,9 +4,12 @@
 //   o_r = sum_j 2^(s - M) 2^ev v_j / sum_j 2^(s - M)     (s in log2 units)
 //
 // with one running reference per row, M = max_j (s[r, j] + ev_j), so that every
-// weight 2^(s + ev - M) of the value product lies in [0, 1] whatever the
+// weight 2^(s + ev - M + 15) of the value product lies in [0, 2^15] whatever the
 // pages' scales are, and is rounded to f16 once; the sum takes the same weight
-// times 2^-ev in FP32.
+// times 2^-(ev + 15) in FP32.  (The 2^15 is f16's range above 1: a weight is rounded
+// to its 11 bits down to 2^-29 of the largest and is lost below 2^-40.  Without it
+// these were 2^-14 and 2^-25, and a key that takes 0.9998 of the weight, or a page of
+// zero values beside pages of scale 2^-20, cost the rest of the output its bits.)
 //
 // q k runs on the codes as they are (m16n8k32 e4m3): a query row is scaled by a
 // power of two and written as e4m3 parts, q = q0 + q1 / 16 + q2 / 256, two for
@@ -50,6 +53,7 @@ constexpr int kMaxBatch = 2048;
 // batch of 384 items of 2 to 1024 tokens took 166 us instead of 86.)
 constexpr int kStart = 3;
 constexpr float kFloor = -1.0e30f;  // reference of a row that has seen nothing
+constexpr int kHeadroom = 15;       // the largest weight is 2^15, within f16; the sum is kept without it
 
 struct AttnParams {
   KvView c;
@@ -506,14 +510,15 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
           }
         }
       }
-      // Weights 2^(s + ev - M): the fragments of p v as they are.
+      // Weights 2^(s + ev - M + kHeadroom): the fragments of p v as they are.
       uint32_t pf[G][4];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const float undo = fp8_pow2(-max(static_cast<int>(meta[n >> 1].y), -127));
+        const float undo = fp8_pow2(-max(static_cast<int>(meta[n >> 1].y), -127) - kHeadroom);
 #pragma unroll
         for (int r = 0; r < G; ++r) {
-          const float a = ex2_approx(s[r][n][0] - top[r]), bb = ex2_approx(s[r][n][1] - top[r]);
+          const float ref = top[r] - kHeadroom;
+          const float a = ex2_approx(s[r][n][0] - ref), bb = ex2_approx(s[r][n][1] - ref);
           sum[r] = fmaf(a + bb, undo, sum[r]);
           pf[r][n] = pack_half2(a, bb);
         }
@@ -587,7 +592,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
         const int row = row0 + 8 * r + 2 * c + e;
         if (row >= p.rows) continue;
         if (whole) {
-          const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];
+          const float inv = l[e] == 0.f ? 0.f : fp8_pow2(-kHeadroom) / l[e];
           T* dst = static_cast<T*>(p.out) + b * p.out_batch + (row / p.group) * p.out_ld +
                    (static_cast<long long>(head) * p.group + row % p.group) * D + g * (D / 8);
           if (D >= 64 && p.out_vec) {
@@ -683,7 +688,7 @@ __global__ void __launch_bounds__(THREADS) kv_attention_merge_kernel(const AttnP
   for (int k = 0; k < kGroups; ++k) sum += reinterpret_cast<const float*>(s_v[k])[threadIdx.x];
   static_cast<T*>(p.out)[at.x * p.out_batch + (row / p.group) * p.out_ld +
                          (static_cast<long long>(head) * p.group + row % p.group) * D + threadIdx.x] =
-      from_f32<T>(l == 0.f ? 0.f : sum / l);
+      from_f32<T>(l == 0.f ? 0.f : sum * fp8_pow2(-kHeadroom) / l);
 }
 
 // Partial rows of every warp, and the pairs left open.

@@ -9,7 +9,11 @@
 // 2^-10 (2^-7) below the row's largest, whose error is 2^-18 of that.  The weights
 // are f16 in TMEM, so the values become f16 (exact) in shared memory on the
 // way: an 8-bit product would need three parts of every weight (2^-11 of each
-// is wanted), split by the softmax warps, which are the busiest as it is.
+// is wanted), split by the softmax warps, which are the busiest as it is.  They are 2^7 at
+// the row's reference, which may lag 2^8 behind its maximum, so that they use f16's
+// range up to 2^15: 11 bits down to 2^-21 of the reference, nothing below 2^-32.
+// (A lag of 2^4 leaves room for 2^4 more, but the prompts below with queries four times as
+// large, a score's spread of 2^5.8, took 551 us instead of 510.)
 //
 // Warps: 0 loads code pages (TMA) and page scales, 1 issues the products, 2-3
 // turn values into f16, 4-7 and 8-11 run the online softmax of tile 0 and 1,
@@ -49,6 +53,7 @@ constexpr int kMeta = 4;     // ring of page factors
 constexpr int kGroups = 8;   // of 16 tokens, each of one page (pages under 64 tokens; else the groups come in fours)
 constexpr float kFloor = -1.0e30f;  // reference of a row that has seen nothing
 constexpr float kGrow = 8.f;        // a reference follows its row's maximum once that is 2^8 above
+constexpr int kHeadroom = 7;        // weights are 2^7 at the reference, 2^15 at most; the sum is kept without it
 
 template <int D, int PARTS>
 struct Cfg {
@@ -63,7 +68,7 @@ struct Cfg {
   static constexpr int kOffK = 2 * PARTS * kPartBytes;
   static constexpr int kOffV = kOffK + kStages * kRawBytes;
   static constexpr int kOffV16 = kOffV + kStages * kRawBytes;
-  static constexpr int kOffMeta = kOffV16 + 2 * kV16Bytes;  // [kMeta][8] (key factor, value exponent, 2^-exponent)
+  static constexpr int kOffMeta = kOffV16 + 2 * kV16Bytes;  // [kMeta][8] (key factor, value exponent, factor of the sum)
   static constexpr int kOffBad = kOffMeta + kMeta * kGroups * 16;  // NaN met among values that not every row sees
   static constexpr int kOffBar = kOffBad + 16;
   static constexpr int kSmem = 1024 + kOffBar + 256;
@@ -251,7 +256,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float gk = __shfl_sync(0xffffffffu, kf, of_group & 31);
         const float ge = __shfl_sync(0xffffffffu, ev, of_group & 31);
         if (lane < kGroups)
-          s_meta[ms * kGroups + lane] = make_float4(gk, ge, fp8_pow2(-max(static_cast<int>(ge), -127)), 0.f);
+          s_meta[ms * kGroups + lane] =
+              make_float4(gk, ge, fp8_pow2(-max(static_cast<int>(ge), -127) - kHeadroom), 0.f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&meta_full[ms]);
         ok = warp_wait(&v_empty[st], ph ^ 1u, abort_flag, status);
@@ -569,7 +575,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c0 = 0; c0 < kN; c0 += kCols) {
         const float4 v = meta[c0 / 16];
         const float f = factor(v.x);
-        const uint64_t f2 = pack2(f, f), shift = pack2(v.y - top, v.y - top);
+        const float ref = top - kHeadroom;
+        const uint64_t f2 = pack2(f, f), shift = pack2(v.y - ref, v.y - ref);
         uint64_t sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
         for (int h = 0; h < kCols; h += 16) {
@@ -606,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ((static_cast<long long>(split) * p.c.batch + sp.b) * p.c.kv_heads + sp.head) * p.rows + row;
       T* dst = static_cast<T*>(p.out) + sp.b * p.out_batch + i * p.out_ld +
                (static_cast<long long>(sp.head) * p.group + gq) * D;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : fp8_pow2(-kHeadroom) / l;
       // (one range: rows to shared memory, where the queries were, and from there D /
       // 8 lanes a row; stored a row per lane they took 6000 cycles at D = 128, now 4200)
       constexpr int kChunks = D / 8, kSpread = kChunks < 8 ? kChunks - 1 : 7;  // 16-byte pieces of an output row
@@ -713,7 +720,7 @@ __global__ void __launch_bounds__(256) kv_tiles_merge_kernel(const KvTileParams 
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) v[c] = fmaf(p.o_part[(s * total + at) * D + 32 * c + lane], f, v[c]);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : fp8_pow2(-kHeadroom) / l;
   const long long pair = at / p.rows;
   const int row = static_cast<int>(at - pair * p.rows);
   const int head = static_cast<int>(pair % p.c.kv_heads);
