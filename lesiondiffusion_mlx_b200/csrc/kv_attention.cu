@@ -416,6 +416,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
     float top[G], sum[G];
 #pragma unroll
     for (int r = 0; r < G; ++r) top[r] = kFloor, sum[r] = 0.f;
+    float ev_top = -INFINITY;  // largest value exponent met
 
     int slot = 0;
 #pragma unroll 1
@@ -497,9 +498,9 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
 #pragma unroll
         for (int r = 0; r < G; ++r) {
           const float m = fmaxf(top[r], mx[r]);
-          const float f = ex2_approx(top[r] - m);
+          const float half = ex2_approx(0.5f * (top[r] - m)), f = half * half;
           top[r] = m;
-          sum[r] *= f;
+          sum[r] = kv_scaled(sum[r], half);
           const float f0 = __shfl_sync(0xffffffffu, f, 8 * c), f1 = __shfl_sync(0xffffffffu, f, 8 * c + 4);
 #pragma unroll
           for (int j = 0; j < kMTiles; ++j) {
@@ -511,10 +512,13 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
         }
       }
       // Weights 2^(s + ev - M + kHeadroom): the fragments of p v as they are.
+      ev_top = fmaxf(ev_top, fmaxf(meta[0].y, meta[1].y));
+      const bool far[2] = {kv_far_below(meta[0].y, ev_top), kv_far_below(meta[1].y, ev_top)};
       uint32_t pf[G][4];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const float undo = fp8_pow2(-max(static_cast<int>(meta[n >> 1].y), -127) - kHeadroom);
+        const float undo =
+            far[n >> 1] ? 0.f : fp8_pow2(-max(static_cast<int>(meta[n >> 1].y), -127) - kHeadroom);
 #pragma unroll
         for (int r = 0; r < G; ++r) {
           const float ref = top[r] - kHeadroom;
@@ -522,6 +526,14 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
           sum[r] = fmaf(a + bb, undo, sum[r]);
           pf[r][n] = pack_half2(a, bb);
         }
+      }
+      if (far[0] || far[1]) {  // (rare)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int r = 0; r < G; ++r)
+            if (far[n >> 1])
+              sum[r] += ex2_approx(s[r][n][0] - meta[n >> 1].y - top[r]) + ex2_approx(s[r][n][1] - meta[n >> 1].y - top[r]);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -662,8 +674,9 @@ __global__ void __launch_bounds__(THREADS) kv_attention_merge_kernel(const AttnP
     const int i = i0 + threadIdx.x;
     if (i < count) {
       const float2 ml = *reinterpret_cast<const float2*>(p.ml_part + part(i) * 2);
-      s_f[threadIdx.x] = ex2_approx(ml.x - m);
-      l = fmaf(ml.y, s_f[threadIdx.x], l);
+      const float half = ex2_approx(0.5f * (ml.x - m));
+      s_f[threadIdx.x] = half * half;
+      l += kv_scaled(ml.y, half);
     }
     __syncthreads();
     const int n = min(count - i0, THREADS);

@@ -42,6 +42,17 @@ __device__ __forceinline__ int kv_query_exponent(float m) {
   return m > 0.f ? min(126, max(-119, static_cast<int>(__float_as_uint(m) >> 23) - 127)) : 0;
 }
 
+// A softmax sum adds up 2^(s - M) with M the maximum of s + ev, as the weight
+// 2^(s + ev - M) times 2^-ev.  That weight is zero in FP32 from 2^-126 on, although the
+// term still counts, where a page's exponent lies far below that of the page
+// that sets M: such pages' terms are computed apart, without ev.  For the others
+// what is lost is below 2^(kKvFar - 126) of a term that the sum has.
+constexpr float kKvFar = 64.f;
+__device__ __forceinline__ bool kv_far_below(float ev, float top) { return ev < top - kKvFar && ev >= -127.f; }
+
+// sum 2^x for x <= 0 that may lie below FP32's range while the result does not: in two halves.
+__device__ __forceinline__ float kv_scaled(float sum, float half) { return sum * half * half; }
+
 struct KvTileParams {
   KvView c;
   const void* q;

@@ -68,7 +68,7 @@ struct Cfg {
   static constexpr int kOffK = 2 * PARTS * kPartBytes;
   static constexpr int kOffV = kOffK + kStages * kRawBytes;
   static constexpr int kOffV16 = kOffV + kStages * kRawBytes;
-  static constexpr int kOffMeta = kOffV16 + 2 * kV16Bytes;  // [kMeta][8] (key factor, value exponent, factor of the sum)
+  static constexpr int kOffMeta = kOffV16 + 2 * kV16Bytes;  // [kMeta][8] (see the page warp)
   static constexpr int kOffBad = kOffMeta + kMeta * kGroups * 16;  // NaN met among values that not every row sees
   static constexpr int kOffBar = kOffBad + 16;
   static constexpr int kSmem = 1024 + kOffBar + 256;
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int box = min(p.c.page, kN), loads = kN / box;  // pages of a block (one where it is a page)
       const int used = (sp.len + p.c.page - 1) >> shift;
       int batch0 = -32, id = -1;
-      float kf = 1.f, ev = 0.f;
+      float kf = 1.f, ev = 0.f, ev_top = -INFINITY;  // (largest value exponent met)
       bool ok = true;
       int k_loads = 0, v_loads = 0;
       for (int j = 0; ok && j < sp.nblocks; ++j) {
@@ -250,14 +250,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (load) tma_load_2d(smem + C::kOffK + st * C::kRawBytes + lane * box * D, &kmap, &k_full[st], 0, row);
         ++k_loads;
-        // Factors of the block's eight groups of 16 tokens, once the loads are on their
-        // way (slot ms: the scores of block j - 2 are done, so the softmax of block j - 4 is).
+        // Factors of the block's eight groups of 16 tokens, once the loads are on their way (slot ms: the
+        // scores of block j - 2 are done, so the softmax of block j - 4 is): of the keys, the value
+        // scale's exponent, what takes that out of a weight again, and a bit for each group far below the others.
         const int of_group = off + ((lane & 7) * 16 >> shift);
         const float gk = __shfl_sync(0xffffffffu, kf, of_group & 31);
         const float ge = __shfl_sync(0xffffffffu, ev, of_group & 31);
+        ev_top = fmaxf(ev_top, ge);
+#pragma unroll
+        for (int o = 1; o < kGroups; o <<= 1) ev_top = fmaxf(ev_top, __shfl_xor_sync(0xffffffffu, ev_top, o));
+        const bool far = kv_far_below(ge, ev_top);
+        const uint32_t all_far = __ballot_sync(0xffffffffu, far && lane < kGroups);
         if (lane < kGroups)
           s_meta[ms * kGroups + lane] =
-              make_float4(gk, ge, fp8_pow2(-max(static_cast<int>(ge), -127) - kHeadroom), 0.f);
+              make_float4(gk, ge, far ? 0.f : fp8_pow2(-max(static_cast<int>(ge), -127) - kHeadroom),
+                          __uint_as_float(all_far));
         __syncwarp();
         if (lane == 0) mbar_arrive(&meta_full[ms]);
         ok = warp_wait(&v_empty[st], ph ^ 1u, abort_flag, status);
@@ -499,109 +506,129 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     float top = kFloor, l = 0.f;
     bool ok = t < sp.tiles;
-    for (int j = 0; ok && j < sp.nblocks; ++j) {
-      ok = warp_wait(&s_full[t], static_cast<uint32_t>(j) & 1u, abort_flag, status) &&
-           warp_wait(&meta_full[j % kMeta], static_cast<uint32_t>(j / kMeta) & 1u, abort_flag, status);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t sr[kN];
-#pragma unroll
-      for (int c0 = 0; c0 < kN; c0 += 32) {
-        uint32_t(&chunk)[32] = *reinterpret_cast<uint32_t(*)[32]>(&sr[c0]);
-        tmem_ld32(tmem_s + c0, chunk);
-      }
-      tmem_wait_ld();
-      if constexpr (C::kSeparateP) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[t]);
-      }
-      const int j0 = (sp.jb0 + j) * kN;
-      if (j0 + kN > sp.open) {  // hidden keys count nothing
-#pragma unroll
-        for (int c = 0; c < kN; ++c)
-          if (j0 + c >= limit) sr[c] = 0xFF800000u;
-      }
-      const float4* meta = s_meta + (j % kMeta) * kGroups;
-      constexpr int kCols = FINE ? 16 : 64;  // columns of one page
-      auto factor = [&](float kf) {
-        const float f = qs * kf;
-        return f < 1.2e-38f ? 1.2e-38f : f;  // (-inf times zero would be a NaN)
-      };
-      float mx = kFloor;
-#pragma unroll
-      for (int c0 = 0; c0 < kN; c0 += kCols) {
-        // independent chains of 3-input maxima, folded
-        float m4[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          m4[k] = fmaxf(__uint_as_float(sr[c0 + 2 * k]), __uint_as_float(sr[c0 + 2 * k + 1]));
-#pragma unroll
-        for (int c = 8; c < kCols; c += 8)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            m4[k] = max3(m4[k], __uint_as_float(sr[c0 + c + 2 * k]), __uint_as_float(sr[c0 + c + 2 * k + 1]));
-        const float4 v = meta[c0 / 16];
-        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), factor(v.x), v.y));
-      }
-      const bool first = j == 0;
-      const bool grow = first || mx - top > kGrow;
-      const float next = grow ? fmaxf(top, mx) : top;
-      const float alpha = first ? 0.f : ex2_approx(top - next);
-      if (j > 0) {
-        // the value product of the block before is done: its weights' place is free, O is whole
-        ok = warp_wait(&pv_done[t], static_cast<uint32_t>(j - 1) & 1u, abort_flag, status);
+    // The blocks from j on; without WITH_FAR, up to the first that has pages far below the others
+    // (rare).  Two loops: with those pages' terms in one, wherever they stood, the
+    // prompts of the head comment took 494 to 526 us where two take 484.
+    auto blocks = [&](int j, auto with_far) {
+      constexpr bool WITH_FAR = decltype(with_far)::value;
+      for (; ok && j < sp.nblocks; ++j) {
+        ok = warp_wait(&s_full[t], static_cast<uint32_t>(j) & 1u, abort_flag, status) &&
+             warp_wait(&meta_full[j % kMeta], static_cast<uint32_t>(j / kMeta) & 1u, abort_flag, status);
         if (!ok) break;
         tc_fence_after();
-        if (__any_sync(0xffffffffu, grow)) {
-          const float scale = grow ? alpha : 1.f;
+        uint32_t sr[kN];
 #pragma unroll
-          for (int c0 = 0; c0 < D; c0 += 16) {
-            uint32_t r[16];
-            tmem_ld16(tmem_o + c0, r);
-            tmem_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * scale);
-            tmem_st16(tmem_o + c0, r);
-          }
-          tmem_wait_st();
+        for (int c0 = 0; c0 < kN; c0 += 32) {
+          uint32_t(&chunk)[32] = *reinterpret_cast<uint32_t(*)[32]>(&sr[c0]);
+          tmem_ld32(tmem_s + c0, chunk);
         }
-      }
-      if (grow) {
-        l *= alpha;
-        top = next;
-      }
-#pragma unroll
-      for (int c0 = 0; c0 < kN; c0 += kCols) {
-        const float4 v = meta[c0 / 16];
-        const float f = factor(v.x);
-        const float ref = top - kHeadroom;
-        const uint64_t f2 = pack2(f, f), shift = pack2(v.y - ref, v.y - ref);
-        uint64_t sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-#pragma unroll
-        for (int h = 0; h < kCols; h += 16) {
-          uint32_t packed[8];
-#pragma unroll
-          for (int c = 0; c < 16; c += 2) {
-            const int at = c0 + h + c;
-            float x0, x1;
-            unpack2(fma2(pack2(__uint_as_float(sr[at]), __uint_as_float(sr[at + 1])), f2, shift), x0, x1);
-            const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
-            sum2[(c >> 1) & 1] = add2(sum2[(c >> 1) & 1], pack2(e0, e1));
-            const __half2 w = __floats2half2_rn(e0, e1);
-            packed[c / 2] = *reinterpret_cast<const uint32_t*>(&w);
-          }
-          tmem_st8(tmem_p + ((c0 + h) >> 1), packed);
+        const float4* meta = s_meta + (j % kMeta) * kGroups;
+        const uint32_t far = __float_as_uint(meta[0].w);  // groups of 16 tokens
+        tmem_wait_ld();
+        if (far && !WITH_FAR) break;
+        if constexpr (C::kSeparateP) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[t]);
         }
-        float a, b;
-        unpack2(add2(sum2[0], sum2[1]), a, b);
-        l = fmaf(a + b, v.z, l);
+        const int j0 = (sp.jb0 + j) * kN;
+        if (j0 + kN > sp.open) {  // hidden keys count nothing
+#pragma unroll
+          for (int c = 0; c < kN; ++c)
+            if (j0 + c >= limit) sr[c] = 0xFF800000u;
+        }
+        constexpr int kCols = FINE ? 16 : 64;  // columns of one page
+        auto factor = [&](float kf) {
+          const float f = qs * kf;
+          return f < 1.2e-38f ? 1.2e-38f : f;  // (-inf times zero would be a NaN)
+        };
+        float mx = kFloor;
+#pragma unroll
+        for (int c0 = 0; c0 < kN; c0 += kCols) {
+          // independent chains of 3-input maxima, folded
+          float m4[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            m4[k] = fmaxf(__uint_as_float(sr[c0 + 2 * k]), __uint_as_float(sr[c0 + 2 * k + 1]));
+#pragma unroll
+          for (int c = 8; c < kCols; c += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              m4[k] = max3(m4[k], __uint_as_float(sr[c0 + c + 2 * k]), __uint_as_float(sr[c0 + c + 2 * k + 1]));
+          const float4 v = meta[c0 / 16];
+          mx = fmaxf(mx, fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), factor(v.x), v.y));
+        }
+        const bool first = j == 0;
+        const bool grow = first || mx - top > kGrow;
+        const float next = grow ? fmaxf(top, mx) : top;
+        const float half = first ? 0.f : ex2_approx(0.5f * (top - next)), alpha = half * half;
+        if (j > 0) {
+          // the value product of the block before is done: its weights' place is free, O is whole
+          ok = warp_wait(&pv_done[t], static_cast<uint32_t>(j - 1) & 1u, abort_flag, status);
+          if (!ok) break;
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, grow)) {
+            const float scale = grow ? alpha : 1.f;
+#pragma unroll
+            for (int c0 = 0; c0 < D; c0 += 16) {
+              uint32_t r[16];
+              tmem_ld16(tmem_o + c0, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * scale);
+              tmem_st16(tmem_o + c0, r);
+            }
+            tmem_wait_st();
+          }
+        }
+        if (grow) {
+          l = kv_scaled(l, half);
+          top = next;
+        }
+        if constexpr (WITH_FAR) {
+#pragma unroll
+          for (int c0 = 0; c0 < kN; c0 += kCols) {
+            if (!((far >> (c0 / 16)) & 1u)) continue;
+            const float f = factor(meta[c0 / 16].x);
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) l += ex2_approx(fmaf(__uint_as_float(sr[c0 + c]), f, -top));
+          }
+        }
+#pragma unroll
+        for (int c0 = 0; c0 < kN; c0 += kCols) {
+          const float4 v = meta[c0 / 16];
+          const float f = factor(v.x);
+          const float ref = top - kHeadroom;
+          const uint64_t f2 = pack2(f, f), shift = pack2(v.y - ref, v.y - ref);
+          uint64_t sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+#pragma unroll
+          for (int h = 0; h < kCols; h += 16) {
+            uint32_t packed[8];
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) {
+              const int at = c0 + h + c;
+              float x0, x1;
+              unpack2(fma2(pack2(__uint_as_float(sr[at]), __uint_as_float(sr[at + 1])), f2, shift), x0, x1);
+              const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
+              sum2[(c >> 1) & 1] = add2(sum2[(c >> 1) & 1], pack2(e0, e1));
+              const __half2 w = __floats2half2_rn(e0, e1);
+              packed[c / 2] = *reinterpret_cast<const uint32_t*>(&w);
+            }
+            tmem_st8(tmem_p + ((c0 + h) >> 1), packed);
+          }
+          float a, b;
+          unpack2(add2(sum2[0], sum2[1]), a, b);
+          l = fmaf(a + b, v.z, l);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[t]);
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[t]);
-    }
+      return j;
+    };
+    const int rest = blocks(0, std::false_type{});
+    if (ok && rest < sp.nblocks) blocks(rest, std::true_type{});
     if (ok && sp.nblocks > 0)
       ok = warp_wait(&pv_done[t], static_cast<uint32_t>(sp.nblocks - 1) & 1u, abort_flag, status) &&
            warp_wait(&v16_full[(sp.nblocks - 1) & 1], static_cast<uint32_t>((sp.nblocks - 1) >> 1) & 1u, abort_flag,
@@ -715,8 +742,8 @@ __global__ void __launch_bounds__(256) kv_tiles_merge_kernel(const KvTileParams 
 #pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     const float2 ml = *reinterpret_cast<const float2*>(p.ml_part + (s * total + at) * 2);
-    const float f = ex2_approx(ml.x - m);
-    l = fmaf(ml.y, f, l);
+    const float half = ex2_approx(0.5f * (ml.x - m)), f = half * half;
+    l += kv_scaled(ml.y, half);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) v[c] = fmaf(p.o_part[(s * total + at) * D + 32 * c + lane], f, v[c]);
   }

@@ -7,7 +7,7 @@
 
 namespace ldb {
 
-constexpr int kKvMaxExponent = 96;  // page scales stay within 2^-96 .. 2^96: FP32 softmax sums of any mix of pages hold
+constexpr int kKvMaxExponent = 96;  // page scales stay within 2^-96 .. 2^96: so do the terms of a softmax sum that count
 
 struct KvView {
   const uint8_t* k;

@@ -106,3 +106,36 @@ def test_a_page_of_zero_values(cuda_device, queries, dim, page, items, zero_page
     exps = [-7] * 5, v_exp
     got = attend(q, k, v, *exps, page, dim ** -0.5, items=items)
     check(got, q, k, v, *exps, page, dim ** -0.5)
+
+
+SPREADS = [[96, -96, 96, -96, -96], [-96, -96, 96, -20, 3], [96, -96, -60, -30, -10], [-96, -80, -96, -90, -96]]
+
+
+@pytest.mark.parametrize("v_exp", SPREADS)
+@pytest.mark.parametrize("queries,dim,page,width,items", [
+    (1, 64, 16, None, 1), (1, 128, 64, None, 1), (9, 32, 32, None, 200), (2, 64, 16, None, 300), (60, 64, 16, None, 1),
+    (60, 128, 64, None, 1), (200, 32, 128, None, 1), (60, 64, 128, 40, 1)])
+def test_pages_at_both_ends_of_the_scales(cuda_device, v_exp, queries, dim, page, width, items):
+    """Every token counts in the sum of the weights, however small its page's values are."""
+    tokens = 5 * page - 3
+    q, k, v = inputs(2, tokens, queries, dim, torch.bfloat16, queries)
+    exps = [-7] * 5, v_exp
+    got = attend(q, k, v, *exps, page, dim ** -0.5, width=width, items=items)
+    check(got, q, k, v, *exps, page, dim ** -0.5)
+
+
+@pytest.mark.parametrize("queries,dim,page,items", [(1, 64, 16, 1), (1, 64, 16, 900), (3, 128, 64, 700), (60, 64, 16, 1),
+                                                    (60, 128, 64, 100)])
+@pytest.mark.parametrize("large", [0, 4])
+def test_large_values_of_tokens_with_little_weight(cuda_device, queries, dim, page, items, large):
+    """The largest page makes the output and the others the sum of the weights: 2^-49 of weight times 2^190."""
+    tokens = 5 * page
+    q, k, v = inputs(2, tokens, queries, dim, torch.bfloat16, queries)
+    scale = dim ** -0.5
+    k[:, large * page : (large + 1) * page, 0] = -320
+    q.view(queries, 2, dim)[..., 0] = 34 / (5 * scale)
+    v_exp = [-96, -95, -96, -94, -96]
+    v_exp[large] = 96
+    exps = [-6] * 5, v_exp
+    got = attend(q, k, v, *exps, page, scale, items=items)
+    check(got, q, k, v, *exps, page, scale)
