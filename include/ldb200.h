@@ -444,8 +444,10 @@ LDB_API int ldb_matmul_fp8(ldb_stream_t stream, const uint8_t* a, long long a_ld
  * head_dim], element strides _ld and _batch) of each item, or the first
  * counts[b] of them, from position start[b] on.  Where a touched page holds
  * older tokens its scale is the larger of its own and the new tokens' and the
- * older codes are rounded to it; otherwise it is the new tokens' alone.  Pages
- * written by one call belong to one item. */
+ * older codes are rounded to it (new tokens without a finite value other than
+ * zero ask for no scale there: the page's stays); otherwise it is the new tokens'
+ * alone, 1 for zeros.  Values past 448 * 2^96 saturate.  Pages written by one call
+ * belong to one item. */
 LDB_API int ldb_kv_append_fp8(ldb_stream_t stream, const void* k, long long k_ld, long long k_batch, const void* v,
                               long long v_ld, long long v_batch, int dtype, uint8_t* k_codes, uint8_t* v_codes,
                               uint8_t* k_scales, uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim,

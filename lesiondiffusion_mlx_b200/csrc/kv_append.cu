@@ -3,12 +3,14 @@
 // One warp or block per touched (page, kv head) of K or V.  With `held` older tokens in
 // the page and e(new) the scale that the new values need (fp8.cuh):
 //
-//   e = held > 0 ? max(e_old, e(new)) : e(new)
+//   e = held > 0 ? max(e_old, e(new)) : e(new)     within -96 .. 96
 //   new codes = e4m3(x 2^-e);  if e > e_old, old codes = e4m3(code 2^(e_old - e))
 //
 // so a page that is filled token by token keeps one scale, and what it holds is
-// rounded again only when that scale grows.  Writing the same tokens at the
-// same place again changes nothing.
+// rounded again only when that scale grows.  New values without a finite one other than
+// zero have no e(new) there: with the scale 1 that they have in a page of their own, a
+// padded token would make a page of scale 2^-9 512 times as coarse.  Writing the same
+// tokens at the same place again changes nothing.
 //
 // Bound: HBM (2 bytes read and 1 written a value); a page's new values stay in
 // registers between the maximum and the rounding.  For one token it is the

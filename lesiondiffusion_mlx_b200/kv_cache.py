@@ -87,7 +87,7 @@ def kv_append(cache: KvCacheFp8, k: torch.Tensor, v: torch.Tensor, table: torch.
 
     Only the first ``counts[b]`` of item ``b``'s tokens where given.  What a
     page holds before ``start`` stays, rounded again if the page's scale has to
-    grow for the new tokens; anything at or after ``start`` in the touched
+    grow for the new tokens (zeros and what is not finite never ask for that); anything at or after ``start`` in the touched
     pages counts as unwritten.  Items written together must not share the
     pages they write.  float16, bfloat16 or float32, any row and item stride."""
     (pages, heads, page, dim), device = _check_cache(cache, "kv_append")
