@@ -107,13 +107,22 @@ class Fp8TokenBlock:
         f = matmul_fp8(rows, self.ff1, self.bias1, act=_lib.LDB_ACT_GELU, out_dtype=h.dtype)
         return matmul_fp8(quantize_rows(f), self.ff2, self.bias2, residual=h, out_dtype=h.dtype)
 
+    def _check(self, x: torch.Tensor, state: KvState) -> None:
+        """Refused here, before anything is written to the state."""
+        if x.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"activations must be float16 or bfloat16, got {x.dtype}")
+        if x.ndim != 3 or x.shape[0] != state.lengths.shape[0]:
+            raise ValueError(f"activations must be ({state.lengths.shape[0]}, L, C), got {tuple(x.shape)}")
+
     def read(self, x: torch.Tensor, state: KvState) -> torch.Tensor:
         """The block with attention over every token of ``state`` (cross-attention to a bound context)."""
+        self._check(x, state)
         rows, h = rms_norm_fp8(x, self.norm1, eps=self.eps)
         return self._rest(rows, h, state, False)
 
     def extend(self, x: torch.Tensor, state: KvState) -> torch.Tensor:
         """The block with causal self-attention: ``x``'s keys and values are written behind the state's tokens."""
+        self._check(x, state)
         rows, h = rms_norm_fp8(x, self.norm1, eps=self.eps)
         state.append(*self._keys_values(rows, x.dtype))
         return self._rest(rows, h, state, True)
