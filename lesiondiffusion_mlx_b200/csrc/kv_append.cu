@@ -14,7 +14,7 @@
 //
 // Bound: HBM (2 bytes read and 1 written a value); a page's new values stay in
 // registers between the maximum and the rounding.  For one token it is the
-// launch.  One B200: 4 x 2049 tokens of 8 x 128 bf16 13.0 us (3.9 TB/s: a unit's
+// launch.  One B200: 4 x 2049 tokens of 8 x 128 bf16 13.1 us (3.8 TB/s: a unit's
 // reads depend on one another, and the grid is not many times what is
 // resident), one token of 32 items 2.6 us.
 
@@ -76,15 +76,18 @@ __device__ __forceinline__ float max_of8(const uint4 (&raw)[sizeof(T) / 2]) {
 }
 
 // WARPS of a unit (a page of one head), VECS vectors of eight values per thread
-// that a whole page takes: a warp up to 256 vectors, eight units to a block, and
-// the fewest warps above, a unit a block.  (4 x 2049 tokens, 8 heads: of 64 in pages
-// of 16, 19.2 us with 256 threads a unit, 6.9 so; of 64 in pages of 64, 8.6 and
-// 7.0; one token of 32 items, 8 heads of 128 in pages of 64, 4.0 and 2.6.)  Only pages
-// of 1024 vectors that are filled whole do better with 256 threads (8 heads of 128:
-// 13.1 and 14.5).  The
-// values stay as they came (four registers a vector in 16 bits) until they are
-// rounded, so that enough warps are resident to cover the chain of dependent
-// reads (position, page number, values).
+// that a whole page takes: a warp up to 256 vectors, eight units to a block, and a
+// unit a block above.  (4 x 2049 tokens, 8 heads of 64 in pages of 16: 19.2 us with 256
+// threads a unit, 6.9 so.)  Above 256 vectors a thread takes eight of them where a call has
+// fewer tokens than a page, which leaves most threads of a unit without work: one token of 32
+// items, 8 heads of 128 in pages of 64, 2.5 us with eight and 4.5 with four, 8 tokens of 64
+// items 6.4 and 8.4.  Else four, up to 1024 vectors, us with eight and with four: pages of 512
+// vectors 3.0 and 2.2 (128 tokens, 8 heads of 128), 6.3 and 5.0 (16 x 600, 2 heads of 128), 13.2
+// and 12.4 (4 x 2049, 8 of 128), 4.6 and 5.4 (the same, of 32); of 1024 3.0 and 2.3,
+// 6.2 and 5.1, 13.2 and 13.2, 7.0 and 7.3 (of 64); of 2048 3.1 and 2.8, 6.4 and 6.7, 13.7
+// and 13.8.  The values stay as they came (four registers a vector in 16 bits) until
+// they are rounded, so that enough warps are resident to cover the chain of
+// dependent reads (position, page number, values).
 template <typename T, int VECS, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? kAppendThreads : WARPS * 32,
                                   (sizeof(T) == 4 ? 3 : (VECS == kMaxVecs ? 4 : 6)) * (WARPS == 1 ? 1 : 8 / WARPS))
@@ -204,18 +207,18 @@ __global__ void __launch_bounds__(WARPS == 1 ? kAppendThreads : WARPS * 32,
 template <typename T>
 int launch_append(cudaStream_t stream, long long units, int batch, const AppendParams& p, unsigned int* status) {
   const int vecs = p.page * p.dim / 8;  // 64 .. 2048, a power of two
-  const bool whole = vecs == 1024 && p.tokens >= p.page;
+  const bool four = p.tokens >= p.page;  // vectors a thread, from 512 to 1024 a page
   auto k = vecs <= 64    ? kv_append_kernel<T, 2, 1>
            : vecs <= 128 ? kv_append_kernel<T, 4, 1>
            : vecs <= 256 ? kv_append_kernel<T, kMaxVecs, 1>
-           : vecs <= 512 ? kv_append_kernel<T, kMaxVecs, 2>
-           : vecs <= 1024 ? (whole ? kv_append_kernel<T, 4, 8> : kv_append_kernel<T, kMaxVecs, 4>)
+           : vecs <= 512 ? (four ? kv_append_kernel<T, 4, 4> : kv_append_kernel<T, kMaxVecs, 2>)
+           : vecs <= 1024 ? (four ? kv_append_kernel<T, 4, 8> : kv_append_kernel<T, kMaxVecs, 4>)
                           : kv_append_kernel<T, kMaxVecs, 8>;
   const long long blocks = vecs <= 256 ? (units + kAppendThreads / 32 - 1) / (kAppendThreads / 32) : units;
   if (blocks > 0x7FFFFFFFll || units > 0x7FFFFF00ll)
     return fail(LDB_ERR_SHAPE, "kv_append: %lld pages and heads of an item", units);
   const dim3 grid(static_cast<unsigned>(blocks), batch, 2);
-  const int threads = vecs <= 256 || whole ? kAppendThreads : vecs / kMaxVecs;
+  const int threads = vecs <= 256 ? kAppendThreads : vecs / (four && vecs <= 1024 ? 4 : kMaxVecs);
   return launch_kernel(k, grid, dim3(threads), 0, stream, "kv_append launch", p, status);
 }
 

@@ -50,3 +50,21 @@ def test_scales_stay_within_their_bounds(cuda_device, heads, dim, page):
         assert (codes[large, :, 0] == -448).all() and (codes[large, :, 1] == 224).all() and (codes[large, :, 2:] == 448).all()
         assert (codes[small, :, 0] == 2.0 ** -8).all() and (codes[small, :, 1] == 0).all()
     assert _lib.device_status(reset=True) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("dim,page", [(128, 32), (64, 64), (32, 128), (128, 64), (64, 128), (128, 128)])
+@pytest.mark.parametrize("fewer", [0, 1])
+def test_calls_of_a_page_and_of_one_token_less(cuda_device, dtype, dim, page, fewer):
+    """Both sides of the number of tokens that decides how a page is shared out."""
+    heads, tokens, start = 2, page - fewer, [0, 5]
+    table, pages = make_table(2, 3, cuda_device, 7)
+    cache = make_cache(pages, heads, dim, page, cuda_device, 8)
+    want = host(cache)
+    g = torch.Generator().manual_seed(page + dim)
+    k, v = ((torch.randn(2, tokens, heads * dim, generator=g) * 30).to(dtype) for _ in range(2))
+    kv_cache.kv_append(cache, k.to(cuda_device), v.to(cuda_device), table.to(cuda_device), ints(start, cuda_device))
+    for (codes, e), new in zip(((want[0], want[1]), (want[2], want[3])), (k, v)):
+        oracle.append(codes, e, new.view(2, tokens, heads, dim), table, start, [tokens] * 2)
+    same_cache(cache, want)
+    assert _lib.device_status(reset=True) == 0
