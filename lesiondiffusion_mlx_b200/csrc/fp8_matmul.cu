@@ -25,10 +25,10 @@
 // KB for 128 x 224 outputs, in and out of shared memory at 128 bytes a cycle,
 // which is what bounds it (704 cycles a K block against 448 of products).
 //
-// One B200: 8190 x 4096 x 4096 bf16 with a residual 124 us (2210 TFLOP/s, 1.32
+// One B200: 8190 x 4096 x 4096 bf16 with a residual 122 us (2240 TFLOP/s, 1.34
 // of the bf16 burst rate; tensor pipe 69 % active, 627 cycles for a K block's 448
 // of products); 6400 x 256 -> 1024 with GELU 14.4 us, bound by the epilogue; one
-// row times 8192 x 2048 8.6 us, the start of the pipeline (2.6 us of weight).
+// row times 8192 x 2048 8.2 us, the start of the pipeline (2.6 us of weight).
 
 #include <algorithm>
 

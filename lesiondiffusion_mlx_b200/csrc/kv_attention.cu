@@ -30,9 +30,9 @@
 // swizzled row are free of bank conflicts, and the orders of channels (in q k)
 // and of output rows (in p v) are chosen so that these bytes are its fragments.
 //
-// One B200, 8 heads of 128 shared by 4 bf16 queries each: 131072 tokens 54.5
+// One B200, 8 heads of 128 shared by 4 bf16 queries each: 131072 tokens 53.4
 // us (50 in this kernel, 5.4 TB/s; the start and the merge are the rest), 48 items
-// of up to 8192 tokens 77 us (5.2 TB/s).  Tiles fetched by one warp per CTA
+// of up to 8192 tokens 74 us (5.4 TB/s).  Tiles fetched by one warp per CTA
 // with TMA and shared by four others took 74 and 154 us: the fetch was bound by
 // the issue of its loads, and every change of pair by the four warps' barriers.
 
@@ -713,10 +713,13 @@ size_t workspace_bytes_of(int warps, int rows, int head_dim) {
 // hold the rows, so that a lane's output stays in registers (8 D / 32 a group).
 int row_groups(long long rows) { return rows <= 8 ? 1 : 2; }
 
-// Rows from which on the 128-row tiles of the many-row kernel are the faster:
-// 16 items of up to 4096 tokens (8 heads of 128) took 48.3 here and 73.1 us there for 32 rows,
-// 64.7 and 73.5 for 48, 82.1 and 73.6 for 64; 32768 tokens of one item 40.3, 51.6
-// and 64.0 here and 50 there.
+// Rows from which on the 128-row tiles of the many-row kernel are the faster in
+// bf16.  16 items of up to 4096 tokens, 8 heads, us here and there: of 128 channels 49 and 74 for
+// 32 rows, 65 and 74 for 48, 83 and 74 for 64; of 64 36 and 50, 48 and 51, 60 and 51; of 32 32 and
+// 49, 43 and 49, 54 and 49.  32768 tokens of one item: of 128 43 and 48, 54 and 49, 66 and 49;
+// of 32 25 and 35, 33 and 35, 47 and 36.  f16, with its third part of the queries and, at 128
+// channels, spilled registers, is past that point at 48 rows (of 128 123 and 79, of 64 66 and 52, of
+// 32 48 and 50); the workspace's size is asked for without the type, so that the rule has none.
 constexpr long long kTileRows = 49;
 
 template <int D, int G, typename T>

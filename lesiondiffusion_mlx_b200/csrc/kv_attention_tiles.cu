@@ -25,8 +25,8 @@
 // Bound: 4 D flops and one exponential per score; at D = 128 the tensor core
 // (1024 cycles per 128 x 128 tile) and the exponentials (1024 cycles) ask for
 // as much.  One B200: 4 prompts of 2048 tokens over up to 8000, 32 heads of 128
-// over 8, bf16, 480 us (764 TFLOP/s); 6400 f16 tokens over 77, 4 heads of 64,
-// 10.0 us.  A block of two tiles takes 4700 cycles: 2000 from a tile's weights to
+// over 8, bf16, 483 us (759 TFLOP/s); 6400 f16 tokens over 77, 4 heads of 64,
+// 9.9 us.  A block of two tiles takes 4700 cycles: 2000 from a tile's weights to
 // its next scores (718 for the value product, 977 for the scores, whose operands
 // take 128 bytes a cycle of shared memory), 420 for the maximum, 340 for the
 // reference, 1600 for the weights.  Slower: four softmax warpgroups with half a row
@@ -794,9 +794,11 @@ int launch_dim(cudaStream_t stream, const KvTileParams& p, int head_dim, unsigne
 
 // Ranges of tokens, from the table's capacity, in the time of a block of 128
 // tokens: a CTA's start and end take about five, the partial rows are written
-// and read once, and there is a second kernel; at most four waves.  (The lengths are
-// on the device; shorter and ragged items leave the order of the counts about as
-// it is.)  7 items of up to 19724 tokens, 523 causal queries, 4 heads of 32: 324 us in
+// and read once, and there is a second kernel; at most four waves.  The lengths are
+// on the device: items much shorter than their table has columns get too many ranges, most of them
+// empty, whose partial rows are written and read all the same (512 queries over 1000 tokens, 32
+// heads of 128 over 8: 30 us in a table of 1024 tokens, 35 of 16384, 81 of 131072; over 8000
+// tokens 99 of 8000 to 32000, 138 of 128000).  7 items of up to 19724 tokens, 523 causal queries, 4 heads of 32: 324 us in
 // one range, 149 in five.
 int kv_tile_splits(int batch, int kv_heads, long long rows, int head_dim, long long capacity) {
   const long long ctas = (rows + 2 * kM - 1) / (2 * kM) * kv_heads * batch, sms = sm_count();

@@ -1,7 +1,8 @@
 """A token block on the 8-bit operators: pre-norm attention over an 8-bit cache and a GELU feed-forward.
 
-One block, as a transformer of the denoiser's kind would run it with its dense
-weights and its keys and values held in 8 bits:
+One block of a token transformer with root-mean-square norms, its dense weights
+and its keys and values held in 8 bits (the denoiser's own blocks have layer norms
+with a bias and run in f16):
 
     rows, h = rms_norm_fp8(x, norm1)                  # codes for the projections, h the residual stream
     q = matmul_fp8(rows, to_q);  a = kv_attention(q, cache, ...)

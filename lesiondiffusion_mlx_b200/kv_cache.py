@@ -85,7 +85,8 @@ def kv_append(cache: KvCacheFp8, k: torch.Tensor, v: torch.Tensor, table: torch.
               counts: torch.Tensor | None = None) -> None:
     """Write ``(B, L, kv_heads * head_dim)`` keys and values at positions ``start[b] ..`` of each item.
 
-    Only the first ``counts[b]`` of item ``b``'s tokens where given.  What a
+    Only the first ``counts[b]`` of item ``b``'s tokens where given (a causal
+    ``kv_attention`` takes an item's last rows for its queries: see there).  What a
     page holds before ``start`` stays, rounded again if the page's scale has to
     grow for the new tokens (zeros and what is not finite never ask for that); anything at or after ``start`` in the touched
     pages counts as unwritten.  Items written together must not share the
@@ -118,9 +119,20 @@ def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, length
     ``heads`` is a multiple of the cache's; query head ``h`` reads key/value
     head ``h // (heads / kv_heads)``.  Item ``b`` has ``lengths[b]`` tokens (0
     included).  With ``causal`` the queries are the item's last ``L`` tokens:
-    query ``i`` sees the keys up to ``lengths[b] - L + i``.  A query that sees
-    no key gives zeros; a NaN among the keys or values a query does not see
-    does not reach it.  float16 or bfloat16, any row and item stride."""
+    query ``i`` sees the keys up to ``lengths[b] - L + i``.  (So an item that was
+    given fewer than ``L`` tokens has its queries in the last rows, not in the
+    first, where ``kv_append`` takes its tokens from: move them there, or attend to
+    it by itself.)  A query that sees no key gives zeros; a NaN among the keys or
+    values a query does not see does not reach it.  float16 or bfloat16, any row
+    and item stride.
+
+    The work is shared out by the table's columns, as the lengths are on the
+    device: hand over ``table[:, :n]`` where the items hold far fewer tokens than
+    they have pages.  A query's channels are exact down to 2^-10 (float16 2^-7) of
+    its row's largest and within 2^-18 of that below, for up to 48 rows of a
+    key/value head (queries times the heads that share it) down to 2^-14; weights
+    are rounded to 11 bits down to 2^-29 of the row's largest, from 49 rows on at
+    least to 2^-21, and lost below 2^-40 and 2^-32."""
     (pages, kv_heads, page, dim), device = _check_cache(cache, "kv_attention")
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"kv_attention: queries must be float16 or bfloat16, got {q.dtype}")
