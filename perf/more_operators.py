@@ -26,7 +26,7 @@ own = False
 EPS = 1e-6
 BASE = 10000.0
 GROUP = 16  # channels per scale of the 4-bit cache
-TOP = 223  # largest scale byte: 1.875 * 2^12
+TOP = 198  # largest scale byte: 1.75 * 2^9
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
@@ -423,7 +423,7 @@ def _exact_rounded(new: torch.Tensor) -> torch.Tensor:
     x = new.to(torch.float64).reshape(*new.shape[:-1], -1, GROUP)
     least = x.abs().amax(-1, keepdim=True) / 7.5
     unit = torch.exp2(torch.floor(torch.log2(least.clamp(min=2.0 ** -14))) - 3)
-    scale = (torch.ceil(least / unit) * unit).clamp(max=1.875 * 2 ** 12)
+    scale = (torch.ceil(least / unit) * unit).clamp(max=1.75 * 2 ** 9)
     times = torch.where(scale > 0, x / scale.clamp(min=2.0 ** -17), 0.0)
     return (torch.round(times).clamp(-8, 7) * scale).reshape(new.shape)
 
