@@ -1,0 +1,81 @@
+// The 4-bit format of the paged key/value cache.
+//
+// A token's channels come in groups of 16 with one scale each:
+//
+//   value = (code - 8) s,   code in 0 .. 15
+//
+// s has five bits of exponent and three of mantissa: its byte is an f16's upper eight
+// bits under the sign, so s is one shift away from an f16 and (code - 8) s is
+// exact in f16, bf16 and FP32.  Quantizing takes the least s with max|x| <= 7.5 s:
+// then no value is further than s / 2 from its code's (7.5 s goes to 7 s, -7.5 s to -8 s).
+// Bytes above kInt4TopScale are not used but for 255, a NaN, the scale of a group that holds a
+// value that is not finite.
+//
+// Codes are packed two to a byte, the lower channel in the low half:
+// codes[page][kv head][token in page][D / 2]; scales lie token by token within a
+// group, scales[page][kv head][D / 16][token in page], so that a group's scales of
+// neighbouring tokens are one word.
+//
+// (Groups of 16 normal values keep 21.8 dB of signal to error so; the 4-bit floating
+// point codes 0, 0.5, 1, 1.5, 2, 3, 4, 6 with the same scales keep 19.3.)
+#pragma once
+
+#include "fp8.cuh"
+
+namespace ldb {
+
+constexpr int kInt4Group = 16;     // channels per scale
+constexpr int kInt4TopScale = 198; // 1.75 * 2^9: 72 times it is within f16 (kernels take codes as 64 + code)
+constexpr int kInt4NanScale = 255;
+constexpr int kInt4Quad = 4;       // tokens whose scales are one word
+
+__device__ __forceinline__ float int4_scale_value(int byte) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(byte << 7)));
+}
+
+// The byte of the least scale with amax <= 7.5 s, for a finite amax >= 0: the
+// quotient's leading bits, and one more where they fall short (7.5 s is exact;
+// the quotient's own rounding may cost a second step for FP32 inputs).
+__device__ __forceinline__ int int4_scale_byte(float amax) {
+  const float t = amax * (1.f / 7.5f);
+  int byte = t < 6.103515625e-05f ? static_cast<int>(t * 131072.f)
+                                  : static_cast<int>(__float_as_uint(t) >> 20) - ((127 - 15) << 3);
+  byte = min(byte, kInt4TopScale);
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+    if (byte < kInt4TopScale && 7.5f * int4_scale_value(byte) < amax) ++byte;
+  return byte;
+}
+
+// 1 / s in two parts: x / s to within 2^-46, so that ties (frequent among 16-bit
+// values) are met exactly and go to the even code.
+struct Int4Inverse {
+  float hi, lo;
+  __device__ __forceinline__ explicit Int4Inverse(int byte) {
+    const float s = int4_scale_value(byte);
+    hi = __frcp_rn(s);
+    lo = hi * fmaf(-s, hi, 1.f);
+    if (byte == 0 || byte == kInt4NanScale) hi = lo = 0.f;
+  }
+};
+
+// Eight values to packed codes.
+__device__ __forceinline__ uint32_t int4_pack8(const float (&x)[8], const Int4Inverse& inv) {
+  // Adding 1.5 * 2^23 rounds to the nearest integer, which the sum's low bits then hold.
+  constexpr uint32_t kBias = 0x4B400000u, kOnes = 0x11111111u;
+  uint32_t word = 0;
+#pragma unroll
+  for (int j = 7; j >= 0; --j) {
+    const float q = fminf(fmaxf(fmaf(x[j], inv.hi, x[j] * inv.lo), -8.f), 7.f);
+    word = word * 16u + __float_as_uint(__fadd_rn(q, 12582912.f + 8.f));
+  }
+  return word - kBias * kOnes;
+}
+
+// Eight values of a packed word times their scale.
+__device__ __forceinline__ void int4_unpack8(uint32_t word, float s, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int>((word >> (4 * j)) & 15u) - 8) * s;
+}
+
+}  // namespace ldb

@@ -1,0 +1,183 @@
+// Reading tokens of a paged key/value cache back as rows.
+//
+//   out[b, i] = value of item b's token start[b] + i where that lies below
+//   lengths[b], else zeros
+//
+// from 4 bits ((code - 8) s, exact in every output type) or from e4m3 with the
+// page's scale (rounded once).  A thread takes 16 channels of four neighbouring
+// tokens of a page, as the 4-bit cache's scales lie.
+//
+// Bound: HBM, 9/16 or 1 byte read and 2 written a value.
+
+#include "host_common.h"
+#include "kv_cache.cuh"
+#include "kv_int4.cuh"
+
+namespace ldb {
+namespace {
+
+struct ReadParams {
+  const uint8_t* codes[2];
+  const uint8_t* scales[2];
+  void* out[2];
+  const int* table;
+  const int* lengths;
+  const int* start;  // [batch] first token read, null: 0
+  long long out_ld[2], out_batch[2], table_ld;
+  int pages, kv_heads, page_shift, width, dim, group_shift, tokens;
+  int vec;  // 16-byte stores
+};
+
+constexpr int kThreads = 128;
+
+template <typename T, bool INT4>
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadParams p, unsigned int* status) {
+  pdl_begin();
+  const int b = blockIdx.y, which = blockIdx.z;
+  const unsigned per = static_cast<unsigned>(p.kv_heads) << p.group_shift;  // groups of a token
+  const unsigned u = blockIdx.x * kThreads + threadIdx.x;
+  const unsigned quad = u / per, rest = u - quad * per;
+  const int head = rest >> p.group_shift, group = rest & ((1 << p.group_shift) - 1);
+  const long long room = static_cast<long long>(p.width) << p.page_shift;
+  int start = p.start ? p.start[b] : 0;
+  long long length = p.lengths[b];
+  if (start < 0 || length < 0 || length > room) {
+    if (u == 0) set_bad_shape(status);
+    length = start < 0 || length < 0 ? 0 : room;
+    start = max(start, 0);
+  }
+  const long long at0 = static_cast<long long>(start & ~(kInt4Quad - 1)) + static_cast<long long>(quad) * kInt4Quad;
+  const int first = static_cast<int>(max(0ll, start - at0));
+  const int last = static_cast<int>(
+      min(static_cast<long long>(kInt4Quad), static_cast<long long>(start) + p.tokens - at0));  // of the rows written
+  if (first >= last) return;
+  const int held = static_cast<int>(max(0ll, min(static_cast<long long>(last), length - at0)));  // of those with a token
+  int id = held > first ? p.table[b * p.table_ld + (at0 >> p.page_shift)] : -1;
+  if (held > first && (id < 0 || id >= p.pages)) {
+    set_bad_shape(status);
+    id = -1;
+  }
+  const int in_page = static_cast<int>(at0 & ((1 << p.page_shift) - 1));
+  const long long unit = static_cast<long long>(max(id, 0)) * p.kv_heads + head;
+  T* out = static_cast<T*>(p.out[which]) + b * p.out_batch[which] + rest * kInt4Group + (at0 - start) * p.out_ld[which];
+  uint4 raw[kInt4Quad];
+  uint32_t scale = 0;
+  if (id >= 0) {
+    if constexpr (INT4) {
+      const uint8_t* codes = p.codes[which] + ((unit << p.page_shift) + in_page) * (p.dim / 2) + group * (kInt4Group / 2);
+#pragma unroll
+      for (int j = 0; j < kInt4Quad; ++j) {  // (all four: the page holds them, written or not)
+        const uint2 w = *reinterpret_cast<const uint2*>(codes + j * (p.dim / 2));
+        raw[j] = make_uint4(w.x, w.y, 0, 0);
+      }
+      scale = *reinterpret_cast<const uint32_t*>(p.scales[which] +
+                                                 ((((unit << p.group_shift) + group) << p.page_shift) + in_page));
+    } else {
+      const uint8_t* codes = p.codes[which] + ((unit << p.page_shift) + in_page) * p.dim + group * kInt4Group;
+#pragma unroll
+      for (int j = 0; j < kInt4Quad; ++j) raw[j] = *reinterpret_cast<const uint4*>(codes + j * p.dim);
+      scale = p.scales[which][unit];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kInt4Quad; ++j) {
+    if (j < first || j >= last) continue;
+    float v[2][8];
+    if (id < 0 || j >= held) {
+#pragma unroll
+      for (int c = 0; c < kInt4Group; ++c) v[c / 8][c % 8] = 0.f;
+    } else if constexpr (INT4) {
+      const float s = int4_scale_value((scale >> (8 * j)) & 0xFFu);
+      int4_unpack8(raw[j].x, s, v[0]);
+      int4_unpack8(raw[j].y, s, v[1]);
+    } else {
+      const float s = fp8_pow2(static_cast<int>(scale) - 127);
+      const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const uint32_t two = fp8_unpack2((w[c / 2] >> (16 * (c % 2))) & 0xFFFFu);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
+        v[c / 4][2 * (c % 4)] = f.x * s, v[c / 4][2 * (c % 4) + 1] = f.y * s;
+      }
+    }
+    T* to = out + j * p.out_ld[which];
+    if (p.vec) {
+      store8<T>(to, v[0]);
+      store8<T>(to + 8, v[1]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < kInt4Group; ++c) to[c] = from_f32<T>(v[c / 8][c % 8]);
+    }
+  }
+}
+
+int kv_read(cudaStream_t stream, bool int4, const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scales,
+            const uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim, const int* table,
+            long long table_ld, int width, const int* lengths, const int* start, void* k, long long k_ld,
+            long long k_batch, void* v, long long v_ld, long long v_batch, int dtype, int batch, int tokens) {
+  if (batch < 0 || tokens < 0) return fail(LDB_ERR_SHAPE, "kv_read: %d items of %d tokens", batch, tokens);
+  if (dtype != LDB_F16 && dtype != LDB_F32 && dtype != LDB_BF16)
+    return fail(LDB_ERR_INVALID, "kv_read: unknown element type %d", dtype);
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return fail(LDB_ERR_SHAPE, "kv_read: head_dim %d (32, 64 or 128)", head_dim);
+  if (page != 16 && page != 32 && page != 64 && page != 128)
+    return fail(LDB_ERR_SHAPE, "kv_read: pages of %d tokens (16, 32, 64 or 128)", page);
+  if (pages <= 0 || kv_heads <= 0 || width <= 0 || table_ld < width)
+    return fail(LDB_ERR_SHAPE, "kv_read: %d pages, %d heads, table of %d", pages, kv_heads, width);
+  if (batch == 0 || tokens == 0) return LDB_OK;
+  if (!k || !v || !k_codes || !v_codes || !k_scales || !v_scales || !table || !lengths)
+    return fail(LDB_ERR_INVALID, "kv_read: null pointer");
+  const long long row = static_cast<long long>(kv_heads) * head_dim;
+  const long long units = ((static_cast<long long>(tokens) + kInt4Quad - 2) / kInt4Quad + 1) * (row / kInt4Group);
+  if ((tokens > 1 && (k_ld < row || v_ld < row)) || (batch > 1 && (k_batch < row || v_batch < row)) || batch > 65535 ||
+      units > 0x7FFFFF00ll)
+    return fail(LDB_ERR_SHAPE, "kv_read: row or item strides below %lld, more than 65535 items, or %lld channels and "
+                "tokens", row, units);
+  for (const uint8_t* t : {k_codes, v_codes})
+    if (reinterpret_cast<uintptr_t>(t) % 16) return fail(LDB_ERR_ALIGNMENT, "kv_read: codes must be 16-byte aligned");
+  if (int4 && (reinterpret_cast<uintptr_t>(k_scales) % 16 || reinterpret_cast<uintptr_t>(v_scales) % 16))
+    return fail(LDB_ERR_ALIGNMENT, "kv_read: scales must be 16-byte aligned");
+  unsigned int* status = device_status_ptr();
+  if (!status) return fail(LDB_ERR_CUDA, "kv_read: no device status word");
+  ReadParams p{};
+  p.codes[0] = k_codes, p.codes[1] = v_codes, p.scales[0] = k_scales, p.scales[1] = v_scales;
+  p.out[0] = k, p.out[1] = v, p.out_ld[0] = k_ld, p.out_ld[1] = v_ld, p.out_batch[0] = k_batch, p.out_batch[1] = v_batch;
+  p.table = table, p.table_ld = table_ld, p.lengths = lengths, p.start = start;
+  p.pages = pages, p.kv_heads = kv_heads, p.width = width, p.dim = head_dim, p.tokens = tokens;
+  p.page_shift = page == 16 ? 4 : (page == 32 ? 5 : (page == 64 ? 6 : 7));
+  p.group_shift = head_dim == 32 ? 1 : (head_dim == 64 ? 2 : 3);
+  const int es = dtype == LDB_F32 ? 4 : 2;
+  p.vec = 1;
+  for (int i = 0; i < 2; ++i)
+    if (reinterpret_cast<uintptr_t>(p.out[i]) % 16 || p.out_ld[i] * es % 16 || p.out_batch[i] * es % 16) p.vec = 0;
+  const dim3 grid(static_cast<unsigned>((units + kThreads - 1) / kThreads), batch, 2);
+  auto run = [&](auto kernel4, auto kernel8) {
+    return launch_kernel(int4 ? kernel4 : kernel8, grid, dim3(kThreads), 0, stream, "kv_read launch", p, status);
+  };
+  if (dtype == LDB_F16) return run(kv_read_kernel<__half, true>, kv_read_kernel<__half, false>);
+  if (dtype == LDB_BF16) return run(kv_read_kernel<__nv_bfloat16, true>, kv_read_kernel<__nv_bfloat16, false>);
+  return run(kv_read_kernel<float, true>, kv_read_kernel<float, false>);
+}
+
+}  // namespace
+}  // namespace ldb
+
+extern "C" {
+
+int ldb_kv_read_fp8(cudaStream_t stream, const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scales,
+                    const uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim, const int* table,
+                    long long table_ld, int width, const int* lengths, const int* start, void* k, long long k_ld,
+                    long long k_batch, void* v, long long v_ld, long long v_batch, int dtype, int batch, int tokens) {
+  return ldb::kv_read(stream, false, k_codes, v_codes, k_scales, v_scales, pages, kv_heads, page, head_dim, table,
+                      table_ld, width, lengths, start, k, k_ld, k_batch, v, v_ld, v_batch, dtype, batch, tokens);
+}
+
+int ldb_kv_read_int4(cudaStream_t stream, const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scales,
+                     const uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim, const int* table,
+                     long long table_ld, int width, const int* lengths, const int* start, void* k, long long k_ld,
+                     long long k_batch, void* v, long long v_ld, long long v_batch, int dtype, int batch, int tokens) {
+  return ldb::kv_read(stream, true, k_codes, v_codes, k_scales, v_scales, pages, kv_heads, page, head_dim, table,
+                      table_ld, width, lengths, start, k, k_ld, k_batch, v, v_ld, v_batch, dtype, batch, tokens);
+}
+
+}  // extern "C"

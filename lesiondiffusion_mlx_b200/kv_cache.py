@@ -1,14 +1,17 @@
-"""Paged 8-bit key/value cache: keys and values that are written once and read many times.
+"""Paged 8- or 4-bit key/value cache: keys and values that are written once and read many times.
 
-The cache holds e4m3 codes in pages of tokens, ``(pages, kv_heads, page,
+The 8-bit cache holds e4m3 codes in pages of tokens, ``(pages, kv_heads, page,
 head_dim)`` for keys and for values, with one power-of-two scale (E8M0) per
-page and head.  An item's tokens lie, in order, in the pages of its row of an
+page and head.  The 4-bit cache holds integers -8 .. 7, two to a byte, with one scale
+for each 16 channels of a token: 9/16 of the bytes, and what is written is never
+rounded again.  An item's tokens lie, in order, in the pages of its row of an
 int32 page table, so items can share pages (several seeds of one text context)
 and grow without moving.
 
-    cache = KvCacheFp8.empty(pages, kv_heads, head_dim, page=64, device="cuda")
+    cache = KvCacheFp8.empty(pages, kv_heads, head_dim, page=64, device="cuda")    # or KvCacheInt4
     kv_append(cache, k, v, table, start)          # tokens start .. start + L of every item
     out = kv_attention(q, cache, table, lengths, scale=head_dim ** -0.5)
+    k, v = kv_read(cache, table, lengths, tokens=77)              # as rows again
 
 Lengths and positions are device tensors; a page number or a length outside
 the cache is left out and sets the device status (``ldb_device_status``).
@@ -26,6 +29,9 @@ from .ops import _DT
 
 HEAD_DIMS = (32, 64, 128)
 PAGES = (16, 32, 64, 128)
+GROUP = 16  # channels per scale of the 4-bit cache
+
+_current_device = torch._C._cuda_getDevice
 
 
 class KvCacheFp8(NamedTuple):
@@ -47,8 +53,51 @@ class KvCacheFp8(NamedTuple):
         return cls(*codes, *scales)
 
 
-def _check_cache(cache: KvCacheFp8, name: str) -> tuple[torch.Size, torch.device]:
+class KvCacheInt4(NamedTuple):
+    """uint8 codes ``k``, ``v`` ``(pages, kv_heads, page, head_dim / 2)``, the lower channel in a byte's low half,
+    and scales ``(pages, kv_heads, head_dim / 16, page)``.
+
+    A code ``c`` of 0 .. 15 stands for ``(c - 8) * s``; a scale byte for the
+    float16 whose upper eight bits under the sign it is."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, head_dim: int, *, page: int = 64,
+              device: torch.device | str = "cuda") -> "KvCacheInt4":
+        """An unwritten cache of ``pages`` pages of ``page`` tokens (16, 32, 64 or 128)."""
+        if page not in PAGES or head_dim not in HEAD_DIMS:
+            raise ValueError(f"pages hold {PAGES} tokens of {HEAD_DIMS} channels, got {page} of {head_dim}")
+        shapes = [(pages, kv_heads, page, head_dim // 2)] * 2 + [(pages, kv_heads, head_dim // GROUP, page)] * 2
+        return cls(*(torch.empty(s, dtype=torch.uint8, device=device) for s in shapes))
+
+
+KvCache = KvCacheFp8 | KvCacheInt4
+
+
+def _check_cache(cache: KvCache, name: str) -> tuple[tuple[int, ...], torch.device]:
+    """((pages, kv_heads, page, head_dim), device)."""
     k, v, k_scale, v_scale = cache
+    if isinstance(cache, KvCacheInt4):
+        shape, device = k.shape, k.device
+        if len(shape) != 4 or v.shape != shape or k.dtype != torch.uint8 or v.dtype != torch.uint8:
+            raise ValueError(f"{name}: k and v must be uint8 (pages, kv_heads, page, head_dim / 2)")
+        pages, heads, page, dim = shape[0], shape[1], shape[2], 2 * shape[3]
+        if page not in PAGES or dim not in HEAD_DIMS:
+            raise ValueError(f"{name}: pages hold {PAGES} tokens of {HEAD_DIMS} channels, got {page} of {dim}")
+        per = (pages, heads, dim // GROUP, page)
+        if (k_scale.shape != per or v_scale.shape != per or k_scale.dtype != torch.uint8
+                or v_scale.dtype != torch.uint8):
+            raise ValueError(f"{name}: scales must be uint8 {per}")
+        if not k.is_cuda:
+            raise ValueError(f"{name}: the cache must be on a CUDA device")
+        if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()
+                and v.device == device and k_scale.device == device and v_scale.device == device):
+            raise ValueError(f"{name}: the cache's tensors must be contiguous and on one device")
+        return (pages, heads, page, dim), device
     shape, device = k.shape, k.device
     if len(shape) != 4 or v.shape != shape or k.dtype != CODES or v.dtype != CODES:
         raise ValueError(f"{name}: k and v must be float8_e4m3fn (pages, kv_heads, page, head_dim)")
@@ -81,17 +130,25 @@ def _check_table(table: torch.Tensor, batch: int, device: torch.device, name: st
     return width, table.stride(0) if batch > 1 else width
 
 
-def kv_append(cache: KvCacheFp8, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, *,
+def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, *,
               counts: torch.Tensor | None = None) -> None:
     """Write ``(B, L, kv_heads * head_dim)`` keys and values at positions ``start[b] ..`` of each item.
 
     Only the first ``counts[b]`` of item ``b``'s tokens where given (a causal
     ``kv_attention`` takes an item's last rows for its queries: see there).  What a
-    page holds before ``start`` stays, rounded again if the page's scale has to
+    page holds before ``start`` stays, in 8 bits rounded again if the page's scale has to
     grow for the new tokens (zeros and what is not finite never ask for that); anything at or after ``start`` in the touched
     pages counts as unwritten.  Items written together must not share the
-    pages they write.  float16, bfloat16 or float32, any row and item stride."""
+    pages they write.  float16, bfloat16 or float32, any row and item stride.
+
+    In 4 bits a value is within half its scale, a 15th of the largest of its 16
+    channels (and up to an eighth more: a scale has four bits); magnitudes past 6720
+    saturate, below 2^-18 they vanish, and 16 channels with one that is not finite are NaN."""
     (pages, heads, page, dim), device = _check_cache(cache, "kv_append")
+    int4 = isinstance(cache, KvCacheInt4)
+    if int4 and device.index != _current_device():
+        with torch.cuda.device(device):
+            return kv_append(cache, k, v, table, start, counts=counts)
     if k.dtype not in _DT or v.dtype != k.dtype:
         raise ValueError("kv_append: k and v must share dtype float16, bfloat16 or float32")
     if k.ndim != 3 or v.shape != k.shape or k.shape[2] != heads * dim:
@@ -106,13 +163,13 @@ def kv_append(cache: KvCacheFp8, k: torch.Tensor, v: torch.Tensor, table: torch.
     _check_index(start, 1, batch, device, "kv_append: start")
     if counts is not None:
         _check_index(counts, 1, batch, device, "kv_append: counts")
-    _launcher("kv_append")("ldb_kv_append_fp8", _raw_stream(k.get_device()), k.data_ptr(), k_ld, k_batch,
+    _launcher("kv_append")("ldb_kv_append_int4" if int4 else "ldb_kv_append_fp8", _raw_stream(k.get_device()), k.data_ptr(), k_ld, k_batch,
             v.data_ptr(), v_ld, v_batch, _DT[k.dtype], cache.k.data_ptr(), cache.v.data_ptr(),
             cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pages, heads, page, dim, table.data_ptr(), table_ld,
             width, start.data_ptr(), None if counts is None else counts.data_ptr(), batch, tokens)
 
 
-def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, lengths: torch.Tensor, *, scale: float,
+def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, *, scale: float,
                  causal: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """``softmax(q k^T * scale) v`` of ``(B, L, heads * head_dim)`` queries over each item's cached tokens.
 
@@ -128,12 +185,17 @@ def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, length
 
     The work is shared out by the table's columns, as the lengths are on the
     device: hand over ``table[:, :n]`` where the items hold far fewer tokens than
-    they have pages.  A query's channels are exact down to 2^-10 (float16 2^-7) of
+    they have pages.  Over 8 bits, a query's channels are exact down to 2^-10 (float16 2^-7) of
     its row's largest and within 2^-18 of that below, for up to 48 rows of a
     key/value head (queries times the heads that share it) down to 2^-14; weights
     are rounded to 11 bits down to 2^-29 of the row's largest, from 49 rows on at
-    least to 2^-21, and lost below 2^-40 and 2^-32."""
+    least to 2^-21, and lost below 2^-40 and 2^-32.  Over 4 bits queries are exact (bfloat16
+    down to 2^-31 of the row's largest) and the weights as over 8."""
     (pages, kv_heads, page, dim), device = _check_cache(cache, "kv_attention")
+    int4 = isinstance(cache, KvCacheInt4)
+    if int4 and device.index != _current_device():
+        with torch.cuda.device(device):
+            return kv_attention(q, cache, table, lengths, scale=scale, causal=causal, out=out)
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"kv_attention: queries must be float16 or bfloat16, got {q.dtype}")
     if q.ndim != 3 or q.device != device or q.shape[2] % (kv_heads * dim) or q.shape[2] == 0:
@@ -152,14 +214,54 @@ def kv_attention(q: torch.Tensor, cache: KvCacheFp8, table: torch.Tensor, length
     out_batch, out_ld, _ = out.stride()
     heads = channels // dim
     index = q.get_device()
-    need = _workspace_bytes("ldb_kv_attention_fp8_table_workspace_size", index, batch, queries, heads, kv_heads, dim,
+    need = _workspace_bytes("ldb_kv_attention_int4_workspace_size" if int4 else
+                            "ldb_kv_attention_fp8_table_workspace_size", index, batch, queries, heads, kv_heads, dim,
                             width * page)
     ws_ptr = None
     if need:
         ws = q.new_empty(need, dtype=torch.uint8)
         ws_ptr = ws.data_ptr()
-    _launcher("kv_attention")("ldb_kv_attention_fp8", _raw_stream(index), q.data_ptr(), q_ld, q_batch,
+    _launcher("kv_attention")("ldb_kv_attention_int4" if int4 else "ldb_kv_attention_fp8", _raw_stream(index), q.data_ptr(), q_ld, q_batch,
             _DT[q.dtype], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
             pages, kv_heads, page, dim, table.data_ptr(), table_ld, width, lengths.data_ptr(), out.data_ptr(), out_ld,
             out_batch, batch, queries, heads, scale, int(causal), ws_ptr, need)
     return out
+
+
+def kv_read(cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, *, tokens: int,
+            start: torch.Tensor | None = None, dtype: torch.dtype = torch.float16,
+            out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values ``(B, tokens, kv_heads * head_dim)`` of each item's tokens ``start[b] ..`` (from 0 without ``start``).
+
+    Rows at or behind ``lengths[b]`` are zeros.  float16, bfloat16 or float32:
+    exact from a 4-bit cache, rounded once from 8 bits.  ``out`` takes a pair of tensors to
+    write, of any row and item stride."""
+    (pages, heads, page, dim), device = _check_cache(cache, "kv_read")
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return kv_read(cache, table, lengths, tokens=tokens, start=start, dtype=dtype, out=out)
+    if lengths.ndim != 1 or tokens < 0:
+        raise ValueError(f"kv_read: lengths must be one number per item and tokens at least 0, got {tokens}")
+    batch = lengths.shape[0]
+    width, table_ld = _check_table(table, batch, device, "kv_read: table")
+    _check_index(lengths, 1, batch, device, "kv_read: lengths")
+    if start is not None:
+        _check_index(start, 1, batch, device, "kv_read: start")
+    shape = (batch, tokens, heads * dim)
+    if out is None:
+        if dtype not in _DT:
+            raise ValueError(f"kv_read: dtype must be float16, bfloat16 or float32, got {dtype}")
+        out = (cache.k.new_empty(shape, dtype=dtype), cache.k.new_empty(shape, dtype=dtype))
+    k, v = out
+    if (k.shape != shape or v.shape != shape or k.dtype not in _DT or v.dtype != k.dtype or k.device != device
+            or v.device != device):
+        raise ValueError(f"kv_read: out must be two tensors {shape} of one float dtype on the cache's device")
+    (k_batch, k_ld, k_step), (v_batch, v_ld, v_step) = k.stride(), v.stride()
+    if k_step != 1 or v_step != 1:
+        raise ValueError("kv_read: channel axis must have unit stride")
+    _launcher("kv_read")("ldb_kv_read_int4" if isinstance(cache, KvCacheInt4) else "ldb_kv_read_fp8",
+            _raw_stream(device.index), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+            cache.v_scale.data_ptr(), pages, heads, page, dim, table.data_ptr(), table_ld, width, lengths.data_ptr(),
+            None if start is None else start.data_ptr(), k.data_ptr(), k_ld, k_batch, v.data_ptr(), v_ld, v_batch,
+            _DT[k.dtype], batch, tokens)
+    return k, v
