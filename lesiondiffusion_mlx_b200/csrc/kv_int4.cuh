@@ -78,4 +78,25 @@ __device__ __forceinline__ void int4_unpack8(uint32_t word, float s, float (&v)[
   for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int>((word >> (4 * j)) & 15u) - 8) * s;
 }
 
+// ------------------------------------------------------------ unpacking to f16
+
+__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+__device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+// The scale bytes of `word` that `sel` names (the lower and the upper one as f16, see scale_selector).
+__device__ __forceinline__ uint32_t scale_pair(uint32_t word, uint32_t sel) { return __byte_perm(word, 0, sel) >> 1; }
+__device__ __forceinline__ uint32_t scale_selector(int lower, int upper) { return 0x0404u | lower << 4 | upper << 12; }
+
+// The four pairs of codes (n, n + 4) of a word's two halves as values: (64 + code) s - 72 s.
+__device__ __forceinline__ void unpack4(uint32_t w, __half2 s, __half2 minus72s, uint32_t (&v)[4]) {
+  constexpr uint32_t kMask = 0x00F000F0u, k64 = 0x54005400u;
+  v[0] = ((w << 4) & kMask) | k64;
+  v[1] = (w & kMask) | k64;
+  v[2] = ((w >> 4) & kMask) | k64;
+  v[3] = ((w >> 8) & kMask) | k64;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) v[n] = as_word(__hfma2(as_half2(v[n]), s, minus72s));
+}
+__device__ __forceinline__ __half2 minus72(uint32_t s) { return __hmul2(as_half2(s), __float2half2_rn(-72.f)); }
+
 }  // namespace ldb

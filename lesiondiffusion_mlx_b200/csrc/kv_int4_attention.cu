@@ -23,6 +23,7 @@
 #include "kv_attention.cuh"
 #include "kv_attention_ranges.cuh"
 #include "kv_int4.cuh"
+#include "kv_int4_attention.cuh"
 
 namespace ldb {
 namespace {
@@ -48,25 +49,6 @@ struct Cfg {
   static constexpr int kOffBase = kWarps * kSlots * kSlotBytes;  // [batch + 1] int
 };
 int ctas_per_sm(int head_dim) { return head_dim == 128 ? Cfg<128, 1>::kCtasPerSm : Cfg<64, 1>::kCtasPerSm; }
-
-__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
-__device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
-
-// The scale bytes of `word` that `sel` names (the lower and the upper one as f16, see scale_selector).
-__device__ __forceinline__ uint32_t scale_pair(uint32_t word, uint32_t sel) { return __byte_perm(word, 0, sel) >> 1; }
-__device__ __forceinline__ uint32_t scale_selector(int lower, int upper) { return 0x0404u | lower << 4 | upper << 12; }
-
-// The four pairs of codes (n, n + 4) of a word's two halves as values: (64 + code) s - 72 s.
-__device__ __forceinline__ void unpack4(uint32_t w, __half2 s, __half2 minus72s, uint32_t (&v)[4]) {
-  constexpr uint32_t kMask = 0x00F000F0u, k64 = 0x54005400u;
-  v[0] = ((w << 4) & kMask) | k64;
-  v[1] = (w & kMask) | k64;
-  v[2] = ((w >> 4) & kMask) | k64;
-  v[3] = ((w >> 8) & kMask) | k64;
-#pragma unroll
-  for (int n = 0; n < 4; ++n) v[n] = as_word(__hfma2(as_half2(v[n]), s, minus72s));
-}
-__device__ __forceinline__ __half2 minus72(uint32_t s) { return __hmul2(as_half2(s), __float2half2_rn(-72.f)); }
 
 // A run of tiles of one (item, head, row tile) pair, and the copies of its tiles into the warp's ring.
 template <int D>
@@ -517,6 +499,9 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
 // Groups of eight query rows that one pass over the cache serves.
 int row_groups(long long rows) { return rows <= 8 ? 1 : 2; }
 
+// Rows from which on the 128-row tiles of the many-row kernel are the faster.
+constexpr long long kTileRows = 49;
+
 template <int D, int G, typename T>
 int launch(cudaStream_t stream, const AttnParams& p, unsigned int* status) {
   static unsigned long long configured = 0;
@@ -553,7 +538,9 @@ int ldb_kv_attention_int4_workspace_size(int batch, int queries, int heads, int 
       (head_dim != 32 && head_dim != 64 && head_dim != 128))
     return fail(LDB_ERR_SHAPE, "kv_attention: %d heads over %d of width %d (32, 64 or 128)", heads, kv_heads, head_dim);
   const long long rows = static_cast<long long>(queries) * (heads / kv_heads);
-  *bytes = workspace_bytes_of(ctas_per_sm(head_dim) * sm_count() * kWarps, kGroupRows * row_groups(rows), head_dim);
+  *bytes = rows >= kTileRows ? kv_int4_tile_workspace(batch, kv_heads, rows, head_dim, capacity)
+                             : workspace_bytes_of(ctas_per_sm(head_dim) * sm_count() * kWarps,
+                                                  kGroupRows * row_groups(rows), head_dim);
   return LDB_OK;
 }
 
@@ -595,12 +582,20 @@ int ldb_kv_attention_int4(cudaStream_t stream, const void* q, long long q_ld, lo
                     table_ld, pages,   kv_heads, page,     width, batch};
   const long long group_rows = static_cast<long long>(queries) * (heads / kv_heads);
   if (group_rows > 0x7FFFFF00ll) return fail(LDB_ERR_SHAPE, "kv_attention: too many query rows");
+  const int q_vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_ld % 8 == 0 && q_batch % 8 == 0;
+  const int out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_ld % 8 == 0 && out_batch % 8 == 0;
+  if (group_rows >= kTileRows) {
+    KvTileParams t{};
+    t.c = view;
+    t.q = q, t.q_ld = q_ld, t.q_batch = q_batch, t.q_vec = q_vec;
+    t.out = out, t.out_ld = out_ld, t.out_batch = out_batch, t.out_vec = out_vec;
+    t.queries = queries, t.group = heads / kv_heads, t.rows = static_cast<int>(group_rows), t.causal = causal != 0;
+    return kv_int4_attention_tiles(stream, t, head_dim, dtype, scale, workspace, status);
+  }
   AttnParams p{};
   p.c = view;
-  p.q = q, p.q_ld = q_ld, p.q_batch = q_batch;
-  p.q_vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_ld % 8 == 0 && q_batch % 8 == 0;
-  p.out = out, p.out_ld = out_ld, p.out_batch = out_batch;
-  p.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_ld % 8 == 0 && out_batch % 8 == 0;
+  p.q = q, p.q_ld = q_ld, p.q_batch = q_batch, p.q_vec = q_vec;
+  p.out = out, p.out_ld = out_ld, p.out_batch = out_batch, p.out_vec = out_vec;
   p.queries = queries, p.group = heads / kv_heads;
   p.tile_rows = kGroupRows * row_groups(group_rows);
   const long long row_tiles = (group_rows + p.tile_rows - 1) / p.tile_rows;

@@ -1,0 +1,608 @@
+// Attention of many query rows over the paged 4-bit key/value cache, on the
+// tcgen05 tensor cores (few rows: kv_int4_attention.cu, whose formulas these are).
+//
+// One CTA owns two 128-row tiles of one (item, key/value head) and streams
+// blocks of 128 tokens once for both.  Keys and values become f16 (exact) on the way: a
+// warpgroup reads a token a thread from the cache into registers, a block ahead,
+// unpacks it and writes its row to shared memory as the products read it.
+// Unpacking leaves eight channels in the order 0, 4, 1, 5, 2, 6, 3, 7: the queries
+// are laid out alike, and an output row is put in order as it leaves.  Queries are f16
+// as they are, or bf16 rows scaled by a power of two.  The weights are f16 in TMEM, 2^7 at the row's
+// reference, which may lag 2^8 behind its maximum: 11 bits down to 2^-21 of the
+// reference, nothing below 2^-32.
+//
+// Warps: 0 issues the products, 4-7 unpack, 8-11 and 12-15 run the online softmax of
+// tile 0 and 1, one row per thread.  Grids that leave SMs idle cut the tokens into ranges, merged
+// by a second kernel (kv_attention_tiles.cuh).
+//
+// Bound: 4 D flops and one exponential per score.
+
+#include <algorithm>
+
+#include "host_common.h"
+#include "kv_attention.cuh"
+#include "kv_attention_tiles.cuh"
+#include "kv_int4.cuh"
+#include "kv_int4_attention.cuh"
+
+namespace ldb {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kRegsWg0 = 48;      // products
+constexpr int kRegsUnpack = 80;
+constexpr int kRegsSoftmax = 192; // a row's 128 scores
+static_assert(128 * (kRegsWg0 + kRegsUnpack + 2 * kRegsSoftmax) <= kThreads * 128, "register split");
+constexpr int kMeta = 4;          // ring of the masks of missing pages
+
+template <int D>
+struct Cfg {
+  static constexpr int kSubD = D == 32 ? 32 : 64;  // channels of one swizzled tile
+  static constexpr int kSubRow = kSubD * 2;
+  static constexpr uint32_t kLayout = kSubD == 64 ? kSwizzle128 : kSwizzle64;
+  static constexpr int kTileBytes = kN * D * 2;    // 128 rows: queries, keys or values
+  static constexpr int kGroups = D / kInt4Group;
+  static constexpr int kOffK = 2 * kTileBytes;
+  static constexpr int kOffV = kOffK + 2 * kTileBytes;
+  static constexpr int kOffMeta = kOffV + 2 * kTileBytes;  // [kMeta][4] bytes: a bit for each 16 tokens of a missing page
+  static constexpr int kOffBad = kOffMeta + kMeta * 4;     // NaN met among values that not every row sees
+  static constexpr int kOffBar = kOffBad + 16;
+  static constexpr int kSmem = 1024 + kOffBar + 256;
+  // TMEM: S_t at 128 t, O_t at 256 + 128 t.  D = 128: the weights overwrite
+  // their scores; narrower heads have room for them behind O_t, so that the next block's
+  // scores need not wait for the value product.
+  static constexpr bool kSeparateP = D <= 64;
+  static_assert(kSmem <= 232448, "shared memory");
+  // Where 16 bytes (channels 8 chunk ..) of a row lie in a tile.
+  static __device__ __forceinline__ int place(int row, int chunk) {
+    constexpr int kPer = kSubRow / 16;
+    return (chunk / kPer) * kN * kSubRow + swizzle_offset(row * kSubRow + (chunk % kPer) * 16, kSubRow);
+  }
+};
+
+// D[tmem] (+)= A[smem] * B[smem]^T of f16 operands, by one elected lane of a convergent warp.
+__device__ __forceinline__ void umma_ss_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// A token's codes and scales of keys or of values.
+template <int D>
+struct Packed {
+  uint4 code[D / 32];
+  uint32_t scale[(D / kInt4Group + 3) / 4];
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTileParams p, unsigned int* status) {
+  using C = Cfg<D>;
+  constexpr bool kScaled = !std::is_same<T, __half>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_meta = smem + C::kOffMeta;
+  uint32_t* s_bad = reinterpret_cast<uint32_t*>(smem + C::kOffBad);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* q_full = bars;              // the queries are written
+  uint64_t* k_full = q_full + 1;        // [2] f16 keys are written
+  uint64_t* k_empty = k_full + 2;       // [2] both tiles' scores have read them
+  uint64_t* v_full = k_empty + 2;       // [2] f16 values are written
+  uint64_t* v_empty = v_full + 2;       // [2] the value products have read them
+  uint64_t* meta_full = v_empty + 2;    // [kMeta] the mask of missing pages is written
+  uint64_t* s_full = meta_full + kMeta; // [2] per tile
+  uint64_t* s_free = s_full + 2;        // [2] scores are in registers
+  uint64_t* p_ready = s_free + 2;       // [2] weights are in TMEM
+  uint64_t* pv_done = p_ready + 2;      // [2]
+  uint64_t* drain = pv_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((1 + 8 + kMeta + 8 + 1) * 8 + 8 <= 256, "barrier block");
+
+  const int warp = warp_id(), lane = lane_id();
+  if (threadIdx.x == 0) {
+    mbar_init(drain, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], 4);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 4);
+      mbar_init(&v_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_free[s], 4);
+      mbar_init(&p_ready[s], 4);
+      mbar_init(&pv_done[s], 1);
+    }
+    for (int s = 0; s < kMeta; ++s) mbar_init(&meta_full[s], 4);
+    mbar_init(q_full, p.rows - (p.row_blocks - 1 - static_cast<int>(blockIdx.x) / p.splits) * 2 * kM > kM ? 8 : 4);
+    *abort_flag = 0;
+    *s_bad = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_begin();
+  const Span sp = span_of(p, status);
+
+  if (warp < 4) {
+    regs_dec<kRegsWg0>();
+    if (warp == 0 && sp.nblocks > 0) {
+      // --------------------------------------------------------- products
+      constexpr uint32_t idesc_qk = make_idesc_f16(kM, kN, 0u, 0u, 0u);
+      constexpr uint32_t idesc_pv = make_idesc_f16(kM, D, 0u, 0u, 1u);
+      auto scores = [&](int t, int j) {
+        const uint32_t q_addr = smem_u32(smem + t * C::kTileBytes);
+        const uint32_t k_addr = smem_u32(smem + C::kOffK + (j & 1) * C::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k * 16 / C::kSubD) * kN * C::kSubRow + (k * 32) % C::kSubRow;
+          umma_ss_warp(tmem + t * 128, make_smem_desc(q_addr + off, 16, 8 * C::kSubRow, C::kLayout),
+                       make_smem_desc(k_addr + off, 16, 8 * C::kSubRow, C::kLayout), idesc_qk, k > 0 ? 1u : 0u);
+        }
+        umma_commit_warp(&s_full[t]);
+      };
+      auto values = [&](int t, int j) {
+        const uint32_t v_addr = smem_u32(smem + C::kOffV + (j & 1) * C::kTileBytes);
+        const uint32_t p_tmem = C::kSeparateP ? tmem + 256 + t * 128 + 64 : tmem + t * 128;
+#pragma unroll
+        for (int k = 0; k < kN / 16; ++k)  // (tiles of 64 channels lie kN rows apart)
+          umma_ts_warp(tmem + 256 + t * 128, p_tmem + k * 8,
+                       make_smem_desc(v_addr + k * 16 * C::kSubRow, kN * C::kSubRow, 8 * C::kSubRow, C::kLayout),
+                       idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+        umma_commit_warp(&pv_done[t]);
+      };
+      bool ok = warp_wait(q_full, 0, abort_flag, status);
+      for (int j = 0; ok && j <= sp.nblocks; ++j) {
+        const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u, was = static_cast<uint32_t>(j - 1) & 1u;
+        if (j < sp.nblocks) ok = warp_wait(&k_full[j & 1], ph, abort_flag, status);
+        if (ok && j > 0)
+          ok = warp_wait(&v_full[(j - 1) & 1], static_cast<uint32_t>((j - 1) >> 1) & 1u, abort_flag, status);
+        if constexpr (C::kSeparateP) {
+          for (int t = 0; ok && j < sp.nblocks && t < sp.tiles; ++t) {
+            // the softmax has the scores of the block before in registers
+            if (j > 0) ok = warp_wait(&s_free[t], was, abort_flag, status);
+            if (!ok) break;
+            tc_fence_after();
+            scores(t, j);
+          }
+          if (ok && j < sp.nblocks) umma_commit_warp(&k_empty[j & 1]);
+          for (int t = 0; ok && j > 0 && t < sp.tiles; ++t) {
+            ok = warp_wait(&p_ready[t], was, abort_flag, status);
+            if (!ok) break;
+            tc_fence_after();
+            values(t, j - 1);
+          }
+        } else {
+          for (int t = 0; ok && t < sp.tiles; ++t) {
+            if (j > 0) {
+              ok = warp_wait(&p_ready[t], was, abort_flag, status);
+              if (!ok) break;
+              tc_fence_after();
+              values(t, j - 1);
+            }
+            if (j < sp.nblocks) {
+              if (j == 0) tc_fence_after();
+              scores(t, j);
+            }
+          }
+          if (ok && j < sp.nblocks) umma_commit_warp(&k_empty[j & 1]);
+        }
+        if (ok && j > 0) umma_commit_warp(&v_empty[(j - 1) & 1]);
+      }
+      umma_commit_warp(drain);
+      volatile int never = 0;
+      mbar_wait(drain, 0, &never, status);
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ unpacking
+    regs_dec<kRegsUnpack>();
+    const int tid = threadIdx.x - 128;  // token of the block
+    const int shift = 31 - __clz(p.c.page);
+    // the page of the thread's token of block j, -1 where it has none
+    auto page_of = [&](int j) {
+      const int tok = (sp.jb0 + j) * kN + tid;
+      if (j >= sp.nblocks || tok >= sp.len) return -1;
+      const int id = p.c.table[sp.b * p.c.table_ld + (tok >> shift)];
+      if (id >= 0 && id < p.c.pages) return id;
+      set_bad_shape(status);
+      return -2;
+    };
+    auto load = [&](int id, const uint8_t* codes, const uint8_t* scales, Packed<D>& to) {
+      if (id < 0) {  // zeros: codes are of no account under a scale of zero
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) to.code[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < (C::kGroups + 3) / 4; ++i) to.scale[i] = 0;
+        return;
+      }
+      const int in = tid & (p.c.page - 1);  // (a block starts a page, or 128 tokens are one)
+      const long long unit = static_cast<long long>(id) * p.c.kv_heads + sp.head;
+      const uint4* from = reinterpret_cast<const uint4*>(codes + (unit * p.c.page + in) * (D / 2));
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) to.code[i] = from[i];
+      const uint8_t* s = scales + unit * C::kGroups * p.c.page + in;
+#pragma unroll
+      for (int i = 0; i < (C::kGroups + 3) / 4; ++i) {
+        to.scale[i] = 0;
+#pragma unroll
+        for (int g = 4 * i; g < C::kGroups && g < 4 * i + 4; ++g)
+          to.scale[i] |= static_cast<uint32_t>(s[g * p.c.page]) << (8 * (g & 3));
+      }
+    };
+    auto unpack = [&](const Packed<D>& from, uint8_t* to) {
+#pragma unroll
+      for (int g = 0; g < C::kGroups; ++g) {
+        const uint32_t sel = scale_selector(g & 3, g & 3);
+        const uint32_t sc = scale_pair(from.scale[g >> 2], sel);
+        const __half2 m = minus72(sc);
+        const uint4 w = from.code[g >> 1];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t v[4];
+          unpack4((g & 1) ? (h ? w.w : w.z) : (h ? w.y : w.x), as_half2(sc), m, v);
+          *reinterpret_cast<uint4*>(to + C::place(tid, 2 * g + h)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    Packed<D> k, v;
+    int id = page_of(0), next = page_of(1);
+    load(id, p.c.k, p.c.k_scale, k);
+    bool ok = true;
+    for (int j = 0; ok && j < sp.nblocks; ++j) {
+      const int st = j & 1, ms = j % kMeta;
+      const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u;
+      const int after = page_of(j + 2);
+      load(id, p.c.v, p.c.v_scale, v);
+      ok = warp_wait(&k_empty[st], ph ^ 1u, abort_flag, status);
+      if (!ok) break;
+      // (the scores of block j - 2 are done, so the softmax has read the mask of block j - 4)
+      const uint32_t missing = __ballot_sync(0xffffffffu, id == -2);
+      if (lane == 0) {
+        s_meta[ms * 4 + (warp & 3)] = ((missing & 0xFFFFu) ? 1 : 0) | ((missing >> 16) ? 2 : 0);
+        mbar_arrive(&meta_full[ms]);
+      }
+      unpack(k, smem + C::kOffK + st * C::kTileBytes);
+      if (lane == 0) mbar_arrive(&k_full[st]);
+      load(next, p.c.k, p.c.k_scale, k);
+      if ((sp.jb0 + j + 1) * kN > sp.open) {
+        // Where some rows may not see a token its NaN becomes zero here, and
+        // the rows that do see it get the NaN at the end.
+#pragma unroll
+        for (int g = 0; g < C::kGroups; ++g) {
+          if (((v.scale[g >> 2] >> (8 * (g & 3))) & 0xFFu) == kInt4NanScale) {
+            v.scale[g >> 2] &= ~(0xFFu << (8 * (g & 3)));
+            *s_bad = 1;
+          }
+        }
+      }
+      ok = warp_wait(&v_empty[st], ph ^ 1u, abort_flag, status);
+      if (!ok) break;
+      unpack(v, smem + C::kOffV + st * C::kTileBytes);
+      if (lane == 0) mbar_arrive(&v_full[st]);
+      id = next;
+      next = after;
+    }
+  } else {
+    regs_inc<kRegsSoftmax>();
+    // ------------------------------------------------------------ softmax
+    const int t = (warp - 8) >> 2;  // tile of this warpgroup
+    const int quarter = warp & 3;   // TMEM lanes this warp may access
+    const int local = quarter * 32 + lane;
+    const int row = sp.row0 + t * kM + local;
+    const bool live = row < p.rows;
+    const int i = live ? row / p.group : 0, gq = live ? row % p.group : 0;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t tmem_s = tmem + t * 128 + lane_base;
+    const uint32_t tmem_o = tmem + 256 + t * 128 + lane_base;
+    const uint32_t tmem_p = C::kSeparateP ? tmem_o + 64 : tmem_s;
+    const int limit = p.causal && live ? min(sp.len, sp.len - p.queries + i + 1) : sp.len;  // keys that the row sees
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes of a row (eight channels each), rows at a time
+    float factor = 1.f;
+    if (t < sp.tiles && sp.nblocks > 0) {
+      // Query rows in the keys' order of channels; the largest magnitude of a bf16
+      // row to [2^14, 2^15).  A NaN stays one, an infinity makes the row's factor one (of a row that
+      // sees any key).
+      const T* src = static_cast<const T*>(p.q) + sp.b * p.q_batch + i * p.q_ld +
+                     (static_cast<long long>(sp.head) * p.group + gq) * D;
+      const int part_lane = lane % kLanes;
+      float top_of = 0.f;  // largest magnitude of the lane's own row
+#pragma unroll 1
+      for (int n0 = 0; n0 < kLanes; n0 += 4) {
+        uint4 raw[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int from = (n0 + n) * kRows + lane / kLanes;  // row of the warp, and the lane that owns it
+          const T* at = reinterpret_cast<const T*>(__shfl_sync(
+                            0xffffffffu, reinterpret_cast<unsigned long long>(src), from)) + 8 * part_lane;
+          raw[n] = make_uint4(0, 0, 0, 0);
+          if (sp.row0 + t * kM + quarter * 32 + from < p.rows) {
+            if (p.q_vec) {
+              raw[n] = *reinterpret_cast<const uint4*>(at);
+            } else {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(at);
+              raw[n] = make_uint4(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16,
+                                  h[4] | static_cast<uint32_t>(h[5]) << 16, h[6] | static_cast<uint32_t>(h[7]) << 16);
+            }
+          }
+        }
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) {
+          const int n = n0 + k4;
+          uint32_t w[4] = {raw[k4].x, raw[k4].y, raw[k4].z, raw[k4].w};
+          float m = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 x = kv_unpack2<T>(w[k]);
+            m = fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y)));
+          }
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const float own = __shfl_sync(0xffffffffu, m, (lane % kRows) * kLanes);
+          if (lane / kRows == n) top_of = own;
+          if constexpr (kScaled) {
+            const float inv = fp8_pow2(7 - kv_query_exponent(m));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 x = kv_unpack2<T>(w[k]);
+              const __half2 h = __floats2half2_rn(x.x * inv * 128.f, x.y * inv * 128.f);
+              w[k] = as_word(h);
+            }
+          }
+          const uint32_t flip = p.negate ? 0x80008000u : 0u;
+          const uint4 out = make_uint4(__byte_perm(w[0], w[2], 0x5410) ^ flip, __byte_perm(w[0], w[2], 0x7632) ^ flip,
+                                       __byte_perm(w[1], w[3], 0x5410) ^ flip, __byte_perm(w[1], w[3], 0x7632) ^ flip);
+          *reinterpret_cast<uint4*>(smem + t * C::kTileBytes +
+                                    C::place(quarter * 32 + n * kRows + lane / kLanes, part_lane)) = out;
+        }
+      }
+      factor = fp8_is_finite(top_of) || limit <= 0
+                   ? (kScaled ? fp8_pow2(kv_query_exponent(top_of) - 7) * 0.0078125f : 1.f) * p.scale_log2
+                   : fp8_nan();
+      if (factor < 1.2e-38f) factor = 1.2e-38f;  // (-inf times zero would be a NaN)
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    float top = kFloor, l = 0.f;
+    bool ok = t < sp.tiles;
+    for (int j = 0; ok && j < sp.nblocks; ++j) {
+      ok = warp_wait(&s_full[t], static_cast<uint32_t>(j) & 1u, abort_flag, status) &&
+           warp_wait(&meta_full[j % kMeta], static_cast<uint32_t>(j / kMeta) & 1u, abort_flag, status);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t sr[kN];
+#pragma unroll
+      for (int c0 = 0; c0 < kN; c0 += 32) {
+        uint32_t(&chunk)[32] = *reinterpret_cast<uint32_t(*)[32]>(&sr[c0]);
+        tmem_ld32(tmem_s + c0, chunk);
+      }
+      const uint32_t missing = *reinterpret_cast<const uint32_t*>(s_meta + (j % kMeta) * 4);
+      tmem_wait_ld();
+      if constexpr (C::kSeparateP) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t]);
+      }
+      const int j0 = (sp.jb0 + j) * kN;
+      if (j0 + kN > sp.open) {  // hidden keys count nothing
+#pragma unroll
+        for (int c = 0; c < kN; ++c)
+          if (j0 + c >= limit) sr[c] = 0xFF800000u;
+      }
+      if (missing) {  // (rare) nor do those of missing pages
+#pragma unroll
+        for (int c = 0; c < kN; ++c)
+          if (missing >> (8 * (c / 32) + (c / 16) % 2) & 1u) sr[c] = 0xFF800000u;
+      }
+      float m4[4];  // independent chains of 3-input maxima, folded
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m4[k] = fmaxf(__uint_as_float(sr[2 * k]), __uint_as_float(sr[2 * k + 1]));
+#pragma unroll
+      for (int c = 8; c < kN; c += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          m4[k] = max3(m4[k], __uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1]));
+      const float mx = fmaxf(kFloor, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * factor);
+      const bool first = j == 0;
+      const bool grow = first || mx - top > kGrow;
+      const float next = grow ? fmaxf(top, mx) : top;
+      const float half = first ? 0.f : ex2_approx(0.5f * (top - next)), alpha = half * half;
+      if (j > 0) {
+        // the value product of the block before is done: its weights' place is free, O is whole
+        ok = warp_wait(&pv_done[t], static_cast<uint32_t>(j - 1) & 1u, abort_flag, status);
+        if (!ok) break;
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, grow)) {
+          const float scale = grow ? alpha : 1.f;
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            uint32_t r[16];
+            tmem_ld16(tmem_o + c0, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * scale);
+            tmem_st16(tmem_o + c0, r);
+          }
+          tmem_wait_st();
+        }
+      }
+      if (grow) {
+        l = kv_scaled(l, half);
+        top = next;
+      }
+      const float ref = kHeadroom - top;
+      const uint64_t f2 = pack2(factor, factor), shift = pack2(ref, ref);
+      uint64_t sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+#pragma unroll
+      for (int h = 0; h < kN; h += 16) {
+        uint32_t packed[8];
+#pragma unroll
+        for (int c = 0; c < 16; c += 2) {
+          float x0, x1;
+          unpack2(fma2(pack2(__uint_as_float(sr[h + c]), __uint_as_float(sr[h + c + 1])), f2, shift), x0, x1);
+          const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
+          sum2[(c >> 1) & 1] = add2(sum2[(c >> 1) & 1], pack2(e0, e1));
+          packed[c / 2] = as_word(__floats2half2_rn(e0, e1));
+        }
+        tmem_st8(tmem_p + (h >> 1), packed);
+      }
+      float a, b;
+      unpack2(add2(sum2[0], sum2[1]), a, b);
+      l += a + b;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[t]);
+    }
+    if (ok && sp.nblocks > 0)
+      ok = warp_wait(&pv_done[t], static_cast<uint32_t>(sp.nblocks - 1) & 1u, abort_flag, status) &&
+           warp_wait(&v_full[(sp.nblocks - 1) & 1], static_cast<uint32_t>((sp.nblocks - 1) >> 1) & 1u, abort_flag,
+                     status);  // (done as well: orders the reads of s_bad)
+    if (ok) {
+      tc_fence_after();
+      const int split = blockIdx.x % p.splits;
+      const long long part =
+          ((static_cast<long long>(split) * p.c.batch + sp.b) * p.c.kv_heads + sp.head) * p.rows + row;
+      T* dst = static_cast<T*>(p.out) + sp.b * p.out_batch + i * p.out_ld +
+               (static_cast<long long>(sp.head) * p.group + gq) * D;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      // (one range: rows to shared memory, where the queries were, and from there D / 8 lanes a row)
+      constexpr int kSpread = kLanes < 8 ? kLanes - 1 : 7;  // 16-byte pieces of an output row
+      uint8_t* rows = smem + t * C::kTileBytes + quarter * 32 * D * 2;
+      constexpr int kOrder[8] = {0, 2, 4, 6, 1, 3, 5, 7};  // where a channel of eight is
+#pragma unroll 2
+      for (int c0 = 0; c0 < D; c0 += 16) {
+        uint32_t r[16];
+        if (sp.nblocks > 0) {
+          tmem_ld16(tmem_o + c0, r);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) r[c] = 0;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) x[c] = __uint_as_float(r[8 * h + kOrder[c]]);
+          if (p.splits > 1) {
+            if (live) {
+              float4* to = reinterpret_cast<float4*>(p.o_part + part * D + c0 + 8 * h);
+              to[0] = make_float4(x[0], x[1], x[2], x[3]);
+              to[1] = make_float4(x[4], x[5], x[6], x[7]);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[c] *= inv;
+            store8<T>(reinterpret_cast<T*>(rows + lane * D * 2 + ((c0 / 8 + h) ^ (lane & kSpread)) * 16), x);
+          }
+        }
+        __syncwarp();  // the next read of TMEM is the whole warp's
+      }
+      if (p.splits == 1) {
+        __syncwarp();
+#pragma unroll 4
+        for (int n = 0; n < kLanes; ++n) {
+          const int from = n * kRows + lane / kLanes, chunk = lane % kLanes;
+          T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from)) +
+                  8 * chunk;
+          if (sp.row0 + t * kM + quarter * 32 + from >= p.rows) continue;
+          const uint4 v = *reinterpret_cast<const uint4*>(rows + from * D * 2 + (chunk ^ (from & kSpread)) * 16);
+          if (p.out_vec) {
+            *reinterpret_cast<uint4*>(to) = v;
+          } else {
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) to[c] = e[c];
+          }
+        }
+        __syncwarp();
+      }
+      if (p.splits > 1 && live)
+        *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(top, l * fp8_pow2(-kHeadroom));
+      tc_fence_before();
+      if (sp.nblocks > 0 && live && *s_bad != 0) {
+        // Rare: NaN among the values of the blocks that `open` cuts, whose product
+        // left them out.  Looked up again in the cache, token by token, by each row.
+        const int to = min(limit, (sp.jb0 + sp.nblocks) * kN);
+        for (int tok = max(sp.jb0, max(sp.open, 0) / kN) * kN; tok < to; ++tok) {
+          const int id = p.c.table[sp.b * p.c.table_ld + tok / p.c.page];
+          if (id < 0 || id >= p.c.pages) continue;
+          const uint8_t* s = p.c.v_scale +
+                             (static_cast<long long>(id) * p.c.kv_heads + sp.head) * C::kGroups * p.c.page +
+                             tok % p.c.page;
+          for (int c = 0; c < D; ++c) {
+            if (s[(c / kInt4Group) * p.c.page] != kInt4NanScale) continue;
+            if (p.splits > 1) {
+              p.o_part[part * D + c] = fp8_nan();
+            } else {
+              dst[c] = from_f32<T>(fp8_nan());
+            }
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, typename T>
+int launch(cudaStream_t stream, const KvTileParams& p, unsigned int* status) {
+  static unsigned long long configured = 0;
+  int rc = ensure_smem_attribute(reinterpret_cast<const void*>(kv_int4_tiles_kernel<D, T>), Cfg<D>::kSmem, &configured,
+                                 "kv_attention shared memory");
+  if (rc != LDB_OK) return rc;
+  rc = launch_kernel(kv_int4_tiles_kernel<D, T>, dim3(p.row_blocks * p.splits, p.c.kv_heads, p.c.batch), dim3(kThreads),
+                     Cfg<D>::kSmem, stream, "kv_attention tiles launch", p, status);
+  if (rc != LDB_OK || p.splits == 1) return rc;
+  const long long rows = static_cast<long long>(p.c.batch) * p.c.kv_heads * p.rows;
+  return launch_kernel(kv_tiles_merge_kernel<D, T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, stream,
+                       "kv_attention tiles merge launch", p);
+}
+
+template <typename T>
+int launch_dim(cudaStream_t stream, const KvTileParams& p, int head_dim, unsigned int* status) {
+  if (head_dim == 32) return launch<32, T>(stream, p, status);
+  if (head_dim == 64) return launch<64, T>(stream, p, status);
+  return launch<128, T>(stream, p, status);
+}
+
+}  // namespace
+
+size_t kv_int4_tile_workspace(int batch, int kv_heads, long long rows, int head_dim, long long capacity) {
+  const long long splits = kv_tile_splits(batch, kv_heads, rows, head_dim, capacity);
+  return splits <= 1 ? 0 : static_cast<size_t>(splits) * batch * kv_heads * rows * (head_dim + 2) * sizeof(float);
+}
+
+int kv_int4_attention_tiles(cudaStream_t stream, KvTileParams p, int head_dim, int dtype, float scale, void* workspace,
+                            unsigned int* status) {
+  p.row_blocks = (p.rows + 2 * kM - 1) / (2 * kM);
+  p.splits = kv_tile_splits(p.c.batch, p.c.kv_heads, p.rows, head_dim, static_cast<long long>(p.c.width) * p.c.page);
+  p.negate = scale < 0.f;
+  p.scale_log2 = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
+  p.o_part = static_cast<float*>(workspace);
+  p.ml_part = p.o_part + static_cast<size_t>(p.splits) * p.c.batch * p.c.kv_heads * p.rows * head_dim;
+  if (static_cast<long long>(p.row_blocks) * p.splits > 0x7FFFFFFFll || p.c.kv_heads > 65535 || p.c.batch > 65535)
+    return fail(LDB_ERR_SHAPE, "kv_attention: %d row blocks, %d heads, %d items", p.row_blocks, p.c.kv_heads,
+                p.c.batch);
+  return dtype == LDB_F16 ? launch_dim<__half>(stream, p, head_dim, status)
+                          : launch_dim<__nv_bfloat16>(stream, p, head_dim, status);
+}
+
+}  // namespace ldb
