@@ -26,6 +26,7 @@ struct AttnParams {
   int tile_rows, row_tiles;
   int causal, q_vec, out_vec;
   float scale_log2;
+  int negate;      // the 4-bit kernel: scale_log2 is a magnitude, the queries are turned
   int warps;       // of the grid
   float* o_part;   // [warp][2][tile rows][D]
   float* ml_part;  // [warp][2][tile rows][2]

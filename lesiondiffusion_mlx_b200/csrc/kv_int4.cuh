@@ -87,13 +87,20 @@ __device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cas
 __device__ __forceinline__ uint32_t scale_pair(uint32_t word, uint32_t sel) { return __byte_perm(word, 0, sel) >> 1; }
 __device__ __forceinline__ uint32_t scale_selector(int lower, int upper) { return 0x0404u | lower << 4 | upper << 12; }
 
+// (a & mask) | bits in one instruction (as plain C, with two constants, it became two).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(bits));
+  return d;
+}
+
 // The four pairs of codes (n, n + 4) of a word's two halves as values: (64 + code) s - 72 s.
 __device__ __forceinline__ void unpack4(uint32_t w, __half2 s, __half2 minus72s, uint32_t (&v)[4]) {
   constexpr uint32_t kMask = 0x00F000F0u, k64 = 0x54005400u;
-  v[0] = ((w << 4) & kMask) | k64;
-  v[1] = (w & kMask) | k64;
-  v[2] = ((w >> 4) & kMask) | k64;
-  v[3] = ((w >> 8) & kMask) | k64;
+  v[0] = and_or(w << 4, kMask, k64);
+  v[1] = and_or(w, kMask, k64);
+  v[2] = and_or(w >> 4, kMask, k64);
+  v[3] = and_or(w >> 8, kMask, k64);
 #pragma unroll
   for (int n = 0; n < 4; ++n) v[n] = as_word(__hfma2(as_half2(v[n]), s, minus72s));
 }

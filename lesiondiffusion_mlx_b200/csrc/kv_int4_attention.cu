@@ -13,7 +13,7 @@
 // M and lost below 2^-40 of it; their sum is FP32.
 //
 // Bound: HBM, (D / 2 + D / 16) 2 bytes a token and key/value head, read once for
-// a group's heads.  The tiles of 64 tokens of all items and heads form one line that the
+// a group's heads.  The tiles of 32 tokens of all items and heads form one line that the
 // warps share out equally (kv_attention_ranges.cuh); a warp copies the next
 // tiles into its own ring (cp.async) while it works on one.
 
@@ -28,11 +28,24 @@
 namespace ldb {
 namespace {
 
-constexpr int kTile = 64;      // tokens per tile
+constexpr int kTile = 32;      // tokens per tile
+constexpr int kKeys = kTile / 8;      // q k products of a tile: eight keys each
+constexpr int kLaneTokens = kTile / 4;
+constexpr int kChunks = kTile / 16;   // of 16 tokens, each of one page
 constexpr int kGroupRows = 8;  // query rows of one value product
 // Positions on the line that the start of a pair counts for.
-constexpr int kStart = 2;
-constexpr int kScaleRow = kTile + 16;  // bytes of a group's scales of a tile (padded: other banks for the next group)
+constexpr int kStart = 3;
+
+// An 8 x 8 matrix of 16-bit values, a pair of a row's neighbours per lane, transposed.
+__device__ __forceinline__ uint32_t transposed8(uint32_t w) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(w));
+  return d;
+}
+
+// As many CTAs as the registers of G groups of eight query rows allow: a warp by itself
+// issues an instruction every third cycle or so.
+constexpr int ctas_of(int head_dim, int groups) { return groups == 1 ? 4 : (head_dim == 128 ? 2 : 3); }
 
 // G groups of eight query rows per row tile.
 template <int D, int G>
@@ -41,93 +54,96 @@ struct Cfg {
   static constexpr int kTokenBytes = D / 2;
   static constexpr int kGroups = D / kInt4Group;
   static constexpr int kCodeBytes = kTile * kTokenBytes;
-  static constexpr int kScaleBytes = kGroups * kScaleRow;
+  static constexpr int kScaleBytes = kGroups * kTile;
   static constexpr int kOffScale = 2 * kCodeBytes;  // in a slot: codes of K and V, then scales of K and V
   static constexpr int kSlotBytes = 2 * (kCodeBytes + kScaleBytes);
-  static constexpr int kSlots = D == 128 ? 3 : (D == 64 ? 4 : 8);
-  static constexpr int kCtasPerSm = D == 128 ? 2 : 3;
+  static constexpr int kSlots = D == 128 ? 3 : (D == 64 ? 6 : 8);
+  static constexpr int kCtasPerSm = ctas_of(D, G);
   static constexpr int kOffBase = kWarps * kSlots * kSlotBytes;  // [batch + 1] int
 };
-int ctas_per_sm(int head_dim) { return head_dim == 128 ? Cfg<128, 1>::kCtasPerSm : Cfg<64, 1>::kCtasPerSm; }
-
 // A run of tiles of one (item, head, row tile) pair, and the copies of its tiles into the warp's ring.
 template <int D>
 struct Fetch {
   using C = Cfg<D, 1>;
+  static constexpr int kUnits = C::kTokenBytes;  // 16-byte units of 16 tokens' codes
   const KvView& c;
-  int b, head, used;  // pages that hold the item's tokens
+  const int* pages;   // of the item
+  int head, used;     // pages that hold the item's tokens
   int batch0;         // first of the 32 pages whose numbers the lanes hold
-  int id;
-  uint32_t holes;     // four bits a slot: 16 tokens of a page that the table names wrongly
+  int id, shift;
+  uint32_t holes;     // two bits a slot: 16 tokens of a page that the table names wrongly
+  // The lane's: 16 bytes of codes in a run of 512, and its 16 tokens of a group's scales (of keys, then of values).
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* scale;
+  int scale_to, group;  // (negative: none)
   unsigned int* status;
 
-  __device__ __forceinline__ Fetch(const KvView& view, unsigned int* st) : c(view), holes(0), status(st) {}
+  __device__ __forceinline__ Fetch(const KvView& view, unsigned int* st) : c(view), holes(0), status(st) {
+    const int lane = lane_id();
+    const int which = lane / (kChunks * C::kGroups);
+    shift = 31 - __clz(view.page);
+    group = (lane / kChunks) % C::kGroups;
+    k = view.k + (lane % kUnits) * 16;
+    v = view.v + (lane % kUnits) * 16;
+    scale = which ? view.v_scale : view.k_scale;
+    scale_to = which < 2 ? C::kOffScale + (which * C::kGroups + group) * kTile + lane % kChunks * 16 : -1;
+  }
 
   __device__ __forceinline__ void start(int item, int h, int len) {
-    b = item;
+    pages = c.table + item * c.table_ld;
     head = h;
-    used = (len + c.page - 1) / c.page;
-    batch0 = -64;
+    used = (len + c.page - 1) >> shift;
+    batch0 = -32;
   }
 
   // Copy tile j into slot `slot` of the ring at `ring` (shared address).
   __device__ __forceinline__ void tile(int j, uint32_t ring, int slot) {
     const uint32_t dst = ring + slot * C::kSlotBytes;
     const int lane = lane_id();
-    const int shift = 31 - __clz(c.page);
     const int first = (j * kTile) >> shift;
-    if (first - batch0 > 28) {  // (a tile has up to four pages)
+    if (first - batch0 > 32 - kChunks) {  // (a tile has up to kChunks pages)
       batch0 = first;
       const int at = batch0 + lane;
-      id = at < used ? c.table[b * c.table_ld + at] : -1;
+      id = at < used ? pages[at] : -1;
       if (at < used && (id < 0 || id >= c.pages)) {
         set_bad_shape(status);
         id = -1;
       }
     }
-    // the page of each 16 tokens, and where in it they start
-    int ids[4];
+    // the page of each 16 tokens, and the first of their rows (the cache has fewer than 2^31)
+    int unit[kChunks], in[kChunks];
+    uint32_t bytes[kChunks];
+    holes &= ~(3u << (2 * slot));
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
-      ids[n] = __shfl_sync(0xffffffffu, id, (((j * kTile) + 16 * n) >> shift) - batch0);
-    holes &= ~(15u << (4 * slot));
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-      if (ids[n] < 0) holes |= 1u << (4 * slot + n);
-    const int inside = (j * kTile) & (c.page - 1);
-    auto chunk_row = [&](int n) { return (inside + 16 * n) & (c.page - 1); };
-    constexpr int kUnits = 16 * C::kTokenBytes / 16;  // 16-byte units of 16 tokens' codes: D / 2
-#pragma unroll
-    for (int i = 0; i < 4 * kUnits / 32; ++i) {
-      const int u = i * 32 + lane;
-      const int n = kUnits >= 32 ? i * 32 / kUnits : u / kUnits;
-      const int page_id = kUnits >= 32 ? ids[n & 3] : ((n & 1) ? ids[(2 * i + 1) & 3] : ids[(2 * i) & 3]);
-      const long long off =
-          ((static_cast<long long>(max(page_id, 0)) * c.kv_heads + head) * c.page + chunk_row(n)) * C::kTokenBytes +
-          (u % kUnits) * 16;
-      const uint32_t bytes = page_id < 0 ? 0u : 16u;  // zeros for what has no page
-      cp_async16(dst + u * 16, c.k + off, bytes);
-      cp_async16(dst + C::kCodeBytes + u * 16, c.v + off, bytes);
+    for (int n = 0; n < kChunks; ++n) {
+      const int page_id = __shfl_sync(0xffffffffu, id, (((j * kTile) + 16 * n) >> shift) - batch0);
+      if (page_id < 0) holes |= 1u << (2 * slot + n);
+      bytes[n] = page_id < 0 ? 0u : 16u;  // zeros for what has no page
+      unit[n] = max(page_id, 0) * c.kv_heads + head;
+      in[n] = (j * kTile + 16 * n) & (c.page - 1);
     }
-    // Scales: 16 tokens of one group a unit; K's and V's side by side over the lanes where they fit.
-    {
-      const int n = lane & 3;
-      const int page_id = (n & 2) ? ((n & 1) ? ids[3] : ids[2]) : ((n & 1) ? ids[1] : ids[0]);
-      const uint32_t bytes = page_id < 0 ? 0u : 16u;
-      const long long unit = static_cast<long long>(max(page_id, 0)) * c.kv_heads + head;
-      const uint32_t to = dst + C::kOffScale;
-      if constexpr (D == 128) {
-        const int group = lane >> 2;
-        const long long off = (unit * C::kGroups + group) * c.page + chunk_row(n);
-        cp_async16(to + group * kScaleRow + n * 16, c.k_scale + off, bytes);
-        cp_async16(to + C::kScaleBytes + group * kScaleRow + n * 16, c.v_scale + off, bytes);
-      } else {
-        const int which = lane / (4 * C::kGroups), group = (lane >> 2) % C::kGroups;
-        const long long off = (unit * C::kGroups + group) * c.page + chunk_row(n);
-        if (which < 2)
-          cp_async16(to + which * C::kScaleBytes + group * kScaleRow + n * 16, (which ? c.v_scale : c.k_scale) + off,
-                     bytes);
+    const uint32_t to = dst + lane * 16;
+    if constexpr (kUnits >= 32) {
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) {
+        const long long off = static_cast<long long>(unit[n] * c.page + in[n]) * C::kTokenBytes;
+#pragma unroll
+        for (int i = 0; i < kUnits / 32; ++i) {
+          cp_async16(to + (n * kUnits + i * 32) * 16, k + off + i * 512, bytes[n]);
+          cp_async16(to + C::kCodeBytes + (n * kUnits + i * 32) * 16, v + off + i * 512, bytes[n]);
+        }
       }
+    } else {  // a chunk per half warp
+      const bool n = lane >= 16;
+      const long long off = static_cast<long long>((n ? unit[1] : unit[0]) * c.page + (n ? in[1] : in[0])) * C::kTokenBytes;
+      cp_async16(to, k + off, n ? bytes[1] : bytes[0]);
+      cp_async16(to + C::kCodeBytes, v + off, n ? bytes[1] : bytes[0]);
+    }
+    if (scale_to >= 0) {
+      const bool n = lane & 1;
+      const long long off = static_cast<long long>((n ? unit[1] : unit[0]) * C::kGroups + group) * c.page + (n ? in[1] : in[0]);
+      cp_async16(dst + scale_to, scale + off, n ? bytes[1] : bytes[0]);
     }
   }
 };
@@ -153,23 +169,23 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
   const uint32_t ring = smem_u32(smem + warp * C::kSlots * C::kSlotBytes);
   const uint8_t* ring_ptr = smem + warp * C::kSlots * C::kSlotBytes;
 
-  // Lane (g, c) holds, in q k, query row g of each group, channels [c D/4, (c + 1) D/4)
-  // of the key in column g of each of eight products, and the scores of the keys
-  // in columns 2c and 2c + 1; in p v, the tokens of those scores, the channels
-  // [g D/8, (g + 1) D/8), and their outputs for rows 2c and 2c + 1.  Column j of
-  // product n is token 16 (j / 2) + 2n + (j % 2, the other way round for odd j / 2): so a
-  // lane's tokens in p v are 16 neighbours, whose scales are one 16-byte read, and no
-  // eight (four) lanes that read at a time meet in a bank more than once (twice).
+  // Lane (g, c) holds, in q k, channels [c D/4, (c + 1) D/4) of query row g of each group and of key
+  // g of each of kKeys blocks of eight (two blocks a product), and key g's scores for
+  // rows 2c and 2c + 1; in p v, the weights of row g for keys 2c and 2c + 1 of each block (the scores
+  // transposed), those tokens' channels [g D/8, (g + 1) D/8), and their outputs for rows 2c and 2c + 1.  Key j of
+  // block n is token 8 (j / 2) + 2n + (j % 2, the other way round for odd j / 2): so a
+  // lane's tokens in p v are eight neighbours, whose scales are one 8-byte read, and
+  // lanes that read codes at a time meet in a bank at most twice.
   const int g = lane >> 2, c = lane & 3;
   constexpr int kSteps = D / 16;            // q k products over the channels
   constexpr int kMTiles = D / 16;           // p v products over the channels
   constexpr int kWk = D / 8;                // bytes of a key's channels: 16, 8 or 4
   constexpr int kWv = D / 16;               // bytes of a value's: 8, 4 or 2
   const int odd_k = (g & 1) ^ ((g >> 1) & 1), odd_v = c & 1;
-  const int at_k = (16 * (g >> 1) + odd_k) * C::kTokenBytes + c * kWk;
-  const int at_v = C::kCodeBytes + 16 * c * C::kTokenBytes + g * kWv;
-  const int at_ks = C::kOffScale + (c * (D / 4) / kInt4Group) * kScaleRow + 16 * (g >> 1);
-  const int at_vs = C::kOffScale + C::kScaleBytes + (g * (D / 8) / kInt4Group) * kScaleRow + 16 * c;
+  const int at_k = (kLaneTokens * (g >> 1) + odd_k) * C::kTokenBytes + c * kWk;
+  const int at_v = C::kCodeBytes + kLaneTokens * c * C::kTokenBytes + g * kWv;
+  const int at_ks = C::kOffScale + (c * (D / 4) / kInt4Group) * kTile + kLaneTokens * (g >> 1);
+  const int at_vs = C::kOffScale + C::kScaleBytes + (g * (D / 8) / kInt4Group) * kTile + kLaneTokens * c;
   const uint32_t sel_k[2] = {scale_selector(odd_k, odd_k), scale_selector(odd_k + 2, odd_k + 2)};
   const uint32_t sel_v[2] = {scale_selector(odd_v, 1 - odd_v), scale_selector(2 + odd_v, 3 - odd_v)};
 
@@ -203,13 +219,18 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
     const int len = kv_length(p.c, b, status);
     // Queries as they are, on their way while the page numbers arrive.
     uint32_t raw[G][D / 8];
-    int limit[G];  // the keys a row sees
+    int limit[G][2];  // the keys that rows 2c and 2c + 1 see
+    float factor[G][2];
 #pragma unroll
     for (int r = 0; r < G; ++r) {
       const int row = row0 + 8 * r + g;
       const bool live = row < p.rows;
       const int i = live ? row / p.group : 0;
-      limit[r] = !live ? len : (p.causal ? min(len, len - p.queries + i + 1) : len);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int of = row0 + 8 * r + 2 * c + e;
+        limit[r][e] = of < p.rows && p.causal ? min(len, len - p.queries + of / p.group + 1) : len;
+      }
       const T* src = static_cast<const T*>(p.q) + b * p.q_batch + i * p.q_ld +
                      (static_cast<long long>(head) * p.group + (live ? row % p.group : 0)) * D + c * (D / 4);
 #pragma unroll
@@ -235,10 +256,9 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
 
     // Queries in the channel order of the unpacked keys, and their rows' factors.
     uint32_t qa[G][kSteps][2];
-    float factor[G];
 #pragma unroll
     for (int r = 0; r < G; ++r) {
-      // a NaN stays one, an infinity makes the row's factor one
+      // a NaN stays one, an infinity makes the row's factor one (of a row that sees any key)
       float m = 0.f;
 #pragma unroll
       for (int k = 0; k < D / 8; ++k) {
@@ -248,7 +268,14 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
       const int e = kv_query_exponent(m);
-      factor[r] = (fp8_is_finite(m) ? (kScaled ? fp8_pow2(e - 7) * 0.0078125f : 1.f) : fp8_nan()) * p.scale_log2;
+      const float own = (kScaled ? fp8_pow2(e - 7) * 0.0078125f : 1.f) * p.scale_log2;
+      const float size = fmaxf(own, 1.2e-38f);  // (-inf times zero would be a NaN)
+      const bool finite = fp8_is_finite(m);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float f = __shfl_sync(0xffffffffu, finite ? size : -size, 8 * c + 4 * x);
+        factor[r][x] = f > 0.f ? f : (limit[r][x] <= 0 ? -f : fp8_nan());
+      }
       if constexpr (kScaled) {
         const float inv = fp8_pow2(7 - e);  // largest magnitude to [2^7, 2^8), and then to [2^14, 2^15)
 #pragma unroll
@@ -257,6 +284,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
           raw[r][k] = pack_half2(x.x * inv * 128.f, x.y * inv * 128.f);
         }
       }
+#pragma unroll
+      for (int w = 0; w < D / 8; ++w) raw[r][w] ^= p.negate ? 0x80008000u : 0u;
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {  // channels 8 w .. 8 w + 7 of the lane's: pairs (n, n + 4)
         qa[r][2 * w][0] = __byte_perm(raw[r][4 * w], raw[r][4 * w + 2], 0x5410);
@@ -274,9 +303,11 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
       for (int j = 0; j < kMTiles; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[r][j][e] = 0.f;
-    float top[G], sum[G];
+    float top[G][2], sum[G][2];
 #pragma unroll
-    for (int r = 0; r < G; ++r) top[r] = kFloor, sum[r] = 0.f;
+    for (int r = 0; r < G; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) top[r][e] = kFloor, sum[r][e] = 0.f;
 
     int slot = 0;
 #pragma unroll 1
@@ -291,55 +322,65 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
       __syncwarp();
       const uint8_t* sk = ring_ptr + slot * C::kSlotBytes;
       const int j0 = (tile0 + t) * kTile;
-      const uint32_t holes = fetch.holes >> (4 * slot) & 15u;
+      const uint32_t holes = fetch.holes >> (2 * slot) & 3u;
       const bool masked = j0 + kTile > open || holes;
 
       // Scores, eight keys at a time.
-      float s[G][8][2];
+      float s[G][kKeys][2];
       {
         constexpr int kKeyGroups = D == 128 ? 2 : 1;  // of the lane's channels
-        uint32_t scales[kKeyGroups][4];
+        uint32_t scales[kKeyGroups][2];
 #pragma unroll
-        for (int h = 0; h < kKeyGroups; ++h) lds_words<16>(sk + at_ks + h * kScaleRow, scales[h]);
+        for (int h = 0; h < kKeyGroups; ++h) lds_words<8>(sk + at_ks + h * kTile, scales[h]);
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          uint32_t w[kWk / 4];
-          lds_words<kWk>(sk + at_k + 2 * n * C::kTokenBytes, w);
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < kKeys; n += 2) {
+          uint32_t w[2][kWk / 4];
+          lds_words<kWk>(sk + at_k + 2 * n * C::kTokenBytes, w[0]);
+          lds_words<kWk>(sk + at_k + 2 * (n + 1) * C::kTokenBytes, w[1]);
+          float d[G][4];
+#pragma unroll
+          for (int r = 0; r < G; ++r) d[r][0] = d[r][1] = d[r][2] = d[r][3] = 0.f;
 #pragma unroll
           for (int i = 0; i < kWk / 4; ++i) {
-            const uint32_t sc = scale_pair(scales[kKeyGroups == 2 ? i >> 1 : 0][n >> 1], sel_k[n & 1]);
-            uint32_t v[4];
-            unpack4(w[i], as_half2(sc), minus72(sc), v);
+            uint32_t v[2][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              mma_f16(d, qa[0][2 * i + h][0], G > 1 ? qa[G - 1][2 * i + h][0] : 0u, qa[0][2 * i + h][1],
-                      G > 1 ? qa[G - 1][2 * i + h][1] : 0u, v[2 * h], v[2 * h + 1]);
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t sc = scale_pair(scales[kKeyGroups == 2 ? i >> 1 : 0][n >> 1], sel_k[h]);
+              unpack4(w[h][i], as_half2(sc), minus72(sc), v[h]);
+            }
+#pragma unroll
+            for (int r = 0; r < G; ++r) {
+              mma_f16(d[r], v[0][0], v[1][0], v[0][1], v[1][1], qa[r][2 * i][0], qa[r][2 * i][1]);
+              mma_f16(d[r], v[0][2], v[1][2], v[0][3], v[1][3], qa[r][2 * i + 1][0], qa[r][2 * i + 1][1]);
+            }
           }
 #pragma unroll
-          for (int r = 0; r < G; ++r) {
-            s[r][n][0] = d[2 * r] * factor[r];
-            s[r][n][1] = d[2 * r + 1] * factor[r];
-          }
+          for (int r = 0; r < G; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s[r][n + h][0] = d[r][2 * h];
+              s[r][n + h][1] = d[r][2 * h + 1];
+            }
         }
       }
-      uint32_t vs[4];  // scales of the values of the lane's 16 tokens
-      lds_words<16>(sk + at_vs, vs);
-      uint64_t bad = 0;  // tokens whose values are NaN in the lane's group, where some rows may not see them
+      uint32_t vs[2];  // scales of the values of the lane's tokens
+      lds_words<8>(sk + at_vs, vs);
+      uint32_t bad = 0;  // tokens whose values are NaN in the lane's group, where some rows may not see them
       if (masked) {
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
+        for (int n = 0; n < kKeys; ++n) {
+          const int tok = kLaneTokens * (g >> 1) + 2 * n + odd_k;
+          const bool gone = holes >> (tok >> 4) & 1u;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int tok = 16 * c + 2 * n + (e ^ odd_v);
+          for (int r = 0; r < G; ++r)
 #pragma unroll
-            for (int r = 0; r < G; ++r)
-              if (j0 + tok >= limit[r] || (holes >> c & 1u)) s[r][n][e] = -INFINITY;
-          }
-        const int left = len - j0 - 16 * c;  // of the lane's tokens, those that exist
+            for (int e = 0; e < 2; ++e)
+              if (j0 + tok >= limit[r][e] || gone) s[r][n][e] = -INFINITY;
+        }
+        const int left = len - j0 - kLaneTokens * c;  // of the lane's tokens, those that exist
         uint32_t mine = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kLaneTokens / 4; ++k) {
           const int n = min(max(left - 4 * k, 0), 4);
           vs[k] = n == 4 ? vs[k] : vs[k] & ((1u << (8 * n)) - 1u);
           if (p.causal && p.queries > 1) {
@@ -352,52 +393,54 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
             }
           }
         }
-        bad = static_cast<uint64_t>(mine) << (16 * c);
+        bad = mine << (kLaneTokens * c);
         bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
         bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
       }
-      float mx[G];
+      float mx[G][2];
       bool grew = false;
 #pragma unroll
-      for (int r = 0; r < G; ++r) {
-        mx[r] = kFloor;
+      for (int r = 0; r < G; ++r)
 #pragma unroll
-        for (int n = 0; n < 8; ++n) mx[r] = fmaxf(mx[r], fmaxf(s[r][n][0], s[r][n][1]));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-        grew |= mx[r] > top[r];
-      }
+        for (int e = 0; e < 2; ++e) {
+          float m = fmaxf(fmaxf(s[r][0][e], s[r][1][e]), fmaxf(s[r][2][e], s[r][3][e]));
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          mx[r][e] = fmaxf(kFloor, m * factor[r][e]);
+          grew |= mx[r][e] > top[r][e];
+        }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-        for (int r = 0; r < G; ++r) {
-          const float m = fmaxf(top[r], mx[r]);
-          const float half = ex2_approx(0.5f * (top[r] - m)), f = half * half;
-          top[r] = m;
-          sum[r] = kv_scaled(sum[r], half);
-          const float f0 = __shfl_sync(0xffffffffu, f, 8 * c), f1 = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+        for (int r = 0; r < G; ++r)
 #pragma unroll
-          for (int j = 0; j < kMTiles; ++j) {
-            o[r][j][0] *= f0;
-            o[r][j][1] *= f1;
-            o[r][j][2] *= f0;
-            o[r][j][3] *= f1;
+          for (int e = 0; e < 2; ++e) {
+            const float m = fmaxf(top[r][e], mx[r][e]);
+            const float half = ex2_approx(0.5f * (top[r][e] - m)), f = half * half;
+            top[r][e] = m;
+            sum[r][e] = kv_scaled(sum[r][e], half);
+#pragma unroll
+            for (int j = 0; j < kMTiles; ++j) {
+              o[r][j][e] *= f;
+              o[r][j][2 + e] *= f;
+            }
           }
-        }
       }
-      // Weights 2^(s - M + kHeadroom): the fragments of p v as they are.
-      uint32_t pf[G][8];
+      // Weights 2^(s - M + kHeadroom), transposed: the fragments of p v.
+      uint32_t pf[G][kKeys];
 #pragma unroll
       for (int r = 0; r < G; ++r) {
-        const float ref = top[r] - kHeadroom;
+        const float ref0 = kHeadroom - top[r][0], ref1 = kHeadroom - top[r][1];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float a = ex2_approx(s[r][n][0] - ref), bb = ex2_approx(s[r][n][1] - ref);
-          sum[r] += a + bb;
-          pf[r][n] = pack_half2(a, bb);
+        for (int n = 0; n < kKeys; ++n) {
+          const float a = ex2_approx(fmaf(s[r][n][0], factor[r][0], ref0));
+          const float bb = ex2_approx(fmaf(s[r][n][1], factor[r][1], ref1));
+          sum[r][0] += a;
+          sum[r][1] += bb;
+          pf[r][n] = transposed8(pack_half2(a, bb));
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kLaneTokens / 4; ++k) {
         // tokens (columns 2c, 2c + 1) of products 2k and 2k + 1, their channels paired by token
         constexpr int kWords = (kWv + 3) / 4;
         uint32_t w[4][kWords];
@@ -431,8 +474,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
         for (int r = 0; r < G; ++r)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int seen = __shfl_sync(0xffffffffu, limit[r], 8 * c + 4 * e) - j0;  // of the tile's tokens
-            const uint64_t in = seen <= 0 ? 0 : (seen >= 64 ? ~0ull : (1ull << seen) - 1);
+            const int seen = limit[r][e] - j0;  // of the tile's tokens
+            const uint32_t in = seen <= 0 ? 0 : (seen >= kTile ? ~0u : (1u << seen) - 1);
             if (bad & in) {
 #pragma unroll
               for (int j = 0; j < kMTiles; ++j) o[r][j][e] = o[r][j][2 + e] = fp8_nan();
@@ -448,21 +491,23 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
     const int part = me * 2 + (tile0 == 0 ? 1 : 0);
 #pragma unroll
     for (int r = 0; r < G; ++r) {
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-      if (!whole && c == 0) {
-        float* ml = p.ml_part + (static_cast<long long>(part) * C::kRows + 8 * r + g) * 2;
-        ml[0] = top[r];
-        ml[1] = sum[r] * fp8_pow2(-kHeadroom);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) sum[r][e] += __shfl_xor_sync(0xffffffffu, sum[r][e], o);
+        if (!whole && g == 0) {
+          float* ml = p.ml_part + (static_cast<long long>(part) * C::kRows + 8 * r + 2 * c + e) * 2;
+          ml[0] = top[r][e];
+          ml[1] = sum[r][e] * fp8_pow2(-kHeadroom);
+        }
       }
-      const float l[2] = {__shfl_sync(0xffffffffu, sum[r], 8 * c), __shfl_sync(0xffffffffu, sum[r], 8 * c + 4)};
       // products j: rows g and g + 8 are channels g D/8 + 2j and + 1
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = row0 + 8 * r + 2 * c + e;
         if (row >= p.rows) continue;
         if (whole) {
-          const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];
+          const float inv = sum[r][e] == 0.f ? 0.f : 1.f / sum[r][e];
           T* dst = static_cast<T*>(p.out) + b * p.out_batch + (row / p.group) * p.out_ld +
                    (static_cast<long long>(head) * p.group + row % p.group) * D + g * (D / 8);
           if (D >= 64 && p.out_vec) {
@@ -538,9 +583,10 @@ int ldb_kv_attention_int4_workspace_size(int batch, int queries, int heads, int 
       (head_dim != 32 && head_dim != 64 && head_dim != 128))
     return fail(LDB_ERR_SHAPE, "kv_attention: %d heads over %d of width %d (32, 64 or 128)", heads, kv_heads, head_dim);
   const long long rows = static_cast<long long>(queries) * (heads / kv_heads);
-  *bytes = rows >= kTileRows ? kv_int4_tile_workspace(batch, kv_heads, rows, head_dim, capacity)
-                             : workspace_bytes_of(ctas_per_sm(head_dim) * sm_count() * kWarps,
-                                                  kGroupRows * row_groups(rows), head_dim);
+  const int groups = row_groups(rows);
+  *bytes = rows >= kTileRows
+               ? kv_int4_tile_workspace(batch, kv_heads, rows, head_dim, capacity)
+               : workspace_bytes_of(ctas_of(head_dim, groups) * sm_count() * kWarps, kGroupRows * groups, head_dim);
   return LDB_OK;
 }
 
@@ -604,8 +650,9 @@ int ldb_kv_attention_int4(cudaStream_t stream, const void* q, long long q_ld, lo
     return fail(LDB_ERR_SHAPE, "kv_attention: too many heads over too long a table");
   p.rows = static_cast<int>(group_rows), p.row_tiles = static_cast<int>(row_tiles);
   p.causal = causal != 0;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.warps = ctas_per_sm(head_dim) * sm_count() * kWarps;
+  p.negate = scale < 0.f;
+  p.scale_log2 = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
+  p.warps = ctas_of(head_dim, row_groups(group_rows)) * sm_count() * kWarps;
   p.o_part = static_cast<float*>(workspace);
   p.ml_part = p.o_part + static_cast<size_t>(p.warps) * 2 * p.tile_rows * head_dim;
   p.open_by_pair = row_tiles * kv_heads * batch <= p.warps;
