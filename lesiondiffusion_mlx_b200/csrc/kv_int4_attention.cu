@@ -32,6 +32,8 @@ constexpr int kTile = 32;      // tokens per tile
 constexpr int kKeys = kTile / 8;      // q k products of a tile: eight keys each
 constexpr int kLaneTokens = kTile / 4;
 constexpr int kChunks = kTile / 16;   // of 16 tokens, each of one page
+constexpr float kLag = 4.f;           // a reference follows its row's maximum once that is 2^4 above
+constexpr int kHeadroomLag = kHeadroom - 4;
 constexpr int kGroupRows = 8;  // query rows of one value product
 // Positions on the line that the start of a pair counts for.
 constexpr int kStart = 3;
@@ -65,13 +67,12 @@ struct Cfg {
 template <int D>
 struct Fetch {
   using C = Cfg<D, 1>;
-  static constexpr int kUnits = C::kTokenBytes;  // 16-byte units of 16 tokens' codes
   const KvView& c;
   const int* pages;   // of the item
   int head, used;     // pages that hold the item's tokens
   int batch0;         // first of the 32 pages whose numbers the lanes hold
   int id, shift;
-  uint32_t holes;     // two bits a slot: 16 tokens of a page that the table names wrongly
+  bool lost;          // the table has named a page wrongly
   // The lane's: 16 bytes of codes in a run of 512, and its 16 tokens of a group's scales (of keys, then of values).
   const uint8_t* k;
   const uint8_t* v;
@@ -79,13 +80,13 @@ struct Fetch {
   int scale_to, group;  // (negative: none)
   unsigned int* status;
 
-  __device__ __forceinline__ Fetch(const KvView& view, unsigned int* st) : c(view), holes(0), status(st) {
+  __device__ __forceinline__ Fetch(const KvView& view, unsigned int* st) : c(view), status(st) {
     const int lane = lane_id();
     const int which = lane / (kChunks * C::kGroups);
     shift = 31 - __clz(view.page);
     group = (lane / kChunks) % C::kGroups;
-    k = view.k + (lane % kUnits) * 16;
-    v = view.v + (lane % kUnits) * 16;
+    k = view.k + lane * 16;
+    v = view.v + lane * 16;
     scale = which ? view.v_scale : view.k_scale;
     scale_to = which < 2 ? C::kOffScale + (which * C::kGroups + group) * kTile + lane % kChunks * 16 : -1;
   }
@@ -95,6 +96,7 @@ struct Fetch {
     head = h;
     used = (len + c.page - 1) >> shift;
     batch0 = -32;
+    lost = false;
   }
 
   // Copy tile j into slot `slot` of the ring at `ring` (shared address).
@@ -111,40 +113,49 @@ struct Fetch {
         id = -1;
       }
     }
-    // the page of each 16 tokens, and the first of their rows (the cache has fewer than 2^31)
-    int unit[kChunks], in[kChunks];
-    uint32_t bytes[kChunks];
-    holes &= ~(3u << (2 * slot));
-#pragma unroll
-    for (int n = 0; n < kChunks; ++n) {
-      const int page_id = __shfl_sync(0xffffffffu, id, (((j * kTile) + 16 * n) >> shift) - batch0);
-      if (page_id < 0) holes |= 1u << (2 * slot + n);
-      bytes[n] = page_id < 0 ? 0u : 16u;  // zeros for what has no page
-      unit[n] = max(page_id, 0) * c.kv_heads + head;
-      in[n] = (j * kTile + 16 * n) & (c.page - 1);
-    }
+    const int at = first - batch0;
     const uint32_t to = dst + lane * 16;
-    if constexpr (kUnits >= 32) {
+    const int page0 = __shfl_sync(0xffffffffu, id, at);
+    lost |= page0 < 0;
+    const uint32_t bytes0 = page0 < 0 ? 0u : 16u;  // zeros for what has no page
+    const int unit0 = max(page0, 0) * c.kv_heads + head;  // (the cache has fewer than 2^31 rows)
+    if (c.page >= kTile) {  // one run of tokens
+      const int in = (j * kTile) & (c.page - 1);
+      const long long off = static_cast<long long>(unit0 * c.page + in) * C::kTokenBytes;
 #pragma unroll
-      for (int n = 0; n < kChunks; ++n) {
-        const long long off = static_cast<long long>(unit[n] * c.page + in[n]) * C::kTokenBytes;
-#pragma unroll
-        for (int i = 0; i < kUnits / 32; ++i) {
-          cp_async16(to + (n * kUnits + i * 32) * 16, k + off + i * 512, bytes[n]);
-          cp_async16(to + C::kCodeBytes + (n * kUnits + i * 32) * 16, v + off + i * 512, bytes[n]);
-        }
+      for (int i = 0; i < kTile * C::kTokenBytes / 512; ++i) {
+        cp_async16(to + i * 512, k + off + i * 512, bytes0);
+        cp_async16(to + C::kCodeBytes + i * 512, v + off + i * 512, bytes0);
       }
-    } else {  // a chunk per half warp
-      const bool n = lane >= 16;
-      const long long off = static_cast<long long>((n ? unit[1] : unit[0]) * c.page + (n ? in[1] : in[0])) * C::kTokenBytes;
-      cp_async16(to, k + off, n ? bytes[1] : bytes[0]);
-      cp_async16(to + C::kCodeBytes, v + off, n ? bytes[1] : bytes[0]);
+      if (scale_to >= 0)
+        cp_async16(dst + scale_to,
+                   scale + static_cast<long long>(unit0 * C::kGroups + group) * c.page + in + (lane & 1) * 16, bytes0);
+    } else {  // two pages of 16
+      const int page1 = __shfl_sync(0xffffffffu, id, at + 1);
+      lost |= page1 < 0 && first + 1 < used;
+      const uint32_t bytes1 = page1 < 0 ? 0u : 16u;
+      const int unit1 = max(page1, 0) * c.kv_heads + head;
+#pragma unroll
+      for (int i = 0; i < kTile * C::kTokenBytes / 512; ++i) {
+        const bool n = (i * 512 + lane * 16) / (16 * C::kTokenBytes);  // second page
+        const long long off =
+            static_cast<long long>(n ? unit1 : unit0) * 16 * C::kTokenBytes + i * 512 - (n ? 16 * C::kTokenBytes : 0);
+        cp_async16(to + i * 512, k + off, n ? bytes1 : bytes0);
+        cp_async16(to + C::kCodeBytes + i * 512, v + off, n ? bytes1 : bytes0);
+      }
+      if (scale_to >= 0) {
+        const bool n = lane & 1;
+        cp_async16(dst + scale_to, scale + static_cast<long long>((n ? unit1 : unit0) * C::kGroups + group) * 16,
+                   n ? bytes1 : bytes0);
+      }
     }
-    if (scale_to >= 0) {
-      const bool n = lane & 1;
-      const long long off = static_cast<long long>((n ? unit[1] : unit[0]) * C::kGroups + group) * c.page + (n ? in[1] : in[0]);
-      cp_async16(dst + scale_to, scale + off, n ? bytes[1] : bytes[0]);
-    }
+  }
+
+  // Whether the table names the page of token `tok` wrongly (asked where `lost` says that it does so anywhere).
+  __device__ __forceinline__ bool is_lost(int tok) const {
+    if (tok >> shift >= used) return false;
+    const int page = pages[tok >> shift];
+    return page < 0 || page >= c.pages;
   }
 };
 
@@ -322,8 +333,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
       __syncwarp();
       const uint8_t* sk = ring_ptr + slot * C::kSlotBytes;
       const int j0 = (tile0 + t) * kTile;
-      const uint32_t holes = fetch.holes >> (2 * slot) & 3u;
-      const bool masked = j0 + kTile > open || holes;
+      const bool masked = j0 + kTile > open || fetch.lost;
 
       // Scores, eight keys at a time.
       float s[G][kKeys][2];
@@ -370,7 +380,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
 #pragma unroll
         for (int n = 0; n < kKeys; ++n) {
           const int tok = kLaneTokens * (g >> 1) + 2 * n + odd_k;
-          const bool gone = holes >> (tok >> 4) & 1u;
+          const bool gone = fetch.lost && fetch.is_lost(j0 + tok);
 #pragma unroll
           for (int r = 0; r < G; ++r)
 #pragma unroll
@@ -397,24 +407,24 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
         bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
         bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
       }
-      float mx[G][2];
+      float mx[G][2];  // the lane's keys
       bool grew = false;
 #pragma unroll
       for (int r = 0; r < G; ++r)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float m = fmaxf(fmaxf(s[r][0][e], s[r][1][e]), fmaxf(s[r][2][e], s[r][3][e]));
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          mx[r][e] = fmaxf(kFloor, m * factor[r][e]);
-          grew |= mx[r][e] > top[r][e];
+          const float m = fmaxf(fmaxf(s[r][0][e], s[r][1][e]), fmaxf(s[r][2][e], s[r][3][e]));
+          mx[r][e] = m * factor[r][e];
+          grew |= mx[r][e] > top[r][e] + kLag;
         }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int r = 0; r < G; ++r)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float m = fmaxf(top[r][e], mx[r][e]);
+            float m = fmaxf(top[r][e], mx[r][e]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             const float half = ex2_approx(0.5f * (top[r][e] - m)), f = half * half;
             top[r][e] = m;
             sum[r][e] = kv_scaled(sum[r][e], half);
@@ -425,11 +435,11 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
             }
           }
       }
-      // Weights 2^(s - M + kHeadroom), transposed: the fragments of p v.
+      // Weights 2^(s - M + kHeadroomLag), transposed: the fragments of p v.
       uint32_t pf[G][kKeys];
 #pragma unroll
       for (int r = 0; r < G; ++r) {
-        const float ref0 = kHeadroom - top[r][0], ref1 = kHeadroom - top[r][1];
+        const float ref0 = kHeadroomLag - top[r][0], ref1 = kHeadroomLag - top[r][1];
 #pragma unroll
         for (int n = 0; n < kKeys; ++n) {
           const float a = ex2_approx(fmaf(s[r][n][0], factor[r][0], ref0));
@@ -498,7 +508,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
         if (!whole && g == 0) {
           float* ml = p.ml_part + (static_cast<long long>(part) * C::kRows + 8 * r + 2 * c + e) * 2;
           ml[0] = top[r][e];
-          ml[1] = sum[r][e] * fp8_pow2(-kHeadroom);
+          ml[1] = sum[r][e] * fp8_pow2(-kHeadroom);  // (as the join takes it; the outputs have 2^kHeadroomLag as the sum)
         }
       }
       // products j: rows g and g + 8 are channels g D/8 + 2j and + 1
