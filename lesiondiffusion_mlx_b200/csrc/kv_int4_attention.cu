@@ -45,9 +45,9 @@ __device__ __forceinline__ uint32_t transposed8(uint32_t w) {
   return d;
 }
 
-// As many CTAs as the registers of G groups of eight query rows allow: a warp by itself
-// issues an instruction every third cycle or so.
-constexpr int ctas_of(int head_dim, int groups) { return groups == 1 ? 4 : (head_dim == 128 ? 2 : 3); }
+// CTAs an SM, as far as registers allow.  One group, 262144 tokens of 128 channels, us: two 72, three 71, four (128 registers
+// a thread) 76; of 64 channels 50 with four, 47 with three.
+constexpr int ctas_of(int head_dim, int groups) { return groups == 1 ? 3 : (head_dim == 128 ? 2 : 3); }
 
 // G groups of eight query rows per row tile.
 template <int D, int G>
