@@ -482,7 +482,7 @@ LDB_API int ldb_kv_attention_fp8(ldb_stream_t stream, const void* q, long long q
  * strides _ld and _batch; a tensor may be its own output with the same strides, and heads or kv_heads
  * may be 0 (null pointers).  positions int32 [batch][tokens][axes], any strides along batch (0: one
  * for all) and tokens.  head_dim a multiple of 16 up to 256; not interleaved, pairs is a multiple of 8.
- * FP32, rounded once. An axis outside [0, axes) sets status bit 1 and counts as axis 0. */
+ * FP32, rounded once.  An axis outside [0, axes) sets status bit 1 and counts as axis 0. */
 LDB_API int ldb_qk_norm_rope(ldb_stream_t stream, const void* q, long long q_ld, long long q_batch, const void* k,
                              long long k_ld, long long k_batch, int dtype, const float* q_gamma, const float* k_gamma,
                              float eps, int norm, const unsigned long long* turns, const int* axis, int pairs, int axes,

@@ -8,6 +8,7 @@
 
 #include "host_common.h"
 #include "kv_attention.cuh"
+#include "packed.cuh"
 
 namespace ldb {
 namespace {
@@ -18,24 +19,6 @@ constexpr float kFloor = -1.0e30f;  // reference of a row that has seen nothing
 constexpr float kGrow = 8.f;        // a reference follows its row's maximum once that is 2^8 above
 constexpr int kHeadroom = 7;        // weights are 2^7 at the reference, 2^15 at most; the sum is kept without it
 
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

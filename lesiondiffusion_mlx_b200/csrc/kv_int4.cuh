@@ -21,6 +21,7 @@
 #pragma once
 
 #include "fp8.cuh"
+#include "packed.cuh"
 
 namespace ldb {
 
@@ -59,23 +60,21 @@ struct Int4Inverse {
   }
 };
 
-// Eight values to packed codes.
-__device__ __forceinline__ uint32_t int4_pack8(const float (&x)[8], const Int4Inverse& inv) {
+// Eight values (pairs of neighbours) within -8.5 s .. 7.5 s to packed codes.
+__device__ __forceinline__ uint32_t int4_pack8(const uint64_t (&x)[4], const Int4Inverse& inv) {
   // Adding 1.5 * 2^23 rounds to the nearest integer, which the sum's low bits then hold.
   constexpr uint32_t kBias = 0x4B400000u, kOnes = 0x11111111u;
+  constexpr float kMagic = 12582912.f + 8.f;
+  const uint64_t hi = pack2(inv.hi, inv.hi), lo = pack2(inv.lo, inv.lo), magic = pack2(kMagic, kMagic);
   uint32_t word = 0;
 #pragma unroll
-  for (int j = 7; j >= 0; --j) {
-    const float q = fminf(fmaxf(fmaf(x[j], inv.hi, x[j] * inv.lo), -8.f), 7.f);
-    word = word * 16u + __float_as_uint(__fadd_rn(q, 12582912.f + 8.f));
+  for (int k = 3; k >= 0; --k) {
+    float a, b;
+    unpack2(fma2(x[k], hi, mul2(x[k], lo)), a, b);
+    unpack2(add2(pack2(fminf(a, 7.f), fminf(b, 7.f)), magic), a, b);
+    word = (word * 16u + __float_as_uint(b)) * 16u + __float_as_uint(a);
   }
   return word - kBias * kOnes;
-}
-
-// Eight values of a packed word times their scale.
-__device__ __forceinline__ void int4_unpack8(uint32_t word, float s, float (&v)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int>((word >> (4 * j)) & 15u) - 8) * s;
 }
 
 // ------------------------------------------------------------ unpacking to f16

@@ -10,6 +10,8 @@
 //
 // Bound: HBM, 2 bytes read and 9/16 written a value; for one token the launch.
 
+#include <type_traits>
+
 #include "host_common.h"
 #include "kv_int4.cuh"
 
@@ -29,6 +31,45 @@ struct AppendParams {
 };
 
 constexpr int kThreads = 128;
+
+// The largest magnitude of a group, infinite where one is not finite.
+template <typename T>
+__device__ __forceinline__ float largest16(const uint4 (&raw)[sizeof(T)]) {
+  constexpr uint32_t kSign = sizeof(T) == 4 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
+  uint32_t m = 0;  // (magnitudes order as their bits do)
+#pragma unroll
+  for (int h = 0; h < static_cast<int>(sizeof(T)); ++h) {
+    const uint32_t w[4] = {raw[h].x, raw[h].y, raw[h].z, raw[h].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = sizeof(T) == 4 ? max(m, w[k] & kSign) : __vmaxu2(m, w[k] & kSign);
+  }
+  if constexpr (sizeof(T) == 4) return __uint_as_float(min(m, 0x7F800000u));
+  constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  const uint32_t top = min(max(m & 0xFFFFu, m >> 16), kInf);
+  return std::is_same<T, __half>::value ? __half2float(__ushort_as_half(static_cast<unsigned short>(top)))
+                                        : __uint_as_float(top << 16);
+}
+
+// A group's values in FP32, in pairs of neighbours.
+template <typename T>
+__device__ __forceinline__ void pairs16(const uint4 (&raw)[sizeof(T)], uint64_t (&x)[2][4]) {
+  constexpr int kWords = 4 * sizeof(T);
+  uint32_t w[kWords];
+#pragma unroll
+  for (int h = 0; h < static_cast<int>(sizeof(T)); ++h)
+    w[4 * h] = raw[h].x, w[4 * h + 1] = raw[h].y, w[4 * h + 2] = raw[h].z, w[4 * h + 3] = raw[h].w;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if constexpr (sizeof(T) == 4) {
+      x[k / 4][k % 4] = pack2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      x[k / 4][k % 4] = pack2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xFFFF0000u));
+    } else {
+      const float2 f = __half22float2(as_half2(w[k]));
+      x[k / 4][k % 4] = pack2(f.x, f.y);
+    }
+  }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) kv_append_int4_kernel(const AppendParams p, unsigned int* status) {
@@ -80,21 +121,20 @@ __global__ void __launch_bounds__(kThreads) kv_append_int4_kernel(const AppendPa
 #pragma unroll
   for (int j = 0; j < kInt4Quad; ++j) {
     if (j < first || j >= last) continue;
-    float x[2][8];
-    const T* v = reinterpret_cast<const T*>(raw[j]);
-    float amax = 0.f;
-    bool finite = true;
-#pragma unroll
-    for (int c = 0; c < kInt4Group; ++c) {
-      x[c / 8][c % 8] = to_f32<T>(v[c]);
-      amax = fmaxf(amax, fabsf(x[c / 8][c % 8]));
-      finite = finite && fp8_is_finite(x[c / 8][c % 8]);
-    }
+    const float amax = largest16<T>(raw[j]);
+    const bool finite = fp8_is_finite(amax);
     const int byte = finite ? int4_scale_byte(amax) : kInt4NanScale;
     const Int4Inverse inv(byte);
-    if (!finite) {
+    uint64_t x[2][4];
+    pairs16<T>(raw[j], x);
+    if (byte >= kInt4TopScale) {  // (rare) past the scales' end, or not finite
+      const float most = finite ? 8.f * int4_scale_value(byte) : 0.f;
 #pragma unroll
-      for (int c = 0; c < kInt4Group; ++c) x[c / 8][c % 8] = 0.f;
+      for (int k = 0; k < 8; ++k) {
+        float a, c;
+        unpack2(x[k / 4][k % 4], a, c);
+        x[k / 4][k % 4] = finite ? pack2(fmaxf(a, -most), fmaxf(c, -most)) : 0;
+      }
     }
     *reinterpret_cast<uint2*>(codes + j * (p.dim / 2)) = make_uint2(int4_pack8(x[0], inv), int4_pack8(x[1], inv));
     bytes |= static_cast<uint32_t>(byte) << (8 * j);

@@ -15,8 +15,12 @@
 //
 // Bound: HBM, each value read and written once; for few tokens the launch.
 
+#include <algorithm>
+#include <type_traits>
+
 #include "host_common.h"
 #include "fp8.cuh"
+#include "packed.cuh"
 
 namespace ldb {
 namespace {
@@ -32,8 +36,8 @@ struct RopeParams {
   long long pos_batch, pos_ld;
   int heads[2];
   int tokens, dim, pairs, axes, interleaved, norm, vec;
-  int rounds, per_warp;  // heads of a token, of a warp, in rounds of as many as fit
-  unsigned splits;       // warps of a token
+  int rounds[2], per_warp[2];  // of heads of a token, of a warp: as many heads as fit at a time
+  unsigned splits;             // warps of a token
   unsigned warps;
   float eps, inv_dim;
 };
@@ -41,11 +45,31 @@ struct RopeParams {
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxPairs = 128;
+// Rounds of values on their way at a time (4 x 4097 tokens of 40 heads of 128: one 92 us, two 72, four 66, six 76).
+constexpr int kAhead = 4;
+
+// Eight channels of a row as they are in memory.
+template <typename T>
+struct Raw {
+  static constexpr int kWords = 2 * sizeof(T);
+  uint32_t w[kWords];
+  // channels 2k and 2k + 1
+  __device__ __forceinline__ uint64_t pair(int k) const {
+    if constexpr (sizeof(T) == 4) {
+      return pack2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return pack2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xFFFF0000u));
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+      return pack2(f.x, f.y);
+    }
+  }
+};
 
 // LANES per head, of eight channels each (the last ones idle where D is not 8 LANES).
-template <typename T, int LANES>
+template <typename T, int LANES, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p, unsigned int* status) {
-  __shared__ __align__(16) float2 s_turn[kWarps][kMaxPairs];  // (cos, sin)
+  __shared__ __align__(16) float2 s_turn[kWarps][kMaxPairs + 8];  // (cos, sin), and eight of no turn
   pdl_begin();
   const int lane = lane_id();
   const unsigned w = blockIdx.x * kWarps + warp_id();
@@ -54,6 +78,13 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p, unsi
   const int split = static_cast<int>(w - row * p.splits);
   const long long b = row / static_cast<unsigned>(p.tokens);
   const long long token = row - static_cast<unsigned>(b) * p.tokens;
+  constexpr int kHeads = 32 / LANES;  // at a time
+  const int sub = lane / LANES, c0 = (lane % LANES) * 8;
+  const bool live = c0 < p.dim;
+  const int turned_to = 2 * p.pairs - c0;  // the lane's channels below this one turn (all or none, in halves)
+  const bool upper = !INTERLEAVED && c0 >= p.pairs;
+  const int away = INTERLEAVED || turned_to <= 0 ? 0 : (upper ? -p.pairs : p.pairs);  // of the other members of its pairs
+  const int partner = lane + away / 8;
   float2* turn = s_turn[warp_id()];
   const int* position = p.positions + b * p.pos_batch + token * p.pos_ld;
   for (int i = lane; i < p.pairs; i += 32) {
@@ -67,77 +98,105 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p, unsi
     sincospif(static_cast<float>(static_cast<int>(phase >> 32)) * 0x1p-31f, &cs.y, &cs.x);
     turn[i] = cs;
   }
+  if (lane < 8) turn[p.pairs + lane] = make_float2(1.f, 0.f);
   __syncwarp();
-  constexpr int kHeads = 32 / LANES;  // at a time
-  const int sub = lane / LANES, c0 = (lane % LANES) * 8;
-  const bool live = c0 < p.dim;
-  // the lane's pairs, and which member of them it holds
-  const int first = p.interleaved ? c0 / 2 : (c0 < p.pairs ? c0 : c0 - p.pairs);
-  const bool turned = c0 < 2 * p.pairs;  // (some of the lane's channels)
-  const bool upper = !p.interleaved && c0 >= p.pairs;
-  const int partner = lane + (p.interleaved || !turned ? 0 : (upper ? -p.pairs / 8 : p.pairs / 8));
-  const int turned_to = min(8, 2 * p.pairs - c0);  // the lane's channels below this one turn
-  float cs[8], sn[8];  // by channel
+
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const int to = min(p.rounds[which], (split + 1) * p.per_warp[which]);
+    int r = split * p.per_warp[which];
+    if (r >= to) continue;
+    // A token's channel becomes f (x own + other times), f its head's norm: sines, cosines and gamma in two factors.
+    uint64_t own[4], times[4];
+    {
+      float g[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f}, mate[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+      if (p.gamma[which] && live) {
+        load8<float>(p.gamma[which] + c0, g);
+        load8<float>(p.gamma[which] + c0 + away, mate);
+      }
+      // the lane's turns: from the first of its pairs, or of no turn
+      const float2* t = turn + (turned_to <= 0 ? p.pairs : (INTERLEAVED ? c0 / 2 : (upper ? c0 - p.pairs : c0)));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int i = p.interleaved ? first + j / 2 : first + j;
-    const float2 t = turned && i < p.pairs ? turn[i] : make_float2(0.f, 0.f);
-    const bool second = p.interleaved ? (j & 1) : upper;
-    cs[j] = t.x;
-    sn[j] = second ? t.y : -t.y;
-  }
-  const int all = p.heads[0] + p.heads[1];
-  const int to = min(p.rounds, (split + 1) * p.per_warp);
-  for (int r = split * p.per_warp; r < to; ++r) {
-    int head = r * kHeads + sub;
-    const bool here = live && head < all;
-    const int which = head >= p.heads[0] ? 1 : 0;
-    if (which) head -= p.heads[0];
-    float x[8];
-    if (here) {
-      const T* src = static_cast<const T*>(p.src[which]) + b * p.src_batch[which] + token * p.src_ld[which] +
-                     static_cast<long long>(head) * p.dim + c0;
+      for (int k = 0; k < 4; ++k) {
+        if (INTERLEAVED) {
+          const float2 cs = t[k];  // (behind the last pair: no turn)
+          own[k] = pack2(cs.x * g[2 * k], cs.x * g[2 * k + 1]);
+          times[k] = pack2(-cs.y * g[2 * k + 1], cs.y * g[2 * k]);
+        } else {
+          const float2 c = t[2 * k], d = t[2 * k + 1];
+          own[k] = pack2(c.x * g[2 * k], d.x * g[2 * k + 1]);
+          const float s0 = c.y * mate[2 * k], s1 = d.y * mate[2 * k + 1];
+          times[k] = upper ? pack2(s0, s1) : pack2(-s0, -s1);
+        }
+      }
+    }
+    const T* src = static_cast<const T*>(p.src[which]) + b * p.src_batch[which] + token * p.src_ld[which] + c0;
+    T* out = static_cast<T*>(p.out[which]) + b * p.out_batch[which] + token * p.out_ld[which] + c0;
+    const int heads = live ? p.heads[which] : 0;
+    auto load = [&](int head, Raw<T>& raw) {
+#pragma unroll
+      for (int k = 0; k < Raw<T>::kWords; ++k) raw.w[k] = 0;
+      if (head >= heads) return;
+      const T* x = src + head * p.dim;
       if (p.vec) {
-        load8<T>(src, x);
+#pragma unroll
+        for (int k = 0; k < Raw<T>::kWords; k += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(x + 4 * k / static_cast<int>(sizeof(T)));
+          raw.w[k] = v.x, raw.w[k + 1] = v.y, raw.w[k + 2] = v.z, raw.w[k + 3] = v.w;
+        }
+      } else {
+        T t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = x[j];
+#pragma unroll
+        for (int k = 0; k < Raw<T>::kWords; ++k) raw.w[k] = reinterpret_cast<const uint32_t*>(t)[k];
+      }
+    };
+    auto finish = [&](int head, const Raw<T>& x) {
+      Raw<T> far;  // the other members (nothing where a channel does not turn: an infinity times zero would reach it)
+#pragma unroll
+      for (int k = 0; k < Raw<T>::kWords; ++k) {
+        uint32_t v;
+        if (!INTERLEAVED) {
+          v = __shfl_sync(0xffffffffu, x.w[k], partner);
+        } else {
+          v = sizeof(T) == 4 ? x.w[k ^ 1] : __byte_perm(x.w[k], 0, 0x1032);
+        }
+        far.w[k] = 4 * k / static_cast<int>(sizeof(T)) < turned_to ? v : 0u;
+      }
+      uint64_t f2 = pack2(1.f, 1.f);
+      if (p.norm) {
+        uint64_t sums = mul2(x.pair(0), x.pair(0));
+#pragma unroll
+        for (int k = 1; k < 4; ++k) sums = fma2(x.pair(k), x.pair(k), sums);
+        float even, odd;
+        unpack2(sums, even, odd);
+        float sum = even + odd;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float f = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
+        f2 = pack2(f, f);
+      }
+      float y[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        unpack2(mul2(f2, fma2(far.pair(k), times[k], mul2(x.pair(k), own[k]))), y[2 * k], y[2 * k + 1]);
+      if (head >= heads) return;
+      T* to_row = out + head * p.dim;
+      if (p.vec) {
+        store8<T>(to_row, y);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = to_f32<T>(src[j]);
+        for (int j = 0; j < 8; ++j) to_row[j] = from_f32<T>(y[j]);
       }
-    } else {
+    };
+    for (; r < to; r += kAhead) {
+      Raw<T> raw[kAhead];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    }
-    if (p.norm) {
-      float sum = 0.f;
+      for (int n = 0; n < kAhead; ++n) load(r + n < to ? (r + n) * kHeads + sub : 0x7FFFFFFF, raw[n]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float f = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= f;
-    }
-    if (here && p.gamma[which]) {
-      float g[8];
-      load8<float>(p.gamma[which] + c0, g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= g[j];
-    }
-    float y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float other = p.interleaved ? x[j ^ 1] : __shfl_sync(0xffffffffu, x[j], partner);
-      y[j] = j < turned_to ? fmaf(x[j], cs[j], other * sn[j]) : x[j];
-    }
-    if (here) {
-      T* out = static_cast<T*>(p.out[which]) + b * p.out_batch[which] + token * p.out_ld[which] +
-               static_cast<long long>(head) * p.dim + c0;
-      if (p.vec) {
-        store8<T>(out, y);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) out[j] = from_f32<T>(y[j]);
-      }
+      for (int n = 0; n < kAhead; ++n)
+        if (r + n < to) finish((r + n) * kHeads + sub, raw[n]);
     }
   }
 }
@@ -146,22 +205,30 @@ template <typename T>
 int launch_rope(cudaStream_t stream, RopeParams& p, long long rows, unsigned int* status) {
   const int lanes = p.dim <= 16 ? 2 : (p.dim <= 32 ? 4 : (p.dim <= 64 ? 8 : (p.dim <= 128 ? 16 : 32)));
   const int at_a_time = 32 / lanes;
-  p.rounds = (p.heads[0] + p.heads[1] + at_a_time - 1) / at_a_time;
+  int most = 0;
+  for (int i = 0; i < 2; ++i) {
+    p.rounds[i] = (p.heads[i] + at_a_time - 1) / at_a_time;
+    most = std::max(most, p.rounds[i]);
+  }
   // A warp per round while all of them are resident at once, else rounds enough to share the sines.
   const long long resident = 32ll * sm_count();
-  p.per_warp = 1;
-  while (p.per_warp < p.rounds && p.per_warp < 8 && rows * ((p.rounds + p.per_warp - 1) / p.per_warp) > resident)
-    p.per_warp *= 2;
-  if (p.per_warp > p.rounds) p.per_warp = p.rounds;
-  p.splits = (p.rounds + p.per_warp - 1) / p.per_warp;
+  int splits = most;
+  while (splits > 1 && rows * splits > resident) splits = (splits + 1) / 2;
+  if (splits > 1 && rows * splits > resident) splits = 1;
+  p.splits = splits;
+  for (int i = 0; i < 2; ++i) p.per_warp[i] = (p.rounds[i] + splits - 1) / splits;
   if (rows * p.splits > 0x7FFFFF00ll) return fail(LDB_ERR_SHAPE, "qk_norm_rope: %lld tokens of %d heads", rows, p.heads[0]);
   p.warps = static_cast<unsigned>(rows * p.splits);
   const unsigned blocks = (p.warps + kWarps - 1) / kWarps;
-  auto kernel = lanes == 2    ? rope_kernel<T, 2>
-                : lanes == 4  ? rope_kernel<T, 4>
-                : lanes == 8  ? rope_kernel<T, 8>
-                : lanes == 16 ? rope_kernel<T, 16>
-                              : rope_kernel<T, 32>;
+  auto pick = [&](auto interleaved) {
+    constexpr bool I = decltype(interleaved)::value;
+    return lanes == 2    ? rope_kernel<T, 2, I>
+           : lanes == 4  ? rope_kernel<T, 4, I>
+           : lanes == 8  ? rope_kernel<T, 8, I>
+           : lanes == 16 ? rope_kernel<T, 16, I>
+                         : rope_kernel<T, 32, I>;
+  };
+  auto kernel = p.interleaved ? pick(std::true_type{}) : pick(std::false_type{});
   return launch_kernel(kernel, dim3(blocks), dim3(kThreads), 0, stream, "qk_norm_rope launch", p,
                        status);
 }
