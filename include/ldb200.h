@@ -473,65 +473,93 @@ LDB_API int ldb_kv_attention_fp8(ldb_stream_t stream, const void* q, long long q
                                  long long out_ld, long long out_batch, int batch, int queries, int heads, float scale,
                                  int causal, void* workspace, size_t workspace_bytes);
 
+/* The operators below take a descriptor: struct_size is its size, checked before anything else; pointers are
+ * device pointers, _ld and _batch element strides of tokens and items. */
+
 /* Each head's queries and keys normed and rotated: x rsqrt(mean(x^2) + eps)
  * gamma over its head_dim channels (norm 0: x gamma; gamma f32 or null = 1, 16-byte
  * aligned), then the first 2 `pairs` channels turned in pairs, (i, i + pairs) or interleaved (2i, 2i
  * + 1), by the angle positions[b][t][axis[i]] * turns[i] (turns: a position's share
  * of a full turn as a 64-bit fraction, so that the angle is exact at any position).  q and
- * q_out [batch][tokens][heads * head_dim], k and k_out [..][kv_heads * head_dim] with element
- * strides _ld and _batch; a tensor may be its own output with the same strides, and heads or kv_heads
- * may be 0 (null pointers).  positions int32 [batch][tokens][axes], any strides along batch (0: one
- * for all) and tokens.  head_dim a multiple of 16 up to 256; not interleaved, pairs is a multiple of 8.
+ * q_out [batch][tokens][heads * head_dim], k and k_out [..][kv_heads * head_dim]; a tensor may
+ * be its own output with the same strides, and heads or kv_heads may be 0 (null pointers).
+ * positions int32 [batch][tokens][axes], any strides along batch (0: one for all) and
+ * tokens.  head_dim a multiple of 16 up to 256; not interleaved, pairs is a multiple of 8.
  * FP32, rounded once.  An axis outside [0, axes) sets status bit 1 and counts as axis 0. */
-LDB_API int ldb_qk_norm_rope(ldb_stream_t stream, const void* q, long long q_ld, long long q_batch, const void* k,
-                             long long k_ld, long long k_batch, int dtype, const float* q_gamma, const float* k_gamma,
-                             float eps, int norm, const unsigned long long* turns, const int* axis, int pairs, int axes,
-                             int interleaved, const int* positions, long long positions_ld, long long positions_batch,
-                             void* q_out, long long qo_ld, long long qo_batch, void* k_out, long long ko_ld,
-                             long long ko_batch, int batch, int tokens, int heads, int kv_heads, int head_dim);
+typedef struct ldb_qk_norm_rope_desc {
+  int struct_size, dtype;
+  const void *q, *k;
+  void *q_out, *k_out;
+  long long q_ld, q_batch, k_ld, k_batch, q_out_ld, q_out_batch, k_out_ld, k_out_batch;
+  const float *q_gamma, *k_gamma;
+  const unsigned long long* turns; /* [pairs] */
+  const int *axis, *positions;     /* [pairs], see above */
+  long long positions_ld, positions_batch;
+  int batch, tokens, heads, kv_heads, head_dim, pairs, axes, interleaved, norm;
+  float eps;
+} ldb_qk_norm_rope_desc;
+LDB_API int ldb_qk_norm_rope(ldb_stream_t stream, const ldb_qk_norm_rope_desc* desc);
 
 /* Paged 4-bit key/value cache, laid out and addressed as the 8-bit one but for:
  * codes [pages][kv_heads][page][head_dim / 2], two to a byte, the lower channel
  * in the low half, and scales [pages][kv_heads][head_dim / 16][page], one for 16
  * channels of a token.  A code c stands for (c - 8) s, a scale byte for the f16 whose
- * upper eight bits under the sign it is (198 = 896 is the largest used, 255 a NaN).
- *
- * ldb_kv_append_int4: the least s with max|x| <= 7.5 s over the 16 channels and
+ * upper eight bits under the sign it is (198 = 896 is the largest used, 255 a NaN).  Codes and scales
+ * 16-byte aligned. */
+typedef struct ldb_kv_cache {
+  uint8_t *k_codes, *v_codes, *k_scales, *v_scales;
+  const int* table;
+  long long table_ld;
+  int pages, kv_heads, page, head_dim, width, batch;
+} ldb_kv_cache;
+
+/* `tokens` rows of k and v of each item, or the first counts[b] of them (counts may be null),
+ * from position start[b] on: the least s with max|x| <= 7.5 s over 16 channels and
  * x / s rounded to nearest even within -8 .. 7, so that no value is further than s / 2
  * away; magnitudes past 6720 saturate.  16 channels that hold a value that is not finite become NaN.
  * Older tokens of a page are neither read nor changed. */
-LDB_API int ldb_kv_append_int4(ldb_stream_t stream, const void* k, long long k_ld, long long k_batch, const void* v,
-                               long long v_ld, long long v_batch, int dtype, uint8_t* k_codes, uint8_t* v_codes,
-                               uint8_t* k_scales, uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim,
-                               const int* table, long long table_ld, int width, const int* start, const int* counts,
-                               int batch, int tokens);
+typedef struct ldb_kv_append_desc {
+  int struct_size, dtype;
+  ldb_kv_cache cache;
+  const void *k, *v;
+  long long k_ld, k_batch, v_ld, v_batch;
+  const int *start, *counts;
+  int tokens;
+} ldb_kv_append_desc;
+LDB_API int ldb_kv_append_int4(ldb_stream_t stream, const ldb_kv_append_desc* desc);
 
-/* Rows of a cache: k and v [batch][tokens][kv_heads * head_dim] (f16, bf16 or f32;
- * element strides _ld and _batch) become item b's tokens start[b] .. start[b] + tokens
- * (start null: from 0), zeros from lengths[b] on and for a page number outside the
- * cache (status bit 1, as for a length outside the table or a negative start).  Exact from 4
- * bits, rounded once from 8. */
-LDB_API int ldb_kv_read_fp8(ldb_stream_t stream, const uint8_t* k_codes, const uint8_t* v_codes,
-                            const uint8_t* k_scales, const uint8_t* v_scales, int pages, int kv_heads, int page,
-                            int head_dim, const int* table, long long table_ld, int width, const int* lengths,
-                            const int* start, void* k, long long k_ld, long long k_batch, void* v, long long v_ld,
-                            long long v_batch, int dtype, int batch, int tokens);
-LDB_API int ldb_kv_read_int4(ldb_stream_t stream, const uint8_t* k_codes, const uint8_t* v_codes,
-                             const uint8_t* k_scales, const uint8_t* v_scales, int pages, int kv_heads, int page,
-                             int head_dim, const int* table, long long table_ld, int width, const int* lengths,
-                             const int* start, void* k, long long k_ld, long long k_batch, void* v, long long v_ld,
-                             long long v_batch, int dtype, int batch, int tokens);
+/* Rows of a cache: k and v [batch][tokens][kv_heads * head_dim] (f16, bf16 or f32) become
+ * item b's tokens start[b] .. start[b] + tokens (start null: from 0), zeros from
+ * lengths[b] on and for a page number outside the cache (status bit 1, as for a
+ * length outside the table or a negative start).  Exact from 4 bits, rounded once from 8. */
+typedef struct ldb_kv_read_desc {
+  int struct_size, dtype;
+  ldb_kv_cache cache;
+  void *k, *v;
+  long long k_ld, k_batch, v_ld, v_batch;
+  const int *lengths, *start;
+  int tokens;
+} ldb_kv_read_desc;
+LDB_API int ldb_kv_read_fp8(ldb_stream_t stream, const ldb_kv_read_desc* desc);
+LDB_API int ldb_kv_read_int4(ldb_stream_t stream, const ldb_kv_read_desc* desc);
 
 /* As ldb_kv_attention_fp8, over the 4-bit cache; workspace for a table of
  * `capacity` = width * page tokens. */
+typedef struct ldb_kv_attention_desc {
+  int struct_size, dtype;
+  ldb_kv_cache cache;
+  const void* q;
+  void* out;
+  long long q_ld, q_batch, out_ld, out_batch;
+  const int* lengths;
+  void* workspace;
+  size_t workspace_bytes;
+  int queries, heads, causal;
+  float scale;
+} ldb_kv_attention_desc;
 LDB_API int ldb_kv_attention_int4_workspace_size(int batch, int queries, int heads, int kv_heads, int head_dim,
                                                  long long capacity, size_t* bytes);
-LDB_API int ldb_kv_attention_int4(ldb_stream_t stream, const void* q, long long q_ld, long long q_batch, int dtype,
-                                  const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scales,
-                                  const uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim,
-                                  const int* table, long long table_ld, int width, const int* lengths, void* out,
-                                  long long out_ld, long long out_batch, int batch, int queries, int heads, float scale,
-                                  int causal, void* workspace, size_t workspace_bytes);
+LDB_API int ldb_kv_attention_int4(ldb_stream_t stream, const ldb_kv_attention_desc* desc);
 
 #ifdef __cplusplus
 }

@@ -9,6 +9,7 @@ library's own message.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -109,18 +110,26 @@ SIGNATURES: dict[str, list] = {
     "ldb_kv_attention_fp8_table_workspace_size": [_I, _I, _I, _I, _I, _L, ctypes.POINTER(_SZ)],
     "ldb_kv_attention_fp8": [_P, _P, _L, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I,
                              _F, _I, _P, _SZ],
-    "ldb_qk_norm_rope": [_P, _P, _L, _L, _P, _L, _L, _I, _P, _P, _F, _I, _P, _P, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P,
-                         _L, _L, _I, _I, _I, _I, _I],
-    "ldb_kv_append_int4": [_P, _P, _L, _L, _P, _L, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _I, _I],
-    "ldb_kv_read_fp8": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _P, _L, _L, _P, _L, _L, _I, _I, _I],
-    "ldb_kv_read_int4": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _P, _L, _L, _P, _L, _L, _I, _I, _I],
+    "ldb_qk_norm_rope": [_P, _P],
+    "ldb_kv_append_int4": [_P, _P],
+    "ldb_kv_read_fp8": [_P, _P],
+    "ldb_kv_read_int4": [_P, _P],
     "ldb_kv_attention_int4_workspace_size": [_I, _I, _I, _I, _I, _L, ctypes.POINTER(_SZ)],
-    "ldb_kv_attention_int4": [_P, _P, _L, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I,
-                              _F, _I, _P, _SZ],
+    "ldb_kv_attention_int4": [_P, _P],
     "ldb_matmul_fp8_workspace_size": [_I, _I, _I, ctypes.POINTER(_SZ)],
     "ldb_matmul_fp8": [_P, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P, _SZ],
 }
 _RESTYPES = {"ldb_last_error": ctypes.c_char_p, "ldb_launch_count": ctypes.c_ulonglong}
+
+# Descriptors, packed as C lays their fields out: one pointer crosses to the library instead of some thirty
+# arguments, whose conversion takes ctypes longer than a launch.  The first field is the size.
+_CACHE = "PPPPPqiiiiii"
+DESCRIPTORS: dict[str, struct.Struct] = {
+    "ldb_qk_norm_rope_desc": struct.Struct("@iiPPPPqqqqqqqqPPPPPqqiiiiiiiiif"),
+    "ldb_kv_append_desc": struct.Struct(f"@ii{_CACHE}PPqqqqPPi0q"),
+    "ldb_kv_read_desc": struct.Struct(f"@ii{_CACHE}PPqqqqPPi0q"),
+    "ldb_kv_attention_desc": struct.Struct(f"@ii{_CACHE}PPqqqqPPNiiif"),
+}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

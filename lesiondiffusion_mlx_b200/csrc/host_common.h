@@ -20,6 +20,16 @@ void set_last_error(const char* fmt, ...);
 // Return `code` after recording a formatted message for ldb_last_error().
 int fail(int code, const char* fmt, ...);
 
+// Whether a descriptor is there and of the size this library was built with.
+template <typename Desc>
+int check_desc(const Desc* desc, const char* what) {
+  if (!desc) return fail(LDB_ERR_INVALID, "%s: descriptor is null", what);
+  if (desc->struct_size != static_cast<int>(sizeof(Desc)))
+    return fail(LDB_ERR_INVALID, "%s: descriptor of %d bytes, %d wanted", what, desc->struct_size,
+                static_cast<int>(sizeof(Desc)));
+  return LDB_OK;
+}
+
 // Map a CUDA runtime error to LDB_ERR_CUDA (recording its text), or LDB_OK.
 int check_cuda(cudaError_t err, const char* what);
 

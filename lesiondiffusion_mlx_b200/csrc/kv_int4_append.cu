@@ -153,12 +153,12 @@ __global__ void __launch_bounds__(kThreads) kv_append_int4_kernel(const AppendPa
 
 extern "C" {
 
-int ldb_kv_append_int4(cudaStream_t stream, const void* k, long long k_ld, long long k_batch, const void* v,
-                       long long v_ld, long long v_batch, int dtype, uint8_t* k_codes, uint8_t* v_codes,
-                       uint8_t* k_scales, uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim,
-                       const int* table, long long table_ld, int width, const int* start, const int* counts, int batch,
-                       int tokens) {
+int ldb_kv_append_int4(cudaStream_t stream, const ldb_kv_append_desc* desc) {
   using namespace ldb;
+  if (const int rc = check_desc(desc, "kv_append")) return rc;
+  const auto& [struct_size, dtype, cache, k, v, k_ld, k_batch, v_ld, v_batch, start, counts, tokens] = *desc;
+  const auto& [k_codes, v_codes, k_scales, v_scales, table, table_ld, pages, kv_heads, page, head_dim, width, batch] =
+      cache;
   if (batch < 0 || tokens < 0) return fail(LDB_ERR_SHAPE, "kv_append: %d items of %d tokens", batch, tokens);
   if (dtype != LDB_F16 && dtype != LDB_F32 && dtype != LDB_BF16)
     return fail(LDB_ERR_INVALID, "kv_append: unknown element type %d", dtype);

@@ -600,13 +600,13 @@ int ldb_kv_attention_int4_workspace_size(int batch, int queries, int heads, int 
   return LDB_OK;
 }
 
-int ldb_kv_attention_int4(cudaStream_t stream, const void* q, long long q_ld, long long q_batch, int dtype,
-                          const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scales,
-                          const uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim, const int* table,
-                          long long table_ld, int width, const int* lengths, void* out, long long out_ld,
-                          long long out_batch, int batch, int queries, int heads, float scale, int causal,
-                          void* workspace, size_t workspace_bytes) {
+int ldb_kv_attention_int4(cudaStream_t stream, const ldb_kv_attention_desc* desc) {
   using namespace ldb;
+  if (const int rc = check_desc(desc, "kv_attention")) return rc;
+  const auto& [struct_size, dtype, cache, q, out, q_ld, q_batch, out_ld, out_batch, lengths, workspace, workspace_bytes,
+               queries, heads, causal, scale] = *desc;
+  const auto& [k_codes, v_codes, k_scales, v_scales, table, table_ld, pages, kv_heads, page, head_dim, width, batch] =
+      cache;
   if (dtype != LDB_F16 && dtype != LDB_BF16) return fail(LDB_ERR_INVALID, "kv_attention: queries must be f16 or bf16");
   size_t need = 0;
   int rc = ldb_kv_attention_int4_workspace_size(batch, queries, heads, kv_heads, head_dim,

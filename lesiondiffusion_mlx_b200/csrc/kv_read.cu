@@ -134,10 +134,11 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadParams p, u
   }
 }
 
-int kv_read(cudaStream_t stream, bool int4, const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scales,
-            const uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim, const int* table,
-            long long table_ld, int width, const int* lengths, const int* start, void* k, long long k_ld,
-            long long k_batch, void* v, long long v_ld, long long v_batch, int dtype, int batch, int tokens) {
+int kv_read(cudaStream_t stream, bool int4, const ldb_kv_read_desc* desc) {
+  if (const int rc = check_desc(desc, "kv_read")) return rc;
+  const auto& [struct_size, dtype, cache, k, v, k_ld, k_batch, v_ld, v_batch, lengths, start, tokens] = *desc;
+  const auto& [k_codes, v_codes, k_scales, v_scales, table, table_ld, pages, kv_heads, page, head_dim, width, batch] =
+      cache;
   if (batch < 0 || tokens < 0) return fail(LDB_ERR_SHAPE, "kv_read: %d items of %d tokens", batch, tokens);
   if (dtype != LDB_F16 && dtype != LDB_F32 && dtype != LDB_BF16)
     return fail(LDB_ERR_INVALID, "kv_read: unknown element type %d", dtype);
@@ -187,20 +188,8 @@ int kv_read(cudaStream_t stream, bool int4, const uint8_t* k_codes, const uint8_
 
 extern "C" {
 
-int ldb_kv_read_fp8(cudaStream_t stream, const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scales,
-                    const uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim, const int* table,
-                    long long table_ld, int width, const int* lengths, const int* start, void* k, long long k_ld,
-                    long long k_batch, void* v, long long v_ld, long long v_batch, int dtype, int batch, int tokens) {
-  return ldb::kv_read(stream, false, k_codes, v_codes, k_scales, v_scales, pages, kv_heads, page, head_dim, table,
-                      table_ld, width, lengths, start, k, k_ld, k_batch, v, v_ld, v_batch, dtype, batch, tokens);
-}
+int ldb_kv_read_fp8(cudaStream_t stream, const ldb_kv_read_desc* desc) { return ldb::kv_read(stream, false, desc); }
 
-int ldb_kv_read_int4(cudaStream_t stream, const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scales,
-                     const uint8_t* v_scales, int pages, int kv_heads, int page, int head_dim, const int* table,
-                     long long table_ld, int width, const int* lengths, const int* start, void* k, long long k_ld,
-                     long long k_batch, void* v, long long v_ld, long long v_batch, int dtype, int batch, int tokens) {
-  return ldb::kv_read(stream, true, k_codes, v_codes, k_scales, v_scales, pages, kv_heads, page, head_dim, table,
-                      table_ld, width, lengths, start, k, k_ld, k_batch, v, v_ld, v_batch, dtype, batch, tokens);
-}
+int ldb_kv_read_int4(cudaStream_t stream, const ldb_kv_read_desc* desc) { return ldb::kv_read(stream, true, desc); }
 
 }  // extern "C"

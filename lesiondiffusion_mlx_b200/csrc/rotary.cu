@@ -238,13 +238,12 @@ int launch_rope(cudaStream_t stream, RopeParams& p, long long rows, unsigned int
 
 extern "C" {
 
-int ldb_qk_norm_rope(cudaStream_t stream, const void* q, long long q_ld, long long q_batch, const void* k,
-                     long long k_ld, long long k_batch, int dtype, const float* q_gamma, const float* k_gamma,
-                     float eps, int norm, const unsigned long long* turns, const int* axis, int pairs, int axes,
-                     int interleaved, const int* positions, long long positions_ld, long long positions_batch,
-                     void* q_out, long long qo_ld, long long qo_batch, void* k_out, long long ko_ld, long long ko_batch,
-                     int batch, int tokens, int heads, int kv_heads, int head_dim) {
+int ldb_qk_norm_rope(cudaStream_t stream, const ldb_qk_norm_rope_desc* desc) {
   using namespace ldb;
+  if (const int rc = check_desc(desc, "qk_norm_rope")) return rc;
+  const auto& [struct_size, dtype, q, k, q_out, k_out, q_ld, q_batch, k_ld, k_batch, qo_ld, qo_batch, ko_ld, ko_batch,
+               q_gamma, k_gamma, turns, axis, positions, positions_ld, positions_batch, batch, tokens, heads, kv_heads,
+               head_dim, pairs, axes, interleaved, norm, eps] = *desc;
   if (batch < 0 || tokens < 0 || heads < 0 || kv_heads < 0)
     return fail(LDB_ERR_SHAPE, "qk_norm_rope: %d items of %d tokens, %d and %d heads", batch, tokens, heads, kv_heads);
   if (dtype != LDB_F16 && dtype != LDB_F32 && dtype != LDB_BF16)

@@ -130,6 +130,42 @@ def _check_table(table: torch.Tensor, batch: int, device: torch.device, name: st
     return width, table.stride(0) if batch > 1 else width
 
 
+def _fields(cache: KvCache, table: torch.Tensor, per_item: torch.Tensor, name: str, what: str) -> tuple[tuple, int, int]:
+    """The library's description of a cache and its table, the channels of a token, and the device's index.
+
+    (All of it is looked at in one expression, as a token's call is bound by the host; what is wrong is found out after that.)"""
+    k, v, k_scale, v_scale = cache
+    shape, index = k.shape, k.get_device()
+    if len(shape) == 4:
+        pages, heads, page, dim = shape
+        if isinstance(cache, KvCacheInt4):
+            codes = scales = torch.uint8
+            dim *= 2
+            per = (pages, heads, dim // GROUP, page)
+        else:
+            codes, scales, per = CODES, SCALES, (pages, heads)
+        if (page in PAGES and dim in HEAD_DIMS and index >= 0 and v.shape == shape and k_scale.shape == per
+                and v_scale.shape == per and k.dtype is codes and v.dtype is codes and k_scale.dtype is scales
+                and v_scale.dtype is scales and k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous()
+                and v_scale.is_contiguous() and v.get_device() == index and k_scale.get_device() == index
+                and v_scale.get_device() == index and per_item.ndim == 1 and table.ndim == 2
+                and per_item.dtype is torch.int32 and table.dtype is torch.int32 and per_item.get_device() == index
+                and table.get_device() == index and per_item.is_contiguous()):
+            (batch,), (rows, width), (table_ld, step) = per_item.shape, table.shape, table.stride()
+            if rows == batch and width and (step == 1 or width == 1):
+                return ((k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
+                         table_ld if batch > 1 else width, pages, heads, page, dim, width, batch), heads * dim, index)
+    _, device = _check_cache(cache, name)
+    if per_item.ndim != 1:
+        raise ValueError(f"{name}: {what} must be one number per item")
+    _check_table(table, per_item.shape[0], device, f"{name}: table")
+    _check_index(per_item, 1, per_item.shape[0], device, f"{name}: {what}")
+    raise ValueError(f"{name}: cache, table and {what} do not fit")
+
+
+_APPEND, _READ, _ATTENTION = (_lib.DESCRIPTORS[f"ldb_kv_{n}_desc"] for n in ("append", "read", "attention"))
+
+
 def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, *,
               counts: torch.Tensor | None = None) -> None:
     """Write ``(B, L, kv_heads * head_dim)`` keys and values at positions ``start[b] ..`` of each item.
@@ -144,11 +180,9 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     In 4 bits a value is within half its scale, a 15th of the largest of its 16
     channels (and up to an eighth more: a scale has four bits); magnitudes past 6720
     saturate, below 2^-18 they vanish, and 16 channels with one that is not finite are NaN."""
+    if isinstance(cache, KvCacheInt4):
+        return _append_int4(cache, k, v, table, start, counts)
     (pages, heads, page, dim), device = _check_cache(cache, "kv_append")
-    int4 = isinstance(cache, KvCacheInt4)
-    if int4 and device.index != _current_device():
-        with torch.cuda.device(device):
-            return kv_append(cache, k, v, table, start, counts=counts)
     if k.dtype not in _DT or v.dtype != k.dtype:
         raise ValueError("kv_append: k and v must share dtype float16, bfloat16 or float32")
     if k.ndim != 3 or v.shape != k.shape or k.shape[2] != heads * dim:
@@ -163,10 +197,34 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     _check_index(start, 1, batch, device, "kv_append: start")
     if counts is not None:
         _check_index(counts, 1, batch, device, "kv_append: counts")
-    _launcher("kv_append")("ldb_kv_append_int4" if int4 else "ldb_kv_append_fp8", _raw_stream(k.get_device()), k.data_ptr(), k_ld, k_batch,
+    _launcher("kv_append")("ldb_kv_append_fp8", _raw_stream(k.get_device()), k.data_ptr(), k_ld, k_batch,
             v.data_ptr(), v_ld, v_batch, _DT[k.dtype], cache.k.data_ptr(), cache.v.data_ptr(),
             cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pages, heads, page, dim, table.data_ptr(), table_ld,
             width, start.data_ptr(), None if counts is None else counts.data_ptr(), batch, tokens)
+
+
+def _append_int4(cache: KvCacheInt4, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
+                 counts: torch.Tensor | None) -> None:
+    fields, channels, index = _fields(cache, table, start, "kv_append", "start")
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return _append_int4(cache, k, v, table, start, counts)
+    dtype = _DT.get(k.dtype)
+    if dtype is None or v.dtype != k.dtype:
+        raise ValueError("kv_append: k and v must share dtype float16, bfloat16 or float32")
+    shape = k.shape
+    if len(shape) != 3 or v.shape != shape or shape[2] != channels or shape[0] != fields[-1]:
+        raise ValueError(f"kv_append: k and v must be ({fields[-1]}, L, {channels}), got {tuple(shape)} and {tuple(v.shape)}")
+    if k.get_device() != index or v.get_device() != index:
+        raise ValueError("kv_append: k and v must be on the cache's device")
+    (k_batch, k_ld, k_step), (v_batch, v_ld, v_step) = k.stride(), v.stride()
+    if k_step != 1 or v_step != 1:
+        raise ValueError("kv_append: channel axis must have unit stride")
+    if counts is not None:
+        _check_index(counts, 1, shape[0], k.device, "kv_append: counts")
+    _launcher("kv_append")("ldb_kv_append_int4", _raw_stream(index), _APPEND.pack(
+        _APPEND.size, dtype, *fields, k.data_ptr(), v.data_ptr(), k_ld, k_batch, v_ld, v_batch, start.data_ptr(),
+        0 if counts is None else counts.data_ptr(), shape[1]))
 
 
 def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, *, scale: float,
@@ -191,11 +249,9 @@ def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, lengths: 
     are rounded to 11 bits down to 2^-29 of the row's largest, from 49 rows on at
     least to 2^-21, and lost below 2^-40 and 2^-32.  Over 4 bits queries are exact (bfloat16
     down to 2^-31 of the row's largest) and the weights as over 8."""
+    if isinstance(cache, KvCacheInt4):
+        return _attention_int4(q, cache, table, lengths, scale, causal, out)
     (pages, kv_heads, page, dim), device = _check_cache(cache, "kv_attention")
-    int4 = isinstance(cache, KvCacheInt4)
-    if int4 and device.index != _current_device():
-        with torch.cuda.device(device):
-            return kv_attention(q, cache, table, lengths, scale=scale, causal=causal, out=out)
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"kv_attention: queries must be float16 or bfloat16, got {q.dtype}")
     if q.ndim != 3 or q.device != device or q.shape[2] % (kv_heads * dim) or q.shape[2] == 0:
@@ -214,17 +270,49 @@ def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, lengths: 
     out_batch, out_ld, _ = out.stride()
     heads = channels // dim
     index = q.get_device()
-    need = _workspace_bytes("ldb_kv_attention_int4_workspace_size" if int4 else
-                            "ldb_kv_attention_fp8_table_workspace_size", index, batch, queries, heads, kv_heads, dim,
+    need = _workspace_bytes("ldb_kv_attention_fp8_table_workspace_size", index, batch, queries, heads, kv_heads, dim,
                             width * page)
     ws_ptr = None
     if need:
         ws = q.new_empty(need, dtype=torch.uint8)
         ws_ptr = ws.data_ptr()
-    _launcher("kv_attention")("ldb_kv_attention_int4" if int4 else "ldb_kv_attention_fp8", _raw_stream(index), q.data_ptr(), q_ld, q_batch,
+    _launcher("kv_attention")("ldb_kv_attention_fp8", _raw_stream(index), q.data_ptr(), q_ld, q_batch,
             _DT[q.dtype], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
             pages, kv_heads, page, dim, table.data_ptr(), table_ld, width, lengths.data_ptr(), out.data_ptr(), out_ld,
             out_batch, batch, queries, heads, scale, int(causal), ws_ptr, need)
+    return out
+
+
+def _attention_int4(q: torch.Tensor, cache: KvCacheInt4, table: torch.Tensor, lengths: torch.Tensor, scale: float,
+                    causal: bool, out: torch.Tensor | None) -> torch.Tensor:
+    fields, row, index = _fields(cache, table, lengths, "kv_attention", "lengths")
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return _attention_int4(q, cache, table, lengths, scale, causal, out)
+    kv_heads, page, dim, width, batch = fields[-5:]
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"kv_attention: queries must be float16 or bfloat16, got {q.dtype}")
+    shape = q.shape
+    if len(shape) != 3 or q.get_device() != index or shape[2] % row or shape[2] == 0 or shape[0] != batch:
+        raise ValueError(f"kv_attention: queries must be ({batch}, L, n * {row}) on the cache's device, got {tuple(shape)}")
+    _, queries, channels = shape
+    q_batch, q_ld, q_step = q.stride()
+    if q_step != 1:
+        raise ValueError("kv_attention: channel axis must have unit stride")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out_ld, out_batch = channels, queries * channels
+    else:
+        if out.shape != shape or out.dtype != q.dtype or out.get_device() != index or out.stride(2) != 1:
+            raise ValueError("kv_attention: out must have q's shape, dtype and device, and unit channel stride")
+        out_batch, out_ld, _ = out.stride()
+    heads = channels // dim
+    need = _workspace_bytes("ldb_kv_attention_int4_workspace_size", index, batch, queries, heads, kv_heads, dim,
+                            width * page)
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
+    _launcher("kv_attention")("ldb_kv_attention_int4", _raw_stream(index), _ATTENTION.pack(
+        _ATTENTION.size, _DT[q.dtype], *fields, q.data_ptr(), out.data_ptr(), q_ld, q_batch, out_ld, out_batch,
+        lengths.data_ptr(), 0 if ws is None else ws.data_ptr(), need, queries, heads, int(causal), scale))
     return out
 
 
@@ -236,32 +324,31 @@ def kv_read(cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, *, token
     Rows at or behind ``lengths[b]`` are zeros.  float16, bfloat16 or float32:
     exact from a 4-bit cache, rounded once from 8 bits.  ``out`` takes a pair of tensors to
     write, of any row and item stride."""
-    (pages, heads, page, dim), device = _check_cache(cache, "kv_read")
-    if device.index != _current_device():
-        with torch.cuda.device(device):
+    fields, channels, index = _fields(cache, table, lengths, "kv_read", "lengths")
+    if index != _current_device():
+        with torch.cuda.device(index):
             return kv_read(cache, table, lengths, tokens=tokens, start=start, dtype=dtype, out=out)
-    if lengths.ndim != 1 or tokens < 0:
-        raise ValueError(f"kv_read: lengths must be one number per item and tokens at least 0, got {tokens}")
-    batch = lengths.shape[0]
-    width, table_ld = _check_table(table, batch, device, "kv_read: table")
-    _check_index(lengths, 1, batch, device, "kv_read: lengths")
+    if tokens < 0:
+        raise ValueError(f"kv_read: tokens must be at least 0, got {tokens}")
+    batch = fields[-1]
     if start is not None:
-        _check_index(start, 1, batch, device, "kv_read: start")
-    shape = (batch, tokens, heads * dim)
+        _check_index(start, 1, batch, lengths.device, "kv_read: start")
+    shape = (batch, tokens, channels)
     if out is None:
         if dtype not in _DT:
             raise ValueError(f"kv_read: dtype must be float16, bfloat16 or float32, got {dtype}")
-        out = (cache.k.new_empty(shape, dtype=dtype), cache.k.new_empty(shape, dtype=dtype))
-    k, v = out
-    if (k.shape != shape or v.shape != shape or k.dtype not in _DT or v.dtype != k.dtype or k.device != device
-            or v.device != device):
-        raise ValueError(f"kv_read: out must be two tensors {shape} of one float dtype on the cache's device")
-    (k_batch, k_ld, k_step), (v_batch, v_ld, v_step) = k.stride(), v.stride()
-    if k_step != 1 or v_step != 1:
-        raise ValueError("kv_read: channel axis must have unit stride")
-    _launcher("kv_read")("ldb_kv_read_int4" if isinstance(cache, KvCacheInt4) else "ldb_kv_read_fp8",
-            _raw_stream(device.index), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-            cache.v_scale.data_ptr(), pages, heads, page, dim, table.data_ptr(), table_ld, width, lengths.data_ptr(),
-            None if start is None else start.data_ptr(), k.data_ptr(), k_ld, k_batch, v.data_ptr(), v_ld, v_batch,
-            _DT[k.dtype], batch, tokens)
+        k, v = cache[0].new_empty(shape, dtype=dtype), cache[0].new_empty(shape, dtype=dtype)
+        k_batch = v_batch = tokens * channels
+        k_ld = v_ld = channels
+    else:
+        k, v = out
+        if (k.shape != shape or v.shape != shape or k.dtype not in _DT or v.dtype != k.dtype or k.get_device() != index
+                or v.get_device() != index):
+            raise ValueError(f"kv_read: out must be two tensors {shape} of one float dtype on the cache's device")
+        (k_batch, k_ld, k_step), (v_batch, v_ld, v_step) = k.stride(), v.stride()
+        if k_step != 1 or v_step != 1:
+            raise ValueError("kv_read: channel axis must have unit stride")
+    _launcher("kv_read")("ldb_kv_read_int4" if isinstance(cache, KvCacheInt4) else "ldb_kv_read_fp8", _raw_stream(index),
+            _READ.pack(_READ.size, _DT[k.dtype], *fields, k.data_ptr(), v.data_ptr(), k_ld, k_batch, v_ld, v_batch,
+                       lengths.data_ptr(), 0 if start is None else start.data_ptr(), tokens))
     return k, v

@@ -20,6 +20,7 @@ from typing import NamedTuple, Sequence
 
 import torch
 
+from . import _lib
 from .fp8 import _check_input, _launcher, _raw_stream
 from .ops import _DT
 
@@ -69,21 +70,25 @@ def grid_positions(*sizes: int, device: torch.device | str = "cuda") -> torch.Te
     return torch.stack(torch.meshgrid(*lines, indexing="ij"), -1).reshape(1, -1, len(sizes))
 
 
+_DESC = _lib.DESCRIPTORS["ldb_qk_norm_rope_desc"]
+
+
 def _check_rows(t: torch.Tensor, like: torch.Tensor, head_dim: int, name: str) -> tuple[int, int, int]:
-    """(heads, row stride, item stride)."""
-    if t.ndim != 3 or t.dtype != like.dtype or t.device != like.device or t.shape[:2] != like.shape[:2]:
+    """(channels, row stride, item stride)."""
+    shape, (batch, ld, step) = t.shape, t.stride() if t.ndim == 3 else (0, 0, 0)
+    if len(shape) != 3 or t.dtype != like.dtype or t.get_device() != like.get_device() or shape[:2] != like.shape[:2]:
         raise ValueError(f"qk_norm_rope: {name} must be (B, L, n * {head_dim}) of q's dtype, device, B and L")
-    batch, ld, step = t.stride()
-    if t.shape[2] % head_dim or (step != 1 and t.shape[2] > 1):
+    channels = shape[2]
+    if channels % head_dim or (step != 1 and channels > 1):
         raise ValueError(f"qk_norm_rope: {name} must hold heads of {head_dim} channels with unit stride")
-    return t.shape[2] // head_dim, ld, batch
+    return channels, ld, batch
 
 
-def _check_gamma(gamma: torch.Tensor | None, like: torch.Tensor, head_dim: int, name: str) -> int | None:
+def _check_gamma(gamma: torch.Tensor | None, like: torch.Tensor, head_dim: int, name: str) -> int:
     if gamma is None:
-        return None
+        return 0
     if (gamma.dtype != torch.float32 or gamma.shape != (head_dim,) or not gamma.is_contiguous()
-            or gamma.device != like.device):
+            or gamma.get_device() != like.get_device()):
         raise ValueError(f"qk_norm_rope: {name} must be contiguous float32 ({head_dim},) on q's device")
     return gamma.data_ptr()
 
@@ -102,57 +107,61 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, *, head_dim: int, q_ga
     head; pairs that are not interleaved come in eights.  float16, bfloat16 or float32, any row
     and item stride; ``k`` may be None, and ``q_out`` / ``k_out`` may be ``q`` / ``k``."""
     _check_input(q, "qk_norm_rope: q")
-    if q.get_device() != _current_device():
-        with torch.cuda.device(q.device):
+    index = q.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
             return qk_norm_rope(q, k, head_dim=head_dim, q_gamma=q_gamma, k_gamma=k_gamma, eps=eps, norm=norm,
                                 rotary=rotary, positions=positions, q_out=q_out, k_out=k_out)
     if head_dim < 16 or head_dim > 256 or head_dim % 16:
         raise ValueError(f"qk_norm_rope: heads have a multiple of 16 channels up to 256, got {head_dim}")
-    heads, q_ld, q_batch = _check_rows(q, q, head_dim, "q")
+    channels, q_ld, q_batch = _check_rows(q, q, head_dim, "q")
     batch, tokens, _ = q.shape
-    kv_heads = k_ld = k_batch = ko_ld = ko_batch = 0
-    k_ptr = ko_ptr = None
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif q_out.shape != q.shape:
-        raise ValueError("qk_norm_rope: q_out must have q's shape")
-    _, qo_ld, qo_batch = _check_rows(q_out, q, head_dim, "q_out")
+        qo_ld, qo_batch = channels, tokens * channels
+    else:
+        if q_out.shape != q.shape:
+            raise ValueError("qk_norm_rope: q_out must have q's shape")
+        _, qo_ld, qo_batch = _check_rows(q_out, q, head_dim, "q_out")
+    k_ptr = ko_ptr = k_channels = k_ld = k_batch = ko_ld = ko_batch = 0
     if k is not None:
-        kv_heads, k_ld, k_batch = _check_rows(k, q, head_dim, "k")
+        k_channels, k_ld, k_batch = _check_rows(k, q, head_dim, "k")
         if k_out is None:
             k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-        elif k_out.shape != k.shape:
-            raise ValueError("qk_norm_rope: k_out must have k's shape")
-        _, ko_ld, ko_batch = _check_rows(k_out, q, head_dim, "k_out")
+            ko_ld, ko_batch = k_channels, tokens * k_channels
+        else:
+            if k_out.shape != k.shape:
+                raise ValueError("qk_norm_rope: k_out must have k's shape")
+            _, ko_ld, ko_batch = _check_rows(k_out, q, head_dim, "k_out")
         k_ptr, ko_ptr = k.data_ptr(), k_out.data_ptr()
     elif k_out is not None:
         raise ValueError("qk_norm_rope: k_out without k")
-    turns_ptr = axis_ptr = at_ptr = None
-    pairs = axes = at_ld = at_batch = interleaved = 0
+    turns_ptr = axis_ptr = at_ptr = pairs = axes = at_ld = at_batch = interleaved = 0
     if rotary is not None:
         turns, axis, axes, interleaved = rotary
         pairs = turns.numel()
-        if (turns.dtype != torch.int64 or axis.dtype != torch.int32 or turns.ndim != 1 or axis.shape != turns.shape
-                or not turns.is_contiguous() or not axis.is_contiguous() or turns.device != q.device
-                or axis.device != q.device):
+        if (turns.dtype != torch.int64 or axis.dtype != torch.int32 or turns.ndim != 1 or axis.ndim != 1
+                or axis.numel() != pairs or not turns.is_contiguous() or not axis.is_contiguous()
+                or turns.get_device() != index or axis.get_device() != index):
             raise ValueError("qk_norm_rope: a plan is int64 turns and int32 axes of its pairs, on q's device")
         if 2 * pairs > head_dim or (not interleaved and pairs % 8):
             raise ValueError(f"qk_norm_rope: {pairs} pairs in heads of {head_dim} channels (in eights, where not interleaved)")
-        if positions is None or positions.dtype != torch.int32 or positions.device != q.device:
+        if positions is None or positions.dtype != torch.int32 or positions.get_device() != index:
             raise ValueError("qk_norm_rope: positions must be int32 on q's device")
-        if positions.ndim == 2 and axes == 1:
-            positions = positions[..., None]
-        if (positions.ndim != 3 or positions.shape[0] not in (1, batch) or positions.shape[1:] != (tokens, axes)
-                or (axes > 1 and positions.stride(2) != 1)):
+        at, step = positions.shape, positions.stride()
+        if len(at) == 2 and axes == 1:
+            at, step = (*at, 1), (*step, 1)
+        if (len(at) != 3 or at[0] not in (1, batch) or at[1] != tokens or at[2] != axes
+                or (axes > 1 and step[2] != 1)):
             raise ValueError(f"qk_norm_rope: positions must be ({batch} or 1, {tokens}, {axes}), got "
                              f"{tuple(positions.shape)}")
-        at_ld, at_batch = positions.stride(1), positions.stride(0) if positions.shape[0] > 1 else 0
+        at_ld, at_batch = step[1], step[0] if at[0] > 1 else 0
         turns_ptr, axis_ptr, at_ptr = turns.data_ptr(), axis.data_ptr(), positions.data_ptr()
     elif positions is not None:
         raise ValueError("qk_norm_rope: positions without a plan")
-    _launcher("qk_norm_rope")("ldb_qk_norm_rope", _raw_stream(q.get_device()), q.data_ptr(), q_ld, q_batch, k_ptr, k_ld,
-            k_batch, _DT[q.dtype], _check_gamma(q_gamma, q, head_dim, "q_gamma"),
-            _check_gamma(k_gamma, q, head_dim, "k_gamma"), eps, int(norm), turns_ptr, axis_ptr, pairs, axes,
-            int(interleaved), at_ptr, at_ld, at_batch, q_out.data_ptr(), qo_ld, qo_batch, ko_ptr, ko_ld, ko_batch, batch,
-            tokens, heads, kv_heads, head_dim)
+    _launcher("qk_norm_rope")("ldb_qk_norm_rope", _raw_stream(index), _DESC.pack(
+        _DESC.size, _DT[q.dtype], q.data_ptr(), k_ptr, q_out.data_ptr(), ko_ptr, q_ld, q_batch, k_ld, k_batch, qo_ld,
+        qo_batch, ko_ld, ko_batch, _check_gamma(q_gamma, q, head_dim, "q_gamma"),
+        _check_gamma(k_gamma, q, head_dim, "k_gamma"), turns_ptr, axis_ptr, at_ptr, at_ld, at_batch, batch, tokens,
+        channels // head_dim, k_channels // head_dim, head_dim, pairs, axes, int(interleaved), int(norm), eps))
     return q_out, k_out

@@ -11,51 +11,66 @@ from lesiondiffusion_mlx_b200 import _lib, kv_cache
 from oracle import kv_int4 as oracle
 
 
-def code(name, args):
-    with pytest.raises(_lib.LdbError) as e:
-        _lib.call(name, None, *args)
-    return e.value.code
+P, ODD = 4096, 4104
+CACHE = dict(k_codes=P, v_codes=P, k_scales=P, v_scales=P, table=P, table_ld=4, pages=4, kv_heads=2, page=64, head_dim=32,
+             width=4, batch=1)
 
 
-def test_library_refuses_bad_caches():
-    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4104)
-    append = [p, 64, 64, p, 64, 64, 0, p, p, p, p, 4, 2, 64, 32, p, 4, 4, p, None, 1, 3]
-    for at, value, want in ((0, None, -1), (6, 9, -1), (7, None, -1), (18, None, -1), (14, 48, -2), (13, 8, -2),
-                            (11, 0, -2), (16, 3, -2), (1, 63, -2), (8, odd, -3), (10, odd, -3), (21, -1, -2),
-                            (20, 70000, -2)):
-        bad = list(append)
-        bad[at] = value
-        assert code("ldb_kv_append_int4", bad) == want, (at, value)
-    read = [p, p, p, p, 4, 2, 64, 32, p, 4, 4, p, None, p, 64, 192, p, 64, 192, 0, 2, 3]
-    for at, value, want in ((0, None, -1), (2, None, -1), (8, None, -1), (11, None, -1), (13, None, -1), (16, None, -1),
-                            (19, 5, -1), (7, 16, -2), (6, 8, -2), (4, 0, -2), (9, 3, -2), (14, 63, -2), (15, 63, -2),
-                            (18, 0, -2), (0, odd, -3), (20, -1, -2), (20, 70000, -2), (21, -1, -2)):
-        bad = list(read)
-        bad[at] = value
-        for name in ("ldb_kv_read_int4", "ldb_kv_read_fp8"):
-            assert code(name, bad) == want, (name, at, value)
-    assert code("ldb_kv_read_int4", [*read[:2], odd, *read[3:]]) == -3
-    attend = [p, 128, 128, 0, p, p, p, p, 4, 2, 64, 32, p, 4, 4, p, p, 128, 128, 1, 3, 4, 1.0, 0, p, 1 << 40]
-    for at, value, want in ((0, None, -1), (3, _lib.LDB_F32, -1), (4, None, -1), (16, None, -1), (21, 5, -2), (11, 96, -2),
-                            (10, 24, -2), (8, 0, -2), (13, 3, -2), (1, 127, -2), (17, 127, -2), (5, odd, -3), (6, odd, -3),
-                            (19, 2049, -2), (24, None, -4), (25, 16, -4), (24, odd, -4), (8, 1 << 30, -2)):
-        bad = list(attend)
-        bad[at] = value
-        assert code("ldb_kv_attention_int4", bad) == want, (at, value)
+def descriptors():
+    """A good call of each operator, by field in the descriptor's order."""
+    size = {n: _lib.DESCRIPTORS[f"ldb_kv_{n}_desc"].size for n in ("append", "read", "attention")}
+    rows = dict(k_ld=64, k_batch=192, v_ld=64, v_batch=192)
+    return {"append": dict(size=size["append"], dtype=0) | CACHE | dict(k=P, v=P) | rows | dict(start=P, counts=0, tokens=3),
+            "read": dict(size=size["read"], dtype=0) | CACHE | dict(k=P, v=P) | rows | dict(lengths=P, start=0, tokens=3),
+            "attention": dict(size=size["attention"], dtype=0) | CACHE | dict(
+                q=P, out=P, q_ld=128, q_batch=384, out_ld=128, out_batch=384, lengths=P, workspace=P,
+                workspace_bytes=1 << 40, queries=3, heads=4, causal=0, scale=1.0)}
+
+
+def call(name, fields, bits="int4"):
+    _lib.call(f"ldb_kv_{name}_{bits}", None, _lib.DESCRIPTORS[f"ldb_kv_{name}_desc"].pack(*fields.values()))
+
+
+SHARED = (("k_codes", 0, -1), ("v_scales", 0, -1), ("table", 0, -1), ("page", 48, -2), ("page", 8, -2), ("head_dim", 24, -2),
+          ("pages", 0, -2), ("table_ld", 3, -2), ("width", 0, -2), ("k_codes", ODD, -3), ("batch", -1, -2), ("dtype", 9, -1),
+          ("size", 8, -1))
+
+
+@pytest.mark.parametrize("name,bits,cases", [
+    ("append", "int4", (("k", 0, -1), ("start", 0, -1), ("k_ld", 63, -2), ("k_scales", ODD, -3), ("tokens", -1, -2),
+                        ("batch", 70000, -2))),
+    ("read", "int4", (("v", 0, -1), ("lengths", 0, -1), ("k_ld", 63, -2), ("v_ld", 63, -2), ("tokens", -1, -2),
+                      ("batch", 70000, -2), ("v_scales", ODD, -3))),
+    ("read", "fp8", (("v", 0, -1), ("lengths", 0, -1), ("k_ld", 63, -2), ("tokens", -1, -2))),
+    ("attention", "int4", (("q", 0, -1), ("dtype", _lib.LDB_F32, -1), ("lengths", 0, -1), ("out", 0, -1), ("heads", 5, -2),
+                           ("q_ld", 127, -2), ("out_ld", 127, -2), ("v_scales", ODD, -3), ("batch", 2049, -2),
+                           ("workspace", 0, -4), ("workspace_bytes", 16, -4), ("workspace", ODD, -4), ("pages", 1 << 30, -2),
+                           ("queries", -1, -2), ("kv_heads", 0, -2)))])
+def test_library_refuses_bad_calls(name, bits, cases):
+    good = descriptors()[name]
+    for field, value, want in SHARED + cases:
+        with pytest.raises(_lib.LdbError) as e:
+            call(name, good | {field: value}, bits)
+        assert e.value.code == want, (field, value)
+    with pytest.raises(_lib.LdbError, match="null"):
+        _lib.call(f"ldb_kv_{name}_{bits}", None, None)
+
+
+def test_item_strides_of_what_is_written():
+    good = descriptors()
+    for name, field in (("read", "v_batch"), ("attention", "out_batch")):
+        with pytest.raises(_lib.LdbError, match="item stride"):
+            call(name, good[name] | {"batch": 2, field: 0})
     need = ctypes.c_size_t(0)
     with pytest.raises(_lib.LdbError, match="heads"):
         _lib.call("ldb_kv_attention_int4_workspace_size", 1, 1, 3, 2, 64, 100, ctypes.byref(need))
 
 
 def test_empty_calls_launch_nothing():
-    before = _lib.launch_count()
-    _lib.call("ldb_kv_append_int4", None, None, 0, 0, None, 0, 0, 0, None, None, None, None, 4, 2, 64, 32, None, 4, 4,
-              None, None, 0, 3)
-    for batch, tokens in ((0, 3), (2, 0)):
-        _lib.call("ldb_kv_read_int4", None, None, None, None, None, 4, 2, 64, 32, None, 4, 4, None, None, None, 0, 0, None,
-                  0, 0, 0, batch, tokens)
-    _lib.call("ldb_kv_attention_int4", None, None, 0, 0, 0, None, None, None, None, 4, 2, 64, 32, None, 4, 4, None, None,
-              0, 0, 0, 3, 4, 1.0, 0, None, 0)
+    before, good = _lib.launch_count(), descriptors()
+    for name, field in (("append", "batch"), ("append", "tokens"), ("read", "batch"), ("read", "tokens"),
+                        ("attention", "batch"), ("attention", "queries")):
+        call(name, good[name] | {field: 0})
     assert _lib.launch_count() == before
 
 

@@ -2,7 +2,6 @@
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import pytest
@@ -40,20 +39,26 @@ def test_grid_positions_count_in_memory_order():
 
 
 def test_library_refuses_bad_calls():
-    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4104)
-    good = [p, 256, 1024, p, 128, 512, 0, p, p, 1e-6, 1, p, p, 32, 1, 0, p, 1, 4, p, 256, 1024, p, 128, 512, 2, 4, 4, 2, 64]
-    for at, value, want in ((0, None, -1), (3, None, -1), (6, 7, -1), (11, None, -1), (12, None, -1), (16, None, -1),
-                            (19, None, -1), (22, None, -1), (29, 72, -2), (29, 272, -2), (29, 0, -2), (13, 33, -2),
-                            (13, 12, -2), (13, -1, -2), (14, 0, -2), (1, 255, -2), (20, 255, -2), (21, 255, -2),
-                            (4, 127, -2), (25, -1, -2), (26, -1, -2), (27, -4, -2), (7, odd, -3), (8, odd, -3)):
-        bad = list(good)
-        bad[at] = value
+    p, odd = 4096, 4104
+    fields = ("size", "dtype", "q", "k", "q_out", "k_out", "q_ld", "q_batch", "k_ld", "k_batch", "q_out_ld", "q_out_batch",
+              "k_out_ld", "k_out_batch", "q_gamma", "k_gamma", "turns", "axis", "positions", "positions_ld",
+              "positions_batch", "batch", "tokens", "heads", "kv_heads", "head_dim", "pairs", "axes", "interleaved", "norm",
+              "eps")
+    desc = _lib.DESCRIPTORS["ldb_qk_norm_rope_desc"]
+    good = dict(zip(fields, (desc.size, 0, p, p, p, p, 256, 1024, 128, 512, 256, 1024, 128, 512, p, p, p, p, p, 1, 4, 2, 4,
+                             4, 2, 64, 32, 1, 0, 1, 1e-6)))
+    for name, value, want in (("q", 0, -1), ("k", 0, -1), ("dtype", 7, -1), ("turns", 0, -1), ("axis", 0, -1),
+                              ("positions", 0, -1), ("q_out", 0, -1), ("k_out", 0, -1), ("size", desc.size - 8, -1),
+                              ("head_dim", 72, -2), ("head_dim", 272, -2), ("head_dim", 0, -2), ("pairs", 33, -2),
+                              ("pairs", 12, -2), ("pairs", -1, -2), ("axes", 0, -2), ("q_ld", 255, -2),
+                              ("q_out_ld", 255, -2), ("q_out_batch", 255, -2), ("k_ld", 127, -2), ("batch", -1, -2),
+                              ("tokens", -1, -2), ("heads", -4, -2), ("q_gamma", odd, -3), ("k_gamma", odd, -3)):
         with pytest.raises(_lib.LdbError) as e:
-            _lib.call("ldb_qk_norm_rope", None, *bad)
-        assert e.value.code == want, (at, value)
+            _lib.call("ldb_qk_norm_rope", None, desc.pack(*(good | {name: value}).values()))
+        assert e.value.code == want, (name, value)
+    with pytest.raises(_lib.LdbError, match="null"):
+        _lib.call("ldb_qk_norm_rope", None, None)
     before = _lib.launch_count()
-    for at in (25, 26):
-        empty = list(good)
-        empty[at] = 0
-        _lib.call("ldb_qk_norm_rope", None, *empty)
+    for name in ("batch", "tokens"):
+        _lib.call("ldb_qk_norm_rope", None, desc.pack(*(good | {name: 0}).values()))
     assert _lib.launch_count() == before
