@@ -9,11 +9,15 @@
 // 64-bit fraction of a turn, so position times turns_i modulo 2^64 is exact integer
 // arithmetic, and its upper 32 bits are the angle to 2^-32 of a turn at any position.
 //
-// A warp takes a token: its P sines and cosines are computed once, a pair per
-// lane, and kept in shared memory for all heads; eight channels per lane, as
-// many heads at a time as fit.
+// A warp takes a token, or a few with few heads: the P sines and cosines of each are
+// computed once, a pair per lane, and kept in shared memory for all heads.
+// Eight channels per lane, as many heads at a time as fit; what a channel becomes is
+// f (x own + other times) with its head's norm f, so that sine, cosine and gamma are
+// two factors for all heads.
 //
-// Bound: HBM, each value read and written once; for few tokens the launch.
+// Bound: HBM, each value read and written once; for few tokens the launch.  One B200: 4 x 4097
+// tokens of 32 + 8 heads of 128 bf16 66 us (5.1 TB/s), 6400 tokens of 4 + 4 heads of 64 7 us (the chain
+// of dependent reads, sines and values), one token of 32 items 3.9 us.
 
 #include <algorithm>
 #include <type_traits>
@@ -38,7 +42,9 @@ struct RopeParams {
   int tokens, dim, pairs, axes, interleaved, norm, vec;
   int rounds[2], per_warp[2];  // of heads of a token, of a warp: as many heads as fit at a time
   unsigned splits;             // warps of a token
-  unsigned warps;
+  int token_shift;            // tokens of a warp, as a power of two
+  unsigned pairs_inverse;     // 2^16 / pairs, rounded up
+  unsigned warps, rows;
   float eps, inv_dim;
 };
 
@@ -69,25 +75,31 @@ struct Raw {
 // LANES per head, of eight channels each (the last ones idle where D is not 8 LANES).
 template <typename T, int LANES, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p, unsigned int* status) {
-  __shared__ __align__(16) float2 s_turn[kWarps][kMaxPairs + 8];  // (cos, sin), and eight of no turn
+  __shared__ __align__(16) float2 s_turn[kWarps][kMaxPairs];  // (cos, sin)
   pdl_begin();
   const int lane = lane_id();
   const unsigned w = blockIdx.x * kWarps + warp_id();
   if (w >= p.warps) return;
-  const unsigned row = w / p.splits;
-  const int split = static_cast<int>(w - row * p.splits);
+  constexpr int kHeads = 32 / LANES;  // at a time, p.at_once of each of the warp's tokens
+  const int sub = lane / LANES, c0 = (lane % LANES) * 8;
+  const unsigned row0 = w / p.splits << p.token_shift;  // the warp's first token
+  const int split = static_cast<int>(w % p.splits);
+  const int at_once = kHeads >> p.token_shift, mine = sub & (at_once - 1), nth = sub / at_once;
+  const unsigned row = min(row0 + nth, p.rows - 1);
   const long long b = row / static_cast<unsigned>(p.tokens);
   const long long token = row - static_cast<unsigned>(b) * p.tokens;
-  constexpr int kHeads = 32 / LANES;  // at a time
-  const int sub = lane / LANES, c0 = (lane % LANES) * 8;
-  const bool live = c0 < p.dim;
+  const bool live = c0 < p.dim && row0 + nth < p.rows;
   const int turned_to = 2 * p.pairs - c0;  // the lane's channels below this one turn (all or none, in halves)
   const bool upper = !INTERLEAVED && c0 >= p.pairs;
   const int away = INTERLEAVED || turned_to <= 0 ? 0 : (upper ? -p.pairs : p.pairs);  // of the other members of its pairs
   const int partner = lane + away / 8;
   float2* turn = s_turn[warp_id()];
-  const int* position = p.positions + b * p.pos_batch + token * p.pos_ld;
-  for (int i = lane; i < p.pairs; i += 32) {
+  const long long at = b * p.pos_batch + token * p.pos_ld;  // of the lane's token's positions
+  const int all = p.pairs << p.token_shift;
+  for (int n0 = 0; n0 < all; n0 += 32) {
+    const int n = min(n0 + lane, all - 1);
+    const int of = static_cast<int>(n * p.pairs_inverse >> 16), i = n - of * p.pairs;  // n / pairs
+    const int* position = p.positions + __shfl_sync(0xffffffffu, at, of * at_once * LANES);
     int axis = p.axis[i];
     if (axis < 0 || axis >= p.axes) {
       set_bad_shape(status);
@@ -96,9 +108,9 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p, unsi
     const unsigned long long phase = p.turns[i] * static_cast<unsigned long long>(static_cast<long long>(position[axis]));
     float2 cs;
     sincospif(static_cast<float>(static_cast<int>(phase >> 32)) * 0x1p-31f, &cs.y, &cs.x);
-    turn[i] = cs;
+    turn[n] = cs;
   }
-  if (lane < 8) turn[p.pairs + lane] = make_float2(1.f, 0.f);
+  turn += nth * p.pairs;
   __syncwarp();
 
 #pragma unroll 1
@@ -114,16 +126,17 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p, unsi
         load8<float>(p.gamma[which] + c0, g);
         load8<float>(p.gamma[which] + c0 + away, mate);
       }
-      // the lane's turns: from the first of its pairs, or of no turn
-      const float2* t = turn + (turned_to <= 0 ? p.pairs : (INTERLEAVED ? c0 / 2 : (upper ? c0 - p.pairs : c0)));
+      // the lane's turns, from the first of its pairs
+      const float2* t = turn + (INTERLEAVED ? c0 / 2 : (upper ? c0 - p.pairs : c0));
+      const float2 none = make_float2(1.f, 0.f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (INTERLEAVED) {
-          const float2 cs = t[k];  // (behind the last pair: no turn)
+          const float2 cs = 2 * k < turned_to ? t[k] : none;
           own[k] = pack2(cs.x * g[2 * k], cs.x * g[2 * k + 1]);
           times[k] = pack2(-cs.y * g[2 * k + 1], cs.y * g[2 * k]);
         } else {
-          const float2 c = t[2 * k], d = t[2 * k + 1];
+          const float2 c = turned_to > 0 ? t[2 * k] : none, d = turned_to > 0 ? t[2 * k + 1] : none;
           own[k] = pack2(c.x * g[2 * k], d.x * g[2 * k + 1]);
           const float s0 = c.y * mate[2 * k], s1 = d.y * mate[2 * k + 1];
           times[k] = upper ? pack2(s0, s1) : pack2(-s0, -s1);
@@ -193,10 +206,10 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p, unsi
     for (; r < to; r += kAhead) {
       Raw<T> raw[kAhead];
 #pragma unroll
-      for (int n = 0; n < kAhead; ++n) load(r + n < to ? (r + n) * kHeads + sub : 0x7FFFFFFF, raw[n]);
+      for (int n = 0; n < kAhead; ++n) load(r + n < to ? (r + n) * at_once + mine : 0x7FFFFFFF, raw[n]);
 #pragma unroll
       for (int n = 0; n < kAhead; ++n)
-        if (r + n < to) finish((r + n) * kHeads + sub, raw[n]);
+        if (r + n < to) finish((r + n) * at_once + mine, raw[n]);
     }
   }
 }
@@ -204,21 +217,26 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p, unsi
 template <typename T>
 int launch_rope(cudaStream_t stream, RopeParams& p, long long rows, unsigned int* status) {
   const int lanes = p.dim <= 16 ? 2 : (p.dim <= 32 ? 4 : (p.dim <= 64 ? 8 : (p.dim <= 128 ? 16 : 32)));
-  const int at_a_time = 32 / lanes;
-  int most = 0;
-  for (int i = 0; i < 2; ++i) {
-    p.rounds[i] = (p.heads[i] + at_a_time - 1) / at_a_time;
-    most = std::max(most, p.rounds[i]);
-  }
-  // A warp per round while all of them are resident at once, else rounds enough to share the sines.
+  if (rows > 0x7FFFFF00ll) return fail(LDB_ERR_SHAPE, "qk_norm_rope: %lld tokens", rows);
   const long long resident = 32ll * sm_count();
-  int splits = most;
-  while (splits > 1 && rows * splits > resident) splits = (splits + 1) / 2;
-  if (splits > 1 && rows * splits > resident) splits = 1;
+  // Tokens of a warp: as many as its lanes have room for (few heads of few channels leave most idle) while
+  // there are tokens enough (183414 tokens of 3 + 3 heads of 32: one a warp 168 us, two 39).
+  auto rounds_of = [&](int shift, int i) { const int n = 32 / lanes >> shift; return (p.heads[i] + n - 1) / n; };
+  p.token_shift = 0;
+  for (int shift = 1; (32 / lanes >> shift) > 0 && (p.pairs << shift) <= kMaxPairs && (rows >> shift) >= resident; ++shift)
+    if (rounds_of(shift, 0) + rounds_of(shift, 1) < (rounds_of(p.token_shift, 0) + rounds_of(p.token_shift, 1))
+                                                        << (shift - p.token_shift))
+      p.token_shift = shift;
+  for (int i = 0; i < 2; ++i) p.rounds[i] = rounds_of(p.token_shift, i);
+  const long long groups = (rows + (1 << p.token_shift) - 1) >> p.token_shift;  // of tokens that share a warp
+  // A warp per round while all of them are resident at once, else all rounds of a token to share its sines.
+  int splits = std::max(p.rounds[0], p.rounds[1]);
+  while (splits > 1 && groups * splits > resident) splits = (splits + 1) / 2 < splits ? (splits + 1) / 2 : 1;
   p.splits = splits;
   for (int i = 0; i < 2; ++i) p.per_warp[i] = (p.rounds[i] + splits - 1) / splits;
-  if (rows * p.splits > 0x7FFFFF00ll) return fail(LDB_ERR_SHAPE, "qk_norm_rope: %lld tokens of %d heads", rows, p.heads[0]);
-  p.warps = static_cast<unsigned>(rows * p.splits);
+  p.rows = static_cast<unsigned>(rows);
+  p.pairs_inverse = (65535u + std::max(p.pairs, 1)) / std::max(p.pairs, 1);
+  p.warps = static_cast<unsigned>(groups * splits);
   const unsigned blocks = (p.warps + kWarps - 1) / kWarps;
   auto pick = [&](auto interleaved) {
     constexpr bool I = decltype(interleaved)::value;

@@ -46,7 +46,8 @@ def frequencies(dims, base=10000.0):
     (1, 1, 1, 1, 64, (64,), False), (2, 5, 4, 2, 128, (128,), True), (3, 7, 3, 1, 80, (48,), False),
     (1, 33, 5, 5, 32, (8, 4, 4), True), (2, 9, 2, 2, 64, (16, 24, 24), False), (1, 4, 1, 0, 16, (16,), False),
     (1, 3, 9, 3, 256, (256,), False), (2, 3, 1, 2, 96, (10,), True), (1, 2, 7, 2, 112, (32, 0, 64), False),
-    (1, 2, 2, 1, 48, (48,), True), (1, 700, 32, 8, 128, (64,), False), (40, 1, 16, 4, 128, (128,), False)])
+    (1, 10007, 3, 3, 32, (16,), False), (2, 9001, 1, 1, 64, (64,), True), (7, 3001, 1, 2, 16, (10,), True),
+    (3, 6500, 2, 0, 48, (16,), False), (1, 2, 2, 1, 48, (48,), True), (1, 700, 32, 8, 128, (64,), False), (40, 1, 16, 4, 128, (128,), False)])
 def test_against_the_definition(cuda_device, dtype, batch, tokens, heads, kv_heads, dim, dims, interleaved):
     q, k, q_gamma, k_gamma = inputs(batch, tokens, heads, max(kv_heads, 1), dim, dtype)
     g = torch.Generator().manual_seed(2)
