@@ -11,8 +11,8 @@
 // reference, which may lag 2^8 behind its maximum: 11 bits down to 2^-21 of the
 // reference, nothing below 2^-32.
 //
-// Warps: 0 issues the products, 4-7 unpack, 8-11 and 12-15 run the online softmax of
-// tile 0 and 1, one row per thread.  Grids that leave SMs idle cut the tokens into ranges, merged
+// Warps: 0 issues the products, 1-7 unpack, 8-15 and 16-23 run the online softmax of
+// tile 0 and 1, half a row a thread.  Grids that leave SMs idle cut the tokens into ranges, merged
 // by a second kernel (kv_attention_tiles.cuh).
 //
 // Bound: 4 D flops and one exponential per score.
@@ -28,11 +28,8 @@
 namespace ldb {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kRegsWg0 = 48;      // products
-constexpr int kRegsUnpack = 80;
-constexpr int kRegsSoftmax = 192; // a row's 128 scores
-static_assert(128 * (kRegsWg0 + kRegsUnpack + 2 * kRegsSoftmax) <= kThreads * 128, "register split");
+constexpr int kThreads = 768;     // of 80 registers: a row's scores are shared by two threads
+constexpr int kUnpackWarps = 7;
 constexpr int kMeta = 4;          // ring of the masks of missing pages
 
 template <int D>
@@ -46,8 +43,10 @@ struct Cfg {
   static constexpr int kOffV = kOffK + 2 * kTileBytes;
   static constexpr int kOffMeta = kOffV + 2 * kTileBytes;  // [kMeta][4] bytes: a bit for each 16 tokens of a missing page
   static constexpr int kOffBad = kOffMeta + kMeta * 4;     // NaN met among values that not every row sees
-  static constexpr int kOffBar = kOffBad + 16;
-  static constexpr int kSmem = 1024 + kOffBar + 256;
+  static constexpr int kOffVote = kOffBad + 16;            // [8 pairs of warps][2][half]: a reference has to grow
+  static constexpr int kOffRow = kOffVote + 128;           // [tile][half][kM] floats that a row's two threads exchange
+  static constexpr int kOffBar = kOffRow + 4 * kM * 4;
+  static constexpr int kSmem = 1024 + kOffBar + 320;
   // TMEM: S_t at 128 t, O_t at 256 + 128 t.  D = 128: the weights overwrite
   // their scores; narrower heads have room for them behind O_t, so that the next block's
   // scores need not wait for the value product.
@@ -72,11 +71,38 @@ __device__ __forceinline__ void umma_ss_warp(uint32_t d_tmem, uint64_t a_desc, u
       : "memory");
 }
 
+// A score of minus infinity where `at` >= `seen`, or where a bit of `mask` is set.  Volatile with the
+// comparison inside, so that blocks without hidden keys branch around them.
+__device__ __forceinline__ void hide_from(uint32_t& score, int at, int seen) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ge.s32 p, %1, %2;\n\t@p mov.b32 %0, 0xFF800000;\n\t}\n"
+               : "+r"(score)
+               : "r"(at), "r"(seen));
+}
+__device__ __forceinline__ void hide_if(uint32_t& score, uint32_t mask, uint32_t bit) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 m;\n\tand.b32 m, %1, %2;\n\tsetp.ne.u32 p, m, 0;\n\t"
+      "@p mov.b32 %0, 0xFF800000;\n\t}\n"
+      : "+r"(score)
+      : "r"(mask), "r"(bit));
+}
+
+// Wait for the loads from TMEM; what uses these registers comes after.
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
 // A token's codes and scales of keys or of values.
 template <int D>
 struct Packed {
   uint4 code[D / 32];
-  uint32_t scale[(D / kInt4Group + 3) / 4];
+  uint32_t scale[D / kInt4Group];  // (a byte each: put together they would be waited for where they are loaded)
 };
 
 template <int D, typename T>
@@ -98,10 +124,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
   uint64_t* s_free = s_full + 2;        // [2] scores are in registers
   uint64_t* p_ready = s_free + 2;       // [2] weights are in TMEM
   uint64_t* pv_done = p_ready + 2;      // [2]
-  uint64_t* drain = pv_done + 2;
+  uint64_t* pair_bar = pv_done + 2;     // [8] the two warps of 32 rows meet
+  uint64_t* drain = pair_bar + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((1 + 8 + kMeta + 8 + 1) * 8 + 8 <= 256, "barrier block");
+  static_assert((1 + 8 + kMeta + 8 + 8 + 1) * 8 + 8 <= 320, "barrier block");
 
   const int warp = warp_id(), lane = lane_id();
   if (threadIdx.x == 0) {
@@ -112,12 +139,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
       mbar_init(&v_full[s], 4);
       mbar_init(&v_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&s_free[s], 4);
-      mbar_init(&p_ready[s], 4);
+      mbar_init(&s_free[s], 8);
+      mbar_init(&p_ready[s], 8);
       mbar_init(&pv_done[s], 1);
     }
     for (int s = 0; s < kMeta; ++s) mbar_init(&meta_full[s], 4);
-    mbar_init(q_full, p.rows - (p.row_blocks - 1 - static_cast<int>(blockIdx.x) / p.splits) * 2 * kM > kM ? 8 : 4);
+    for (int s = 0; s < 8; ++s) mbar_init(&pair_bar[s], 2);
+    mbar_init(q_full, p.rows - (p.row_blocks - 1 - static_cast<int>(blockIdx.x) / p.splits) * 2 * kM > kM ? 16 : 8);
     *abort_flag = 0;
     *s_bad = 0;
     fence_mbarrier_init();
@@ -133,9 +161,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
   pdl_begin();
   const Span sp = span_of(p, status);
 
-  if (warp < 4) {
-    regs_dec<kRegsWg0>();
-    if (warp == 0 && sp.nblocks > 0) {
+  if (warp == 0) {
+    if (sp.nblocks > 0) {
       // --------------------------------------------------------- products
       constexpr uint32_t idesc_qk = make_idesc_f16(kM, kN, 0u, 0u, 0u);
       constexpr uint32_t idesc_pv = make_idesc_f16(kM, D, 0u, 0u, 1u);
@@ -152,10 +179,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
       };
       auto values = [&](int t, int j) {
         const uint32_t v_addr = smem_u32(smem + C::kOffV + (j & 1) * C::kTileBytes);
+        // weights of the keys' second half: over their own scores, too
         const uint32_t p_tmem = C::kSeparateP ? tmem + 256 + t * 128 + 64 : tmem + t * 128;
 #pragma unroll
         for (int k = 0; k < kN / 16; ++k)  // (tiles of 64 channels lie kN rows apart)
-          umma_ts_warp(tmem + 256 + t * 128, p_tmem + k * 8,
+          umma_ts_warp(tmem + 256 + t * 128, p_tmem + k * 8 + (C::kSeparateP || k < 4 ? 0 : 32),
                        make_smem_desc(v_addr + k * 16 * C::kSubRow, kN * C::kSubRow, 8 * C::kSubRow, C::kLayout),
                        idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
         umma_commit_warp(&pv_done[t]);
@@ -204,124 +232,130 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------ unpacking
-    regs_dec<kRegsUnpack>();
-    const int tid = threadIdx.x - 128;  // token of the block
+    // Pieces of 32 tokens, a token per lane: four of the keys, then four of the values of each block, dealt out
+    // in turn; a warp reads its next piece into registers while it unpacks one.
     const int shift = 31 - __clz(p.c.page);
-    // the page of the thread's token of block j, -1 where it has none
-    auto page_of = [&](int j) {
-      const int tok = (sp.jb0 + j) * kN + tid;
-      if (j >= sp.nblocks || tok >= sp.len) return -1;
-      const int id = p.c.table[sp.b * p.c.table_ld + (tok >> shift)];
-      if (id >= 0 && id < p.c.pages) return id;
-      set_bad_shape(status);
-      return -2;
+    const int pieces = sp.nblocks * 8;
+    // What the table says for the lane's token of piece n, kNone where it has none.  (Looked at a piece
+    // later, when it is used: a test here would wait for it.)
+    constexpr int kNone = -0x7FFFFFFF - 1;
+    auto page_of = [&](int n) {
+      const int tok = (sp.jb0 + (n >> 3)) * kN + (n & 3) * 32 + lane;
+      return n < pieces && tok < sp.len ? p.c.table[sp.b * p.c.table_ld + (tok >> shift)] : kNone;
     };
-    auto load = [&](int id, const uint8_t* codes, const uint8_t* scales, Packed<D>& to) {
-      if (id < 0) {  // zeros: codes are of no account under a scale of zero
+    auto known = [&](int id) { return id >= 0 && id < p.c.pages; };
+    auto load = [&](int n, int id, Packed<D>& to) {
+      if (!known(id)) {  // zeros: codes are of no account under a scale of zero
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) to.code[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < (C::kGroups + 3) / 4; ++i) to.scale[i] = 0;
+        for (int g = 0; g < C::kGroups; ++g) to.scale[g] = 0;
         return;
       }
-      const int in = tid & (p.c.page - 1);  // (a block starts a page, or 128 tokens are one)
+      const int in = ((n & 3) * 32 + lane) & (p.c.page - 1);  // (a block starts a page, or 128 tokens are one)
       const long long unit = static_cast<long long>(id) * p.c.kv_heads + sp.head;
-      const uint4* from = reinterpret_cast<const uint4*>(codes + (unit * p.c.page + in) * (D / 2));
+      const uint4* from =
+          reinterpret_cast<const uint4*>((n & 4 ? p.c.v : p.c.k) + (unit * p.c.page + in) * (D / 2));
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) to.code[i] = from[i];
-      const uint8_t* s = scales + unit * C::kGroups * p.c.page + in;
+      const uint8_t* s = (n & 4 ? p.c.v_scale : p.c.k_scale) + unit * C::kGroups * p.c.page + in;
 #pragma unroll
-      for (int i = 0; i < (C::kGroups + 3) / 4; ++i) {
-        to.scale[i] = 0;
-#pragma unroll
-        for (int g = 4 * i; g < C::kGroups && g < 4 * i + 4; ++g)
-          to.scale[i] |= static_cast<uint32_t>(s[g * p.c.page]) << (8 * (g & 3));
-      }
+      for (int g = 0; g < C::kGroups; ++g) to.scale[g] = s[g * p.c.page];
     };
-    auto unpack = [&](const Packed<D>& from, uint8_t* to) {
+    Packed<D> now, next;
+    int n = warp - 1, id = page_of(n), id_next = page_of(n + kUnpackWarps);
+    load(n, id, now);
+    for (; n < pieces; n += kUnpackWarps) {
+      const int j = n >> 3, st = j & 1, ms = j % kMeta, quarter = n & 3;
+      const bool values = n & 4;
+      const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u;
+      const int id_after = page_of(n + 2 * kUnpackWarps);
+      load(n + kUnpackWarps, id_next, next);
+      if (!warp_wait(values ? &v_empty[st] : &k_empty[st], ph ^ 1u, abort_flag, status)) break;
+      if (values) {
+        if ((sp.jb0 + j + 1) * kN > sp.open) {
+          // Where some rows may not see a token its NaN becomes zero here, and
+          // the rows that do see it get the NaN at the end.
+#pragma unroll
+          for (int g = 0; g < C::kGroups; ++g) {
+            if (now.scale[g] == kInt4NanScale) {
+              now.scale[g] = 0;
+              *s_bad = 1;
+            }
+          }
+        }
+      } else {
+        // (the scores of block j - 2 are done, so the softmax has read the mask of block j - 4)
+        const bool lost = id != kNone && !known(id);
+        if (lost) set_bad_shape(status);
+        const uint32_t missing = __ballot_sync(0xffffffffu, lost);
+        if (lane == 0) {
+          s_meta[ms * 4 + quarter] = ((missing & 0xFFFFu) ? 1 : 0) | ((missing >> 16) ? 2 : 0);
+          mbar_arrive(&meta_full[ms]);
+        }
+      }
+      uint8_t* to = smem + (values ? C::kOffV : C::kOffK) + st * C::kTileBytes;
+      const int row = quarter * 32 + lane;
 #pragma unroll
       for (int g = 0; g < C::kGroups; ++g) {
-        const uint32_t sel = scale_selector(g & 3, g & 3);
-        const uint32_t sc = scale_pair(from.scale[g >> 2], sel);
+        const uint32_t sc = now.scale[g] * 0x00800080u;  // twice as f16
         const __half2 m = minus72(sc);
-        const uint4 w = from.code[g >> 1];
+        const uint4 w = now.code[g >> 1];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t v[4];
           unpack4((g & 1) ? (h ? w.w : w.z) : (h ? w.y : w.x), as_half2(sc), m, v);
-          *reinterpret_cast<uint4*>(to + C::place(tid, 2 * g + h)) = make_uint4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<uint4*>(to + C::place(row, 2 * g + h)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-    };
-    Packed<D> k, v;
-    int id = page_of(0), next = page_of(1);
-    load(id, p.c.k, p.c.k_scale, k);
-    bool ok = true;
-    for (int j = 0; ok && j < sp.nblocks; ++j) {
-      const int st = j & 1, ms = j % kMeta;
-      const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u;
-      const int after = page_of(j + 2);
-      load(id, p.c.v, p.c.v_scale, v);
-      ok = warp_wait(&k_empty[st], ph ^ 1u, abort_flag, status);
-      if (!ok) break;
-      // (the scores of block j - 2 are done, so the softmax has read the mask of block j - 4)
-      const uint32_t missing = __ballot_sync(0xffffffffu, id == -2);
-      if (lane == 0) {
-        s_meta[ms * 4 + (warp & 3)] = ((missing & 0xFFFFu) ? 1 : 0) | ((missing >> 16) ? 2 : 0);
-        mbar_arrive(&meta_full[ms]);
-      }
-      unpack(k, smem + C::kOffK + st * C::kTileBytes);
-      if (lane == 0) mbar_arrive(&k_full[st]);
-      load(next, p.c.k, p.c.k_scale, k);
-      if ((sp.jb0 + j + 1) * kN > sp.open) {
-        // Where some rows may not see a token its NaN becomes zero here, and
-        // the rows that do see it get the NaN at the end.
-#pragma unroll
-        for (int g = 0; g < C::kGroups; ++g) {
-          if (((v.scale[g >> 2] >> (8 * (g & 3))) & 0xFFu) == kInt4NanScale) {
-            v.scale[g >> 2] &= ~(0xFFu << (8 * (g & 3)));
-            *s_bad = 1;
-          }
-        }
-      }
-      ok = warp_wait(&v_empty[st], ph ^ 1u, abort_flag, status);
-      if (!ok) break;
-      unpack(v, smem + C::kOffV + st * C::kTileBytes);
-      if (lane == 0) mbar_arrive(&v_full[st]);
-      id = next;
-      next = after;
+      if (lane == 0) mbar_arrive(values ? &v_full[st] : &k_full[st]);
+      now = next;
+      id = id_next;
+      id_next = id_after;
     }
   } else {
-    regs_inc<kRegsSoftmax>();
     // ------------------------------------------------------------ softmax
-    const int t = (warp - 8) >> 2;  // tile of this warpgroup
-    const int quarter = warp & 3;   // TMEM lanes this warp may access
+    const int t = (warp - 8) >> 3;         // tile
+    const int half = (warp >> 2) & 1;      // keys 64 half .. of a block, channels D / 2 half .. of the output
+    const int quarter = warp & 3;          // TMEM lanes this warp may access
+    const int pair = t * 4 + quarter;      // with the warp of the other half
     const int local = quarter * 32 + lane;
     const int row = sp.row0 + t * kM + local;
     const bool live = row < p.rows;
     const int i = live ? row / p.group : 0, gq = live ? row % p.group : 0;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t tmem_s = tmem + t * 128 + lane_base;
+    const uint32_t tmem_s = tmem + t * 128 + lane_base + 64 * half;
     const uint32_t tmem_o = tmem + 256 + t * 128 + lane_base;
-    const uint32_t tmem_p = C::kSeparateP ? tmem_o + 64 : tmem_s;
+    const uint32_t tmem_p = C::kSeparateP ? tmem_o + 64 + 32 * half : tmem_s;
     const int limit = p.causal && live ? min(sp.len, sp.len - p.queries + i + 1) : sp.len;  // keys that the row sees
+    float* s_row = reinterpret_cast<float*>(smem + C::kOffRow) + t * 2 * kM + local;  // [half * kM]
+    volatile uint32_t* s_vote = reinterpret_cast<volatile uint32_t*>(smem + C::kOffVote) + pair * 4;
+    uint32_t meets = 0;
+    bool ok = t < sp.tiles;
+    // The two warps of the rows wait for each other; what either has written to shared memory before is there for the other.
+    auto meet = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pair_bar[pair]);
+      ok = warp_wait(&pair_bar[pair], meets & 1u, abort_flag, status);
+      ++meets;
+    };
     constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes of a row (eight channels each), rows at a time
+    const T* src = static_cast<const T*>(p.q) + sp.b * p.q_batch + i * p.q_ld +
+                   (static_cast<long long>(sp.head) * p.group + gq) * D;
     float factor = 1.f;
-    if (t < sp.tiles && sp.nblocks > 0) {
-      // Query rows in the keys' order of channels; the largest magnitude of a bf16
+    if (ok && sp.nblocks > 0) {
+      // Query rows in the keys' order of channels, half of them each warp; the largest magnitude of a bf16
       // row to [2^14, 2^15).  A NaN stays one, an infinity makes the row's factor one (of a row that
       // sees any key).
-      const T* src = static_cast<const T*>(p.q) + sp.b * p.q_batch + i * p.q_ld +
-                     (static_cast<long long>(sp.head) * p.group + gq) * D;
       const int part_lane = lane % kLanes;
-      float top_of = 0.f;  // largest magnitude of the lane's own row
+      constexpr int kTurns = kLanes / 2, kAtOnce = kTurns < 4 ? kTurns : 4;
 #pragma unroll 1
-      for (int n0 = 0; n0 < kLanes; n0 += 4) {
-        uint4 raw[4];
+      for (int n0 = half * kTurns; n0 < (half + 1) * kTurns; n0 += kAtOnce) {
+        uint4 raw[kAtOnce];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < kAtOnce; ++n) {
           const int from = (n0 + n) * kRows + lane / kLanes;  // row of the warp, and the lane that owns it
           const T* at = reinterpret_cast<const T*>(__shfl_sync(
                             0xffffffffu, reinterpret_cast<unsigned long long>(src), from)) + 8 * part_lane;
@@ -337,8 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
           }
         }
 #pragma unroll
-        for (int k4 = 0; k4 < 4; ++k4) {
-          const int n = n0 + k4;
+        for (int k4 = 0; k4 < kAtOnce; ++k4) {
+          const int from = (n0 + k4) * kRows + lane / kLanes;
           uint32_t w[4] = {raw[k4].x, raw[k4].y, raw[k4].z, raw[k4].w};
           float m = 0.f;
 #pragma unroll
@@ -348,118 +382,125 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
           }
 #pragma unroll
           for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          const float own = __shfl_sync(0xffffffffu, m, (lane % kRows) * kLanes);
-          if (lane / kRows == n) top_of = own;
+          if (part_lane == 0) s_row[from - lane] = m;
           if constexpr (kScaled) {
             const float inv = fp8_pow2(7 - kv_query_exponent(m));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float2 x = kv_unpack2<T>(w[k]);
-              const __half2 h = __floats2half2_rn(x.x * inv * 128.f, x.y * inv * 128.f);
-              w[k] = as_word(h);
+              w[k] = as_word(__floats2half2_rn(x.x * inv * 128.f, x.y * inv * 128.f));
             }
           }
           const uint32_t flip = p.negate ? 0x80008000u : 0u;
           const uint4 out = make_uint4(__byte_perm(w[0], w[2], 0x5410) ^ flip, __byte_perm(w[0], w[2], 0x7632) ^ flip,
                                        __byte_perm(w[1], w[3], 0x5410) ^ flip, __byte_perm(w[1], w[3], 0x7632) ^ flip);
-          *reinterpret_cast<uint4*>(smem + t * C::kTileBytes +
-                                    C::place(quarter * 32 + n * kRows + lane / kLanes, part_lane)) = out;
+          *reinterpret_cast<uint4*>(smem + t * C::kTileBytes + C::place(quarter * 32 + from, part_lane)) = out;
         }
       }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      meet();
+      const float top_of = *s_row;  // largest magnitude of the thread's row
       factor = fp8_is_finite(top_of) || limit <= 0
                    ? (kScaled ? fp8_pow2(kv_query_exponent(top_of) - 7) * 0.0078125f : 1.f) * p.scale_log2
                    : fp8_nan();
       if (factor < 1.2e-38f) factor = 1.2e-38f;  // (-inf times zero would be a NaN)
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
+      if (ok) meet();  // (s_row is free again)
     }
     float top = kFloor, l = 0.f;
-    bool ok = t < sp.tiles;
+    const uint64_t f2 = pack2(factor, factor);
     for (int j = 0; ok && j < sp.nblocks; ++j) {
       ok = warp_wait(&s_full[t], static_cast<uint32_t>(j) & 1u, abort_flag, status) &&
            warp_wait(&meta_full[j % kMeta], static_cast<uint32_t>(j / kMeta) & 1u, abort_flag, status);
       if (!ok) break;
       tc_fence_after();
-      uint32_t sr[kN];
+      const uint32_t missing = *reinterpret_cast<const uint32_t*>(s_meta + (j % kMeta) * 4) >> (16 * half);
+      const int j0 = (sp.jb0 + j) * kN + 64 * half;
+      const bool hidden = j0 + 64 > sp.open || missing;
+      uint32_t packed[32];
+      uint64_t sum2[2];
+      float mx;
+      // Weights against the reference as it is, and the thread's largest score.
+      auto weights = [&] {
+        const uint64_t shift = pack2(kHeadroom - top, kHeadroom - top);
+        sum2[0] = sum2[1] = 0;
+        mx = -INFINITY;
 #pragma unroll
-      for (int c0 = 0; c0 < kN; c0 += 32) {
-        uint32_t(&chunk)[32] = *reinterpret_cast<uint32_t(*)[32]>(&sr[c0]);
-        tmem_ld32(tmem_s + c0, chunk);
-      }
-      const uint32_t missing = *reinterpret_cast<const uint32_t*>(s_meta + (j % kMeta) * 4);
-      tmem_wait_ld();
-      if constexpr (C::kSeparateP) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[t]);
-      }
-      const int j0 = (sp.jb0 + j) * kN;
-      if (j0 + kN > sp.open) {  // hidden keys count nothing
+        for (int c = 0; c < 2; ++c) {
+          uint32_t sr[32];
+          tmem_ld32(tmem_s + 32 * c, sr);
+          tmem_wait_ld32(sr);
+          if (hidden) {  // hidden keys count nothing, nor do those of missing pages
 #pragma unroll
-        for (int c = 0; c < kN; ++c)
-          if (j0 + c >= limit) sr[c] = 0xFF800000u;
-      }
-      if (missing) {  // (rare) nor do those of missing pages
+            for (int k = 0; k < 32; ++k) {
+              hide_from(sr[k], 32 * c + k, limit - j0);
+              hide_if(sr[k], missing, 1u << (8 * c + k / 16));
+            }
+          }
 #pragma unroll
-        for (int c = 0; c < kN; ++c)
-          if (missing >> (8 * (c / 32) + (c / 16) % 2) & 1u) sr[c] = 0xFF800000u;
-      }
-      float m4[4];  // independent chains of 3-input maxima, folded
-#pragma unroll
-      for (int k = 0; k < 4; ++k) m4[k] = fmaxf(__uint_as_float(sr[2 * k]), __uint_as_float(sr[2 * k + 1]));
-#pragma unroll
-      for (int c = 8; c < kN; c += 8)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          m4[k] = max3(m4[k], __uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1]));
-      const float mx = fmaxf(kFloor, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * factor);
-      const bool first = j == 0;
-      const bool grow = first || mx - top > kGrow;
-      const float next = grow ? fmaxf(top, mx) : top;
-      const float half = first ? 0.f : ex2_approx(0.5f * (top - next)), alpha = half * half;
-      if (j > 0) {
-        // the value product of the block before is done: its weights' place is free, O is whole
-        ok = warp_wait(&pv_done[t], static_cast<uint32_t>(j - 1) & 1u, abort_flag, status);
+          for (int k = 0; k < 32; k += 2) {
+            mx = max3(mx, __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
+            float x0, x1;
+            unpack2(fma2(pack2(__uint_as_float(sr[k]), __uint_as_float(sr[k + 1])), f2, shift), x0, x1);
+            const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
+            sum2[(k >> 1) & 1] = add2(sum2[(k >> 1) & 1], pack2(e0, e1));
+            packed[16 * c + k / 2] = as_word(__floats2half2_rn(e0, e1));
+          }
+        }
+      };
+      weights();
+      // A reference seldom grows; where one of 32 rows' does, both warps scale what there is and begin again.
+      const bool mine = __any_sync(0xffffffffu, j == 0 || mx * factor > top + kGrow);
+      const uint32_t side = (meets & 1u) * 2;
+      if (lane == 0) s_vote[side + half] = mine;
+      meet();
+      if (!ok) break;
+      if (mine || s_vote[side + 1 - half]) {
+        s_row[half * kM] = mx * factor;
+        meet();
         if (!ok) break;
-        tc_fence_after();
-        if (__any_sync(0xffffffffu, grow)) {
-          const float scale = grow ? alpha : 1.f;
+        const float all = fmaxf(s_row[0], s_row[kM]);
+        const float next = j == 0 || all > top + kGrow ? fmaxf(top, all) : top;
+        const float scale_half = ex2_approx(0.5f * (top - next)), alpha = scale_half * scale_half;
+        if (j > 0) {
+          // the value product of the block before is done: the output is whole
+          ok = warp_wait(&pv_done[t], static_cast<uint32_t>(j - 1) & 1u, abort_flag, status);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-          for (int c0 = 0; c0 < D; c0 += 16) {
+          for (int c0 = 0; c0 < D / 2; c0 += 16) {
             uint32_t r[16];
-            tmem_ld16(tmem_o + c0, r);
+            tmem_ld16(tmem_o + half * (D / 2) + c0, r);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * scale);
-            tmem_st16(tmem_o + c0, r);
+            for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * alpha);
+            tmem_st16(tmem_o + half * (D / 2) + c0, r);
           }
           tmem_wait_st();
         }
-      }
-      if (grow) {
-        l = kv_scaled(l, half);
+        l = kv_scaled(l, scale_half);
         top = next;
-      }
-      const float ref = kHeadroom - top;
-      const uint64_t f2 = pack2(factor, factor), shift = pack2(ref, ref);
-      uint64_t sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-#pragma unroll
-      for (int h = 0; h < kN; h += 16) {
-        uint32_t packed[8];
-#pragma unroll
-        for (int c = 0; c < 16; c += 2) {
-          float x0, x1;
-          unpack2(fma2(pack2(__uint_as_float(sr[h + c]), __uint_as_float(sr[h + c + 1])), f2, shift), x0, x1);
-          const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
-          sum2[(c >> 1) & 1] = add2(sum2[(c >> 1) & 1], pack2(e0, e1));
-          packed[c / 2] = as_word(__floats2half2_rn(e0, e1));
-        }
-        tmem_st8(tmem_p + (h >> 1), packed);
+        weights();
+        meet();  // (s_row is free again)
+        if (!ok) break;
       }
       float a, b;
       unpack2(add2(sum2[0], sum2[1]), a, b);
       l += a + b;
+      if constexpr (C::kSeparateP) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t]);
+        if (j > 0) {
+          // the value product of the block before has read its weights
+          ok = warp_wait(&pv_done[t], static_cast<uint32_t>(j - 1) & 1u, abort_flag, status);
+          if (!ok) break;
+          tc_fence_after();
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) tmem_st16(tmem_p + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(&packed[16 * c]));
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -470,7 +511,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
            warp_wait(&v_full[(sp.nblocks - 1) & 1], static_cast<uint32_t>((sp.nblocks - 1) >> 1) & 1u, abort_flag,
                      status);  // (done as well: orders the reads of s_bad)
     if (ok) {
+      s_row[half * kM] = l;
+      meet();
+    }
+    if (ok) {
       tc_fence_after();
+      l = s_row[0] + s_row[kM];
       const int split = blockIdx.x % p.splits;
       const long long part =
           ((static_cast<long long>(split) * p.c.batch + sp.b) * p.c.kv_heads + sp.head) * p.rows + row;
@@ -482,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
       uint8_t* rows = smem + t * C::kTileBytes + quarter * 32 * D * 2;
       constexpr int kOrder[8] = {0, 2, 4, 6, 1, 3, 5, 7};  // where a channel of eight is
 #pragma unroll 2
-      for (int c0 = 0; c0 < D; c0 += 16) {
+      for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 16) {
         uint32_t r[16];
         if (sp.nblocks > 0) {
           tmem_ld16(tmem_o + c0, r);
@@ -511,9 +557,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
         __syncwarp();  // the next read of TMEM is the whole warp's
       }
       if (p.splits == 1) {
-        __syncwarp();
+        meet();
 #pragma unroll 4
-        for (int n = 0; n < kLanes; ++n) {
+        for (int n = half * (kLanes / 2); ok && n < (half + 1) * (kLanes / 2); ++n) {
           const int from = n * kRows + lane / kLanes, chunk = lane % kLanes;
           T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from)) +
                   8 * chunk;
@@ -529,12 +575,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
         }
         __syncwarp();
       }
-      if (p.splits > 1 && live)
+      if (p.splits > 1 && live && half == 0)
         *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(top, l * fp8_pow2(-kHeadroom));
       tc_fence_before();
-      if (sp.nblocks > 0 && live && *s_bad != 0) {
+      const bool bad = sp.nblocks > 0 && *s_bad != 0;  // (of the CTA: both warps go on or neither)
+      if (bad && ok) meet();  // (the rows are written)
+      if (bad && ok && live) {
         // Rare: NaN among the values of the blocks that `open` cuts, whose product
-        // left them out.  Looked up again in the cache, token by token, by each row.
+        // left them out.  Looked up again in the cache, token by token, by each row's threads.
         const int to = min(limit, (sp.jb0 + sp.nblocks) * kN);
         for (int tok = max(sp.jb0, max(sp.open, 0) / kN) * kN; tok < to; ++tok) {
           const int id = p.c.table[sp.b * p.c.table_ld + tok / p.c.page];
@@ -542,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
           const uint8_t* s = p.c.v_scale +
                              (static_cast<long long>(id) * p.c.kv_heads + sp.head) * C::kGroups * p.c.page +
                              tok % p.c.page;
-          for (int c = 0; c < D; ++c) {
+          for (int c = half * (D / 2); c < (half + 1) * (D / 2); ++c) {
             if (s[(c / kInt4Group) * p.c.page] != kInt4NanScale) continue;
             if (p.splits > 1) {
               p.o_part[part * D + c] = fp8_nan();
