@@ -5,7 +5,8 @@ and its keys and values held in 8 bits (the denoiser's own blocks have layer nor
 with a bias and run in f16):
 
     rows, h = rms_norm_fp8(x, norm1)                  # codes for the projections, h the residual stream
-    q = matmul_fp8(rows, to_q);  a = kv_attention(q, cache, ...)
+    q, k = qk_norm_rope(matmul_fp8(rows, to_q), ...)  # where the block norms its heads or tokens have positions
+    a = kv_attention(q, cache, ...)
     o = matmul_fp8(quantize_rows(a), to_out)
     rows, h = rms_norm_fp8(o, norm2, residual=h)      # adds the attention's output on the way
     y = matmul_fp8(quantize_rows(matmul_fp8(rows, ff1, gelu)), ff2, residual=h)
@@ -13,6 +14,8 @@ with a bias and run in f16):
 ``bind`` projects a context into a cache once, ``read`` attends to it at every
 step (cross-attention); ``extend`` writes the tokens' own keys and values behind
 those of earlier calls and attends causally (a prompt, then token by token).
+Caches hold 8 bits or 4, and positions run along one axis (a sequence: ``extend`` counts
+them by itself) or several (a volume's tokens).
 
 Run as a command it times both on random weights:
 ``python -m lesiondiffusion_mlx_b200.fp8_block``.
@@ -26,7 +29,8 @@ import torch
 
 from . import _lib
 from .fp8 import Fp8Weight, matmul_fp8, pack_weight_fp8, quantize_rows, rms_norm_fp8
-from .kv_cache import KvCacheFp8, kv_append, kv_attention
+from .kv_cache import KvCache, KvCacheFp8, KvCacheInt4, kv_append, kv_attention
+from .rotary import Rotary, grid_positions, qk_norm_rope
 
 WEIGHTS = ("norm1", "norm2", "to_q", "to_k", "to_v", "to_out", "ff1", "ff2")
 
@@ -35,7 +39,7 @@ WEIGHTS = ("norm1", "norm2", "to_q", "to_k", "to_v", "to_out", "ff1", "ff2")
 class KvState:
     """A cache, the pages of each item and how many of their tokens are written."""
 
-    cache: KvCacheFp8
+    cache: KvCache
     table: torch.Tensor
     lengths: torch.Tensor
     room: int     # tokens an item's pages hold
@@ -56,10 +60,12 @@ class Fp8TokenBlock:
     ``weights`` holds ``norm1``, ``norm2`` ``(C,)``, ``to_q`` ``(heads * d, C)``,
     ``to_k`` / ``to_v`` ``(kv_heads * d, C_context)``, ``to_out`` ``(C, heads *
     d)``, ``ff1`` ``(F, C)``, ``ff2`` ``(C, F)`` and optionally ``ff1.bias`` /
-    ``ff2.bias``; activations are float16 or bfloat16 ``(B, L, C)``."""
+    ``ff2.bias`` and the norms of each head's queries and keys, ``q_norm`` and ``k_norm``
+    ``(d,)``; activations are float16 or bfloat16 ``(B, L, C)``.  With a
+    ``rotary`` plan queries and keys turn by their tokens' positions where a call has them."""
 
     def __init__(self, weights: dict[str, torch.Tensor], *, heads: int, kv_heads: int, eps: float = 1e-6,
-                 device: torch.device | str = "cuda"):
+                 rotary: Rotary | None = None, device: torch.device | str = "cuda"):
         missing = [n for n in WEIGHTS if n not in weights]
         if missing:
             raise ValueError(f"weights are missing {missing}")
@@ -69,6 +75,9 @@ class Fp8TokenBlock:
                              f"to_k {tuple(weights['to_k'].shape)}")
         self.heads, self.kv_heads, self.head_dim, self.eps = heads, kv_heads, width // heads, eps
         self.device = torch.device(device)
+        self.rotary = rotary
+        if ("q_norm" in weights) != ("k_norm" in weights):
+            raise ValueError("q_norm and k_norm come together")
 
         def vector(name: str) -> torch.Tensor | None:
             w = weights.get(name)
@@ -79,14 +88,18 @@ class Fp8TokenBlock:
 
         self.norm1, self.norm2 = vector("norm1"), vector("norm2")
         self.bias1, self.bias2 = vector("ff1.bias"), vector("ff2.bias")
+        self.q_norm, self.k_norm = vector("q_norm"), vector("k_norm")
         self.to_q, self.to_kv, self.to_out = packed("to_q"), packed("to_k", "to_v"), packed("to_out")
         self.ff1, self.ff2 = packed("ff1"), packed("ff2")
 
-    def new_state(self, batch: int, tokens: int, *, page: int = 64) -> KvState:
-        """Room for ``tokens`` tokens of each of ``batch`` items, none written."""
+    def new_state(self, batch: int, tokens: int, *, page: int = 64, bits: int = 8) -> KvState:
+        """Room for ``tokens`` tokens of each of ``batch`` items in 8 or 4 bits, none written."""
+        if bits not in (4, 8):
+            raise ValueError(f"caches hold 4 or 8 bits, got {bits}")
         per = -(-tokens // page)
         table = torch.arange(batch * per, dtype=torch.int32, device=self.device).view(batch, per)
-        cache = KvCacheFp8.empty(batch * per, self.kv_heads, self.head_dim, page=page, device=self.device)
+        kind = KvCacheInt4 if bits == 4 else KvCacheFp8
+        cache = kind.empty(batch * per, self.kv_heads, self.head_dim, page=page, device=self.device)
         return KvState(cache, table, torch.zeros(batch, dtype=torch.int32, device=self.device), per * page, 0)
 
     def _keys_values(self, rows, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
@@ -94,14 +107,29 @@ class Fp8TokenBlock:
         width = self.kv_heads * self.head_dim
         return kv[..., :width], kv[..., width:]
 
-    def bind(self, context: torch.Tensor, *, page: int = 64) -> KvState:
+    def _queries(self, rows, dtype: torch.dtype) -> torch.Tensor:
+        return matmul_fp8(rows, self.to_q, out_dtype=dtype)
+
+    def _turned(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor | None, *,
+                q_norm: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """Heads normed where the block has norms for them, and turned where there are positions."""
+        if positions is not None and self.rotary is None:
+            raise ValueError("positions without a rotary plan")
+        if q_norm is None and positions is None:
+            return q, k
+        return qk_norm_rope(q, k, head_dim=self.head_dim, q_gamma=q_norm, k_gamma=self.k_norm, eps=self.eps,
+                            norm=q_norm is not None, rotary=None if positions is None else self.rotary,
+                            positions=positions)
+
+    def bind(self, context: torch.Tensor, *, positions: torch.Tensor | None = None, page: int = 64,
+             bits: int = 8) -> KvState:
         """The keys and values of a ``(B, L, C_context)`` context, projected and written once."""
-        state = self.new_state(int(context.shape[0]), int(context.shape[1]), page=page)
-        state.append(*self._keys_values(quantize_rows(context), context.dtype))
+        state = self.new_state(int(context.shape[0]), int(context.shape[1]), page=page, bits=bits)
+        k, v = self._keys_values(quantize_rows(context), context.dtype)
+        state.append(self._turned(k, None, positions, q_norm=self.k_norm)[0], v)
         return state
 
-    def _rest(self, rows, h: torch.Tensor, state: KvState, causal: bool) -> torch.Tensor:
-        q = matmul_fp8(rows, self.to_q, out_dtype=h.dtype)
+    def _rest(self, q: torch.Tensor, h: torch.Tensor, state: KvState, causal: bool) -> torch.Tensor:
         a = kv_attention(q, state.cache, state.table, state.lengths, scale=self.head_dim ** -0.5, causal=causal)
         o = matmul_fp8(quantize_rows(a), self.to_out, out_dtype=h.dtype)
         rows, h = rms_norm_fp8(o, self.norm2, residual=h, eps=self.eps)
@@ -115,18 +143,27 @@ class Fp8TokenBlock:
         if x.ndim != 3 or x.shape[0] != state.lengths.shape[0]:
             raise ValueError(f"activations must be ({state.lengths.shape[0]}, L, C), got {tuple(x.shape)}")
 
-    def read(self, x: torch.Tensor, state: KvState) -> torch.Tensor:
+    def read(self, x: torch.Tensor, state: KvState, *, positions: torch.Tensor | None = None) -> torch.Tensor:
         """The block with attention over every token of ``state`` (cross-attention to a bound context)."""
         self._check(x, state)
         rows, h = rms_norm_fp8(x, self.norm1, eps=self.eps)
-        return self._rest(rows, h, state, False)
+        q, _ = self._turned(self._queries(rows, h.dtype), None, positions, q_norm=self.q_norm)
+        return self._rest(q, h, state, False)
 
-    def extend(self, x: torch.Tensor, state: KvState) -> torch.Tensor:
-        """The block with causal self-attention: ``x``'s keys and values are written behind the state's tokens."""
+    def extend(self, x: torch.Tensor, state: KvState, *, positions: torch.Tensor | None = None) -> torch.Tensor:
+        """The block with causal self-attention: ``x``'s keys and values are written behind the state's tokens.
+
+        Positions along one axis count on from the state's tokens where none are given."""
         self._check(x, state)
+        if positions is None and self.rotary is not None:
+            if self.rotary.axes != 1:
+                raise ValueError(f"positions along {self.rotary.axes} axes have to be given")
+            positions = state.lengths[:, None] + torch.arange(x.shape[1], dtype=torch.int32, device=x.device)
         rows, h = rms_norm_fp8(x, self.norm1, eps=self.eps)
-        state.append(*self._keys_values(rows, x.dtype))
-        return self._rest(rows, h, state, True)
+        k, v = self._keys_values(rows, x.dtype)
+        q, k = self._turned(self._queries(rows, h.dtype), k, positions, q_norm=self.q_norm)
+        state.append(k, v)
+        return self._rest(q, h, state, True)
 
 
 def random_weights(channels: int, context: int, heads: int, kv_heads: int, head_dim: int, hidden: int, *,
@@ -169,6 +206,20 @@ def main() -> None:
     block.extend(torch.randn(16, 2048, 2048, device="cuda", dtype=torch.bfloat16), state)
     token = torch.randn(16, 1, 2048, device="cuda", dtype=torch.bfloat16)
     timed("one token of 16 sequences behind 2048", lambda: block.extend(token, state))
+
+    # the same with normed heads and positions, over a 4-bit cache
+    weights = random_weights(2048, 2048, 16, 4, 128, 8192) | {"q_norm": torch.ones(128), "k_norm": torch.ones(128)}
+    block = Fp8TokenBlock(weights, heads=16, kv_heads=4, rotary=Rotary.build((128,)))
+    state = block.new_state(16, 2048 + 64, bits=4)
+    block.extend(torch.randn(16, 2048, 2048, device="cuda", dtype=torch.bfloat16), state)
+    timed("with normed heads and positions, in 4 bits", lambda: block.extend(token, state))
+
+    # the 16x20x20 level's tokens over their own, bound in 4 bits with their places in the volume
+    volume = Fp8TokenBlock(random_weights(256, 256, 4, 4, 64, 1024), heads=4, kv_heads=4,
+                           rotary=Rotary.build((16, 24, 24)))
+    at = grid_positions(16, 20, 20)
+    bound = volume.bind(x, positions=at, bits=4)
+    timed("6400 tokens over 6400 of a volume, in 4 bits", lambda: volume.read(x, bound, positions=at))
 
 
 if __name__ == "__main__":
