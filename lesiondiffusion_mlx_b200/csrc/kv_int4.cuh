@@ -16,8 +16,8 @@
 // group, scales[page][kv head][D / 16][token in page], so that a group's scales of
 // neighbouring tokens are one word.
 //
-// (Groups of 16 normal values keep 21.8 dB of signal to error so; the 4-bit floating
-// point codes 0, 0.5, 1, 1.5, 2, 3, 4, 6 with the same scales keep 19.3.)
+// (Groups of 16 normal values keep 21.4 dB of signal to error so; the 4-bit floating
+// point codes 0, 0.5, 1, 1.5, 2, 3, 4, 6 with the same scales keep 20.0.)
 #pragma once
 
 #include "fp8.cuh"

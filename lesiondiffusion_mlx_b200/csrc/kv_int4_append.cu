@@ -8,7 +8,9 @@
 // neighbouring threads read neighbouring groups (whole rows of all heads) and four
 // reads are on their way at a time.
 //
-// Bound: HBM, 2 bytes read and 9/16 written a value; for one token the launch.
+// Bound: HBM, 2 bytes read and 9/16 written a value; for one token the launch.  One B200, 4 x 4097
+// tokens of 8 heads of 128 bf16 with the read back that follows 35 us (172 MB at 4.9 TB/s), one token of 32 items with its
+// read back 3.9 us.  Eight channels a thread instead of a group find each group's maximum twice, and took longer.
 
 #include <type_traits>
 

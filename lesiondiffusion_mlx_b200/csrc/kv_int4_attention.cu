@@ -9,13 +9,19 @@
 // come out as pairs of channels, so the queries are paired like them; values of two
 // neighbouring tokens are paired by exchanging half words first, and their scales come
 // as pairs too.  Queries are f16 as they are, or bf16 rows scaled by a power of
-// two (exact down to 2^-17 of the row's largest).  Weights are rounded to f16 once, 2^15 at
-// M and lost below 2^-40 of it; their sum is FP32.
+// two (exact down to 2^-31 of the row's largest).  M follows a row's maximum only once that is 2^4 above
+// it, so that most tiles scale nothing.  Weights are rounded to f16 once, 2^11 at M (within f16 at 2^15), with
+// 11 bits down to 2^-25 of M and lost below 2^-36; their sum is FP32.
 //
 // Bound: HBM, (D / 2 + D / 16) 2 bytes a token and key/value head, read once for
 // a group's heads.  The tiles of 32 tokens of all items and heads form one line that the
 // warps share out equally (kv_attention_ranges.cuh); a warp copies the next
 // tiles into its own ring (cp.async) while it works on one.
+//
+// One B200, one bf16 token of 32 heads of 128 over 8: behind 262144 tokens 69 us (302 MB at
+// 4.4 TB/s: 60 in this kernel, 8 in the join of its warps' parts), behind 32 items of up to 16384 70 us.  Of
+// the kernel's issue slots 65 % are taken, most by unpacking; without the unpacking it would be
+// bound by HBM.
 
 #include <algorithm>
 
@@ -554,7 +560,11 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
 // Groups of eight query rows that one pass over the cache serves.
 int row_groups(long long rows) { return rows <= 8 ? 1 : 2; }
 
-// Rows from which on the 128-row tiles of the many-row kernel are the faster.
+// Rows from which on the 128-row tiles of the many-row kernel are the faster.  8 key/value heads and 65536
+// tokens, us here and there: of 128 channels 48 rows 71 and 79, 128 rows 168 and 81; of 64 channels 53 and 60, 108 and
+// 60; of 32 channels 42 and 54, 80 and 55.  Where lengths differ much the tiles' ranges do, too (8 items, none to
+// 16384 tokens each, 128 channels: 48 rows 74 and 149, 128 rows 178 and 153); over 2048 tokens 17 rows are enough (16 and
+// 15).  Lengths are on the device, so the rule has the rows alone.
 constexpr long long kTileRows = 49;
 
 template <int D, int G, typename T>

@@ -9,7 +9,8 @@
 // are whole sectors (with 16 channels a thread, 32 bytes in two halves, items of up to 16384
 // tokens took 137 us instead of 93, and with 8 or 16 tokens a thread 96).
 //
-// Bound: HBM, 9/16 or 1 byte read and 2 written a value.
+// Bound: HBM, 9/16 or 1 byte read and 2 written a value.  One B200, 8 items of up to 16384 tokens, 8 heads
+// of 128 in 4 bits: 93 us (610 MB at 6.5 TB/s); 77 tokens of 4 items of 4 heads of 64 in 8 bits 2.3 us.
 
 #include <type_traits>
 

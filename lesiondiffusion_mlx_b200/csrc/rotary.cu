@@ -231,7 +231,7 @@ int launch_rope(cudaStream_t stream, RopeParams& p, long long rows, unsigned int
   const long long groups = (rows + (1 << p.token_shift) - 1) >> p.token_shift;  // of tokens that share a warp
   // A warp per round while all of them are resident at once, else all rounds of a token to share its sines.
   int splits = std::max(p.rounds[0], p.rounds[1]);
-  while (splits > 1 && groups * splits > resident) splits = (splits + 1) / 2 < splits ? (splits + 1) / 2 : 1;
+  while (splits > 1 && groups * splits > resident) splits = (splits + 1) / 2;
   p.splits = splits;
   for (int i = 0; i < 2; ++i) p.per_warp[i] = (p.rounds[i] + splits - 1) / splits;
   p.rows = static_cast<unsigned>(rows);
