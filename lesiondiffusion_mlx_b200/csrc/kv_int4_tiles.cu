@@ -16,8 +16,8 @@
 // by a second kernel (kv_attention_tiles.cuh).
 //
 // Bound: 4 D flops and one exponential per score.  One B200, 1024 causal bf16 queries of 2 items, 32 heads of
-// 128 over 8, behind 16384 tokens: 450 us (868 TFLOP/s), 256 CTAs on 148 SMs in two waves of 3450 cycles
-// a block, of which the products need 2048 and read 128 bytes of shared memory a cycle all the while; 6400 f16
+// 128 over 8, behind 8192 and 16384 tokens: 450 us (868 TFLOP/s), 4400 cycles a block on SMs that share 256 CTAs out
+// unevenly; the products need 2048 of them and read 128 bytes of shared memory a cycle all the while.  6400 f16
 // queries of 4 heads of 64 over 6477 tokens 117 us, 4060 cycles a block for 2048 of exponentials.  Each tile is a
 // chain: scores, weights (1500 cycles alone, 1024 of them exponentials), votes, value product.  Slower or
 // no faster, the first case's us: one row a thread with four unpacking warps (485) or seven (583); two
