@@ -131,6 +131,16 @@ DESCRIPTORS: dict[str, struct.Struct] = {
     "ldb_kv_attention_desc": struct.Struct(f"@ii{_CACHE}PPqqqqPPNiiif"),
 }
 
+
+
+def packed(name: str, desc: struct.Struct, *fields) -> bytes:
+    """A descriptor's bytes behind its size; ``ValueError`` where a number does not fit its field."""
+    try:
+        return desc.pack(desc.size, *fields)
+    except struct.error as error:
+        raise ValueError(f"{name}: {error}") from None
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 

@@ -624,11 +624,10 @@ int ldb_kv_attention_int4(cudaStream_t stream, const ldb_kv_attention_desc* desc
   if (rc != LDB_OK) return rc;
   if (page != 16 && page != 32 && page != 64 && page != 128)
     return fail(LDB_ERR_SHAPE, "kv_attention: pages of %d tokens (16, 32, 64 or 128)", page);
-  if (pages <= 0 || width <= 0 || table_ld < width || static_cast<long long>(width) * page > 0x7FFFFFFFll)
+  if (pages <= 0 || width <= 0 || table_ld < width || static_cast<long long>(width) * page > 0x7FFFFF00ll)
     return fail(LDB_ERR_SHAPE, "kv_attention: %d pages, table of %d", pages, width);
-  const long long rows_all = static_cast<long long>(pages) * kv_heads * page;
-  if (rows_all > 0x7FFFFFFFll)
-    return fail(LDB_ERR_SHAPE, "kv_attention: cache of %lld token rows (2^31 - 1)", rows_all);
+  if (static_cast<long long>(pages) * kv_heads > 0x7FFFFFFFll / page)
+    return fail(LDB_ERR_SHAPE, "kv_attention: cache of %d pages, %d heads and %d tokens (2^31 - 1 rows)", pages, kv_heads, page);
   if (batch > kMaxBatch) return fail(LDB_ERR_SHAPE, "kv_attention: at most %d items, got %d", kMaxBatch, batch);
   if (batch == 0 || queries == 0) return LDB_OK;
   if (!q || !k_codes || !v_codes || !k_scales || !v_scales || !table || !lengths || !out)
@@ -666,7 +665,7 @@ int ldb_kv_attention_int4(cudaStream_t stream, const ldb_kv_attention_desc* desc
   p.tile_rows = kGroupRows * row_groups(group_rows);
   const long long row_tiles = (group_rows + p.tile_rows - 1) / p.tile_rows;
   const long long tiles = kStart + (static_cast<long long>(width) * page + kTile - 1) / kTile;
-  if (row_tiles * kv_heads > 0x7FFFFFFFll || row_tiles * kv_heads * batch * tiles > 0x7FFFFFFFll)
+  if (row_tiles * kv_heads * batch > 0x7FFFFFFFll / tiles)
     return fail(LDB_ERR_SHAPE, "kv_attention: too many heads over too long a table");
   p.rows = static_cast<int>(group_rows), p.row_tiles = static_cast<int>(row_tiles);
   p.causal = causal != 0;

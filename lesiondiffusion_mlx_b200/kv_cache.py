@@ -222,8 +222,8 @@ def _append_int4(cache: KvCacheInt4, k: torch.Tensor, v: torch.Tensor, table: to
         raise ValueError("kv_append: channel axis must have unit stride")
     if counts is not None:
         _check_index(counts, 1, shape[0], k.device, "kv_append: counts")
-    _launcher("kv_append")("ldb_kv_append_int4", _raw_stream(index), _APPEND.pack(
-        _APPEND.size, dtype, *fields, k.data_ptr(), v.data_ptr(), k_ld, k_batch, v_ld, v_batch, start.data_ptr(),
+    _launcher("kv_append")("ldb_kv_append_int4", _raw_stream(index), _lib.packed(
+        "kv_append", _APPEND, dtype, *fields, k.data_ptr(), v.data_ptr(), k_ld, k_batch, v_ld, v_batch, start.data_ptr(),
         0 if counts is None else counts.data_ptr(), shape[1]))
 
 
@@ -311,8 +311,8 @@ def _attention_int4(q: torch.Tensor, cache: KvCacheInt4, table: torch.Tensor, le
     need = _workspace_bytes("ldb_kv_attention_int4_workspace_size", index, batch, queries, heads, kv_heads, dim,
                             width * page)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
-    _launcher("kv_attention")("ldb_kv_attention_int4", _raw_stream(index), _ATTENTION.pack(
-        _ATTENTION.size, _DT[q.dtype], *fields, q.data_ptr(), out.data_ptr(), q_ld, q_batch, out_ld, out_batch,
+    _launcher("kv_attention")("ldb_kv_attention_int4", _raw_stream(index), _lib.packed(
+        "kv_attention", _ATTENTION, _DT[q.dtype], *fields, q.data_ptr(), out.data_ptr(), q_ld, q_batch, out_ld, out_batch,
         lengths.data_ptr(), 0 if ws is None else ws.data_ptr(), need, queries, heads, int(causal), scale))
     return out
 
@@ -329,8 +329,8 @@ def kv_read(cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, *, token
     if index != _current_device():
         with torch.cuda.device(index):
             return kv_read(cache, table, lengths, tokens=tokens, start=start, dtype=dtype, out=out)
-    if tokens < 0:
-        raise ValueError(f"kv_read: tokens must be at least 0, got {tokens}")
+    if not 0 <= tokens < 2 ** 31:
+        raise ValueError(f"kv_read: tokens must be at least 0 and below 2^31, got {tokens}")
     batch = fields[-1]
     if start is not None:
         _check_index(start, 1, batch, lengths.device, "kv_read: start")
@@ -350,6 +350,6 @@ def kv_read(cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, *, token
         if k_step != 1 or v_step != 1:
             raise ValueError("kv_read: channel axis must have unit stride")
     _launcher("kv_read")("ldb_kv_read_int4" if isinstance(cache, KvCacheInt4) else "ldb_kv_read_fp8", _raw_stream(index),
-            _READ.pack(_READ.size, _DT[k.dtype], *fields, k.data_ptr(), v.data_ptr(), k_ld, k_batch, v_ld, v_batch,
+            _lib.packed("kv_read", _READ, _DT[k.dtype], *fields, k.data_ptr(), v.data_ptr(), k_ld, k_batch, v_ld, v_batch,
                        lengths.data_ptr(), 0 if start is None else start.data_ptr(), tokens))
     return k, v

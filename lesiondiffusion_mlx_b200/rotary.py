@@ -159,8 +159,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, *, head_dim: int, q_ga
         turns_ptr, axis_ptr, at_ptr = turns.data_ptr(), axis.data_ptr(), positions.data_ptr()
     elif positions is not None:
         raise ValueError("qk_norm_rope: positions without a plan")
-    _launcher("qk_norm_rope")("ldb_qk_norm_rope", _raw_stream(index), _DESC.pack(
-        _DESC.size, _DT[q.dtype], q.data_ptr(), k_ptr, q_out.data_ptr(), ko_ptr, q_ld, q_batch, k_ld, k_batch, qo_ld,
+    _launcher("qk_norm_rope")("ldb_qk_norm_rope", _raw_stream(index), _lib.packed(
+        "qk_norm_rope", _DESC, _DT[q.dtype], q.data_ptr(), k_ptr, q_out.data_ptr(), ko_ptr, q_ld, q_batch, k_ld, k_batch, qo_ld,
         qo_batch, ko_ld, ko_batch, _check_gamma(q_gamma, q, head_dim, "q_gamma"),
         _check_gamma(k_gamma, q, head_dim, "k_gamma"), turns_ptr, axis_ptr, at_ptr, at_ld, at_batch, batch, tokens,
         channels // head_dim, k_channels // head_dim, head_dim, pairs, axes, int(interleaved), int(norm), eps))

@@ -44,7 +44,7 @@ SHARED = (("k_codes", 0, -1), ("v_scales", 0, -1), ("table", 0, -1), ("page", 48
     ("read", "fp8", (("v", 0, -1), ("lengths", 0, -1), ("k_ld", 63, -2), ("tokens", -1, -2))),
     ("attention", "int4", (("q", 0, -1), ("dtype", _lib.LDB_F32, -1), ("lengths", 0, -1), ("out", 0, -1), ("heads", 5, -2),
                            ("q_ld", 127, -2), ("out_ld", 127, -2), ("v_scales", ODD, -3), ("batch", 2049, -2),
-                           ("workspace", 0, -4), ("workspace_bytes", 16, -4), ("workspace", ODD, -4), ("pages", 1 << 30, -2),
+                           ("workspace", 0, -4), ("workspace_bytes", 16, -4), ("workspace", ODD, -4), ("pages", 1 << 30, -2), ("pages", (1 << 31) - 1, -2),
                            ("queries", -1, -2), ("kv_heads", 0, -2)))])
 def test_library_refuses_bad_calls(name, bits, cases):
     good = descriptors()[name]
@@ -64,6 +64,23 @@ def test_item_strides_of_what_is_written():
     need = ctypes.c_size_t(0)
     with pytest.raises(_lib.LdbError, match="heads"):
         _lib.call("ldb_kv_attention_int4_workspace_size", 1, 1, 3, 2, 64, 100, ctypes.byref(need))
+
+
+def test_tables_past_the_last_block():
+    # 2^31 - 256 tokens: the number of the token behind a last block of 128 still has a sign to spare
+    attention = descriptors()["attention"] | dict(page=16, width=0x7FFFFF1, table_ld=0x7FFFFF1)
+    with pytest.raises(_lib.LdbError, match="table of") as e:
+        call("attention", attention)
+    assert e.value.code == -2
+
+
+def test_numbers_past_their_fields():
+    desc = _lib.DESCRIPTORS["ldb_kv_attention_desc"]
+    fields = list(descriptors()["attention"].values())[1:]
+    assert _lib.packed("kv_attention", desc, *fields) == desc.pack(desc.size, *fields)
+    for at, value in ((-4, 2 ** 31), (-4, 1.5), (-1, None)):
+        with pytest.raises(ValueError, match="kv_attention"):
+            _lib.packed("kv_attention", desc, *fields[:at], value, *(fields[at + 1:] if at + 1 else []))
 
 
 def test_empty_calls_launch_nothing():

@@ -472,6 +472,8 @@ def test_refusals(cuda_device):
                        (lambda: kv_cache.kv_read(cache, table, one.long(), tokens=3), "lengths"),
                        (lambda: kv_cache.kv_read(cache, table[0], one, tokens=3), "table"),
                        (lambda: kv_cache.kv_read(cache, table, one, tokens=-1), "tokens"),
+                       (lambda: kv_cache.kv_read(cache, table, one, tokens=2 ** 31), "tokens"),
+                       (lambda: kv_cache.kv_attention(q, cache, table, one, scale=None), "kv_attention"),
                        (lambda: kv_cache.kv_read(cache, table, one, tokens=1, dtype=torch.int32), "dtype"),
                        (lambda: kv_cache.kv_read(cache, table, one, tokens=3, start=one.long()), "start"),
                        (lambda: kv_cache.kv_read(cache, table, one, tokens=3, out=(q, q)), "out must")):
