@@ -338,9 +338,11 @@ def kv_read(cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, *, token
     if out is None:
         if dtype not in _DT:
             raise ValueError(f"kv_read: dtype must be float16, bfloat16 or float32, got {dtype}")
-        k, v = cache[0].new_empty(shape, dtype=dtype), cache[0].new_empty(shape, dtype=dtype)
         k_batch = v_batch = tokens * channels
         k_ld = v_ld = channels
+        # (3.0 us of the host's; new_empty twice 4.2)
+        k = torch.empty_strided(shape, (k_batch, k_ld, 1), dtype=dtype, device=cache[0].device)
+        v = torch.empty_like(k)
     else:
         k, v = out
         if (k.shape != shape or v.shape != shape or k.dtype not in _DT or v.dtype != k.dtype or k.get_device() != index

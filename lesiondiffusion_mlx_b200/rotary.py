@@ -73,15 +73,14 @@ def grid_positions(*sizes: int, device: torch.device | str = "cuda") -> torch.Te
 _DESC = _lib.DESCRIPTORS["ldb_qk_norm_rope_desc"]
 
 
-def _check_rows(t: torch.Tensor, like: torch.Tensor, head_dim: int, name: str) -> tuple[int, int, int]:
-    """(channels, row stride, item stride)."""
-    shape, (batch, ld, step) = t.shape, t.stride() if t.ndim == 3 else (0, 0, 0)
-    if len(shape) != 3 or t.dtype != like.dtype or t.get_device() != like.get_device() or shape[:2] != like.shape[:2]:
-        raise ValueError(f"qk_norm_rope: {name} must be (B, L, n * {head_dim}) of q's dtype, device, B and L")
-    channels = shape[2]
-    if channels % head_dim or (step != 1 and channels > 1):
-        raise ValueError(f"qk_norm_rope: {name} must hold heads of {head_dim} channels with unit stride")
-    return channels, ld, batch
+def _check_rows(t: torch.Tensor, like: torch.Tensor, index: int, head_dim: int, name: str) -> tuple[int, ...]:
+    """(channels, row stride, item stride, tokens, items)."""
+    if t.ndim == 3 and t.dtype is like.dtype and t.get_device() == index:
+        (items, tokens, channels), (batch, ld, step) = t.shape, t.stride()
+        if channels % head_dim or (step != 1 and channels > 1):
+            raise ValueError(f"qk_norm_rope: {name} must hold heads of {head_dim} channels with unit stride")
+        return channels, ld, batch, tokens, items
+    raise ValueError(f"qk_norm_rope: {name} must be (B, L, n * {head_dim}) of q's dtype, device, B and L")
 
 
 def _check_gamma(gamma: torch.Tensor | None, like: torch.Tensor, head_dim: int, name: str) -> int:
@@ -114,25 +113,26 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, *, head_dim: int, q_ga
                                 rotary=rotary, positions=positions, q_out=q_out, k_out=k_out)
     if head_dim < 16 or head_dim > 256 or head_dim % 16:
         raise ValueError(f"qk_norm_rope: heads have a multiple of 16 channels up to 256, got {head_dim}")
-    channels, q_ld, q_batch = _check_rows(q, q, head_dim, "q")
-    batch, tokens, _ = q.shape
+    channels, q_ld, q_batch, tokens, batch = _check_rows(q, q, index, head_dim, "q")
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         qo_ld, qo_batch = channels, tokens * channels
     else:
         if q_out.shape != q.shape:
             raise ValueError("qk_norm_rope: q_out must have q's shape")
-        _, qo_ld, qo_batch = _check_rows(q_out, q, head_dim, "q_out")
+        _, qo_ld, qo_batch, _, _ = _check_rows(q_out, q, index, head_dim, "q_out")
     k_ptr = ko_ptr = k_channels = k_ld = k_batch = ko_ld = ko_batch = 0
     if k is not None:
-        k_channels, k_ld, k_batch = _check_rows(k, q, head_dim, "k")
+        k_channels, k_ld, k_batch, k_tokens, k_items = _check_rows(k, q, index, head_dim, "k")
+        if k_tokens != tokens or k_items != batch:
+            raise ValueError(f"qk_norm_rope: k must be (B, L, n * {head_dim}) of q's dtype, device, B and L")
         if k_out is None:
             k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
             ko_ld, ko_batch = k_channels, tokens * k_channels
         else:
             if k_out.shape != k.shape:
                 raise ValueError("qk_norm_rope: k_out must have k's shape")
-            _, ko_ld, ko_batch = _check_rows(k_out, q, head_dim, "k_out")
+            _, ko_ld, ko_batch, _, _ = _check_rows(k_out, q, index, head_dim, "k_out")
         k_ptr, ko_ptr = k.data_ptr(), k_out.data_ptr()
     elif k_out is not None:
         raise ValueError("qk_norm_rope: k_out without k")
@@ -140,7 +140,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, *, head_dim: int, q_ga
     if rotary is not None:
         turns, axis, axes, interleaved = rotary
         pairs = turns.numel()
-        if (turns.dtype != torch.int64 or axis.dtype != torch.int32 or turns.ndim != 1 or axis.ndim != 1
+        if (turns.dtype is not torch.int64 or axis.dtype is not torch.int32 or turns.ndim != 1 or axis.ndim != 1
                 or axis.numel() != pairs or not turns.is_contiguous() or not axis.is_contiguous()
                 or turns.get_device() != index or axis.get_device() != index):
             raise ValueError("qk_norm_rope: a plan is int64 turns and int32 axes of its pairs, on q's device")
