@@ -561,10 +561,10 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
 int row_groups(long long rows) { return rows <= 8 ? 1 : 2; }
 
 // Rows from which on the 128-row tiles of the many-row kernel are the faster.  8 key/value heads and 65536
-// tokens, us here and there: of 128 channels 48 rows 71 and 79, 128 rows 168 and 81; of 64 channels 53 and 60, 108 and
-// 60; of 32 channels 42 and 54, 80 and 55.  Where lengths differ much the tiles' ranges do, too (8 items, none to
-// 16384 tokens each, 128 channels: 48 rows 74 and 149, 128 rows 178 and 153); over 2048 tokens 17 rows are enough (16 and
-// 15).  Lengths are on the device, so the rule has the rows alone.
+// tokens, us here and there: of 128 channels 32 rows 55 and 65, 48 rows 71 and 67, 128 rows 168 and 71; of 64 channels 39
+// and 52, 53 and 53, 108 and 55; of 32 channels 31 and 50, 42 and 51, 80 and 53.  Where lengths differ much the tiles'
+// ranges do, too (8 items, none to 16384 tokens each, 128 channels: 48 rows 74 and 110, 128 rows 178 and 117); over 2048
+// tokens 17 rows are enough (16 and 15).  Lengths are on the device, so the rule has the rows alone.
 constexpr long long kTileRows = 49;
 
 template <int D, int G, typename T>

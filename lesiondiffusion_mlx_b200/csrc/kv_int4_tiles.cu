@@ -113,7 +113,9 @@ struct Packed {
   uint32_t scale[D / kInt4Group];  // (a byte each: put together they would be waited for where they are loaded)
 };
 
-template <int D, typename T>
+// ALT: one tile of rows, alternating: tile t is the rows over the blocks of parity t, so that the softmax of one block
+// runs beside the products of the next; each leaves its part for the merge.
+template <int D, typename T, bool ALT>
 __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTileParams p, unsigned int* status) {
   using C = Cfg<D>;
   constexpr bool kScaled = !std::is_same<T, __half>::value;
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
     }
     for (int s = 0; s < kMeta; ++s) mbar_init(&meta_full[s], 4);
     for (int s = 0; s < 8; ++s) mbar_init(&pair_bar[s], 2);
-    mbar_init(q_full, p.rows - (p.row_blocks - 1 - static_cast<int>(blockIdx.x) / p.splits) * 2 * kM > kM ? 16 : 8);
+    mbar_init(q_full, ALT || p.rows - (p.row_blocks - 1 - static_cast<int>(blockIdx.x) / p.splits) * 2 * kM > kM ? 16 : 8);
     *abort_flag = 0;
     *s_bad = 0;
     fence_mbarrier_init();
@@ -193,11 +195,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
         for (int k = 0; k < kN / 16; ++k)  // (tiles of 64 channels lie kN rows apart)
           umma_ts_warp(tmem + 256 + t * 128, p_tmem + k * 8 + (C::kSeparateP || k < 4 ? 0 : 32),
                        make_smem_desc(v_addr + k * 16 * C::kSubRow, kN * C::kSubRow, 8 * C::kSubRow, C::kLayout),
-                       idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+                       idesc_pv, (j > (ALT ? 1 : 0) || k > 0) ? 1u : 0u);
         umma_commit_warp(&pv_done[t]);
       };
       bool ok = warp_wait(q_full, 0, abort_flag, status);
-      for (int j = 0; ok && j <= sp.nblocks; ++j) {
+      // (the blocks that tile j & 1 has had before block j are j >> 1)
+      for (int j = 0; ALT && ok && j < sp.nblocks + (C::kSeparateP ? 1 : 2); ++j) {
+        const int t = j & 1, last = C::kSeparateP ? j - 1 : j - 2;  // of the value product
+        auto value_product = [&] {
+          if (last < 0) return;
+          ok = warp_wait(&v_full[last & 1], static_cast<uint32_t>(last >> 1) & 1u, abort_flag, status) &&
+               warp_wait(&p_ready[last & 1], static_cast<uint32_t>(last >> 1) & 1u, abort_flag, status);
+          if (!ok) return;
+          tc_fence_after();
+          values(last & 1, last);
+          umma_commit_warp(&v_empty[last & 1]);
+        };
+        if (!C::kSeparateP) value_product();
+        if (ok && j < sp.nblocks) {
+          ok = warp_wait(&k_full[t], static_cast<uint32_t>(j >> 1) & 1u, abort_flag, status) &&
+               (!C::kSeparateP || j < 2 || warp_wait(&s_free[t], static_cast<uint32_t>((j >> 1) - 1) & 1u, abort_flag, status));
+          if (!ok) break;
+          tc_fence_after();
+          scores(t, j);
+          umma_commit_warp(&k_empty[t]);
+        }
+        if (ok && C::kSeparateP) value_product();
+      }
+      for (int j = 0; !ALT && ok && j <= sp.nblocks; ++j) {
         const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u, was = static_cast<uint32_t>(j - 1) & 1u;
         if (j < sp.nblocks) ok = warp_wait(&k_full[j & 1], ph, abort_flag, status);
         if (ok && j > 0)
@@ -330,7 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
     const int quarter = warp & 3;          // TMEM lanes this warp may access
     const int pair = t * 4 + quarter;      // with the warp of the other half
     const int local = quarter * 32 + lane;
-    const int row = sp.row0 + t * kM + local;
+    const int row = sp.row0 + (ALT ? 0 : t * kM) + local;
+    const int blocks = ALT ? (sp.nblocks - t + 1) >> 1 : sp.nblocks;  // of the tile
     const bool live = row < p.rows;
     const int i = live ? row / p.group : 0, gq = live ? row % p.group : 0;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
@@ -341,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
     float* s_row = reinterpret_cast<float*>(smem + C::kOffRow) + t * 2 * kM + local;  // [half * kM]
     volatile uint32_t* s_vote = reinterpret_cast<volatile uint32_t*>(smem + C::kOffVote) + pair * 4;
     uint32_t meets = 0;
-    bool ok = t < sp.tiles;
+    bool ok = ALT || t < sp.tiles;
     // The two warps of the rows wait for each other; what either has written to shared memory before is there for the other.
     auto meet = [&] {
       __syncwarp();
@@ -368,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
           const T* at = reinterpret_cast<const T*>(__shfl_sync(
                             0xffffffffu, reinterpret_cast<unsigned long long>(src), from)) + 8 * part_lane;
           raw[n] = make_uint4(0, 0, 0, 0);
-          if (sp.row0 + t * kM + quarter * 32 + from < p.rows) {
+          if (row - lane + from < p.rows) {
             if (p.q_vec) {
               raw[n] = *reinterpret_cast<const uint4*>(at);
             } else {
@@ -418,8 +444,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
     }
     float top = kFloor, l = 0.f;
     const uint64_t f2 = pack2(factor, factor);
-    for (int j = 0; ok && j < sp.nblocks; ++j) {
-      ok = warp_wait(&s_full[t], static_cast<uint32_t>(j) & 1u, abort_flag, status) &&
+    for (int nth = 0; ok && nth < blocks; ++nth) {
+      const int j = ALT ? 2 * nth + t : nth;
+      ok = warp_wait(&s_full[t], static_cast<uint32_t>(nth) & 1u, abort_flag, status) &&
            warp_wait(&meta_full[j % kMeta], static_cast<uint32_t>(j / kMeta) & 1u, abort_flag, status);
       if (!ok) break;
       tc_fence_after();
@@ -459,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
       };
       weights();
       // A reference seldom grows; where one of 32 rows' does, both warps scale what there is and begin again.
-      const bool mine = __any_sync(0xffffffffu, j == 0 || mx * factor > top + kGrow);
+      const bool mine = __any_sync(0xffffffffu, nth == 0 || mx * factor > top + kGrow);
       const uint32_t side = (meets & 1u) * 2;
       if (lane == 0) s_vote[side + half] = mine;
       meet();
@@ -469,11 +496,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
         meet();
         if (!ok) break;
         const float all = fmaxf(s_row[0], s_row[kM]);
-        const float next = j == 0 || all > top + kGrow ? fmaxf(top, all) : top;
+        const float next = nth == 0 || all > top + kGrow ? fmaxf(top, all) : top;
         const float scale_half = ex2_approx(0.5f * (top - next)), alpha = scale_half * scale_half;
-        if (j > 0) {
+        if (nth > 0) {
           // the value product of the block before is done: the output is whole
-          ok = warp_wait(&pv_done[t], static_cast<uint32_t>(j - 1) & 1u, abort_flag, status);
+          ok = warp_wait(&pv_done[t], static_cast<uint32_t>(nth - 1) & 1u, abort_flag, status);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -500,9 +527,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[t]);
-        if (j > 0) {
+        if (nth > 0) {
           // the value product of the block before has read its weights
-          ok = warp_wait(&pv_done[t], static_cast<uint32_t>(j - 1) & 1u, abort_flag, status);
+          ok = warp_wait(&pv_done[t], static_cast<uint32_t>(nth - 1) & 1u, abort_flag, status);
           if (!ok) break;
           tc_fence_after();
         }
@@ -514,10 +541,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[t]);
     }
-    if (ok && sp.nblocks > 0)
-      ok = warp_wait(&pv_done[t], static_cast<uint32_t>(sp.nblocks - 1) & 1u, abort_flag, status) &&
-           warp_wait(&v_full[(sp.nblocks - 1) & 1], static_cast<uint32_t>((sp.nblocks - 1) >> 1) & 1u, abort_flag,
-                     status);  // (done as well: orders the reads of s_bad)
+    if (ok && blocks > 0) {
+      const int j = ALT ? 2 * (blocks - 1) + t : blocks - 1;
+      ok = warp_wait(&pv_done[t], static_cast<uint32_t>(blocks - 1) & 1u, abort_flag, status) &&
+           warp_wait(&v_full[j & 1], static_cast<uint32_t>(j >> 1) & 1u, abort_flag, status);  // (done as well: orders the reads of s_bad)
+    }
+    if (ALT) asm volatile("bar.sync 1, 512;" ::: "memory");  // (and those of the other tile's blocks)
     if (ok) {
       s_row[half * kM] = l;
       meet();
@@ -525,7 +554,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
     if (ok) {
       tc_fence_after();
       l = s_row[0] + s_row[kM];
-      const int split = blockIdx.x % p.splits;
+      const bool parts = ALT || p.splits > 1;
+      const int split = ALT ? 2 * (blockIdx.x % p.splits) + t : blockIdx.x % p.splits;
       const long long part =
           ((static_cast<long long>(split) * p.c.batch + sp.b) * p.c.kv_heads + sp.head) * p.rows + row;
       T* dst = static_cast<T*>(p.out) + sp.b * p.out_batch + i * p.out_ld +
@@ -538,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
 #pragma unroll 2
       for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 16) {
         uint32_t r[16];
-        if (sp.nblocks > 0) {
+        if (blocks > 0) {
           tmem_ld16(tmem_o + c0, r);
           tmem_wait_ld();
         } else {
@@ -550,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
           float x[8];
 #pragma unroll
           for (int c = 0; c < 8; ++c) x[c] = __uint_as_float(r[8 * h + kOrder[c]]);
-          if (p.splits > 1) {
+          if (parts) {
             if (live) {
               float4* to = reinterpret_cast<float4*>(p.o_part + part * D + c0 + 8 * h);
               to[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -564,14 +594,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
         }
         __syncwarp();  // the next read of TMEM is the whole warp's
       }
-      if (p.splits == 1) {
+      if (!parts) {
         meet();
 #pragma unroll 4
         for (int n = half * (kLanes / 2); ok && n < (half + 1) * (kLanes / 2); ++n) {
           const int from = n * kRows + lane / kLanes, chunk = lane % kLanes;
           T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from)) +
                   8 * chunk;
-          if (sp.row0 + t * kM + quarter * 32 + from >= p.rows) continue;
+          if (row - lane + from >= p.rows) continue;
           const uint4 v = *reinterpret_cast<const uint4*>(rows + from * D * 2 + (chunk ^ (from & kSpread)) * 16);
           if (p.out_vec) {
             *reinterpret_cast<uint4*>(to) = v;
@@ -583,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
         }
         __syncwarp();
       }
-      if (p.splits > 1 && live && half == 0)
+      if (parts && live && half == 0)
         *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(top, l * fp8_pow2(-kHeadroom));
       tc_fence_before();
       const bool bad = sp.nblocks > 0 && *s_bad != 0;  // (of the CTA: both warps go on or neither)
@@ -600,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
                              tok % p.c.page;
           for (int c = half * (D / 2); c < (half + 1) * (D / 2); ++c) {
             if (s[(c / kInt4Group) * p.c.page] != kInt4NanScale) continue;
-            if (p.splits > 1) {
+            if (parts) {
               p.o_part[part * D + c] = fp8_nan();
             } else {
               dst[c] = from_f32<T>(fp8_nan());
@@ -618,47 +648,70 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
   }
 }
 
-template <int D, typename T>
-int launch(cudaStream_t stream, const KvTileParams& p, unsigned int* status) {
+template <int D, typename T, bool ALT>
+int launch(cudaStream_t stream, KvTileParams p, unsigned int* status) {
   static unsigned long long configured = 0;
-  int rc = ensure_smem_attribute(reinterpret_cast<const void*>(kv_int4_tiles_kernel<D, T>), Cfg<D>::kSmem, &configured,
-                                 "kv_attention shared memory");
+  int rc = ensure_smem_attribute(reinterpret_cast<const void*>(kv_int4_tiles_kernel<D, T, ALT>), Cfg<D>::kSmem,
+                                 &configured, "kv_attention shared memory");
   if (rc != LDB_OK) return rc;
-  rc = launch_kernel(kv_int4_tiles_kernel<D, T>, dim3(p.row_blocks * p.splits, p.c.kv_heads, p.c.batch), dim3(kThreads),
-                     Cfg<D>::kSmem, stream, "kv_attention tiles launch", p, status);
-  if (rc != LDB_OK || p.splits == 1) return rc;
+  rc = launch_kernel(kv_int4_tiles_kernel<D, T, ALT>, dim3(p.row_blocks * p.splits, p.c.kv_heads, p.c.batch),
+                     dim3(kThreads), Cfg<D>::kSmem, stream, "kv_attention tiles launch", p, status);
+  if (rc != LDB_OK || (!ALT && p.splits == 1)) return rc;
   const long long rows = static_cast<long long>(p.c.batch) * p.c.kv_heads * p.rows;
+  if (ALT) p.splits *= 2;  // (parts)
   return launch_kernel(kv_tiles_merge_kernel<D, T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, stream,
                        "kv_attention tiles merge launch", p);
 }
 
-template <typename T>
+template <typename T, bool ALT>
 int launch_dim(cudaStream_t stream, const KvTileParams& p, int head_dim, unsigned int* status) {
-  if (head_dim == 32) return launch<32, T>(stream, p, status);
-  if (head_dim == 64) return launch<64, T>(stream, p, status);
-  return launch<128, T>(stream, p, status);
+  if (head_dim == 32) return launch<32, T, ALT>(stream, p, status);
+  if (head_dim == 64) return launch<64, T, ALT>(stream, p, status);
+  return launch<128, T, ALT>(stream, p, status);
+}
+
+// How the tokens are cut: ranges, and parts that they leave.
+struct Cuts {
+  int ranges, parts;
+  bool alternate;
+};
+
+// One tile of rows alternates where its ranges are long: it stages its queries twice and leaves two parts a range, but two
+// blocks are on their way.  8 key/value heads of 128, 64 rows, us alternating and not: 16384 tokens (8 blocks a
+// range) 33 and 31, 32768 (14) 45 and 47, 131072 (57) 109 and 133; 16 items of up to 4096 tokens (32) 65 and 73, of up to
+// 16384 (128) 208 and 268; of 64 channels 26 and 24, 36 and 36, 89 and 102, 53 and 56, 174 and 204.
+Cuts cuts_of(int batch, int kv_heads, long long rows, int head_dim, long long capacity) {
+  const int ranges = kv_tile_splits(batch, kv_heads, rows, head_dim, capacity);
+  if (rows > kM || capacity < 25ll * kN * ranges) return {ranges, ranges, false};
+  // (twice the parts, in half the time of as many blocks)
+  const int pairs = kv_tile_splits(batch, kv_heads, rows, 2 * head_dim, (capacity + 1) / 2);
+  return {pairs, 2 * pairs, true};
 }
 
 }  // namespace
 
 size_t kv_int4_tile_workspace(int batch, int kv_heads, long long rows, int head_dim, long long capacity) {
-  const long long splits = kv_tile_splits(batch, kv_heads, rows, head_dim, capacity);
-  return splits <= 1 ? 0 : static_cast<size_t>(splits) * batch * kv_heads * rows * (head_dim + 2) * sizeof(float);
+  const long long parts = cuts_of(batch, kv_heads, rows, head_dim, capacity).parts;
+  return parts <= 1 ? 0 : static_cast<size_t>(parts) * batch * kv_heads * rows * (head_dim + 2) * sizeof(float);
 }
 
 int kv_int4_attention_tiles(cudaStream_t stream, KvTileParams p, int head_dim, int dtype, float scale, void* workspace,
                             unsigned int* status) {
+  const Cuts cuts = cuts_of(p.c.batch, p.c.kv_heads, p.rows, head_dim, static_cast<long long>(p.c.width) * p.c.page);
   p.row_blocks = (p.rows + 2 * kM - 1) / (2 * kM);
-  p.splits = kv_tile_splits(p.c.batch, p.c.kv_heads, p.rows, head_dim, static_cast<long long>(p.c.width) * p.c.page);
+  p.splits = cuts.ranges;
   p.negate = scale < 0.f;
   p.scale_log2 = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
   p.o_part = static_cast<float*>(workspace);
-  p.ml_part = p.o_part + static_cast<size_t>(p.splits) * p.c.batch * p.c.kv_heads * p.rows * head_dim;
+  p.ml_part = p.o_part + static_cast<size_t>(cuts.parts) * p.c.batch * p.c.kv_heads * p.rows * head_dim;
   if (static_cast<long long>(p.row_blocks) * p.splits > 0x7FFFFFFFll || p.c.kv_heads > 65535 || p.c.batch > 65535)
     return fail(LDB_ERR_SHAPE, "kv_attention: %d row blocks, %d heads, %d items", p.row_blocks, p.c.kv_heads,
                 p.c.batch);
-  return dtype == LDB_F16 ? launch_dim<__half>(stream, p, head_dim, status)
-                          : launch_dim<__nv_bfloat16>(stream, p, head_dim, status);
+  if (cuts.alternate)
+    return dtype == LDB_F16 ? launch_dim<__half, true>(stream, p, head_dim, status)
+                            : launch_dim<__nv_bfloat16, true>(stream, p, head_dim, status);
+  return dtype == LDB_F16 ? launch_dim<__half, false>(stream, p, head_dim, status)
+                          : launch_dim<__nv_bfloat16, false>(stream, p, head_dim, status);
 }
 
 }  // namespace ldb

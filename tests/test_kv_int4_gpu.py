@@ -8,6 +8,8 @@ rounded once."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -218,12 +220,17 @@ def reference(q, cache, table, lengths, group, scale, causal):
     return oracle.attention(q, oracle.values(k, ks), oracle.values(v, vs), table, lengths, group, scale, causal)
 
 
+# as many pairs as SMs, so that a tile of rows has all tokens to itself: its blocks alternate
+LONG = [3200, 0, 1, 128, 129, 255, 256, 257, 3199, 2000, 640] + [5] * 26
 CASES = [  # lengths, queries, kv heads, group, dim, page, causal
     ([1], 1, 1, 1, 64, 64, False), ([0, 3, 64, 65, 200], 1, 2, 4, 128, 64, True), ([77], 50, 4, 1, 64, 64, False),
     ([129, 17], 5, 1, 3, 32, 16, True), ([40, 0, 7], 12, 2, 2, 64, 32, True), ([300], 1, 1, 16, 128, 128, False),
     ([500, 30], 1, 1, 17, 64, 128, False), ([1500], 1, 2, 1, 128, 16, False), ([260], 130, 1, 2, 128, 64, True),
     ([5], 30, 1, 8, 32, 64, True), ([200, 128, 1], 64, 2, 4, 128, 128, True), ([333], 300, 1, 1, 64, 16, False),
-    ([63, 62, 66, 127], 2, 1, 4, 32, 32, True), ([700], 257, 1, 1, 32, 128, True), ([130], 513, 1, 1, 128, 16, False)]
+    ([63, 62, 66, 127], 2, 1, 4, 32, 32, True), ([700], 257, 1, 1, 32, 128, True), ([130], 513, 1, 1, 128, 16, False),
+    ([1100, 0, 1, 128, 129, 640, 1025], 20, 2, 4, 128, 64, True), ([1300, 257, 3], 50, 1, 1, 64, 16, False),
+    (LONG, 25, 4, 4, 128, 64, True), (LONG, 64, 4, 1, 64, 16, False), (LONG, 32, 4, 4, 32, 128, True),
+    (LONG, 49, 4, 1, 128, 32, False), ([130000, 70000], 50, 1, 1, 32, 128, True)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -274,6 +281,38 @@ def test_attention_nan_reaches_its_channels_and_the_queries_that_see_it(cuda_dev
     assert torch.equal(torch.isnan(got.cpu().view(nan.shape)), nan)
     finite = {k: torch.where(torch.isnan(x), torch.zeros_like(x), x) for k, x in ref.items()}
     finite["peak"] = torch.full_like(finite["peak"], 310 * 8 * 30.0)
+    check_attention(torch.where(nan.to(cuda_device), 0.0, got.view(nan.shape)), finite, dtype)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("queries,dim,page", [(60, 128, 64), (100, 64, 16), (128, 32, 128)])
+def test_attention_nan_and_lost_pages_among_many_blocks(cuda_device, causal, queries, dim, page):
+    """NaN groups of values in blocks of either parity that some queries see, and a page that is not there."""
+    heads, lengths, lost, dtype = 4, [1310, 1100] + [1] * 35, 5, torch.float16
+    table, pages = make_table(len(lengths), 3264 // page, 21)
+    cache = make_cache(pages, heads, dim, page, cuda_device, 22, 96, 112)
+    q = torch.randn(len(lengths), queries, heads * dim, generator=torch.Generator().manual_seed(23)).to(dtype)
+    need = ctypes.c_size_t()
+    _lib.call("ldb_kv_attention_int4_workspace_size", len(lengths), queries, heads, heads, dim, table.shape[1] * page,
+              ctypes.byref(need))
+    assert need.value == 2 * len(lengths) * heads * queries * (dim + 2) * 4  # (two parts: blocks alternate)
+    args = (q.to(cuda_device), cache)
+    kept, holes = table.clone(), table.clone()
+    kept[:, lost:-1] = table[:, lost + 1:]
+    holes[:, lost] = -1
+    if not causal:  # (a query's place among the tokens would be another)
+        got = kv_cache.kv_attention(*args, holes.to(cuda_device), ints(lengths, cuda_device), scale=dim ** -0.5)
+        assert _lib.device_status(reset=True) == 2
+        check_attention(got, reference(q, cache, kept, [max(n - page, 1) for n in lengths], 1, dim ** -0.5, False), dtype)
+    for b, head, tok, group_at in ((0, 0, 1309, 0), (0, 1, 1275, 1), (1, 0, 1099, 0), (1, 2, 1060, 1)):
+        cache.v_scale[int(table[b, tok // page]), head, group_at, tok % page] = oracle.NAN
+    ref = reference(q, cache, table, lengths, 1, dim ** -0.5, causal)
+    got = kv_cache.kv_attention(*args, table.to(cuda_device), ints(lengths, cuda_device), scale=dim ** -0.5, causal=causal)
+    nan = torch.isnan(ref["out"])
+    assert nan.any() and _lib.device_status(reset=True) == 0  # (32 channels without a mask: all of it)
+    assert torch.equal(torch.isnan(got.cpu().view(nan.shape)), nan)
+    finite = {k: torch.where(torch.isnan(x), torch.zeros_like(x), x) for k, x in ref.items()}
+    finite["peak"] = torch.full_like(finite["peak"], 1310 * 8 * 30.0)
     check_attention(torch.where(nan.to(cuda_device), 0.0, got.view(nan.shape)), finite, dtype)
 
 
