@@ -444,6 +444,36 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
     }
     float top = kFloor, l = 0.f;
     const uint64_t f2 = pack2(factor, factor);
+    // The first block's largest scores are the first reference.
+    if (ok && blocks > 0) {
+      ok = warp_wait(&s_full[t], 0, abort_flag, status) && warp_wait(&meta_full[ALT ? t : 0], 0, abort_flag, status);
+      if (ok) {
+        tc_fence_after();
+        const uint32_t missing = *reinterpret_cast<const uint32_t*>(s_meta + (ALT ? t : 0) * 4) >> (16 * half);
+        const int j0 = (sp.jb0 + (ALT ? t : 0)) * kN + 64 * half;
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t sr[32];
+          tmem_ld32(tmem_s + 32 * c, sr);
+          tmem_wait_ld32(sr);
+          if (j0 + 64 > sp.open || missing) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              hide_from(sr[k], 32 * c + k, limit - j0);
+              hide_if(sr[k], missing, 1u << (8 * c + k / 16));
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 32; k += 2)
+            m4[(k >> 1) & 3] = max3(m4[(k >> 1) & 3], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
+        }
+        s_row[half * kM] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * factor;
+        meet();
+        if (ok) top = fmaxf(top, fmaxf(s_row[0], s_row[kM]));
+        if (ok) meet();  // (s_row is free again)
+      }
+    }
     for (int nth = 0; ok && nth < blocks; ++nth) {
       const int j = ALT ? 2 * nth + t : nth;
       ok = warp_wait(&s_full[t], static_cast<uint32_t>(nth) & 1u, abort_flag, status) &&
@@ -486,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
       };
       weights();
       // A reference seldom grows; where one of 32 rows' does, both warps scale what there is and begin again.
-      const bool mine = __any_sync(0xffffffffu, nth == 0 || mx * factor > top + kGrow);
+      const bool mine = __any_sync(0xffffffffu, mx * factor > top + kGrow);
       const uint32_t side = (meets & 1u) * 2;
       if (lane == 0) s_vote[side + half] = mine;
       meet();
@@ -496,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
         meet();
         if (!ok) break;
         const float all = fmaxf(s_row[0], s_row[kM]);
-        const float next = nth == 0 || all > top + kGrow ? fmaxf(top, all) : top;
+        const float next = all > top + kGrow ? all : top;
         const float scale_half = ex2_approx(0.5f * (top - next)), alpha = scale_half * scale_half;
         if (nth > 0) {
           // the value product of the block before is done: the output is whole
