@@ -16,9 +16,9 @@
 // by a second kernel (kv_attention_tiles.cuh).
 //
 // Bound: 4 D flops and one exponential per score.  One B200, 1024 causal bf16 queries of 2 items, 32 heads of
-// 128 over 8, behind 8192 and 16384 tokens: 450 us (868 TFLOP/s), 4400 cycles a block on SMs that share 256 CTAs out
+// 128 over 8, behind 8192 and 16384 tokens: 443 us (890 TFLOP/s), 4400 cycles a block on SMs that share 256 CTAs out
 // unevenly; the products need 2048 of them and read 128 bytes of shared memory a cycle all the while.  6400 f16
-// queries of 4 heads of 64 over 6477 tokens 117 us, 4060 cycles a block for 2048 of exponentials.  Each tile is a
+// queries of 4 heads of 64 over 6477 tokens 116 us, 4060 cycles a block for 2048 of exponentials.  Each tile is a
 // chain: scores, weights (1500 cycles alone, 1024 of them exponentials), votes, value product.  Slower or
 // no faster, the first case's us: one row a thread with four unpacking warps (485) or seven (583); two
 // issuing warps (637); packed rows through a ring of cp.async (606); blocks of 64 keys with two places for each tile's scores
