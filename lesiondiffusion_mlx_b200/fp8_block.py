@@ -158,7 +158,9 @@ class Fp8TokenBlock:
         if positions is None and self.rotary is not None:
             if self.rotary.axes != 1:
                 raise ValueError(f"positions along {self.rotary.axes} axes have to be given")
-            positions = state.lengths[:, None] + torch.arange(x.shape[1], dtype=torch.int32, device=x.device)
+            positions = state.lengths[:, None]
+            if x.shape[1] != 1:
+                positions = positions + torch.arange(x.shape[1], dtype=torch.int32, device=x.device)
         rows, h = rms_norm_fp8(x, self.norm1, eps=self.eps)
         k, v = self._keys_values(rows, x.dtype)
         q, k = self._turned(self._queries(rows, h.dtype), k, positions, q_norm=self.q_norm)
