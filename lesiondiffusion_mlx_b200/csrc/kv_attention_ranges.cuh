@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(THREADS) kv_attention_merge_kernel(const AttnP
   const int group = threadIdx.x / kLanes, lane4 = threadIdx.x % kLanes;
   // slot 1 of the warp that starts the pair, slot 0 of those that go on with it
   auto part = [&](int i) { return (static_cast<long long>(first + i) * 2 + (i == 0 ? 1 : 0)) * p.tile_rows + r; };
-  float m = kFloor;
+  float m = -INFINITY;  // (no part is: a row that has seen nothing has its kernel's least reference)
   for (int i = threadIdx.x; i < count; i += THREADS) m = fmaxf(m, p.ml_part[part(i) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));

@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256) kv_tiles_merge_kernel(const KvTileParams 
   const long long at = blockIdx.x * 8ll + warp_id();
   if (at >= total) return;
   const int lane = lane_id();
-  float m = kFloor;
+  float m = -INFINITY;  // (no part is: a row that has seen nothing has its kernel's least reference)
   for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.ml_part[(s * total + at) * 2]);
   float l = 0.f, v[D / 32];
 #pragma unroll

@@ -324,7 +324,10 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
 #pragma unroll
     for (int r = 0; r < G; ++r)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) top[r][e] = kFloor, sum[r][e] = 0.f;
+      for (int e = 0; e < 2; ++e) top[r][e] = kUnseen, sum[r][e] = 0.f;
+    // Where a reference is far: the references and factors, in whose place `top` and `factor` are zero and one.
+    bool far = false;
+    float far_top[G][2], far_factor[G][2];
 
     int slot = 0;
 #pragma unroll 1
@@ -420,18 +423,21 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float m = fmaxf(fmaxf(s[r][0][e], s[r][1][e]), fmaxf(s[r][2][e], s[r][3][e]));
-          mx[r][e] = m * factor[r][e];
+          mx[r][e] = __fmul_rn(m, factor[r][e]);
           grew |= mx[r][e] > top[r][e] + kLag;
         }
-      if (__any_sync(0xffffffffu, grew)) {
+      if (__any_sync(0xffffffffu, grew) || far) {
+        bool wide = false;  // (of a far reference)
 #pragma unroll
         for (int r = 0; r < G; ++r)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float m = fmaxf(top[r][e], mx[r][e]);
+            const float was = far ? far_top[r][e] : top[r][e];
+            float m = fmaxf(was, far ? __fmul_rn(mx[r][e], far_factor[r][e]) : mx[r][e]);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float half = ex2_approx(0.5f * (top[r][e] - m)), f = half * half;
+            const float half = ex2_approx(0.5f * (was - m)), f = half * half;
+            wide |= is_far(m);
             top[r][e] = m;
             sum[r][e] = kv_scaled(sum[r][e], half);
 #pragma unroll
@@ -440,6 +446,18 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
               o[r][j][2 + e] *= f;
             }
           }
+        if (far || __any_sync(0xffffffffu, wide)) {
+#pragma unroll
+          for (int r = 0; r < G; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (!far) far_factor[r][e] = factor[r][e];
+              far_top[r][e] = top[r][e], top[r][e] = 0.f, factor[r][e] = 1.f;
+#pragma unroll
+              for (int n = 0; n < kKeys; ++n) s[r][n][e] = __fmul_rn(s[r][n][e], far_factor[r][e]) - far_top[r][e];
+            }
+          far = true;
+        }
       }
       // Weights 2^(s - M + kHeadroomLag), transposed: the fragments of p v.
       uint32_t pf[G][kKeys];
@@ -503,6 +521,12 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, G>::kCtasPerSm)
     }
 
     // The pair's rows, or this range's part of them.
+    if (far) {
+#pragma unroll
+      for (int r = 0; r < G; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) top[r][e] = far_top[r][e];
+    }
     const bool whole = tiles == item_tiles;
     const int part = me * 2 + (tile0 == 0 ? 1 : 0);
 #pragma unroll

@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
       if (factor < 1.2e-38f) factor = 1.2e-38f;  // (-inf times zero would be a NaN)
       if (ok) meet();  // (s_row is free again)
     }
-    float top = kFloor, l = 0.f;
+    float top = kUnseen, l = 0.f;
     const uint64_t f2 = pack2(factor, factor);
     // The first block's largest scores are the first reference.
     if (ok && blocks > 0) {
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
           for (int k = 0; k < 32; k += 2)
             m4[(k >> 1) & 3] = max3(m4[(k >> 1) & 3], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
         }
-        s_row[half * kM] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * factor;
+        s_row[half * kM] = __fmul_rn(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), factor);
         meet();
         if (ok) top = fmaxf(top, fmaxf(s_row[0], s_row[kM]));
         if (ok) meet();  // (s_row is free again)
@@ -486,9 +486,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
       uint32_t packed[32];
       uint64_t sum2[2];
       float mx;
-      // Weights against the reference as it is, and the thread's largest score.
-      auto weights = [&] {
-        const uint64_t shift = pack2(kHeadroom - top, kHeadroom - top);
+      // Weights 2^(by s + kHeadroom - off), and the thread's largest score.
+      auto weights = [&](uint64_t by, float off) {
+        const uint64_t shift = pack2(kHeadroom - off, kHeadroom - off);
         sum2[0] = sum2[1] = 0;
         mx = -INFINITY;
 #pragma unroll
@@ -507,26 +507,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
           for (int k = 0; k < 32; k += 2) {
             mx = max3(mx, __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
             float x0, x1;
-            unpack2(fma2(pack2(__uint_as_float(sr[k]), __uint_as_float(sr[k + 1])), f2, shift), x0, x1);
+            unpack2(fma2(pack2(__uint_as_float(sr[k]), __uint_as_float(sr[k + 1])), by, shift), x0, x1);
             const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
             sum2[(k >> 1) & 1] = add2(sum2[(k >> 1) & 1], pack2(e0, e1));
             packed[16 * c + k / 2] = as_word(__floats2half2_rn(e0, e1));
           }
         }
       };
-      weights();
-      // A reference seldom grows; where one of 32 rows' does, both warps scale what there is and begin again.
-      const bool mine = __any_sync(0xffffffffu, mx * factor > top + kGrow);
+      weights(f2, top);  // (against the reference as it is)
+      // A reference seldom grows; where one of 32 rows' does, both warps scale what there is and begin again (as they do
+      // wherever one is far).
+      const bool mine =
+          __any_sync(0xffffffffu, __fmul_rn(mx, factor) > (fabsf(top) > kFarReference ? -INFINITY : top + kGrow));
       const uint32_t side = (meets & 1u) * 2;
       if (lane == 0) s_vote[side + half] = mine;
       meet();
       if (!ok) break;
       if (mine || s_vote[side + 1 - half]) {
-        s_row[half * kM] = mx * factor;
+        s_row[half * kM] = __fmul_rn(mx, factor);
         meet();
         if (!ok) break;
         const float all = fmaxf(s_row[0], s_row[kM]);
-        const float next = all > top + kGrow ? all : top;
+        const float next = all - top > kGrow ? all : top;
         const float scale_half = ex2_approx(0.5f * (top - next)), alpha = scale_half * scale_half;
         if (nth > 0) {
           // the value product of the block before is done: the output is whole
@@ -546,7 +548,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv_int4_tiles_kernel(const KvTile
         }
         l = kv_scaled(l, scale_half);
         top = next;
-        weights();
+        const bool far = __any_sync(0xffffffffu, is_far(top));
+        if (far) {
+          // (rare) What is above the references takes the scores' place.
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(tmem_s + c, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__fmul_rn(__uint_as_float(r[k]), factor) - top);
+            tmem_st16(tmem_s + c, r);
+          }
+          tmem_wait_st();
+        }
+        const float by = far ? 1.f : factor;
+        weights(pack2(by, by), far ? 0.f : top);
         meet();  // (s_row is free again)
         if (!ok) break;
       }
