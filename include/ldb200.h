@@ -531,7 +531,8 @@ LDB_API int ldb_kv_append_int4(ldb_stream_t stream, const ldb_kv_append_desc* de
 /* Rows of a cache: k and v [batch][tokens][kv_heads * head_dim] (f16, bf16 or f32) become
  * item b's tokens start[b] .. start[b] + tokens (start null: from 0), zeros from
  * lengths[b] on and for a page number outside the cache (status bit 1, as for a
- * length outside the table or a negative start).  Exact from 4 bits, rounded once from 8. */
+ * length outside the table or a negative start).  Exact from 4 bits, rounded once from 8 (under a scale byte of
+ * 255 NaN). */
 typedef struct ldb_kv_read_desc {
   int struct_size, dtype;
   ldb_kv_cache cache;

@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadParams p, u
                                    __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)};
       store_half8<T>(value, ordered);
     } else {
-      const float s = fp8_pow2(static_cast<int>(scale) - 127);
+      const float s = scale == 255 ? fp8_nan() : fp8_pow2(static_cast<int>(scale) - 127);
       float f[8];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
