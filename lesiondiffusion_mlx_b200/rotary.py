@@ -8,14 +8,17 @@ with its own share of the channels):
     at = grid_positions(16, 20, 20, device="cuda")             # of a (B, 6400, C) volume's tokens
     q, k = qk_norm_rope(q, k, head_dim=64, q_gamma=qg, k_gamma=kg, rotary=plan, positions=at)
 
-A plan holds a position's share of a full turn as a 64-bit fraction, so that the
-angles are exact at any 32-bit position.  Inputs are channels-last ``torch`` CUDA tensors;
+A plan holds a position's share of a full turn as a 64-bit fraction, rounded once, whose product
+with a position is exact: an angle is within 2^-25 of a turn at any 32-bit position.  Inputs are channels-last ``torch`` CUDA tensors;
 the call checks shapes, dtypes and devices and launches on the current stream.
 """
 
 from __future__ import annotations
 
+import decimal
+import functools
 import math
+from fractions import Fraction
 from typing import NamedTuple, Sequence
 
 import torch
@@ -25,6 +28,30 @@ from .fp8 import _check_input, _launcher, _raw_stream
 from .ops import _DT
 
 _current_device = torch._C._cuda_getDevice
+
+
+@functools.lru_cache
+def _full_turn(bits: int) -> int:
+    """2 pi * 2^bits, within one (Machin: pi / 4 = 4 atan(1/5) - atan(1/239))."""
+    one = 1 << (bits + 32)
+
+    def atan_of_inverse(n: int) -> int:
+        total, term, k = 0, one // n, 0
+        while term:
+            total += (term // (2 * k + 1)) * (-1) ** k
+            term, k = term // (n * n), k + 1
+        return total
+
+    return 8 * (4 * atan_of_inverse(5) - atan_of_inverse(239)) >> 32
+
+
+def _turns(frequency: Fraction) -> int:
+    """``frequency / (2 pi)`` modulo 1 as a 64-bit fraction, rounded to nearest.
+
+    (In doubles it has 53 bits: 100 radians a step are off by 2^-21 of a turn at position 2^31.)"""
+    bits = 160 + max(0, abs(frequency.numerator).bit_length() - frequency.denominator.bit_length())
+    n, d = frequency.numerator << (64 + bits), frequency.denominator * _full_turn(bits)
+    return (2 * n + d) // (2 * d) % 2 ** 64
 
 
 class Rotary(NamedTuple):
@@ -41,15 +68,16 @@ class Rotary(NamedTuple):
     interleaved: bool = False
 
     @classmethod
-    def from_frequencies(cls, frequencies: Sequence[float], axis: Sequence[int] | None = None, *,
+    def from_frequencies(cls, frequencies: Sequence[float | Fraction], axis: Sequence[int] | None = None, *,
                          interleaved: bool = False, device: torch.device | str = "cuda") -> "Rotary":
         """Pairs of these frequencies (radians a step), all along one axis where ``axis`` is not given."""
         axis = [0] * len(frequencies) if axis is None else [int(a) for a in axis]
         if len(axis) != len(frequencies) or not axis or min(axis) < 0:
             raise ValueError(f"Rotary: {len(frequencies)} frequencies along {len(axis)} axes")
-        if not all(math.isfinite(f) for f in frequencies):
+        exact = [f if isinstance(f, Fraction) else float(f) for f in frequencies]
+        if not all(isinstance(f, Fraction) or math.isfinite(f) for f in exact):
             raise ValueError("Rotary: frequencies must be finite")
-        turns = [int(float(f) / (2 * math.pi) * 2 ** 64) % 2 ** 64 for f in frequencies]
+        turns = [_turns(Fraction(f)) for f in exact]
         return cls(torch.tensor([t - 2 ** 64 * (t >> 63) for t in turns], dtype=torch.int64, device=device),
                    torch.tensor(axis, dtype=torch.int32, device=device), max(axis) + 1, interleaved)
 
@@ -57,9 +85,12 @@ class Rotary(NamedTuple):
     def build(cls, dims: Sequence[int], *, base: float = 10000.0, interleaved: bool = False,
               device: torch.device | str = "cuda") -> "Rotary":
         """``dims[a]`` channels (an even number) along axis ``a``, pair ``i`` of an axis at ``base^(-2 i / dims[a])``."""
-        if not dims or any(d < 0 or d % 2 for d in dims) or base <= 0:
+        if not dims or any(d < 0 or d % 2 for d in dims) or not base > 0:
             raise ValueError(f"Rotary: {tuple(dims)} channels along the axes (even numbers), base {base}")
-        pairs = [(base ** (-2 * i / d), a) for a, d in enumerate(dims) for i in range(d // 2)]
+        with decimal.localcontext() as context:
+            context.prec = 50
+            pairs = [(Fraction(decimal.Decimal(base) ** (decimal.Decimal(-2 * i) / d)), a)
+                     for a, d in enumerate(dims) for i in range(d // 2)]
         plan = cls.from_frequencies([f for f, _ in pairs], [a for _, a in pairs], interleaved=interleaved, device=device)
         return plan._replace(axes=len(dims))
 
