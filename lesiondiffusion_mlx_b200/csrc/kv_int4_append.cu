@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_int4_kernel(const AppendPa
 #pragma unroll
       for (int h = 0; h < static_cast<int>(sizeof(T)); ++h) raw[j][h] = reinterpret_cast<const uint4*>(x)[h];
     } else {
-      T t[kInt4Group];
+      __align__(16) T t[kInt4Group];
 #pragma unroll
       for (int c = 0; c < kInt4Group; ++c) t[c] = x[c];
 #pragma unroll

@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p, unsi
           raw.w[k] = v.x, raw.w[k + 1] = v.y, raw.w[k + 2] = v.z, raw.w[k + 3] = v.w;
         }
       } else {
-        T t[8];
+        __align__(16) T t[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) t[j] = x[j];
 #pragma unroll
