@@ -545,7 +545,7 @@ LDB_API int ldb_kv_read_fp8(ldb_stream_t stream, const ldb_kv_read_desc* desc);
 LDB_API int ldb_kv_read_int4(ldb_stream_t stream, const ldb_kv_read_desc* desc);
 
 /* As ldb_kv_attention_fp8, over the 4-bit cache; workspace for a table of
- * `capacity` = width * page tokens. */
+ * `capacity` = width * page tokens.  `scale` is finite, and so is log2(e) times it. */
 typedef struct ldb_kv_attention_desc {
   int struct_size, dtype;
   ldb_kv_cache cache;

@@ -24,6 +24,7 @@
 // bound by HBM.
 
 #include <algorithm>
+#include <cmath>
 
 #include "host_common.h"
 #include "kv_attention.cuh"
@@ -642,6 +643,9 @@ int ldb_kv_attention_int4(cudaStream_t stream, const ldb_kv_attention_desc* desc
   const auto& [k_codes, v_codes, k_scales, v_scales, table, table_ld, pages, kv_heads, page, head_dim, width, batch] =
       cache;
   if (dtype != LDB_F16 && dtype != LDB_BF16) return fail(LDB_ERR_INVALID, "kv_attention: queries must be f16 or bf16");
+  // (a NaN would not reach the rows: factors are kept above zero by a maximum)
+  if (!std::isfinite(scale * 1.4426950408889634f))
+    return fail(LDB_ERR_INVALID, "kv_attention: scale %g (finite, as a power of two's factor too)", scale);
   size_t need = 0;
   int rc = ldb_kv_attention_int4_workspace_size(batch, queries, heads, kv_heads, head_dim,
                                                 static_cast<long long>(std::max(width, 0)) * std::max(page, 0), &need);
