@@ -137,7 +137,7 @@ def packed(name: str, desc: struct.Struct, *fields) -> bytes:
     """A descriptor's bytes behind its size; ``ValueError`` where a number does not fit its field."""
     try:
         return desc.pack(desc.size, *fields)
-    except (struct.error, OverflowError) as error:  # (an integer past its field, a float past its)
+    except struct.error as error:
         raise ValueError(f"{name}: {error}") from None
 
 

@@ -16,11 +16,3 @@ def test_attention_refuses_scales_that_are_not_finite(scale):
     with pytest.raises(_lib.LdbError, match="scale") as e:
         call("attention", descriptors()["attention"] | {"scale": scale})
     assert e.value.code == -1
-
-
-def test_floats_past_their_field():
-    desc = _lib.DESCRIPTORS["ldb_kv_attention_desc"]
-    fields = list(descriptors()["attention"].values())[1:]
-    for value in (1e39, -1e300):
-        with pytest.raises(ValueError, match="kv_attention"):
-            _lib.packed("kv_attention", desc, *fields[:-1], value)
