@@ -177,8 +177,9 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     pages counts as unwritten.  Items written together must not share the
     pages they write.  float16, bfloat16 or float32, any row and item stride.
 
-    In 4 bits a value is within half its scale, a 15th of the largest of its 16
-    channels (and up to an eighth more: a scale has four bits); magnitudes past 6720
+    In 4 bits a value is within half its scale: a 15th of the largest of its 16
+    channels and up to an eighth of that more (a scale has four bits), or up to 2^-18 more where that is
+    greater (scales below 2^-14 lie 2^-17 apart).  Magnitudes past 6720
     saturate, below 2^-18 they vanish, and 16 channels with one that is not finite are NaN."""
     if isinstance(cache, KvCacheInt4):
         return _append_int4(cache, k, v, table, start, counts)

@@ -1,4 +1,4 @@
-"""4-bit cache: numbers that a call's descriptor cannot hold, a scale that is not a number, and the bound on a value's error."""
+"""4-bit cache: scales that are not finite numbers, and the bound on the error of a value."""
 
 from __future__ import annotations
 
@@ -16,3 +16,18 @@ def test_attention_refuses_scales_that_are_not_finite(scale):
     with pytest.raises(_lib.LdbError, match="scale") as e:
         call("attention", descriptors()["attention"] | {"scale": scale})
     assert e.value.code == -1
+
+
+def test_error_of_a_value():
+    """Half the scale that is taken: a 15th of the group's largest and an eighth more while scales have a leading bit, and
+    2^-18 more below (the statement of ``kv_append``)."""
+    g = torch.Generator().manual_seed(1)
+    past_an_eighth = 0
+    for top in torch.exp2(torch.linspace(-20, -9, 1200, dtype=torch.float64)).tolist():
+        x = top * (2 * torch.rand(16, generator=g, dtype=torch.float64) - 1)
+        x[3] = top
+        codes, byte = oracle.quantize(x)
+        error = float(((codes.double() - 8) * oracle.SCALES[byte] - x).abs().max())
+        assert error <= max(top / 15 * 9 / 8, top / 15 + 2.0 ** -18)
+        past_an_eighth += error > top / 15 * 9 / 8
+    assert past_an_eighth
