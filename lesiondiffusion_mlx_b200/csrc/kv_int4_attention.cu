@@ -18,9 +18,9 @@
 // warps share out equally (kv_attention_ranges.cuh); a warp copies the next
 // tiles into its own ring (cp.async) while it works on one.
 //
-// One B200, one bf16 token of 32 heads of 128 over 8: behind 262144 tokens 69 us (302 MB at
-// 4.4 TB/s: 60 in this kernel, 8 in the join of its warps' parts), behind 32 items of up to 16384 70 us.  Of
-// the kernel's issue slots 65 % are taken, most by unpacking; without the unpacking it would be
+// One B200, one bf16 token of 32 heads of 128 over 8: behind 262144 tokens 70 us (302 MB at
+// 4.3 TB/s: 8 of them in the join of its warps' parts), behind 32 items of up to 16384 71 us.  Of
+// the kernel's issue slots 62 % are taken, most by unpacking; without the unpacking it would be
 // bound by HBM.
 
 #include <algorithm>

@@ -16,11 +16,12 @@
 // by a second kernel (kv_attention_tiles.cuh).
 //
 // Bound: 4 D flops and one exponential per score.  One B200, 1024 causal bf16 queries of 2 items, 32 heads of
-// 128 over 8, behind 8192 and 16384 tokens: 443 us (890 TFLOP/s), 4400 cycles a block on SMs that share 256 CTAs out
+// 128 over 8, behind 8192 and 16384 tokens: 458 us (862 TFLOP/s), some 4400 cycles a block on SMs that share 256 CTAs out
 // unevenly; the products need 2048 of them and read 128 bytes of shared memory a cycle all the while.  6400 f16
-// queries of 4 heads of 64 over 6477 tokens 116 us, 4060 cycles a block for 2048 of exponentials.  Each tile is a
-// chain: scores, weights (1500 cycles alone, 1024 of them exponentials), votes, value product.  Slower or
-// no faster, the first case's us: one row a thread with four unpacking warps (485) or seven (583); two
+// queries of 4 heads of 64 over 6477 tokens 118 us, some 4060 cycles a block for 2048 of exponentials.  Each tile is a
+// chain: scores, weights (1500 cycles alone, 1024 of them exponentials), votes, value product.  (Cycles of the kernel without
+// far references, 2 % faster.  At 80 registers a thread two tiles of 128 channels spill 20 bytes, narrower ones 12 and
+// alternating ones none.)  Slower or no faster, the first case's us, where it took 443: one row a thread with four unpacking warps (485) or seven (583); two
 // issuing warps (637); packed rows through a ring of cp.async (606); blocks of 64 keys with two places for each tile's scores
 // (476: products of 64 columns read the queries twice); the tiles' weights in strict turn (498); maxima before weights, scores
 // read from TMEM twice (481); the line of all blocks cut in equal ranges (508); polynomial exponentials.

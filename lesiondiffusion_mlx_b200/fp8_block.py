@@ -216,7 +216,8 @@ def main() -> None:
     block.extend(torch.randn(16, 2048, 2048, device="cuda", dtype=torch.bfloat16), state)
     timed("with normed heads and positions, in 4 bits", lambda: block.extend(token, state))
 
-    # the 16x20x20 level's tokens over their own, bound in 4 bits with their places in the volume
+    # The 16x20x20 level's tokens over their own, bound in 4 bits with their places in the volume.  (Over a context this
+    # short a cache saves memory, not time: the f16 attention over the same tokens takes 88 us of the GPU, this one 117.)
     volume = Fp8TokenBlock(random_weights(256, 256, 4, 4, 64, 1024), heads=4, kv_heads=4,
                            rotary=Rotary.build((16, 24, 24)))
     at = grid_positions(16, 20, 20)

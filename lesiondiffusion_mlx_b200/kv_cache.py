@@ -248,9 +248,10 @@ def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, lengths: 
     its row's largest and within 2^-18 of that below, for up to 48 rows of a
     key/value head (queries times the heads that share it) down to 2^-14; weights
     are rounded to 11 bits down to 2^-29 of the row's largest, from 49 rows on at
-    least to 2^-21, and lost below 2^-40 and 2^-32.  Over 4 bits queries are exact (bfloat16
+    least to 2^-21, and lost below 2^-40 and 2^-32; scores (as powers of two: times scale log2(e)) are to stay below
+    2^24, as weights overflow from there on.  Over 4 bits queries are exact (bfloat16
     down to 2^-31 of the row's largest); the weights have 11 bits down to 2^-25, from 49 rows on
-    2^-21, and are lost below 2^-36 and 2^-32."""
+    2^-21, and are lost below 2^-36 and 2^-32; scores may be as large as 2^127."""
     if isinstance(cache, KvCacheInt4):
         return _attention_int4(q, cache, table, lengths, scale, causal, out)
     (pages, kv_heads, page, dim), device = _check_cache(cache, "kv_attention")
