@@ -14,7 +14,7 @@ import torch
 
 from lesiondiffusion_mlx_b200 import _lib, kv_cache
 from oracle import kv_int4 as oracle
-from tests.test_kv_int4_gpu import TINY, UNIT, host, ints, make_cache, make_table
+from tests.test_kv_int4_gpu import TINY, UNIT, check_attention, host, ints, make_cache, make_table
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,42 @@ def test_scores_far_past_their_rounding(cuda_device, dtype, keys, sign, lengths,
         bad = ~((got.cpu().double().view(out.shape) - out).abs() <= bound)
         assert not bad.any(), (power, int(bad.sum()), int((~torch.isfinite(got)).sum()))
     assert _lib.device_status(reset=True) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lost", [False, True])
+@pytest.mark.parametrize("lengths,queries,heads,group,dim,page,causal", [
+    ([300, 0, 5, 64], 7, 2, 1, 128, 64, True), ([700, 33], 3, 2, 5, 64, 16, False), ([2100], 4, 1, 12, 32, 128, True),
+    ([300, 129], 60, 2, 1, 128, 64, True), ([700], 300, 1, 1, 64, 16, False), ([3000], 130, 1, 2, 32, 128, True),
+    ([3200, 2000] + [5] * 35, 60, 4, 1, 128, 64, True), ([3200, 2000] + [5] * 35, 32, 4, 4, 32, 128, False)])
+def test_rows_beside_far_ones(cuda_device, dtype, lost, lengths, queries, heads, group, dim, page, causal):
+    """Every third query's scores are about 2^25, one query is NaN and one has an infinity: the others' outputs are theirs."""
+    if lost and causal:
+        pytest.skip("a query's place among the tokens would be another")
+    table, pages = make_table(len(lengths), -(-max(lengths) // page) + 1, 11)
+    cache = make_cache(pages, heads, dim, page, cuda_device, 12, 96, 112)
+    q = torch.randn(len(lengths), queries, heads * group * dim, generator=torch.Generator().manual_seed(13))
+    scale = 2.0 ** 14 * dim ** -0.5
+    q *= 2.0 ** -13
+    q[:, ::3] *= 2.0 ** 20
+    q[0, -2, 3], q[0, -1, 0] = float("nan"), float("inf")
+    q = q.to(dtype)
+    seen, kept = lengths, table
+    if lost:  # the first item's second page
+        kept = table.clone()
+        kept[0, 1:-1] = table[0, 2:]
+        seen = [lengths[0] - page, *lengths[1:]]
+        table = table.clone()
+        table[0, 1] = pages
+    got = kv_cache.kv_attention(q.to(cuda_device), cache, table.to(cuda_device), ints(lengths, cuda_device), scale=scale,
+                                causal=causal).cpu()
+    assert _lib.device_status(reset=True) == (2 if lost else 0)
+    heads_of = got.view(len(lengths), queries, -1, dim)
+    assert torch.isnan(heads_of[0, -2, 0]).all() and torch.isnan(heads_of[0, -1, 0]).all()
+    far = [i for i in range(0, queries, 3) if i < queries - 2]
+    codes_k, codes_v, scales_k, scales_v = host(cache)
+    v = oracle.values(codes_v, scales_v)
+    assert (got[:, far].abs().double() <= v.abs().max() * (1 + 2.0 ** -7)).all()
+    rest = [i for i in range(queries) if i % 3 and i < queries - 2]
+    ref = oracle.attention(q, oracle.values(codes_k, scales_k), v, kept, seen, group, scale, causal)
+    check_attention(got[:, rest], {k: x[:, rest] for k, x in ref.items()}, dtype)
